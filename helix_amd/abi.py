@@ -29,6 +29,11 @@ ABI_SYMBOLS = (
 )
 HOST_SYMBOLS = ("helix_ctx_create_host", "helix_scan_plan_info", "helix_scan_run_info", "helix_scan_run",
                 "helix_scan_encode_noalloc")
+# include/helix/helix_layer.h
+LAYER_SYMBOLS = ("helix_norm_encode", "helix_quantize_fp8_encode", "helix_norm_backward_scratch_size",
+                 "helix_norm_backward_encode", "helix_matmul_fp8_encode", "helix_gated_scan_scratch_size",
+                 "helix_gated_scan_encode", "helix_gated_scan_backward_scratch_size",
+                 "helix_gated_scan_backward_encode")
 # include/helix/helix_host.h HELIX_PASS_B_*: where Pass B's segment scan runs
 PASS_B_LAUNCHED, PASS_B_IN_C = 0, 1
 # include/helix/helix_host.h HELIX_NOALLOC_SCRATCH_BYTES
@@ -82,6 +87,12 @@ class HelixRunInfo(ctypes.Structure):
 # struct.pack: filling ctypes fields one by one cost more than the launches.
 DESC_STRUCT = struct.Struct("=6i24q5i?3x2f")
 ARGS_STRUCT = struct.Struct("=11Q")
+# The argument structs of include/helix/helix_layer.h, field by field.
+NORM_STRUCT = struct.Struct("=q3if8Q6q")
+NORM_BACKWARD_STRUCT = struct.Struct("=q4i9Q4q")
+MATMUL_FP8_STRUCT = struct.Struct("=4i5Q5q")
+GATED_SCAN_STRUCT = struct.Struct("=4i7Q6q")
+GATED_SCAN_BACKWARD_STRUCT = struct.Struct("=4i11Q12q")
 assert DESC_STRUCT.size == ctypes.sizeof(HelixScanDesc)
 
 
@@ -136,6 +147,13 @@ def lib():
     L.helix_scan_plan_info.restype = c_int
     L.helix_scan_run_info.argtypes = [c_void_p, dp, POINTER(HelixRunInfo)]
     L.helix_scan_run_info.restype = c_int
+    # The arguments as packed bytes (NORM_STRUCT and the others).
+    for name in LAYER_SYMBOLS:
+        fn = getattr(L, name)
+        if name.endswith("_size"):
+            fn.argtypes, fn.restype = [c_char_p], c_size_t
+        else:
+            fn.argtypes, fn.restype = [c_void_p, c_void_p, c_char_p], c_int
     _lib = L
     return L
 

@@ -9,3 +9,6 @@
 #include "pass_c_walk16.hip"
 #include "pass_c_walk_x6.hip"
 #include "pass_single.hip"
+#include "rms_norm.hip"
+#include "matmul_fp8.hip"
+#include "gated_scan.hip"

@@ -104,6 +104,11 @@ extern "C" helix_status helix_ctx_create(helix_ctx** out, void* device, const ch
             }
             ctx->kernels[names[i]] = f;
         }
+        for (const std::string& name : helix::rt::layer_kernel_names()) {
+            hipFunction_t f = nullptr;
+            if (hipModuleGetFunction(&f, ctx->module, name.c_str()) == hipSuccess && f) ctx->kernels[name] = f;
+            else (void)hipGetLastError();
+        }
     }
     if (prev >= 0 && prev != dev) (void)hipSetDevice(prev);
 

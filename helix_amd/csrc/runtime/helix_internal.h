@@ -10,6 +10,7 @@
 #include <cstdint>
 #include <string>
 #include <unordered_map>
+#include <vector>
 
 #include "helix/helix.h"
 #include "../kernels/helix_params.h"
@@ -122,6 +123,10 @@ helix_tuning tuning_from_env();
 
 // Every kernel name in the traits tables; all are resolved at context creation.
 const char* const* all_kernel_names(size_t* count);
+
+// The layer operators' kernels (layer.cpp). A code object without them serves
+// the scan alone; their entry points then fail.
+const std::vector<std::string>& layer_kernel_names();
 
 // Never fails: falls back to the fp32 path whenever bf16 is not requested or
 // not serviceable. A pure function of the context's tuning and the

@@ -1,0 +1,387 @@
+// layer.cpp -- the entry points of the layer operators (helix_layer.h): checks,
+// choice of the kernel, launches. As in dispatch.cpp every check comes before the
+// first launch, and nothing is allocated, synchronized or waited for.
+#include <algorithm>
+#include <cmath>
+#include <cstdint>
+#include <exception>
+#include <string>
+
+#include "helix/helix_layer.h"
+#include "helix_internal.h"
+#include "../kernels/layer_params.h"
+
+using helix::rt::set_error;
+
+namespace {
+
+const char* const kTags[] = {"f32", "f16", "bf16"};   // by helix_dtype
+const size_t kBytes[] = {4, 2, 2};
+
+bool dtype_ok(int32_t t) { return t == HELIX_F32 || t == HELIX_F16 || t == HELIX_BF16; }
+
+bool aligned(const void* p, size_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
+
+struct Bad {
+    helix_status st;
+    std::string why;
+};
+
+void need(bool ok, const char* why, helix_status st = HELIX_ERR_INVALID_ARG) {
+    if (!ok) throw Bad{st, why};
+}
+
+// A matrix of `rows` rows of `dim` elements of `es` bytes, `ld` apart: present,
+// aligned to its elements, and with rows that do not overlap where it is written.
+void matrix(const char* name, const void* p, long long rows, long long dim, long long ld, size_t es, bool written) {
+    const std::string n = name;
+    if (!p) throw Bad{HELIX_ERR_INVALID_ARG, n + " is NULL"};
+    if (!aligned(p, es)) throw Bad{HELIX_ERR_INVALID_ARG, n + " is not aligned to its elements"};
+    if (ld < 0 || (written && rows > 1 && ld < dim))
+        throw Bad{HELIX_ERR_INVALID_ARG, n + (written ? ": rows overlap" : ": negative stride")};
+}
+
+// The current device is the context's while it lives.
+class OnDevice {
+public:
+    explicit OnDevice(int device) : device_(device) {
+        (void)hipGetDevice(&prev_);
+        if (prev_ != device_ && hipSetDevice(device_) != hipSuccess) {
+            (void)hipGetLastError();
+            throw Bad{HELIX_ERR_NO_DEVICE, "hipSetDevice failed"};
+        }
+    }
+    ~OnDevice() {
+        if (prev_ >= 0 && prev_ != device_) (void)hipSetDevice(prev_);
+    }
+
+private:
+    int device_, prev_ = -1;
+};
+
+hipFunction_t kernel(const helix_ctx* ctx, const std::string& name) {
+    need(ctx->module != nullptr, "context has no device (host-only context)", HELIX_ERR_NO_DEVICE);
+    const auto it = ctx->kernels.find(name);
+    if (it == ctx->kernels.end()) throw Bad{HELIX_ERR_PIPELINE, "kernel " + name + " is not in the code object"};
+    return it->second;
+}
+
+template <typename P>
+void launch(hipFunction_t f, void* stream, unsigned gx, unsigned gy, unsigned threads, P& params) {
+    void* args[] = {&params};
+    const hipError_t e = hipModuleLaunchKernel(f, gx, gy, 1, threads, 1, 1, 0, static_cast<hipStream_t>(stream), args,
+                                               nullptr);
+    if (e != hipSuccess) {
+        (void)hipGetLastError();
+        throw Bad{HELIX_ERR_PIPELINE, std::string("kernel launch failed: ") + hipGetErrorString(e)};
+    }
+}
+
+unsigned grid(long long n) {
+    need(n <= 0x7fffffffLL, "launch grid exceeds 2^31 workgroups");
+    return (unsigned)n;
+}
+
+long long ceil_div(long long a, long long b) { return (a + b - 1) / b; }
+
+// Runs an entry point's body: no exception leaves it.
+template <typename F>
+helix_status entry(helix_ctx* ctx, F&& body) {
+    try {
+        body();
+        return HELIX_OK;
+    } catch (const Bad& b) {
+        set_error(ctx, b.why);
+        return b.st;
+    } catch (const std::exception& e) {
+        set_error(ctx, e.what());
+        return HELIX_ERR_PIPELINE;
+    }
+}
+
+constexpr int kNormThreads = 256;
+
+void norm(helix_ctx* ctx, void* stream, const helix_norm_args* a, bool quantize) {
+    need(ctx && a, "NULL context or arguments");
+    need(a->rows >= 0 && a->dim >= 1 && a->dim <= HELIX_LAYER_MAX_DIM, "rows or dim out of range",
+         HELIX_ERR_UNSUPPORTED_SHAPE);
+    need(dtype_ok(a->io_dtype), "io_dtype is none of HELIX_F32, HELIX_F16 and HELIX_BF16");
+    if (a->rows == 0) return;   // an empty tensor may have no address
+    if (quantize) {
+        need(!a->weight && !a->rstd && !a->y, "quantisation takes no weight, rstd or y");
+        need(a->q != nullptr, "q is NULL");
+    } else {
+        need(a->weight_dtype == HELIX_F32 || a->weight_dtype == a->io_dtype,
+             "weight_dtype is neither HELIX_F32 nor io_dtype");
+        need(!a->y != !a->q, "exactly one of y and q is wanted");
+        need(std::isfinite(a->eps) && a->eps >= 0, "eps is negative or not finite");
+    }
+    const size_t es = kBytes[a->io_dtype];
+    const long long blocks = ceil_div(a->dim, HELIX_FP8_BLOCK);
+    matrix("x", a->x, a->rows, a->dim, a->ld_x, es, false);
+    if (a->residual) matrix("residual", a->residual, a->rows, a->dim, a->ld_residual, es, false);
+    if (!quantize) matrix("weight", a->weight, 1, a->dim, 0, kBytes[a->weight_dtype], false);
+    if (a->h) matrix("h", a->h, a->rows, a->dim, a->ld_h, es, true);
+    if (a->y) matrix("y", a->y, a->rows, a->dim, a->ld_y, es, true);
+    if (a->q) {
+        matrix("q", a->q, a->rows, a->dim, a->ld_q, 1, true);
+        matrix("scale", a->scale, a->rows, blocks, a->ld_scale, 1, true);
+    }
+    need(aligned(a->rstd, 4), "rstd is not aligned to its elements");
+
+    HelixNormParams p{};
+    p.x = a->x;
+    p.residual = a->residual;
+    p.weight = a->weight;
+    p.h = a->h;
+    p.y = a->y;
+    p.q = static_cast<uint8_t*>(a->q);
+    p.scale = static_cast<uint8_t*>(a->scale);
+    p.rstd = a->rstd;
+    p.ld_x = a->ld_x;
+    p.ld_residual = a->ld_residual;
+    p.ld_h = a->ld_h;
+    p.ld_y = a->ld_y;
+    p.ld_q = a->ld_q;
+    p.ld_scale = a->ld_scale;
+    p.rows = a->rows;
+    p.dim = a->dim;
+    p.w_f32 = a->weight_dtype == HELIX_F32;
+    p.eps = a->eps;
+    const unsigned gx = grid(a->rows);
+    const hipFunction_t f = kernel(ctx, std::string("helix_norm_") + kTags[a->io_dtype]);
+    const OnDevice on(ctx->device);
+    launch(f, stream, gx, 1, kNormThreads, p);
+}
+
+// Parts that dweight's rows are summed in: as many as give every CU four
+// workgroups of 256 channels, of 16 rows at least.
+long long norm_parts(long long rows, long long dim) {
+    const long long most = ceil_div(1024, ceil_div(dim, kNormThreads));
+    return std::max(1LL, std::min(most, rows / 16));
+}
+
+}  // namespace
+
+namespace helix::rt {
+
+const std::vector<std::string>& layer_kernel_names() {
+    static const std::vector<std::string> names = [] {
+        std::vector<std::string> v{"helix_norm_dw"};
+        for (const char* t : kTags)
+            for (const char* k : {"helix_norm_", "helix_norm_bwd_", "helix_norm_dw_part_", "helix_matmul_fp8_",
+                                  "helix_gated_scan_", "helix_gated_scan_bwd_"})
+                v.push_back(std::string(k) + t);
+        return v;
+    }();
+    return names;
+}
+
+}  // namespace helix::rt
+
+extern "C" helix_status helix_norm_encode(helix_ctx* ctx, void* stream, const helix_norm_args* args) {
+    return entry(ctx, [&] { norm(ctx, stream, args, false); });
+}
+
+extern "C" helix_status helix_quantize_fp8_encode(helix_ctx* ctx, void* stream, const helix_norm_args* args) {
+    return entry(ctx, [&] { norm(ctx, stream, args, true); });
+}
+
+extern "C" size_t helix_norm_backward_scratch_size(const helix_norm_backward_args* a) {
+    if (!a || !a->dweight || a->rows <= 0 || a->dim <= 0) return 0;
+    return (size_t)norm_parts(a->rows, a->dim) * a->dim * sizeof(float);
+}
+
+extern "C" helix_status helix_norm_backward_encode(helix_ctx* ctx, void* stream, const helix_norm_backward_args* a) {
+    return entry(ctx, [&] {
+        need(ctx && a, "NULL context or arguments");
+        need(a->rows >= 0 && a->dim >= 1 && a->dim <= HELIX_LAYER_MAX_DIM, "rows or dim out of range",
+             HELIX_ERR_UNSUPPORTED_SHAPE);
+        need(dtype_ok(a->io_dtype), "io_dtype is none of HELIX_F32, HELIX_F16 and HELIX_BF16");
+        need(a->weight_dtype == HELIX_F32 || a->weight_dtype == a->io_dtype,
+             "weight_dtype is neither HELIX_F32 nor io_dtype");
+        need(a->reserved == 0, "reserved is not 0");
+        need(aligned(a->dweight, 4), "dweight is not aligned to its elements");
+        const size_t es = kBytes[a->io_dtype];
+        if (a->rows) {
+            matrix("dy", a->dy, a->rows, a->dim, a->ld_dy, es, false);
+            matrix("h", a->h, a->rows, a->dim, a->ld_h, es, false);
+            matrix("weight", a->weight, 1, a->dim, 0, kBytes[a->weight_dtype], false);
+            matrix("rstd", a->rstd, 1, a->rows, 0, 4, false);
+            if (a->dh) matrix("dh", a->dh, a->rows, a->dim, a->ld_dh, es, false);
+            matrix("dx", a->dx, a->rows, a->dim, a->ld_dx, es, true);
+            const size_t want = helix_norm_backward_scratch_size(a);
+            need(want == 0 || (a->scratch && a->scratch_bytes >= want),
+                 "scratch smaller than helix_norm_backward_scratch_size()", HELIX_ERR_SCRATCH_TOO_SMALL);
+            need(aligned(a->scratch, 16), "scratch is not 16-byte aligned");
+        } else if (!a->dweight) {
+            return;
+        }
+        HelixNormBwdParams p{};
+        p.dy = a->dy;
+        p.h = a->h;
+        p.weight = a->weight;
+        p.rstd = a->rstd;
+        p.dh = a->dh;
+        p.dx = a->dx;
+        p.dweight = a->dweight;
+        p.part = static_cast<float*>(a->scratch);
+        p.ld_dy = a->ld_dy;
+        p.ld_h = a->ld_h;
+        p.ld_dh = a->ld_dh;
+        p.ld_dx = a->ld_dx;
+        p.rows = a->rows;
+        p.dim = a->dim;
+        p.w_f32 = a->weight_dtype == HELIX_F32;
+        p.parts = a->rows ? (int)norm_parts(a->rows, a->dim) : 0;   // no rows: dweight is 0
+        p.part_rows = p.parts ? ceil_div(a->rows, p.parts) : 0;
+        const std::string tag = kTags[a->io_dtype];
+        const unsigned gx = grid(a->rows);
+        const unsigned gc = (unsigned)ceil_div(a->dim, kNormThreads);
+        const hipFunction_t dx = kernel(ctx, "helix_norm_bwd_" + tag), part = kernel(ctx, "helix_norm_dw_part_" + tag),
+                            dw = kernel(ctx, "helix_norm_dw");
+        const OnDevice on(ctx->device);
+        if (p.dweight) {   // first: dx may be dy
+            if (p.parts) launch(part, stream, gc, (unsigned)p.parts, kNormThreads, p);
+            launch(dw, stream, gc, 1, kNormThreads, p);
+        }
+        if (a->rows) launch(dx, stream, gx, 1, kNormThreads, p);
+    });
+}
+
+extern "C" helix_status helix_matmul_fp8_encode(helix_ctx* ctx, void* stream, const helix_matmul_fp8_args* a) {
+    return entry(ctx, [&] {
+        need(ctx && a, "NULL context or arguments");
+        need(a->m >= 0 && a->n >= 0 && a->k >= 1 && a->k <= HELIX_LAYER_MAX_DIM, "m, n or k out of range",
+             HELIX_ERR_UNSUPPORTED_SHAPE);
+        need(dtype_ok(a->out_dtype), "out_dtype is none of HELIX_F32, HELIX_F16 and HELIX_BF16");
+        if (a->m == 0 || a->n == 0) return;
+        const long long blocks = ceil_div(a->k, HELIX_FP8_BLOCK);
+        matrix("a", a->a, a->m, a->k, a->ld_a, 16, false);
+        matrix("b", a->b, a->n, a->k, a->ld_b, 16, false);
+        matrix("a_scale", a->a_scale, a->m, blocks, a->ld_a_scale, 1, false);
+        matrix("b_scale", a->b_scale, a->n, blocks, a->ld_b_scale, 1, false);
+        matrix("c", a->c, a->m, a->n, a->ld_c, kBytes[a->out_dtype], true);
+        need((a->m == 1 || a->ld_a % 16 == 0) && (a->n == 1 || a->ld_b % 16 == 0),
+             "ld_a and ld_b have to be multiples of 16");
+        HelixMatmulParams p{};
+        p.a = static_cast<const uint8_t*>(a->a);
+        p.a_scale = static_cast<const uint8_t*>(a->a_scale);
+        p.b = static_cast<const uint8_t*>(a->b);
+        p.b_scale = static_cast<const uint8_t*>(a->b_scale);
+        p.c = a->c;
+        p.ld_a = a->ld_a;
+        p.ld_a_scale = a->ld_a_scale;
+        p.ld_b = a->ld_b;
+        p.ld_b_scale = a->ld_b_scale;
+        p.ld_c = a->ld_c;
+        p.m = a->m;
+        p.n = a->n;
+        p.k = a->k;
+        const unsigned gx = grid(ceil_div(a->m, 16) * ceil_div(a->n, 16));
+        const hipFunction_t f = kernel(ctx, std::string("helix_matmul_fp8_") + kTags[a->out_dtype]);
+        const OnDevice on(ctx->device);
+        launch(f, stream, gx, 1, 64, p);
+    });
+}
+
+namespace {
+
+constexpr int kScanThreads = 256;
+
+template <typename A>
+bool scan_shape(const A& a) {
+    need(a.n_seq >= 0 && a.n_tok >= 0 && a.n_chan >= 0, "n_seq, n_tok or n_chan is negative",
+         HELIX_ERR_UNSUPPORTED_SHAPE);
+    need(dtype_ok(a.io_dtype), "io_dtype is none of HELIX_F32, HELIX_F16 and HELIX_BF16");
+    return a.n_seq && a.n_chan;
+}
+
+// A tensor (n_seq, n_tok, n_chan) with contiguous channels.
+template <typename A>
+void tokens(const char* name, const A& a, const void* p, long long seq, long long tok, bool written) {
+    if (!a.n_tok) return;
+    matrix(name, p, a.n_tok, a.n_chan, tok, kBytes[a.io_dtype], written);
+    need(seq >= 0 && (!written || a.n_seq == 1 || seq >= a.n_chan), "sequences overlap or have a negative stride");
+}
+
+}  // namespace
+
+extern "C" size_t helix_gated_scan_scratch_size(const helix_gated_scan_args*) { return 0; }
+
+extern "C" helix_status helix_gated_scan_encode(helix_ctx* ctx, void* stream, const helix_gated_scan_args* a) {
+    return entry(ctx, [&] {
+        need(ctx && a, "NULL context or arguments");
+        if (!scan_shape(*a)) return;
+        tokens("g", *a, a->g, a->seq_g, a->tok_g, false);
+        tokens("v", *a, a->v, a->seq_v, a->tok_v, false);
+        tokens("h", *a, a->h, a->seq_h, a->tok_h, true);
+        need(aligned(a->h0, 4) && aligned(a->last, 4), "h0 or last is not aligned to its elements");
+        HelixGatedScanParams p{};
+        p.g = a->g;
+        p.v = a->v;
+        p.h0 = a->h0;
+        p.h = a->h;
+        p.last = a->last;
+        p.seq_g = a->seq_g;
+        p.tok_g = a->tok_g;
+        p.seq_v = a->seq_v;
+        p.tok_v = a->tok_v;
+        p.seq_h = a->seq_h;
+        p.tok_h = a->tok_h;
+        p.n_seq = a->n_seq;
+        p.n_tok = a->n_tok;
+        p.n_chan = a->n_chan;
+        const unsigned gx = grid(ceil_div((long long)a->n_seq * a->n_chan, kScanThreads));
+        const hipFunction_t f = kernel(ctx, std::string("helix_gated_scan_") + kTags[a->io_dtype]);
+        const OnDevice on(ctx->device);
+        launch(f, stream, gx, 1, kScanThreads, p);
+    });
+}
+
+extern "C" size_t helix_gated_scan_backward_scratch_size(const helix_gated_scan_backward_args*) { return 0; }
+
+extern "C" helix_status helix_gated_scan_backward_encode(helix_ctx* ctx, void* stream,
+                                                         const helix_gated_scan_backward_args* a) {
+    return entry(ctx, [&] {
+        need(ctx && a, "NULL context or arguments");
+        if (!scan_shape(*a)) return;
+        tokens("dh", *a, a->dh, a->seq_dh, a->tok_dh, false);
+        tokens("g", *a, a->g, a->seq_g, a->tok_g, false);
+        tokens("v", *a, a->v, a->seq_v, a->tok_v, false);
+        tokens("h", *a, a->h, a->seq_h, a->tok_h, false);
+        tokens("dg", *a, a->dg, a->seq_dg, a->tok_dg, true);
+        tokens("dv", *a, a->dv, a->seq_dv, a->tok_dv, true);
+        need(aligned(a->h0, 4) && aligned(a->dh_last, 4) && aligned(a->dh0, 4),
+             "h0, dh_last or dh0 is not aligned to its elements");
+        HelixGatedScanBwdParams p{};
+        p.dh = a->dh;
+        p.g = a->g;
+        p.v = a->v;
+        p.h = a->h;
+        p.h0 = a->h0;
+        p.dh_last = a->dh_last;
+        p.dg = a->dg;
+        p.dv = a->dv;
+        p.dh0 = a->dh0;
+        p.seq_dh = a->seq_dh;
+        p.tok_dh = a->tok_dh;
+        p.seq_g = a->seq_g;
+        p.tok_g = a->tok_g;
+        p.seq_v = a->seq_v;
+        p.tok_v = a->tok_v;
+        p.seq_h = a->seq_h;
+        p.tok_h = a->tok_h;
+        p.seq_dg = a->seq_dg;
+        p.tok_dg = a->tok_dg;
+        p.seq_dv = a->seq_dv;
+        p.tok_dv = a->tok_dv;
+        p.n_seq = a->n_seq;
+        p.n_tok = a->n_tok;
+        p.n_chan = a->n_chan;
+        const unsigned gx = grid(ceil_div((long long)a->n_seq * a->n_chan, kScanThreads));
+        const hipFunction_t f = kernel(ctx, std::string("helix_gated_scan_bwd_") + kTags[a->io_dtype]);
+        const OnDevice on(ctx->device);
+        launch(f, stream, gx, 1, kScanThreads, p);
+    });
+}

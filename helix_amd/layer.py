@@ -1,0 +1,86 @@
+"""What the layer operators' bindings (helix_amd.norm, helix_amd.matmul, helix_amd.recurrence) share: checks of
+tensors, streams, scratch and errors. The arithmetic runs in the HIP kernels of libhelix.so
+(include/helix/helix_layer.h)."""
+from __future__ import annotations
+
+import torch
+
+from .abi import HelixError
+from .desc import HELIX_BF16, HELIX_F16, HELIX_F32, HELIX_OK
+from .scan import _capturing, _contexts, _scratch_for, _under, context
+
+IO_DTYPES = {torch.float32: HELIX_F32, torch.bfloat16: HELIX_BF16, torch.float16: HELIX_F16}
+FP8 = torch.float8_e4m3fn
+FP8_SCALE = torch.float8_e8m0fnu
+# HELIX_FP8_BLOCK: elements of a row that share a scale
+FP8_BLOCK = 128
+
+
+def device_index(op: str, t: torch.Tensor) -> int:
+    dev = t.device
+    if dev.type != "cuda":
+        raise ValueError(f"{op} runs on a HIP device; got {dev}")
+    return dev.index if dev.index is not None else torch.cuda.current_device()
+
+
+def io_code(name: str, t: torch.Tensor) -> int:
+    code = IO_DTYPES.get(t.dtype)
+    if code is None:
+        raise ValueError(f"{name} must be float32, bfloat16 or float16; got {t.dtype}")
+    return code
+
+
+def expect(name: str, t: torch.Tensor, dtype: torch.dtype, shape, like: torch.Tensor) -> None:
+    if t.dtype != dtype or t.device != like.device:
+        raise ValueError(f"{name} must be {dtype} on {like.device}; got {t.dtype} on {t.device}")
+    if t.shape != shape:
+        raise ValueError(f"{name} must have shape {tuple(shape)}; got {tuple(t.shape)}")
+
+
+def row_stride(name: str, t: torch.Tensor) -> int:
+    """The one stride of the rows of t [..., dim], whose leading dimensions have to collapse into one."""
+    if t.is_contiguous():
+        return t.shape[-1]
+    if t.stride(-1) != 1 and t.shape[-1] > 1:
+        raise ValueError(f"{name}: the last dimension must be contiguous")
+    ld = None     # stride of the rows so far, from the inside out
+    span = 0      # stride that the next dimension has to have
+    for n, s in zip(reversed(t.shape[:-1]), reversed(t.stride()[:-1])):
+        if n == 1:
+            continue
+        if ld is None:
+            ld = s
+        elif s != span:
+            raise ValueError(f"{name}: the leading dimensions must collapse into rows of one stride")
+        span = s * n
+    return t.shape[-1] if ld is None else ld
+
+
+def stream_handle(index: int, stream) -> int:
+    return stream.cuda_stream if stream is not None else torch._C._cuda_getCurrentRawStream(index)
+
+
+def under(index: int, stream):
+    """The context that outputs are allocated in, so that their memory is the stream's own."""
+    return _under(index, 0 if stream is None else stream.cuda_stream, stream)
+
+
+def scratch(index: int, st: int, stream, nbytes: int) -> torch.Tensor | None:
+    """Scratch of the calling thread for the stream; work under capture gets memory of the graph's own."""
+    if not nbytes:
+        return None
+    if torch.cuda.is_current_stream_capturing() if stream is None else _capturing(index, st, stream):
+        with _under(index, st, stream):
+            return torch.empty(nbytes, dtype=torch.uint8, device=f"cuda:{index}")
+    return _scratch_for(index, st, nbytes, stream)
+
+
+def run(fn, index: int, st: int, args: bytes) -> None:
+    ctx = _contexts.get(index) or context(index)
+    rc = fn(ctx.handle, st, args)
+    if rc != HELIX_OK:
+        raise HelixError(rc, ctx.last_error())
+
+
+def ptr(t: torch.Tensor | None) -> int:
+    return 0 if t is None else t.data_ptr()
