@@ -52,6 +52,22 @@ typedef struct {
     int            m, n, k;
 } HelixMatmulParams;
 
+/* Gated recurrence: tokens of a thread's run, forward and backward, chunks of a
+ * group, and most tokens that one thread walks by itself. */
+#define HELIX_GS_RUN 8
+#define HELIX_GS_RUN_BWD 4
+#define HELIX_GS_GROUP 8
+#define HELIX_GS_STEPS 16
+
+/* Scratch that the chunks of a stream (64 channels of a sequence) are joined
+ * through, filled with ones; unused with one chunk. */
+typedef struct {
+    unsigned*           ticket;   /* one less than the next ticket             */
+    unsigned long long* part;     /* [stream][chunk][64] (A, B) of a chunk     */
+    unsigned*           left;     /* [stream][group][64] state after a group   */
+    int                 n_chunk, n_group;
+} HelixGatedScanJoin;
+
 typedef struct {
     const void*  g;
     const void*  v;
@@ -60,6 +76,8 @@ typedef struct {
     float*       last;      /* may be null                                     */
     long long    seq_g, tok_g, seq_v, tok_v, seq_h, tok_h;
     int          n_seq, n_tok, n_chan;
+    int          n_slab;    /* ceil(n_chan / 64)                               */
+    HelixGatedScanJoin join;
 } HelixGatedScanParams;
 
 typedef struct {
@@ -74,6 +92,8 @@ typedef struct {
     float*       dh0;       /* may be null                                     */
     long long    seq_dh, tok_dh, seq_g, tok_g, seq_v, tok_v, seq_h, tok_h, seq_dg, tok_dg, seq_dv, tok_dv;
     int          n_seq, n_tok, n_chan;
+    int          n_slab;    /* ceil(n_chan / 64)                               */
+    HelixGatedScanJoin join;
 } HelixGatedScanBwdParams;
 
 #endif

@@ -66,15 +66,19 @@ hipFunction_t kernel(const helix_ctx* ctx, const std::string& name) {
     return it->second;
 }
 
-template <typename P>
-void launch(hipFunction_t f, void* stream, unsigned gx, unsigned gy, unsigned threads, P& params) {
-    void* args[] = {&params};
+void launch_args(hipFunction_t f, void* stream, unsigned gx, unsigned gy, unsigned threads, void** args) {
     const hipError_t e = hipModuleLaunchKernel(f, gx, gy, 1, threads, 1, 1, 0, static_cast<hipStream_t>(stream), args,
                                                nullptr);
     if (e != hipSuccess) {
         (void)hipGetLastError();
         throw Bad{HELIX_ERR_PIPELINE, std::string("kernel launch failed: ") + hipGetErrorString(e)};
     }
+}
+
+template <typename P>
+void launch(hipFunction_t f, void* stream, unsigned gx, unsigned gy, unsigned threads, P& params) {
+    void* args[] = {&params};
+    launch_args(f, stream, gx, gy, threads, args);
 }
 
 unsigned grid(long long n) {
@@ -167,11 +171,14 @@ namespace helix::rt {
 
 const std::vector<std::string>& layer_kernel_names() {
     static const std::vector<std::string> names = [] {
-        std::vector<std::string> v{"helix_norm_dw"};
+        std::vector<std::string> v{"helix_norm_dw", "helix_gated_scan_fill"};
         for (const char* t : kTags)
-            for (const char* k : {"helix_norm_", "helix_norm_bwd_", "helix_norm_dw_part_", "helix_matmul_fp8_",
-                                  "helix_gated_scan_", "helix_gated_scan_bwd_"})
+            for (const char* k : {"helix_norm_", "helix_norm_bwd_", "helix_norm_dw_part_", "helix_matmul_fp8_"})
                 v.push_back(std::string(k) + t);
+        for (const char* t : kTags)
+            for (const char* k : {"helix_gated_scan_", "helix_gated_scan_bwd_"})
+                for (const char* x : {"_v_", "_s_"})
+                    for (const char* w : {"steps", "w4", "w8"}) v.push_back(std::string(k) + t + x + w);
         return v;
     }();
     return names;
@@ -289,6 +296,84 @@ namespace {
 
 constexpr int kScanThreads = 256;
 
+// How the recurrence of a shape is cut (kernels/gated_scan.hip).
+struct ScanPlan {
+    int waves = 0;               // of a workgroup; 0: one thread walks all tokens of four channels
+    int n_slab = 0, n_chunk = 1, n_group = 0;
+    long long streams = 0;
+    size_t part_at = 0, left_at = 0, bytes = 0;   // scratch: the ticket, then these
+};
+
+// run: tokens of a thread's run. As few tokens as one thread walks quickly, and
+// rows so far apart that a wave's reach past 32-bit offsets, go token by token. Four
+// waves where they hold the whole sequence, else eight: over 8192 tokens of 4096
+// channels (bf16) chunks of 4, 8 and 16 waves took 67, 52 and 54 us, backward over 8 x
+// 4096 tokens of 5120 channels 534, 419 and 422.
+ScanPlan scan_plan(long long n_seq, long long n_tok, long long n_chan, int run, bool far) {
+    ScanPlan p;
+    if (n_seq <= 0 || n_tok < 0 || n_chan <= 0) return p;
+    p.n_slab = (int)ceil_div(n_chan, 64);
+    p.streams = n_seq * p.n_slab;
+    if (n_tok <= HELIX_GS_STEPS || far) return p;
+    p.waves = n_tok <= 4LL * run * 4 ? 4 : 8;
+    p.n_chunk = (int)ceil_div(n_tok, 4LL * run * p.waves);
+    p.n_group = (int)ceil_div(p.n_chunk, HELIX_GS_GROUP);
+    if (p.n_chunk > 1) {
+        p.part_at = 256;
+        p.left_at = p.part_at + (size_t)p.streams * p.n_chunk * 64 * 8;
+        p.bytes = p.left_at + (size_t)p.streams * p.n_group * 64 * 4;
+    }
+    return p;
+}
+
+// Whether rows of four channels can be moved together.
+bool quads(const void* p, long long seq, long long tok, long long n_chan, size_t es) {
+    return !(n_chan % 4) && !(seq % 4) && !(tok % 4) && aligned(p, 4 * es);
+}
+
+// Whether a wave's rows (4 runs of 8 tokens at most, and one before them) reach
+// beyond 2^29 bytes.
+bool far_rows(long long tok, size_t es) { return tok >= (1LL << 29) / 33 / (long long)es; }
+
+// Fills in a plan, and runs it: P is HelixGatedScanParams or its backward form.
+template <typename A, typename P>
+void run_scan(helix_ctx* ctx, void* stream, const A& a, P& p, const char* name, int run, bool vec, bool far) {
+    const ScanPlan plan = scan_plan(a.n_seq, a.n_tok, a.n_chan, run, far);
+    need(plan.bytes == 0 || (a.scratch && a.scratch_bytes >= plan.bytes), "scratch smaller than its _scratch_size()",
+         HELIX_ERR_SCRATCH_TOO_SMALL);
+    need(aligned(a.scratch, 16), "scratch is not 16-byte aligned");
+    p.n_seq = a.n_seq;
+    p.n_tok = a.n_tok;
+    p.n_chan = a.n_chan;
+    p.n_slab = plan.n_slab;
+    p.join = HelixGatedScanJoin{};
+    p.join.n_chunk = plan.n_chunk;
+    p.join.n_group = plan.n_group;
+    const std::string base = std::string(name) + kTags[a.io_dtype] + (vec ? "_v" : "_s");
+    const unsigned gx = grid(plan.waves ? plan.streams * plan.n_chunk
+                                        : ceil_div(a.n_seq * ceil_div(a.n_chan, 4), kScanThreads));
+    const hipFunction_t f = kernel(ctx, plan.waves ? base + "_w" + std::to_string(plan.waves) : base + "_steps");
+    if (!plan.bytes) {
+        const OnDevice on(ctx->device);
+        launch(f, stream, gx, 1, plan.waves ? 64 * plan.waves : kScanThreads, p);
+        return;
+    }
+    char* sc = static_cast<char*>(a.scratch);
+    p.join.ticket = reinterpret_cast<unsigned*>(sc);
+    p.join.part = reinterpret_cast<unsigned long long*>(sc + plan.part_at);
+    p.join.left = reinterpret_cast<unsigned*>(sc + plan.left_at);
+    struct {
+        void* p;
+        long long n;
+    } fill{sc, (long long)(plan.bytes / 16)};
+    const hipFunction_t ff = kernel(ctx, "helix_gated_scan_fill");
+    const unsigned gf = grid(ceil_div(fill.n, kScanThreads));
+    const OnDevice on(ctx->device);
+    void* args[] = {&fill.p, &fill.n};
+    launch_args(ff, stream, gf, 1, kScanThreads, args);
+    launch(f, stream, gx, 1, 64 * plan.waves, p);
+}
+
 template <typename A>
 bool scan_shape(const A& a) {
     need(a.n_seq >= 0 && a.n_tok >= 0 && a.n_chan >= 0, "n_seq, n_tok or n_chan is negative",
@@ -307,7 +392,9 @@ void tokens(const char* name, const A& a, const void* p, long long seq, long lon
 
 }  // namespace
 
-extern "C" size_t helix_gated_scan_scratch_size(const helix_gated_scan_args*) { return 0; }
+extern "C" size_t helix_gated_scan_scratch_size(const helix_gated_scan_args* a) {
+    return a ? scan_plan(a->n_seq, a->n_tok, a->n_chan, HELIX_GS_RUN, false).bytes : 0;
+}
 
 extern "C" helix_status helix_gated_scan_encode(helix_ctx* ctx, void* stream, const helix_gated_scan_args* a) {
     return entry(ctx, [&] {
@@ -329,17 +416,18 @@ extern "C" helix_status helix_gated_scan_encode(helix_ctx* ctx, void* stream, co
         p.tok_v = a->tok_v;
         p.seq_h = a->seq_h;
         p.tok_h = a->tok_h;
-        p.n_seq = a->n_seq;
-        p.n_tok = a->n_tok;
-        p.n_chan = a->n_chan;
-        const unsigned gx = grid(ceil_div((long long)a->n_seq * a->n_chan, kScanThreads));
-        const hipFunction_t f = kernel(ctx, std::string("helix_gated_scan_") + kTags[a->io_dtype]);
-        const OnDevice on(ctx->device);
-        launch(f, stream, gx, 1, kScanThreads, p);
+        const size_t es = kBytes[a->io_dtype];
+        const long long D = a->n_chan;
+        const bool vec = quads(a->g, a->seq_g, a->tok_g, D, es) && quads(a->v, a->seq_v, a->tok_v, D, es) && quads(a->h, a->seq_h, a->tok_h, D, es);
+        bool far = false;
+        for (const long long tok : {(long long)a->tok_g, (long long)a->tok_v, (long long)a->tok_h}) far |= far_rows(tok, es);
+        run_scan(ctx, stream, *a, p, "helix_gated_scan_", HELIX_GS_RUN, vec, far);
     });
 }
 
-extern "C" size_t helix_gated_scan_backward_scratch_size(const helix_gated_scan_backward_args*) { return 0; }
+extern "C" size_t helix_gated_scan_backward_scratch_size(const helix_gated_scan_backward_args* a) {
+    return a ? scan_plan(a->n_seq, a->n_tok, a->n_chan, HELIX_GS_RUN_BWD, false).bytes : 0;
+}
 
 extern "C" helix_status helix_gated_scan_backward_encode(helix_ctx* ctx, void* stream,
                                                          const helix_gated_scan_backward_args* a) {
@@ -376,12 +464,11 @@ extern "C" helix_status helix_gated_scan_backward_encode(helix_ctx* ctx, void* s
         p.tok_dg = a->tok_dg;
         p.seq_dv = a->seq_dv;
         p.tok_dv = a->tok_dv;
-        p.n_seq = a->n_seq;
-        p.n_tok = a->n_tok;
-        p.n_chan = a->n_chan;
-        const unsigned gx = grid(ceil_div((long long)a->n_seq * a->n_chan, kScanThreads));
-        const hipFunction_t f = kernel(ctx, std::string("helix_gated_scan_bwd_") + kTags[a->io_dtype]);
-        const OnDevice on(ctx->device);
-        launch(f, stream, gx, 1, kScanThreads, p);
+        const size_t es = kBytes[a->io_dtype];
+        const long long D = a->n_chan;
+        const bool vec = quads(a->dh, a->seq_dh, a->tok_dh, D, es) && quads(a->g, a->seq_g, a->tok_g, D, es) && quads(a->v, a->seq_v, a->tok_v, D, es) && quads(a->h, a->seq_h, a->tok_h, D, es) && quads(a->dg, a->seq_dg, a->tok_dg, D, es) && quads(a->dv, a->seq_dv, a->tok_dv, D, es);
+        bool far = false;
+        for (const long long tok : {(long long)a->tok_dh, (long long)a->tok_g, (long long)a->tok_v, (long long)a->tok_h, (long long)a->tok_dg, (long long)a->tok_dv}) far |= far_rows(tok, es);
+        run_scan(ctx, stream, *a, p, "helix_gated_scan_bwd_", HELIX_GS_RUN_BWD, vec, far);
     });
 }

@@ -149,7 +149,7 @@ typedef struct {
     int64_t      seq_g, tok_g, seq_v, tok_v, seq_h, tok_h;
 } helix_gated_scan_args;
 
-/* From n_seq, n_tok, n_chan and io_dtype; the other fields are not read. */
+/* From n_seq, n_tok and n_chan; the other fields are not read. */
 size_t       helix_gated_scan_scratch_size(const helix_gated_scan_args* args);
 helix_status helix_gated_scan_encode(helix_ctx* ctx, void* stream, const helix_gated_scan_args* args);
 

@@ -112,6 +112,21 @@ def test_strides(gpu):
     check(wide[:, :, 3:100], wide[:, :, 101:198], normal(2, 97, seed=19))
 
 
+def test_rows_far_apart(gpu):
+    # Sequences more than 2^32 bytes apart, and tokens so far apart that a wave's reach past 2^29 bytes.
+    far = torch.empty(2, (1 << 31) + 64, device="cuda", dtype=torch.bfloat16)
+    g, v = (far[:, k * 4096:k * 4096 + 40 * 64].unflatten(1, (40, 64)) for k in (0, 1))
+    g.copy_(2 + normal(2, 40, 64, seed=70))
+    v.copy_(normal(2, 40, 64, seed=71))
+    check(g, v, normal(2, 64, seed=72))
+    del far, g, v
+    far = torch.empty(20, 9_000_000, device="cuda", dtype=torch.bfloat16)
+    g, v = (far[None, :, k * 4096:k * 4096 + 72] for k in (0, 1))
+    g.copy_(2 + normal(1, 20, 72, seed=73))
+    v.copy_(normal(1, 20, 72, seed=74))
+    check(g, v, normal(1, 72, seed=75))
+
+
 def test_parts_join_as_one(gpu):
     # A sequence in two calls, the state carried: the same values as in one, up to the roundings of the joins.
     g, v, h0 = problem(2, 1200, 64, seed=20)

@@ -73,6 +73,26 @@ def test_leading_dimensions_strides_and_out(gpu):
     assert lead.shape == (7, 10, n) and torch.equal(lead.view(m, n), want)
 
 
+@pytest.mark.parametrize("m", [3, 200])
+def test_rows_far_apart(gpu, m):
+    # Rows of both operands, their scales and the result reach past 2^32 bytes.
+    k, n = 300, 70
+    a, sa, b, sb = operands(m, n, k, seed=6)
+
+    def spread(t, rows):
+        ld = (1 << 33) // rows // 256 * 256
+        far = torch.empty(rows, ld // t.element_size(), device="cuda", dtype=torch.uint8 if t.element_size() == 1 else t.dtype)
+        view = far.view(t.dtype)[:, :t.shape[1]]
+        view.copy_(t)
+        return view
+
+    want = matmul_fp8(a, sa, b, sb)
+    out = spread(want, m)
+    out.zero_()
+    got = matmul_fp8(spread(a, m), spread(sa, m), spread(b, n), spread(sb, n), out=out)
+    assert torch.equal(got, want)
+
+
 def test_every_code_and_wide_scales(gpu):
     # All finite codes, in every place of a block, against ones; scales up to the range's ends.
     codes = torch.arange(256, dtype=torch.uint8, device="cuda")

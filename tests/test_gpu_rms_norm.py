@@ -61,6 +61,16 @@ def test_norm_strided_and_unaligned(gpu, dim, dtype):
     check_norm(lead, w, lead.flip(0))
 
 
+def test_rows_far_apart(gpu):
+    far = torch.empty(3, (1 << 30) + (1 << 29) + 8, device="cuda", dtype=torch.bfloat16)
+    x = far[:, :1000]
+    x.copy_(normal(3, 1000, seed=80))
+    w = 1 + 0.1 * normal(1000, seed=81)
+    check_norm(x, w, x)
+    _, _, rstd = rms_norm(x, w)
+    check_backward(x, x, w, rstd, x)
+
+
 def test_norm_values(gpu):
     # A zero row, a row of subnormal squares, large values, one lone value, the sum cancelling to zero.
     x = normal(6, 300, seed=9)
