@@ -31,7 +31,7 @@ HOST_SYMBOLS = ("helix_ctx_create_host", "helix_scan_plan_info", "helix_scan_run
                 "helix_scan_encode_noalloc")
 # include/helix/helix_layer.h
 LAYER_SYMBOLS = ("helix_norm_encode", "helix_quantize_fp8_encode", "helix_norm_backward_scratch_size",
-                 "helix_norm_backward_encode", "helix_matmul_fp8_encode", "helix_gated_scan_scratch_size",
+                 "helix_norm_backward_encode", "helix_matmul_fp8_scratch_size", "helix_matmul_fp8_encode", "helix_gated_scan_scratch_size",
                  "helix_gated_scan_encode", "helix_gated_scan_backward_scratch_size",
                  "helix_gated_scan_backward_encode")
 # include/helix/helix_host.h HELIX_PASS_B_*: where Pass B's segment scan runs
@@ -90,7 +90,7 @@ ARGS_STRUCT = struct.Struct("=11Q")
 # The argument structs of include/helix/helix_layer.h, field by field.
 NORM_STRUCT = struct.Struct("=q3if8Q6q")
 NORM_BACKWARD_STRUCT = struct.Struct("=q4i9Q4q")
-MATMUL_FP8_STRUCT = struct.Struct("=4i5Q5q")
+MATMUL_FP8_STRUCT = struct.Struct("=4i7Q5q")
 GATED_SCAN_STRUCT = struct.Struct("=4i7Q6q")
 GATED_SCAN_BACKWARD_STRUCT = struct.Struct("=4i11Q12q")
 assert DESC_STRUCT.size == ctypes.sizeof(HelixScanDesc)

@@ -50,6 +50,12 @@ typedef struct {
     void*          c;
     long long      ld_a, ld_a_scale, ld_b, ld_b_scale, ld_c;
     int            m, n, k;
+    int            wide;    /* rows of c are 16-byte aligned (16-bit types)    */
+    /* Tiled kernel: bands of gm rows of tiles, band = gm x columns of tiles, and
+     * 2^32 / d + 1 of band, gm and the last band's rows. */
+    int            gm;
+    unsigned       band, inv_band, inv_gm, inv_rest;
+    int            stride;  /* workgroups: tiles from one to a workgroup's next  */
 } HelixMatmulParams;
 
 /* Gated recurrence: tokens of a thread's run, forward and backward, chunks of a

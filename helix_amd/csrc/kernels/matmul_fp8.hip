@@ -73,7 +73,8 @@ HELIX_DEV f32x4 block_sum(i32x8 a, i32x8 b) {
     return s;
 }
 
-// One wave per 16 x 16 tile of c, operands straight from memory.
+// One wave per 16 x 16 tile of c, operands straight from memory: for the shapes that
+// nothing else takes.
 template <typename T>
 __device__ void matmul_tile(const HelixMatmulParams& p) {
     const int lane = lane_id(), lo = lane & 15, kq = lane >> 4;
@@ -104,10 +105,448 @@ __device__ void matmul_tile(const HelixMatmulParams& p) {
     }
 }
 
+// ---- few rows of a ------------------------------------------------------------
+//
+// A workgroup per 16 rows of b, its W waves each a stretch of the sum and all of up to
+// 16 MT rows of a; they meet in LDS, in the order of the waves. b is read once, straight
+// into registers, which is what bounds it; a comes from the caches.
+template <typename T, int MT, int W>
+__device__ void matmul_rows(const HelixMatmulParams& p) {
+    __shared__ float sum[W][MT * 16][17];
+    const int lane = lane_id(), wave = wave_uniform(), lo = lane & 15, kq = lane >> 4;
+    const int j0 = blockIdx.x * 16, i0 = blockIdx.y * 16 * MT;
+    const int nkb = (p.k + 127) >> 7, each = (nkb + W - 1) / W;
+    const int first = wave * each, last = min(first + each, nkb);
+    const long long rb = min(j0 + lo, p.n - 1);
+    const uint8_t* b = p.b + rb * p.ld_b;
+    const uint8_t* eb = p.b_scale + rb * p.ld_b_scale;
+    const uint8_t *a[MT], *ea[MT];
+#pragma unroll
+    for (int t = 0; t < MT; ++t) {
+        const long long ra = min(i0 + 16 * t + lo, p.m - 1);
+        a[t] = p.a + ra * p.ld_a;
+        ea[t] = p.a_scale + ra * p.ld_a_scale;
+    }
+    f32x4 acc[MT];
+#pragma unroll
+    for (int t = 0; t < MT; ++t) acc[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int kb = first; kb < last; ++kb) {
+        const i32x8 x = row_block(b, kb, kq, p.k);
+        const int ex = eb[kb];
+#pragma unroll
+        for (int t = 0; t < MT; ++t) {
+            const i32x8 y = row_block(a[t], kb, kq, p.k);
+            if constexpr (sizeof(T) == 4) {
+                const f32x4 s = block_sum(x, y);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const long long row = min(j0 + 4 * kq + r, p.n - 1);
+                    acc[t][r] += scaled(s[r], p.b_scale[row * p.ld_b_scale + kb], ea[t][kb]);
+                }
+            } else {
+                acc[t] = mfma_fp8(x, y, acc[t], ex, ea[t][kb]);
+            }
+        }
+    }
+    // Register r of a lane: row 4 kq + r of b, row lo of a's tile.
+#pragma unroll
+    for (int t = 0; t < MT; ++t)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) sum[wave][16 * t + lo][4 * kq + r] = acc[t][r];
+    __syncthreads();
+    for (int e = threadIdx.x; e < MT * 256; e += 64 * W) {
+        const int i = e >> 4, j = e & 15;
+        float s = 0.0f;
+#pragma unroll
+        for (int w = 0; w < W; ++w) s += sum[w][i][j];
+        if (i0 + i < p.m && j0 + j < p.n) static_cast<T*>(p.c)[(i0 + i) * p.ld_c + j0 + j] = (T)s;
+    }
+}
+
+// ---- large products ----------------------------------------------------------
+//
+// A workgroup of four waves takes tiles of 32 TM columns (rows of b, X) by 32 TN
+// rows (of a, Y) of c, a wave a quarter: 16 TM by 16 TN. Its accumulators fill up to
+// 256 accumulation registers, so each SIMD holds one wave, and nothing but the
+// wave's own order hides anything. What the order has to respect:
+//
+//  - A scaled product takes 32 cycles. Whatever else is issued between two of them
+//    costs nothing while it takes less, so that reads of LDS, loads and scalar work
+//    are dealt out singly between products (`repeat` over their places). Branches
+//    and waits for scalars are kept out of the steps: with them 8192 x 8192 x 8192
+//    took 431 us, as here 392.
+//  - Products are volatile assembly: the compiler keeps their order and that of the
+//    reads, and accumulates in place. Loads into LDS are, too (the compiler would
+//    wait for all of them before any read of LDS); their waits are counted by hand.
+//  - LDS holds two steps (128 along the sum each). The fragments of a step are read
+//    in two halves: X and the first half of Y while the step before multiplies its
+//    second half, the second half of Y while this one multiplies its first. So X and
+//    half of Y are free again when a step begins, the rest at its middle, and loads go
+//    one and a half steps ahead: WINDOW of a wave's later loads may be under way at
+//    either of a step's two barriers.
+//  - Tiles follow each other without a pause: the loads of the next tile's first steps
+//    go out during the last steps of this one, and its first waits count this one's
+//    stores (vmcnt counts both, in order) instead of waiting for them.
+//
+// A row's eight 16-byte chunks lie exchanged in LDS (chunk c at c ^ its row's number),
+// so that the eight rows that are read together lie in different banks; the loads
+// write them there by reading the row's chunks in that order.
+//
+// The power limit binds it: 8192 x 8192 x 8192 take 392 us (2.81 PFLOP/s) at 2.0 GHz,
+// two thirds of the products' own rate at that clock. Smaller tiles: 192 rows 440 us,
+// 128 rows 496, 128 x 128 in two workgroups per CU 573. Products of 32 x 32 x 64 run at
+// 3.5 PFLOP/s where those of 16 x 16 x 128 run at 4.1, and took 526 us in this loop's
+// first form, against 457.
+
+struct TileAt {
+    int i, j;
+};
+
+HELIX_DEV void mm_first(i32x8 a, i32x8 b, f32x4& c, int ea, int eb) {
+    asm volatile("v_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, 0, %3, %4 op_sel_hi:[0,0,0]"
+                 : "=a"(c) : "v"(a), "v"(b), "v"(ea), "v"(eb));
+}
+HELIX_DEV void mm_next(i32x8 a, i32x8 b, f32x4& c, int ea, int eb) {
+    asm volatile("v_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel_hi:[0,0,0]"
+                 : "+a"(c) : "v"(a), "v"(b), "v"(ea), "v"(eb));
+}
+
+// Sixteen wait states before anything reads these: twice the products' latency, for
+// what nothing else would wait for.
+HELIX_DEV void mm_settle(f32x4& a, f32x4& b) { asm volatile("s_nop 15" : "+a"(a), "+a"(b)); }
+
+// A wave's 64 x 16 or 64 x 4 bytes from a resource into LDS at `lds` + ADD. The
+// compiler does not see a memory instruction here: scalars that vector instructions
+// write need five wait states before it reads them, which rarely happens (spilled
+// scalars) and which tests/test_layer_host.py looks for in the built code.
+template <int ADD>
+HELIX_DEV void load_lds16(i32x4 r, int voff, int soff, unsigned lds) {
+    asm volatile("s_add_u32 m0, %3, %4\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, %2 offen lds"
+                 ::"v"(voff), "s"(r), "s"(soff), "s"(lds), "n"(ADD) : "memory", "scc");
+}
+HELIX_DEV void load_lds4(i32x4 r, int voff, int soff, unsigned lds) {
+    asm volatile("s_mov_b32 m0, %3\n\ts_nop 4\n\tbuffer_load_dword %0, %1, %2 offen lds"
+                 ::"v"(voff), "s"(r), "s"(soff), "s"(lds) : "memory");
+}
+HELIX_DEV i32x4 lds_rsrc(const uint8_t* base, long long bytes) {
+    const unsigned long long u = (unsigned long long)base;
+    return i32x4{__builtin_amdgcn_readfirstlane((int)u), __builtin_amdgcn_readfirstlane((int)(u >> 32)),
+                 __builtin_amdgcn_readfirstlane((int)min(bytes, 0xfffffff0LL)), 0x00020000};
+}
+
+template <int N> using num = std::integral_constant<int, N>;
+template <int N, typename F>
+HELIX_DEV void repeat(F&& f) {
+    if constexpr (N > 0) {
+        repeat<N - 1>(f);
+        f(num<N - 1>{});
+    }
+}
+
+template <typename T, int TM, int TN>
+__device__ void matmul_tiles(const HelixMatmulParams& p) {
+    constexpr int BN = 32 * TM, BM = 32 * TN, ROWS = BN + BM, STAGE = ROWS * 128, SLOT = ROWS * 4;
+    constexpr int NX = BN / 32, NY = BM / 32;      // loads of a wave in a stage: 8 rows each
+    constexpr int WINDOW = NX + NY;                // loads issued after the ones that a barrier waits for
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[2 * STAGE + 4 * SLOT];
+    const int lane = lane_id(), wave = wave_uniform();
+    const int mt = (p.m + BM - 1) / BM, nt = (p.n + BN - 1) / BN, tiles = mt * nt;
+    const int nkb = (p.k + 127) >> 7, ngr = (nkb + 3) >> 2;
+    // Tiles go down columns of GM tiles, a column beside the other, band by band: what runs on an XCD at a time shares rows of
+    // both matrices. Divisions by products with reciprocals of the host's (mulhi of x with 2^32 / d + 1).
+    auto tile_at = [&](int t) {
+        const unsigned per = tiles >> 3, id = (unsigned)t < 8 * per ? (t & 7) * per + (t >> 3) : t;
+        const unsigned g = p.band == 1 ? id : __umulhi(id, p.inv_band), r = id - g * p.band;
+        const int rows = min(p.gm, mt - (int)g * p.gm);
+        const unsigned c = rows == 1 ? r : __umulhi(r, rows == p.gm ? p.inv_gm : p.inv_rest);
+        return TileAt{__builtin_amdgcn_readfirstlane(((int)g * p.gm + (int)(r - c * rows)) * BM), __builtin_amdgcn_readfirstlane((int)c * BN)};
+    };
+    // X: rows of b, the instruction's first operand; Y: rows of a.
+    const int wx = (wave >> 1) * 16 * TM, wy = (wave & 1) * 16 * TN;
+    const unsigned lds0 = (unsigned)(unsigned long long)(__attribute__((address_space(3))) uint8_t*)lds;
+
+    // ---- loads: data two steps ahead, scales two groups of four steps ahead
+    // row of the tile that load i of the wave starts at
+    auto xrow = [&](int i) { return 8 * (wave * NX + i); };
+    auto yrow = [&](int i) {
+        const int h = i / (NY / 2), u = wave * (NY / 2) + i % (NY / 2);   // half h: rows 8 u of the waves' tiles j in it
+        return (u / TN) * 16 * TN + h * 8 * TN + (u % TN) * 8;
+    };
+    i32x4 rx, ry, rsx, rsy;
+    int vx[NX], vy[NY], vsx, vsy;
+    const int stride = p.stride;
+    int pkb = 0, qt = blockIdx.x, qg = 0;   // where the data's and the scales' loads are
+    // Rows and columns past the matrices are out of the resources' range and come as zeros.
+    auto aim_data = [&](int t) {
+        const TileAt at = tile_at(t);
+        const int k16 = (p.k + 15) & ~15;
+        rx = lds_rsrc(p.b + at.j * p.ld_b, (min(BN, p.n - at.j) - 1) * p.ld_b + k16);
+        ry = lds_rsrc(p.a + at.i * p.ld_a, (min(BM, p.m - at.i) - 1) * p.ld_a + k16);
+    };
+    auto aim_scales = [&](int t) {
+        const TileAt at = tile_at(t);
+        rsx = lds_rsrc(p.b_scale + at.j * p.ld_b_scale, (min(BN, p.n - at.j) - 1) * p.ld_b_scale + 4 * ngr);
+        rsy = lds_rsrc(p.a_scale + at.i * p.ld_a_scale, (min(BM, p.m - at.i) - 1) * p.ld_a_scale + 4 * ngr);
+    };
+    // a row's 16-byte chunk c is kept at c ^ (what its row's number says)
+#pragma unroll
+    for (int i = 0; i < NX; ++i) {
+        const int r = xrow(i) + (lane >> 3), s = (r & 3) | ((r >> 1) & 4);
+        vx[i] = r * (int)p.ld_b + (((lane & 7) ^ s) << 4);
+    }
+#pragma unroll
+    for (int i = 0; i < NY; ++i) vy[i] = (yrow(i) + (lane >> 3)) * (int)p.ld_a + (((lane & 7) ^ (lane >> 3)) << 4);
+    vsx = (64 * wave + lane) * (int)p.ld_b_scale;
+    vsy = (64 * wave + lane) * (int)p.ld_a_scale;
+    // where the wave's loads go: X's, and those of both halves of Y's, a kilobyte apart
+    const unsigned to_x = lds0 + xrow(0) * 128, to_y0 = lds0 + BN * 128 + yrow(0) * 128, to_y1 = lds0 + BN * 128 + yrow(NY / 2) * 128;
+    auto load = [&](auto which, unsigned into) {
+        constexpr int E = decltype(which)::value;
+        if constexpr (E < NX) load_lds16<E * 1024>(rx, vx[E], pkb * 128, to_x + into);
+        else if constexpr (E < NX + NY / 2) load_lds16<(E - NX) * 1024>(ry, vy[E - NX], pkb * 128, to_y0 + into);
+        else load_lds16<(E - NX - NY / 2) * 1024>(ry, vy[E - NX], pkb * 128, to_y1 + into);
+    };
+    auto load_scales = [&](int slot) {
+        if (64 * wave < BN) load_lds4(rsx, vsx, 4 * qg, lds0 + 2 * STAGE + slot * SLOT + 256 * wave);
+        if (64 * wave < BM) load_lds4(rsy, vsy, 4 * qg, lds0 + 2 * STAGE + slot * SLOT + 4 * BN + 256 * wave);
+    };
+    // Past the last tile the loads repeat it, into buffers that are not read any more.
+    auto next_tile = [&](int t) { return t + stride < tiles ? t + stride : t; };
+    auto next_scales = [&] {
+        if (++qg == ngr) {
+            qg = 0;
+            qt = next_tile(qt);
+            aim_scales(qt);
+        }
+    };
+
+    // ---- fragments
+    const int fr = lane & 15, fq = lane >> 4;
+    // Row fr of X's tile i is n = 32 (i / 2) + 8 (fr / 4) + 4 (i % 2) + fr % 4: a lane's results of tiles i and i + 1 are eight neighbours.
+    const int xr = 8 * (fr >> 2) + (fr & 3), xs = (fr & 3) | (fr & 4);
+    const uint8_t* fx = lds + (wx + xr) * 128 + ((fq ^ xs) << 4);
+    const uint8_t* fy = lds + BN * 128 + (wy + fr) * 128 + ((fq ^ (fr & 7)) << 4);
+    const int flip_x = ((fq ^ xs) & 4) ? -64 : 64, flip_y = ((fq ^ (fr & 7)) & 4) ? -64 : 64;
+    auto frag = [&](const uint8_t* q, int flip) {
+        const i32x4 lo = *reinterpret_cast<const i32x4*>(q), hi = *reinterpret_cast<const i32x4*>(q + flip);
+        return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+    };
+    auto frag_x = [&](int buf, int i) { return frag(fx + buf * STAGE + (i >> 1) * 4096 + (i & 1) * 512, flip_x); };
+    auto frag_y = [&](int buf, int j) { return frag(fy + buf * STAGE + j * 2048, flip_y); };
+    auto at_x = [&](int buf, int i) { return fx + buf * STAGE + (i >> 1) * 4096 + (i & 1) * 512; };
+    auto at_y = [&](int buf, int j) { return fy + buf * STAGE + j * 2048; };
+    auto lo = [&](i32x8& w, const uint8_t* q) { w = __builtin_shufflevector(__builtin_shufflevector(*reinterpret_cast<const i32x4*>(q), i32x4{}, 0, 1, 2, 3, 0, 1, 2, 3), w, 0, 1, 2, 3, 12, 13, 14, 15); };
+    auto hi = [&](i32x8& w, const uint8_t* q) { w = __builtin_shufflevector(__builtin_shufflevector(*reinterpret_cast<const i32x4*>(q), i32x4{}, 0, 1, 2, 3, 0, 1, 2, 3), w, 8, 9, 10, 11, 0, 1, 2, 3); };
+    const uint8_t* fsx = lds + 2 * STAGE + (wx + xr) * 4;
+    const uint8_t* fsy = lds + 2 * STAGE + 4 * BN + (wy + fr) * 4;
+    auto scale_x = [&](int slot, int i) { return *reinterpret_cast<const int*>(fsx + slot * SLOT + (i >> 1) * 128 + (i & 1) * 16); };
+    auto scale_y = [&](int slot, int j) { return *reinterpret_cast<const int*>(fsy + slot * SLOT + j * 64); };
+
+    i32x8 X[TM], Y[TN];
+    int ex[TM], ey[TN];
+    f32x4 acc[TM][TN];
+
+    // prologue: two steps, two groups
+    aim_data(blockIdx.x);
+    aim_scales(qt);
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+        load_scales(s);
+        next_scales();
+        repeat<NX + NY>([&](auto e) { load(e, s * STAGE); });
+        ++pkb;
+    }
+    asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(WINDOW) : "memory");
+#pragma unroll
+    for (int i = 0; i < TM; ++i) { X[i] = frag_x(0, i); ex[i] = scale_x(0, i); }
+#pragma unroll
+    for (int j = 0; j < TN / 2; ++j) { Y[j] = frag_y(0, j); ey[j] = scale_y(0, j); }
+
+    int buf = 0, slot = 0;   // of the step at hand
+    // A last block that k ends in: clears what a lane's 32 bytes (16 fq on, and 64 + 16 fq on) hold past it.
+    const int kt = p.k & 127;
+    auto cut = [&](i32x8& w) {
+#pragma unroll
+        for (int d = 0; d < 8; ++d) {
+            const int keep = kt - (64 * (d >> 2) + 16 * fq + 4 * (d & 3));   // bytes of this word
+            w[d] &= keep >= 4 ? -1 : keep <= 0 ? 0 : (1 << (8 * keep)) - 1;
+        }
+    };
+    // The waits of a tile's first step, and the first one of its second, count the stores of the tile before.
+    constexpr int STORES = TM / 2 * TN < 63 - WINDOW ? TM / 2 * TN : 63 - WINDOW;
+    // One step: STORED_S and STORED_M, whether its waits have the stores of the tile before among what may be under way; Q, its place
+    // in a group of four (-1: any, `q`); TURN, whether a group ends with it (-1: where q is 3); CUT, whether k may end in it.
+    auto step = [&](auto first, auto stored_s, auto stored_m, auto place, auto turns, auto cuts, int q) {
+        constexpr bool FIRST = decltype(first)::value, CUT = decltype(cuts)::value;
+        constexpr int Q = decltype(place)::value, TURN = decltype(turns)::value;
+        constexpr int WS = WINDOW + (decltype(stored_s)::value ? STORES : 0), WM = WINDOW + (decltype(stored_m)::value ? STORES : 0);
+        if constexpr (Q >= 0) q = Q;
+        const bool turn = TURN >= 0 ? TURN == 1 : q == 3;
+        const int sh = 8 * q, other = buf ^ 1, sn = turn ? (slot + 1) & 3 : slot;
+        constexpr int H = TM * TN / 2, LEAD = TN / 2;   // products of a half; those before its barrier
+        constexpr int L1 = NX + NY / 2, L2 = NY / 2;    // loads of a half
+        const unsigned into = buf * STAGE;
+        if (CUT && kt) {
+#pragma unroll
+            for (int i = 0; i < TM; ++i) cut(X[i]);
+#pragma unroll
+            for (int j = 0; j < TN / 2; ++j) cut(Y[j]);
+        }
+#pragma unroll
+        for (int i = 0; i < TM; ++i) ex[i] = vgpr_fresh((unsigned)ex[i] >> sh);
+#pragma unroll
+        for (int j = 0; j < TN / 2; ++j) ey[j] = vgpr_fresh((unsigned)ey[j] >> sh);
+        asm volatile("s_nop 1");
+        auto product = [&](int i, int j) {
+            if constexpr (FIRST) mm_first(X[i], Y[j], acc[i][j], ex[i], ey[j]);
+            else mm_next(X[i], Y[j], acc[i][j], ex[i], ey[j]);
+        };
+        repeat<H>([&](auto slot_) {
+            constexpr int t = decltype(slot_)::value;
+            product(t / (TN / 2), t % (TN / 2));
+            if constexpr (t == LEAD - 1) {
+                // The first halves of this step's stage have been read by every wave, and its second half has landed.
+                asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(WS) : "memory");
+                if (Q == 0 || (Q < 0 && q == 0)) {
+                    load_scales((slot + 2) & 3);
+                    next_scales();
+                }
+            }
+            constexpr int u = t - LEAD, U = H - LEAD;   // places after the barrier
+            if constexpr (u >= 0) {
+                repeat<TN / 2>([&](auto y) {
+                    constexpr int j = TN / 2 + y;
+                    if constexpr (u == 2 * (2 * y) * (U / 2) / TN) lo(Y[j], at_y(buf, j));
+                    if constexpr (u == 2 * (2 * y + 1) * (U / 2) / TN) hi(Y[j], at_y(buf, j) + flip_y);
+                    if constexpr (u == 2 * (2 * y + 1) * (U / 2) / TN && (y % 2 == 1 || y == TN / 2 - 1)) { if constexpr (y % 2 == 1) ey[j - 1] = scale_y(slot, j - 1); ey[j] = scale_y(slot, j); }
+                });
+                repeat<L1>([&](auto l) {
+                    if constexpr (u == l * U / L1 + (U >= 2 * L1 ? 1 : 0)) load(l, into);
+                });
+            }
+        });
+        if (CUT && kt) {
+#pragma unroll
+            for (int j = TN / 2; j < TN; ++j) cut(Y[j]);
+        }
+#pragma unroll
+        for (int j = TN / 2; j < TN; ++j) ey[j] = vgpr_fresh((unsigned)ey[j] >> sh);
+        asm volatile("s_nop 1");
+        repeat<H>([&](auto slot_) {
+            constexpr int t = decltype(slot_)::value, W = TN / 2, i = t / W;
+            product(i, W + t % W);
+            if constexpr (t == LEAD - 1) {
+                // The second half has been read, and the next stage's first halves have landed.
+                asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(WM) : "memory");
+            }
+            // X of the row before, from the next stage
+            if constexpr (t >= W && t % W == 0) lo(X[i - 1], at_x(other, i - 1));
+            if constexpr (t >= W && t % W == (W > 1 ? 1 : 0)) hi(X[i - 1], at_x(other, i - 1) + flip_x);
+            if constexpr (t >= W && t % W == W - 1 && i % 2 == 0) { ex[i - 2] = scale_x(sn, i - 2); ex[i - 1] = scale_x(sn, i - 1); }
+            constexpr int u = t - LEAD, U = H - LEAD, SPAN = U > 4 ? U - 4 : 0, FROM = U > 4 ? 3 : U - 1;
+            if constexpr (u >= 0) {
+                repeat<TN / 2>([&](auto y) {
+                    if constexpr (u == 2 + (2 * y) * SPAN / TN) lo(Y[y], at_y(other, y));
+                    if constexpr (u == 2 + (2 * y + 1) * SPAN / TN) hi(Y[y], at_y(other, y) + flip_y);
+                    if constexpr (u == 2 + (2 * y + 1) * SPAN / TN && (y % 2 == 1 || y == TN / 2 - 1)) { if constexpr (y % 2 == 1) ey[y - 1] = scale_y(sn, y - 1); ey[y] = scale_y(sn, y); }
+                });
+                repeat<L2>([&](auto l) {
+                    if constexpr (u == FROM + l * SPAN / L2) load(num<L1 + l>{}, into);
+                });
+            }
+        });
+        lo(X[TM - 1], at_x(other, TM - 1));
+        hi(X[TM - 1], at_x(other, TM - 1) + flip_x);
+        ex[TM - 2] = scale_x(sn, TM - 2);
+        ex[TM - 1] = scale_x(sn, TM - 1);
+        ++pkb;
+        buf = other;
+        slot = sn;
+    };
+    for (int t = blockIdx.x; t < tiles; t += stride) {
+        // nkb is 4 at least. Two steps before the end the loads go over to the next tile.
+        constexpr std::true_type yes{};
+        constexpr std::false_type no{};
+        step(yes, yes, yes, num<0>{}, num<0>{}, no, 0);
+        step(no, yes, no, num<1>{}, num<0>{}, no, 1);
+        int kb = 2;
+#pragma clang loop unroll(disable)
+        for (; kb + 4 <= nkb - 2; kb += 4) {
+            step(no, no, no, num<2>{}, num<0>{}, no, 2);
+            step(no, no, no, num<3>{}, num<1>{}, no, 3);
+            step(no, no, no, num<0>{}, num<0>{}, no, 0);
+            step(no, no, no, num<1>{}, num<0>{}, no, 1);
+        }
+#pragma clang loop unroll(disable)
+        for (; kb < nkb - 2; ++kb) step(no, no, no, num<-1>{}, num<-1>{}, no, kb & 3);
+        aim_data(next_tile(t));
+        pkb = 0;
+        step(no, no, no, num<-1>{}, num<-1>{}, no, kb & 3);
+        step(no, no, no, num<-1>{}, num<1>{}, yes, (kb + 1) & 3);
+        // The last products' results are there before anything reads them.
+#pragma unroll
+        for (int j = TN / 2; j < TN; ++j) mm_settle(acc[TM - 2][j], acc[TM - 1][j]);
+        // Every store is issued, whatever its lanes may write: the waits of the next steps count them.
+        const TileAt at = tile_at(t);
+        const int left_n = p.n - at.j, left_m = p.m - at.i;
+        const helix_rsrc rc = make_rsrc_u(static_cast<T*>(p.c) + at.i * p.ld_c + at.j, (unsigned)(((min(left_m, BM) - 1) * p.ld_c + min(left_n, BN)) * 2));
+        const int ldc = (int)p.ld_c * 2;
+#pragma unroll
+        for (int j = 0; j < TN; ++j) {
+            const int row = (wy + 16 * j + vgpr_fresh(fr)) * ldc;
+#pragma unroll
+            for (int i = 0; i < TM; i += 2) {
+                const int col = wx + 16 * i + 8 * vgpr_fresh(fq);
+                const f32x4 u = acc[i][j], v = acc[i + 1][j];
+                const u32x4 w = {narrow2<T>(u[0], u[1]), narrow2<T>(u[2], u[3]), narrow2<T>(v[0], v[1]), narrow2<T>(v[2], v[3])};
+                if (p.wide) {
+                    __builtin_amdgcn_raw_buffer_store_b128(w, rc, col < left_n ? row + 2 * col : (int)0x80000000, 0, 0);
+                } else {
+#pragma unroll
+                    for (int r = 0; r < 8; ++r)
+                        __builtin_amdgcn_raw_buffer_store_b16((unsigned short)(w[r >> 1] >> (16 * (r & 1))), rc, col + r < left_n ? row + 2 * (col + r) : (int)0x80000000, 0, 0);
+                }
+            }
+        }
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+}
 }  // namespace
 
-#define MATMUL_KERNELS(TAG, T) \
-    extern "C" __global__ __launch_bounds__(64) void helix_matmul_fp8_##TAG(HelixMatmulParams p) { matmul_tile<T>(p); }
+// Scales into rows of `pitch` bytes, a multiple of four, for the tiles' loads.
+extern "C" __global__ __launch_bounds__(256) void helix_fp8_scales(const uint8_t* from, uint8_t* to, long long ld,
+                                                                   long long rows, int blocks, int pitch) {
+    const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+    const long long row = i / pitch;
+    const int c = (int)(i % pitch);
+    if (row < rows) to[i] = c < blocks ? from[row * ld + c] : 0;
+}
+
+#define MATMUL_TILES(TAG, T, TM, TN, BOUND)                                                                  \
+    extern "C" __global__ __launch_bounds__(256, BOUND) void helix_matmul_fp8_##TAG##_t##TM##TN(HelixMatmulParams p) { \
+        matmul_tiles<T, TM, TN>(p);                                                                          \
+    }
+#define MATMUL_TILED(TAG, T)         \
+    MATMUL_TILES(TAG, T, 8, 8, 1)    \
+    MATMUL_TILES(TAG, T, 8, 6, 1)    \
+    MATMUL_TILES(TAG, T, 8, 4, 1)    \
+    MATMUL_TILES(TAG, T, 4, 4, 2)    \
+    MATMUL_TILES(TAG, T, 4, 2, 2)
+MATMUL_TILED(f16, _Float16)
+MATMUL_TILED(bf16, __bf16)
+
+#define MATMUL_ROWS(TAG, T, MT)                                                                              \
+    extern "C" __global__ __launch_bounds__(512) void helix_matmul_fp8_##TAG##_r##MT(HelixMatmulParams p) {  \
+        matmul_rows<T, MT, 8>(p);                                                                            \
+    }
+#define MATMUL_KERNELS(TAG, T)                                                                               \
+    MATMUL_ROWS(TAG, T, 1)                                                                                   \
+    MATMUL_ROWS(TAG, T, 2)                                                                                   \
+    MATMUL_ROWS(TAG, T, 4)                                                                                   \
+    MATMUL_ROWS(TAG, T, 8)                                                                                   \
+    extern "C" __global__ __launch_bounds__(64) void helix_matmul_fp8_##TAG##_any(HelixMatmulParams p) {     \
+        matmul_tile<T>(p);                                                                                   \
+    }
 MATMUL_KERNELS(f32, float)
 MATMUL_KERNELS(f16, _Float16)
 MATMUL_KERNELS(bf16, __bf16)

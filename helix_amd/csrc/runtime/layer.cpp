@@ -171,10 +171,13 @@ namespace helix::rt {
 
 const std::vector<std::string>& layer_kernel_names() {
     static const std::vector<std::string> names = [] {
-        std::vector<std::string> v{"helix_norm_dw", "helix_gated_scan_fill"};
+        std::vector<std::string> v{"helix_norm_dw", "helix_fp8_scales", "helix_gated_scan_fill"};
         for (const char* t : kTags)
-            for (const char* k : {"helix_norm_", "helix_norm_bwd_", "helix_norm_dw_part_", "helix_matmul_fp8_"})
+            for (const char* k : {"helix_norm_", "helix_norm_bwd_", "helix_norm_dw_part_"})
                 v.push_back(std::string(k) + t);
+        for (const char* tag : kTags)
+            for (const char* k : {"_any", "_r1", "_r2", "_r4", "_r8", "_t88", "_t86", "_t84", "_t44", "_t42"})
+                if (tag != kTags[HELIX_F32] || k[1] != 't') v.push_back(std::string("helix_matmul_fp8_") + tag + k);
         for (const char* t : kTags)
             for (const char* k : {"helix_gated_scan_", "helix_gated_scan_bwd_"})
                 for (const char* x : {"_v_", "_s_"})
@@ -256,6 +259,72 @@ extern "C" helix_status helix_norm_backward_encode(helix_ctx* ctx, void* stream,
     });
 }
 
+namespace {
+
+// How a product is computed (kernels/matmul_fp8.hip).
+struct MatmulPlan {
+    const char* kernel = "_any";
+    int rows = 0;                            // > 0: rows of a that a workgroup takes at once
+    int bm = 0, bn = 0, per_cu = 1;          // > 0: tiles
+    size_t pitch = 0, a_bytes = 0, b_bytes = 0;   // copies of the scales, in scratch
+};
+
+struct Tiling {
+    const char* kernel;
+    int bm, bn, per_cu;
+    double step, tile;   // us of a step of 128 and of the rest of a tile, with every CU at work
+};
+// Fitted to 8192 x 8192 x 8192, 8192 x 10304 x 2048 and 32768 x 2560 x 5120: the large tiles take 20e-6 us per element
+// and step, the small ones up to 33e-6, but waste less of a last round.
+const Tiling kTilings[] = {
+    {"_t88", 256, 256, 1, 1.38, 6.4}, {"_t86", 192, 256, 1, 1.04, 6.4}, {"_t84", 128, 256, 1, 0.93, 2.2},
+    {"_t44", 128, 128, 2, 1.10, 1.5}, {"_t42", 64, 128, 2, 0.75, 1.2},
+};
+
+MatmulPlan matmul_plan(const helix_matmul_fp8_args& a) {
+    MatmulPlan p;
+    const long long blocks = ceil_div(a.k, HELIX_FP8_BLOCK);
+    // Few rows: b's bytes are what counts, and every wave reads all of a.
+    if (a.m <= 128) {
+        p.rows = a.m <= 16 ? 16 : a.m <= 32 ? 32 : a.m <= 64 ? 64 : 128;
+        p.kernel = a.m <= 16 ? "_r1" : a.m <= 32 ? "_r2" : a.m <= 64 ? "_r4" : "_r8";
+        return p;
+    }
+    // The tiles' loads and stores reach a tile's rows by 32-bit offsets, and their loop is four steps long at least. fp32
+    // results do not come from its instruction.
+    const long long reach = (1LL << 31) / 256 / 2;
+    if (a.out_dtype == HELIX_F32 || blocks < 4 || a.ld_a >= reach || a.ld_b >= reach || a.ld_c >= reach / 2 ||
+        a.ld_a_scale >= reach || a.ld_b_scale >= reach)
+        return p;
+    double best = 0;
+    for (const Tiling& t : kTilings) {
+        const long long tiles = ceil_div(a.m, t.bm) * ceil_div(a.n, t.bn);
+        const double us = ceil_div(tiles, 256 * t.per_cu) * (blocks * t.step + t.tile);
+        if (p.bm && us >= best) continue;
+        best = us;
+        p.kernel = t.kernel;
+        p.bm = t.bm;
+        p.bn = t.bn;
+        p.per_cu = t.per_cu;
+    }
+    p.pitch = (size_t)ceil_div(blocks, 4) * 4;
+    // Scales are loaded as words of four.
+    if (a.ld_a_scale % 4 || !aligned(a.a_scale, 4)) p.a_bytes = ((size_t)a.m * p.pitch + 255) & ~(size_t)255;
+    if (a.ld_b_scale % 4 || !aligned(a.b_scale, 4)) p.b_bytes = ((size_t)a.n * p.pitch + 255) & ~(size_t)255;
+    return p;
+}
+
+// 2^32 / d + 1: the high word of its product with x is x / d while x d is below 2^32 (d above 1).
+unsigned reciprocal(unsigned d) { return d > 1 ? (unsigned)((1ULL << 32) / d + 1) : 0; }
+
+}  // namespace
+
+extern "C" size_t helix_matmul_fp8_scratch_size(const helix_matmul_fp8_args* a) {
+    if (!a || a->m <= 0 || a->n <= 0 || a->k <= 0) return 0;
+    const MatmulPlan p = matmul_plan(*a);
+    return p.a_bytes + p.b_bytes;
+}
+
 extern "C" helix_status helix_matmul_fp8_encode(helix_ctx* ctx, void* stream, const helix_matmul_fp8_args* a) {
     return entry(ctx, [&] {
         need(ctx && a, "NULL context or arguments");
@@ -271,6 +340,10 @@ extern "C" helix_status helix_matmul_fp8_encode(helix_ctx* ctx, void* stream, co
         matrix("c", a->c, a->m, a->n, a->ld_c, kBytes[a->out_dtype], true);
         need((a->m == 1 || a->ld_a % 16 == 0) && (a->n == 1 || a->ld_b % 16 == 0),
              "ld_a and ld_b have to be multiples of 16");
+        const MatmulPlan plan = matmul_plan(*a);
+        need(a->scratch_bytes >= plan.a_bytes + plan.b_bytes && (a->scratch || !(plan.a_bytes + plan.b_bytes)),
+             "scratch smaller than helix_matmul_fp8_scratch_size()", HELIX_ERR_SCRATCH_TOO_SMALL);
+        need(aligned(a->scratch, 16), "scratch is not 16-byte aligned");
         HelixMatmulParams p{};
         p.a = static_cast<const uint8_t*>(a->a);
         p.a_scale = static_cast<const uint8_t*>(a->a_scale);
@@ -279,16 +352,50 @@ extern "C" helix_status helix_matmul_fp8_encode(helix_ctx* ctx, void* stream, co
         p.c = a->c;
         p.ld_a = a->ld_a;
         p.ld_a_scale = a->ld_a_scale;
-        p.ld_b = a->ld_b;
+        p.ld_b = a->n == 1 ? ceil_div(a->k, 16) * 16 : a->ld_b;   // a single row's may be anything
         p.ld_b_scale = a->ld_b_scale;
         p.ld_c = a->ld_c;
         p.m = a->m;
         p.n = a->n;
         p.k = a->k;
-        const unsigned gx = grid(ceil_div(a->m, 16) * ceil_div(a->n, 16));
-        const hipFunction_t f = kernel(ctx, std::string("helix_matmul_fp8_") + kTags[a->out_dtype]);
+        const hipFunction_t f = kernel(ctx, std::string("helix_matmul_fp8_") + kTags[a->out_dtype] + plan.kernel);
+        if (plan.rows) {
+            const unsigned gx = grid(ceil_div(a->n, 16)), gy = (unsigned)ceil_div(a->m, plan.rows);
+            const OnDevice on(ctx->device);
+            launch(f, stream, gx, gy, 512, p);
+            return;
+        }
+        if (!plan.bm) {
+            const unsigned gx = grid(ceil_div(a->m, 16) * ceil_div(a->n, 16));
+            const OnDevice on(ctx->device);
+            launch(f, stream, gx, 1, 64, p);
+            return;
+        }
+        const long long mt = ceil_div(a->m, plan.bm), nt = ceil_div(a->n, plan.bn), tiles = mt * nt;
+        need(tiles <= 0x7fffffffLL, "launch grid exceeds 2^31 workgroups");
+        // Bands of 2048 rows, or of one row of tiles where c is so large that a band's number would not come out exactly.
+        p.gm = std::max(1, 2048 / plan.bm);
+        if (tiles * p.gm * nt >= (1LL << 32)) p.gm = 1;
+        need(tiles * p.gm * nt < (1LL << 32), "m and n are too large", HELIX_ERR_UNSUPPORTED_SHAPE);
+        p.band = (unsigned)(p.gm * nt);
+        p.inv_band = reciprocal(p.band);
+        p.inv_gm = reciprocal(p.gm);
+        p.inv_rest = reciprocal((unsigned)(mt % p.gm));
+        p.stride = (int)std::min<long long>(tiles, 256LL * plan.per_cu);
+        p.wide = a->n % 8 == 0 && a->ld_c % 8 == 0 && aligned(a->c, 16);
+        const unsigned ga = grid(ceil_div((long long)a->m * plan.pitch, 256)), gb = grid(ceil_div((long long)a->n * plan.pitch, 256));
+        const hipFunction_t copy = kernel(ctx, "helix_fp8_scales");
         const OnDevice on(ctx->device);
-        launch(f, stream, gx, 1, 64, p);
+        auto repack = [&](const uint8_t*& scale, long long& ld, long long rows, uint8_t* to, unsigned gx) {
+            int nb = (int)blocks, pitch = (int)plan.pitch;
+            void* args[] = {&scale, &to, &ld, &rows, &nb, &pitch};
+            launch_args(copy, stream, gx, 1, 256, args);
+            scale = to;
+            ld = pitch;
+        };
+        if (plan.a_bytes) repack(p.a_scale, p.ld_a_scale, a->m, static_cast<uint8_t*>(a->scratch), ga);
+        if (plan.b_bytes) repack(p.b_scale, p.ld_b_scale, a->n, static_cast<uint8_t*>(a->scratch) + plan.a_bytes, gb);
+        launch(f, stream, (unsigned)p.stride, 1, 256, p);
     });
 }
 

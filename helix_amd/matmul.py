@@ -4,7 +4,8 @@ from __future__ import annotations
 import torch
 
 from . import abi
-from .layer import FP8, FP8_BLOCK, FP8_SCALE, IO_DTYPES, device_index, expect, row_stride, run, stream_handle, under
+from .layer import (FP8, FP8_BLOCK, FP8_SCALE, IO_DTYPES, device_index, expect, ptr, row_stride, run, scratch,
+                    stream_handle, under)
 
 
 def matmul_fp8(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale: torch.Tensor, *,
@@ -37,9 +38,14 @@ def matmul_fp8(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale:
             raise ValueError(f"out must be float32, bfloat16 or float16; got {out.dtype}")
         expect("out", out, out.dtype, (*lead, n), a)
         ld_c = row_stride("out", out)
-    args = abi.MATMUL_FP8_STRUCT.pack(a.numel() // k, n, k, IO_DTYPES[out.dtype], a.data_ptr(), a_scale.data_ptr(),
-                                      b.data_ptr(), b_scale.data_ptr(), out.data_ptr(), row_stride("a", a),
-                                      row_stride("a_scale", a_scale), row_stride("b", b),
-                                      row_stride("b_scale", b_scale), ld_c)
-    run(abi.lib().helix_matmul_fp8_encode, index, stream_handle(index, stream), args)
+    st = stream_handle(index, stream)
+    dims = (a.numel() // k, n, k, IO_DTYPES[out.dtype], a.data_ptr(), a_scale.data_ptr(), b.data_ptr(),
+            b_scale.data_ptr(), out.data_ptr())
+    strides = (row_stride("a", a), row_stride("a_scale", a_scale), row_stride("b", b), row_stride("b_scale", b_scale), ld_c)
+    lib = abi.lib()
+    args = abi.MATMUL_FP8_STRUCT.pack(*dims, 0, 0, *strides)
+    need = lib.helix_matmul_fp8_scratch_size(args)
+    if need:
+        args = abi.MATMUL_FP8_STRUCT.pack(*dims, ptr(scratch(index, st, stream, need)), need, *strides)
+    run(lib.helix_matmul_fp8_encode, index, st, args)
     return out

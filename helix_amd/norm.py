@@ -26,13 +26,14 @@ def _weight_code(weight: torch.Tensor, x: torch.Tensor) -> int:
 
 
 def fp8_rows(shape, device) -> tuple[torch.Tensor, torch.Tensor]:
-    """Uninitialised 8-bit rows and their scales; a row starts at a multiple of 16 bytes, as matmul_fp8 wants it."""
+    """Uninitialised 8-bit rows and their scales; rows start at multiples of 16 bytes, those of the scales of 4, as
+    matmul_fp8 wants them."""
     dim = shape[-1]
-    pitch = -(-dim // 16) * 16
+    blocks = -(-dim // FP8_BLOCK)
+    pitch, s_pitch = -(-dim // 16) * 16, -(-blocks // 4) * 4
     q = torch.empty((*shape[:-1], pitch), dtype=FP8, device=device)
-    if pitch != dim:
-        q = q[..., :dim]
-    return q, torch.empty((*shape[:-1], -(-dim // FP8_BLOCK)), dtype=FP8_SCALE, device=device)
+    scale = torch.empty((*shape[:-1], s_pitch), dtype=FP8_SCALE, device=device)
+    return q if pitch == dim else q[..., :dim], scale if s_pitch == blocks else scale[..., :blocks]
 
 
 def _norm(op, fn, x, weight, residual, eps, fp8, want_rstd, stream):
@@ -63,7 +64,7 @@ def _norm(op, fn, x, weight, residual, eps, fp8, want_rstd, stream):
     pitch = -(-dim // 16) * 16
     args = abi.NORM_STRUCT.pack(x.numel() // dim, dim, io, w_code, eps, x.data_ptr(), ptr(residual), ptr(weight),
                                 0 if h is x else h.data_ptr(), ptr(y), ptr(q), ptr(scale), ptr(rstd), ld_x, ld_r, dim,
-                                dim, pitch, -(-dim // FP8_BLOCK))
+                                dim, pitch, -(-dim // (4 * FP8_BLOCK)) * 4)
     run(fn, index, stream_handle(index, stream), args)
     return y, q, scale, h, rstd
 

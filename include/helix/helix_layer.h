@@ -120,9 +120,15 @@ typedef struct {
     const void* b;             /* (n, k) e4m3                                 */
     const void* b_scale;       /* (n, ceil(k / 128))                          */
     void*       c;             /* (m, n)                                      */
+    void*       scratch;       /* helix_matmul_fp8_scratch_size() bytes,
+                                  16-byte aligned; none is needed where rows of
+                                  scales start at multiples of four bytes     */
+    uint64_t    scratch_bytes;
     int64_t     ld_a, ld_a_scale, ld_b, ld_b_scale, ld_c;
 } helix_matmul_fp8_args;
 
+/* From the arguments without their scratch; addresses count by their alignment. */
+size_t       helix_matmul_fp8_scratch_size(const helix_matmul_fp8_args* args);
 helix_status helix_matmul_fp8_encode(helix_ctx* ctx, void* stream, const helix_matmul_fp8_args* args);
 
 /* ------------------------------------------------------------------------- */

@@ -111,8 +111,9 @@ def test_norm_backward_checks(host, change, status):
     assert call(host, "helix_norm_backward_encode", bwd_args(**change)) == status
 
 
-def mm_args(m=4, n=8, k=300, out=2, a=P, sa=P, b=P, sb=P, c=P, lda=304, ldsa=3, ldb=304, ldsb=3, ldc=8):
-    return abi.MATMUL_FP8_STRUCT.pack(m, n, k, out, a, sa, b, sb, c, lda, ldsa, ldb, ldsb, ldc)
+def mm_args(m=4, n=8, k=300, out=2, a=P, sa=P, b=P, sb=P, c=P, scratch=P, nbytes=1 << 20, lda=304, ldsa=3,
+            ldb=304, ldsb=3, ldc=8):
+    return abi.MATMUL_FP8_STRUCT.pack(m, n, k, out, a, sa, b, sb, c, scratch, nbytes, lda, ldsa, ldb, ldsb, ldc)
 
 
 @pytest.mark.parametrize("change,status", [
@@ -120,6 +121,9 @@ def mm_args(m=4, n=8, k=300, out=2, a=P, sa=P, b=P, sb=P, c=P, lda=304, ldsa=3, 
     (dict(k=0), HELIX_ERR_UNSUPPORTED_SHAPE), (dict(k=(1 << 20) + 1), HELIX_ERR_UNSUPPORTED_SHAPE),
     (dict(out=3), HELIX_ERR_INVALID_ARG), (dict(a=0), HELIX_ERR_INVALID_ARG), (dict(a=P + 8), HELIX_ERR_INVALID_ARG),
     (dict(b=P + 1), HELIX_ERR_INVALID_ARG), (dict(sa=0), HELIX_ERR_INVALID_ARG), (dict(lda=312), HELIX_ERR_INVALID_ARG),
+    (dict(m=1000, k=600, lda=608, ldb=608, ldsa=5, nbytes=10), HELIX_ERR_SCRATCH_TOO_SMALL),
+    (dict(m=1000, k=600, lda=608, ldb=608, ldsa=5, scratch=0), HELIX_ERR_SCRATCH_TOO_SMALL),
+    (dict(m=1000, k=600, lda=608, ldb=608, ldsa=8, ldsb=8, scratch=0, nbytes=0), HELIX_ERR_NO_DEVICE),
     (dict(ldb=-304), HELIX_ERR_INVALID_ARG), (dict(ldc=7), HELIX_ERR_INVALID_ARG), (dict(c=P + 1), HELIX_ERR_INVALID_ARG),
 ])
 def test_matmul_checks(host, change, status):
@@ -200,3 +204,68 @@ def test_the_checks_see_a_mistake():
         lo.within(lo.scan(g, v, None)[0].float(), h, bh)
     with pytest.raises(AssertionError):
         lo.within(h[:, -2].float(), last, bl)
+
+
+# ---- what the compiler cannot see in the tiles' assembly ------------------------
+
+HSACO = os.path.join(ROOT, "helix_amd", "csrc", "_build", "helix_kernels.hsaco")
+OBJDUMP = "/opt/rocm/llvm/bin/llvm-objdump"
+
+
+def _registers(token):
+    m = re.match(r"([vas])\[(\d+):(\d+)\]", token)
+    if m:
+        return {(m.group(1), k) for k in range(int(m.group(2)), int(m.group(3)) + 1)}
+    m = re.match(r"([vas])(\d+)$", token)
+    return {(m.group(1), int(m.group(2)))} if m else set()
+
+
+def _missing_waits(lines):
+    """Products that read a register a vector instruction wrote less than two wait states before, and loads into LDS
+    that read a scalar one wrote less than five before."""
+    def operands(line):
+        return [t.split(" ")[0] for t in re.split(r",\s*(?![^\[]*\])", line.split(None, 1)[1])] if " " in line else []
+
+    found = []
+    for i, line in enumerate(lines):
+        if line.startswith("v_mfma_scale"):
+            reads, states = set().union(*(_registers(t) for t in operands(line)[1:])), 2
+        elif line.startswith("buffer_load") and line.endswith("lds"):
+            reads, states = set().union(*(_registers(t) for t in operands(line))), 5
+        else:
+            continue
+        passed = 0
+        for before in reversed(lines[max(0, i - 8):i]):
+            if before.startswith("v_") and not before.startswith("v_mfma") and operands(before):
+                wrote = _registers(operands(before)[0])
+                if wrote & reads and passed < states:
+                    found.append((before, line))
+            m = re.match(r"s_nop (\d+)", before)
+            passed += int(m.group(1)) + 1 if m else 1
+            if passed >= states:
+                break
+    return found
+
+
+def test_missing_waits_are_seen():
+    product = "v_mfma_scale_f32_16x16x128_f8f6f4 a[0:3], v[8:15], v[16:23], a[0:3], v30, v31 op_sel_hi:[0,0,0]"
+    load = "buffer_load_dwordx4 v2, s[4:7], s9 offen lds"
+    assert _missing_waits(["v_lshrrev_b32_e32 v30, s2, v30", product])
+    assert _missing_waits(["v_mov_b32_e32 v10, v11", "s_mov_b32 s0, 0", product])
+    assert not _missing_waits(["v_mov_b32_e32 v10, v11", "s_nop 1", product])
+    assert _missing_waits(["v_readlane_b32 s9, v255, 3", "s_add_u32 m0, s1, 0x400", "s_nop 0", load])
+    assert not _missing_waits(["v_readlane_b32 s9, v255, 3", "s_mov_b32 m0, s1", "s_nop 4", load])
+
+
+@pytest.mark.skipif(not (os.path.exists(HSACO) and os.path.exists(OBJDUMP)), reason="needs the built code object and llvm-objdump")
+def test_tiles_assembly_waits_for_its_operands():
+    out = subprocess.run([OBJDUMP, "-d", HSACO], check=True, capture_output=True, text=True).stdout
+    kernels = 0
+    for block in re.split(r"\n(?=[0-9a-f]+ <)", out):
+        name = re.match(r"[0-9a-f]+ <(\w+)>", block)
+        if not name or not re.match(r"helix_matmul_fp8_\w+_t\d", name.group(1)):
+            continue
+        kernels += 1
+        lines = [re.sub(r"\s+", " ", ln.split("//")[0]).strip() for ln in block.splitlines()[1:]]
+        assert _missing_waits([ln for ln in lines if ln]) == [], name.group(1)
+    assert kernels == 10
