@@ -231,7 +231,7 @@ def _missing_waits(lines):
         if line.startswith("v_mfma_scale"):
             reads, states = set().union(*(_registers(t) for t in operands(line)[1:])), 2
         elif line.startswith("buffer_load") and line.endswith("lds"):
-            reads, states = set().union(*(_registers(t) for t in operands(line))), 5
+            reads, states = {r for t in operands(line) for r in _registers(t) if r[0] == "s"}, 5
         else:
             continue
         passed = 0
