@@ -120,4 +120,47 @@ HELIX_DEV void buf_store4(helix_rsrc r, const float (&v)[4], int voff, int own) 
     }
 }
 
+// Eight neighbouring elements as they are stored, at byte offset voff.
+template <typename T> struct Raw8 { u32x4 w[sizeof(T) / 2]; };
+template <typename T>
+HELIX_DEV Raw8<T> buf_load8(helix_rsrc r, int voff) {
+    Raw8<T> o;
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) o.w[i] = __builtin_amdgcn_raw_buffer_load_b128(r, voff + 16 * i, 0, 0);
+    return o;
+}
+template <typename T>
+HELIX_DEV float at8(const Raw8<T>& v, int i) {
+    if constexpr (sizeof(T) == 4) {
+        return as_f32(v.w[i >> 2][i & 3]);
+    } else {
+        const unsigned x = v.w[0][i >> 1];
+        return io_f32<T>((unsigned short)(i & 1 ? x >> 16 : x & 0xffffu));
+    }
+}
+template <typename T>
+HELIX_DEV void buf_store8(helix_rsrc r, const float (&v)[8], int voff) {
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+            __builtin_amdgcn_raw_buffer_store_b128(
+                u32x4{as_u32(v[4 * i]), as_u32(v[4 * i + 1]), as_u32(v[4 * i + 2]), as_u32(v[4 * i + 3])}, r, voff + 16 * i, 0, 0);
+    } else {
+        __builtin_amdgcn_raw_buffer_store_b128(
+            u32x4{narrow2<T>(v[0], v[1]), narrow2<T>(v[2], v[3]), narrow2<T>(v[4], v[5]), narrow2<T>(v[6], v[7])}, r, voff, 0, 0);
+    }
+}
+
+// The largest over each sixteen lanes, by moves within a row of lanes; all have it.
+template <int CTRL>
+HELIX_DEV float max_dpp(float v) {
+    return fmaxf(v, as_f32((unsigned)__builtin_amdgcn_update_dpp(0, (int)as_u32(v), CTRL, 0xf, 0xf, true)));
+}
+HELIX_DEV float row16_max(float v) {
+    v = max_dpp<0xb1>(v);    // lane ^ 1
+    v = max_dpp<0x4e>(v);    // lane ^ 2
+    v = max_dpp<0x141>(v);   // mirrored in eight
+    return max_dpp<0x140>(v);   // mirrored in sixteen
+}
+
 #endif

@@ -243,7 +243,7 @@ HELIX_DEV void repeat(F&& f) {
     }
 }
 
-template <typename T, int TM, int TN>
+template <int TM, int TN>
 __device__ void matmul_tiles(const HelixMatmulParams& p) {
     constexpr int BN = 32 * TM, BM = 32 * TN, ROWS = BN + BM, STAGE = ROWS * 128, SLOT = ROWS * 4;
     constexpr int NX = BN / 32, NY = BM / 32;      // loads of a wave in a stage: 8 rows each
@@ -489,7 +489,9 @@ __device__ void matmul_tiles(const HelixMatmulParams& p) {
         // Every store is issued, whatever its lanes may write: the waits of the next steps count them.
         const TileAt at = tile_at(t);
         const int left_n = p.n - at.j, left_m = p.m - at.i;
-        const helix_rsrc rc = make_rsrc_u(static_cast<T*>(p.c) + at.i * p.ld_c + at.j, (unsigned)(((min(left_m, BM) - 1) * p.ld_c + min(left_n, BN)) * 2));
+        const helix_rsrc rc =
+            make_rsrc_u(static_cast<uint16_t*>(p.c) + at.i * p.ld_c + at.j,
+                        (unsigned)(((min(left_m, BM) - 1) * p.ld_c + min(left_n, BN)) * 2));
         const int ldc = (int)p.ld_c * 2;
 #pragma unroll
         for (int j = 0; j < TN; ++j) {
@@ -498,13 +500,16 @@ __device__ void matmul_tiles(const HelixMatmulParams& p) {
             for (int i = 0; i < TM; i += 2) {
                 const int col = wx + 16 * i + 8 * vgpr_fresh(fq);
                 const f32x4 u = acc[i][j], v = acc[i + 1][j];
-                const u32x4 w = {narrow2<T>(u[0], u[1]), narrow2<T>(u[2], u[3]), narrow2<T>(v[0], v[1]), narrow2<T>(v[2], v[3])};
+                u32x4 w;
+                if (p.f16) w = u32x4{narrow2<_Float16>(u[0], u[1]), narrow2<_Float16>(u[2], u[3]), narrow2<_Float16>(v[0], v[1]), narrow2<_Float16>(v[2], v[3])};
+                else w = u32x4{narrow2<__bf16>(u[0], u[1]), narrow2<__bf16>(u[2], u[3]), narrow2<__bf16>(v[0], v[1]), narrow2<__bf16>(v[2], v[3])};
                 if (p.wide) {
                     __builtin_amdgcn_raw_buffer_store_b128(w, rc, col < left_n ? row + 2 * col : (int)0x80000000, 0, 0);
                 } else {
 #pragma unroll
                     for (int r = 0; r < 8; ++r)
-                        __builtin_amdgcn_raw_buffer_store_b16((unsigned short)(w[r >> 1] >> (16 * (r & 1))), rc, col + r < left_n ? row + 2 * (col + r) : (int)0x80000000, 0, 0);
+                        __builtin_amdgcn_raw_buffer_store_b16((unsigned short)(w[r >> 1] >> (16 * (r & 1))), rc,
+                                                              col + r < left_n ? row + 2 * (col + r) : (int)0x80000000, 0, 0);
                 }
             }
         }
@@ -522,18 +527,15 @@ extern "C" __global__ __launch_bounds__(256) void helix_fp8_scales(const uint8_t
     if (row < rows) to[i] = c < blocks ? from[row * ld + c] : 0;
 }
 
-#define MATMUL_TILES(TAG, T, TM, TN, BOUND)                                                                  \
-    extern "C" __global__ __launch_bounds__(256, BOUND) void helix_matmul_fp8_##TAG##_t##TM##TN(HelixMatmulParams p) { \
-        matmul_tiles<T, TM, TN>(p);                                                                          \
+#define MATMUL_TILES(TM, TN, BOUND)                                                                           \
+    extern "C" __global__ __launch_bounds__(256, BOUND) void helix_matmul_fp8_t##TM##TN(HelixMatmulParams p) { \
+        matmul_tiles<TM, TN>(p);                                                                              \
     }
-#define MATMUL_TILED(TAG, T)         \
-    MATMUL_TILES(TAG, T, 8, 8, 1)    \
-    MATMUL_TILES(TAG, T, 8, 6, 1)    \
-    MATMUL_TILES(TAG, T, 8, 4, 1)    \
-    MATMUL_TILES(TAG, T, 4, 4, 2)    \
-    MATMUL_TILES(TAG, T, 4, 2, 2)
-MATMUL_TILED(f16, _Float16)
-MATMUL_TILED(bf16, __bf16)
+MATMUL_TILES(8, 8, 1)
+MATMUL_TILES(8, 6, 1)
+MATMUL_TILES(8, 4, 1)
+MATMUL_TILES(4, 4, 2)
+MATMUL_TILES(4, 2, 2)
 
 #define MATMUL_ROWS(TAG, T, MT)                                                                              \
     extern "C" __global__ __launch_bounds__(512) void helix_matmul_fp8_##TAG##_r##MT(HelixMatmulParams p) {  \

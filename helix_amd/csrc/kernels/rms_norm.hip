@@ -1,5 +1,16 @@
 // rms_norm.hip -- root-mean-square norm with the residual's addition, into the
 // storage type or 8 bits with scales, and its backward pass (helix_layer.h).
+//
+// Memory binds all of it, so every tensor is read and written once: a row stays in
+// registers between its sum and its outputs. A lane holds eight neighbouring channels
+// of every chunk of 512 (16-byte accesses; sixteen lanes are a block of 128), and a row
+// is a wave's (W = 1: no barrier) or a workgroup's of four waves (W = 4), which divide
+// the registers of a wide row, or of one of few.
+// Accesses past a row's end are out of the resource's range: they read zeros, which add
+// nothing to a sum or a largest magnitude, and write nothing.
+//
+// Rows wider than that, or whose elements do not start at multiples of 16 bytes, go
+// through the forms below that read a row twice, element by element.
 #include "layer_common.h"
 
 namespace {
@@ -20,6 +31,198 @@ HELIX_DEV float group_sum(float v, float* red) {
 template <typename T>
 HELIX_DEV float weight_at(const void* w, int w_f32, int c) {
     return w_f32 ? static_cast<const float*>(w)[c] : (float)static_cast<const T*>(w)[c];
+}
+
+// A row's resource: `dim` elements of T.
+template <typename T>
+HELIX_DEV helix_rsrc row_rsrc(const void* base, long long row, long long ld, int dim) {
+    return make_rsrc_u(static_cast<const T*>(base) + row * ld, (unsigned)dim * (unsigned)sizeof(T));
+}
+
+// The weights of a lane's channels in fp32.
+template <typename T, int NC>
+HELIX_DEV void load_weights(const void* w, int w_f32, int dim, const int (&c)[NC], float (&o)[NC][8]) {
+    if (w_f32) {
+        const helix_rsrc r = make_rsrc_u(w, dim * 4u);
+#pragma unroll
+        for (int j = 0; j < NC; ++j) {
+            const Raw8<float> v = buf_load8<float>(r, c[j] * 4);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) o[j][i] = at8(v, i);
+        }
+    } else {
+        const helix_rsrc r = make_rsrc_u(w, dim * (unsigned)sizeof(T));
+#pragma unroll
+        for (int j = 0; j < NC; ++j) {
+            const Raw8<T> v = buf_load8<T>(r, c[j] * (int)sizeof(T));
+#pragma unroll
+            for (int i = 0; i < 8; ++i) o[j][i] = at8(v, i);
+        }
+    }
+}
+
+// Sum over the row's waves.
+template <int W>
+HELIX_DEV float row_sum(float v, float* red) {
+    if constexpr (W == 1) return wave_sum(v);
+    else return group_sum(v, red);
+}
+
+template <typename T, int W, int NC>
+__device__ void norm_rows(const HelixNormParams& p) {
+    __shared__ float red[NORM_THREADS / 64];
+    constexpr int ES = sizeof(T);
+    const int lane = lane_id(), wave = wave_uniform();
+    const long long row = W == 1 ? (long long)blockIdx.x * 4 + wave : blockIdx.x;
+    if (W == 1 && row >= p.rows) return;
+    int c[NC];
+#pragma unroll
+    for (int j = 0; j < NC; ++j) c[j] = (W == 1 ? j : 4 * j + wave) * 512 + 8 * lane;
+    Raw8<T> x[NC], r[NC];
+    const helix_rsrc rx = row_rsrc<T>(p.x, row, p.ld_x, p.dim);
+#pragma unroll
+    for (int j = 0; j < NC; ++j) x[j] = buf_load8<T>(rx, c[j] * ES);
+    if (p.residual) {
+        const helix_rsrc rr = row_rsrc<T>(p.residual, row, p.ld_residual, p.dim);
+#pragma unroll
+        for (int j = 0; j < NC; ++j) r[j] = buf_load8<T>(rr, c[j] * ES);
+    }
+    float w[NC][8], v[NC][8];
+    if (p.weight) load_weights<T>(p.weight, p.w_f32, p.dim, c, w);
+    float ss = 0.0f;
+#pragma unroll
+    for (int j = 0; j < NC; ++j)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[j][i] = at8(x[j], i);
+    if (p.residual) {
+#pragma unroll
+        for (int j = 0; j < NC; ++j)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[j][i] += at8(r[j], i);
+    }
+    if (p.h) {
+        const helix_rsrc rh = row_rsrc<T>(p.h, row, p.ld_h, p.dim);
+#pragma unroll
+        for (int j = 0; j < NC; ++j) buf_store8<T>(rh, v[j], c[j] * ES);
+    }
+    if (p.weight) {
+#pragma unroll
+        for (int j = 0; j < NC; ++j)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) ss += v[j][i] * v[j][i];
+        const float rstd = 1.0f / sqrtf(row_sum<W>(ss, red) / (float)p.dim + p.eps);
+        if (p.rstd && lane == 0 && (W == 1 || wave == 0)) p.rstd[row] = rstd;
+#pragma unroll
+        for (int j = 0; j < NC; ++j)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[j][i] = v[j][i] * rstd * w[j][i];
+    }
+    if (p.y) {
+        const helix_rsrc ry = row_rsrc<T>(p.y, row, p.ld_y, p.dim);
+#pragma unroll
+        for (int j = 0; j < NC; ++j) buf_store8<T>(ry, v[j], c[j] * ES);
+        return;
+    }
+    const helix_rsrc rq = row_rsrc<uint8_t>(p.q, row, p.ld_q, p.dim);
+    const helix_rsrc rs = row_rsrc<uint8_t>(p.scale, row, p.ld_scale, (p.dim + HELIX_BLOCK - 1) / HELIX_BLOCK);
+#pragma unroll
+    for (int j = 0; j < NC; ++j) {
+        float top = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(v[j][i]));
+        const int e = block_exponent(row16_max(top));
+        const float inv = exponent_recip(e);
+        u32x2 q;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            int d = __builtin_amdgcn_cvt_pk_fp8_f32(v[j][4 * i] * inv, v[j][4 * i + 1] * inv, 0, false);
+            q[i] = (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(v[j][4 * i + 2] * inv, v[j][4 * i + 3] * inv, d, true);
+        }
+        __builtin_amdgcn_raw_buffer_store_b64(q, rq, c[j], 0, 0);
+        __builtin_amdgcn_raw_buffer_store_b8((unsigned char)e, rs, lane & 15 ? (int)0x80000000 : c[j] >> 7, 0, 0);
+    }
+}
+
+// dx, and dweight's sum over the rows of a part: a workgroup's, row by row in each of
+// its waves (W = 1) or in all of them (W = 4). The waves' sums are added in their order.
+template <typename T, int W, int NC>
+__device__ void norm_bwd_rows(const HelixNormBwdParams& p) {
+    __shared__ float red[2][NORM_THREADS / 64];
+    __shared__ float sums[W == 1 ? 3 : 1][W == 1 ? NC * 512 : 1];
+    constexpr int ES = sizeof(T);
+    const int lane = lane_id(), wave = wave_uniform();
+    int c[NC];
+#pragma unroll
+    for (int j = 0; j < NC; ++j) c[j] = (W == 1 ? j : 4 * j + wave) * 512 + 8 * lane;
+    float w[NC][8], dw[NC][8];
+    load_weights<T>(p.weight, p.w_f32, p.dim, c, w);
+#pragma unroll
+    for (int j = 0; j < NC; ++j)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) dw[j][i] = 0.0f;
+    const long long first = blockIdx.x * p.part_rows, end = min(p.rows, first + p.part_rows);
+    int turn = 0;
+    for (long long row = first + (W == 1 ? wave : 0); row < end; row += W == 1 ? 4 : 1) {
+        Raw8<T> dy[NC], h[NC], dh[NC];
+        const helix_rsrc rd = row_rsrc<T>(p.dy, row, p.ld_dy, p.dim), rh = row_rsrc<T>(p.h, row, p.ld_h, p.dim);
+#pragma unroll
+        for (int j = 0; j < NC; ++j) dy[j] = buf_load8<T>(rd, c[j] * ES);
+#pragma unroll
+        for (int j = 0; j < NC; ++j) h[j] = buf_load8<T>(rh, c[j] * ES);
+        if (p.dh) {
+            const helix_rsrc rg = row_rsrc<T>(p.dh, row, p.ld_dh, p.dim);
+#pragma unroll
+            for (int j = 0; j < NC; ++j) dh[j] = buf_load8<T>(rg, c[j] * ES);
+        }
+        const float rstd = p.rstd[row];
+        float dot = 0.0f;
+#pragma unroll
+        for (int j = 0; j < NC; ++j)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float n = at8(h[j], i) * rstd, g = at8(dy[j], i);
+                dot += g * w[j][i] * n;
+                dw[j][i] += g * n;
+            }
+        // Two places in turn: a wave may be at the next row's sum while another reads this one's.
+        const float mean = row_sum<W>(dot, red[turn]) / (float)p.dim;
+        turn ^= 1;
+        const helix_rsrc rx = row_rsrc<T>(p.dx, row, p.ld_dx, p.dim);
+#pragma unroll
+        for (int j = 0; j < NC; ++j) {
+            float o[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float n = at8(h[j], i) * rstd;
+                o[i] = rstd * (at8(dy[j], i) * w[j][i] - n * mean);
+            }
+            if (p.dh) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) o[i] += at8(dh[j], i);
+            }
+            buf_store8<T>(rx, o, c[j] * ES);
+        }
+    }
+    if (!p.dweight) return;
+    const helix_rsrc rp = row_rsrc<float>(p.part, blockIdx.x, p.dim, p.dim);
+    if constexpr (W == 1) {
+        if (wave > 0) {
+#pragma unroll
+            for (int j = 0; j < NC; ++j)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) sums[wave - 1][(j * 8 + i) * 64 + lane] = dw[j][i];
+        }
+        __syncthreads();
+        if (wave > 0) return;
+#pragma unroll
+        for (int j = 0; j < NC; ++j)
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+#pragma unroll
+                for (int o = 0; o < 3; ++o) dw[j][i] += sums[o][(j * 8 + i) * 64 + lane];
+    }
+#pragma unroll
+    for (int j = 0; j < NC; ++j) buf_store8<float>(rp, dw[j], c[j] * 4);
 }
 
 // One workgroup per row, which is read twice (the second time from the caches).
@@ -104,11 +307,19 @@ __device__ void norm_dw_part(const HelixNormBwdParams& p) {
 
 }  // namespace
 
-extern "C" __global__ __launch_bounds__(NORM_THREADS) void helix_norm_dw(HelixNormBwdParams p) {
-    const int c = blockIdx.x * NORM_THREADS + threadIdx.x;
-    if (c >= p.dim) return;
+// dweight from the parts: 64 channels a workgroup, a sixteenth of the parts a wave, the
+// sixteen added in their order.
+extern "C" __global__ __launch_bounds__(1024) void helix_norm_dw(HelixNormBwdParams p) {
+    __shared__ float sum[16][64];
+    const int lane = lane_id(), wave = wave_id(), c = blockIdx.x * 64 + lane;
     float s = 0.0f;
-    for (int i = 0; i < p.parts; ++i) s += p.part[(long long)i * p.dim + c];
+    if (c < p.dim)
+        for (int i = wave; i < p.parts; i += 16) s += p.part[(long long)i * p.dim + c];
+    sum[wave][lane] = s;
+    __syncthreads();
+    if (wave || c >= p.dim) return;
+#pragma unroll
+    for (int w = 1; w < 16; ++w) s += sum[w][lane];
     p.dweight[c] = s;
 }
 
@@ -125,3 +336,34 @@ extern "C" __global__ __launch_bounds__(NORM_THREADS) void helix_norm_dw(HelixNo
 NORM_KERNELS(f32, float)
 NORM_KERNELS(f16, _Float16)
 NORM_KERNELS(bf16, __bf16)
+
+#define NORM_FWD(TAG, T, KIND, W, NC)                                                                             \
+    extern "C" __global__ __launch_bounds__(NORM_THREADS) void helix_norm_##TAG##_##KIND##NC(HelixNormParams p) { \
+        norm_rows<T, W, NC>(p);                                                                                   \
+    }
+#define NORM_BWD(TAG, T, KIND, W, NC)                                                                                    \
+    extern "C" __global__ __launch_bounds__(NORM_THREADS) void helix_norm_bwd_##TAG##_##KIND##NC(HelixNormBwdParams p) { \
+        norm_bwd_rows<T, W, NC>(p);                                                                                      \
+    }
+#define NORM_ROWS(TAG, T)     \
+    NORM_FWD(TAG, T, w, 1, 1) \
+    NORM_FWD(TAG, T, w, 1, 2) \
+    NORM_FWD(TAG, T, w, 1, 3) \
+    NORM_FWD(TAG, T, w, 1, 4) \
+    NORM_FWD(TAG, T, g, 4, 1) \
+    NORM_FWD(TAG, T, g, 4, 2) \
+    NORM_FWD(TAG, T, g, 4, 3) \
+    NORM_FWD(TAG, T, g, 4, 4) \
+    NORM_FWD(TAG, T, g, 4, 6) \
+    NORM_FWD(TAG, T, g, 4, 8) \
+    NORM_BWD(TAG, T, w, 1, 1) \
+    NORM_BWD(TAG, T, w, 1, 2) \
+    NORM_BWD(TAG, T, g, 4, 1) \
+    NORM_BWD(TAG, T, g, 4, 2) \
+    NORM_BWD(TAG, T, g, 4, 3) \
+    NORM_BWD(TAG, T, g, 4, 4) \
+    NORM_BWD(TAG, T, g, 4, 6) \
+    NORM_BWD(TAG, T, g, 4, 8)
+NORM_ROWS(f32, float)
+NORM_ROWS(f16, _Float16)
+NORM_ROWS(bf16, __bf16)

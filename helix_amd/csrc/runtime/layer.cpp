@@ -105,6 +105,23 @@ helix_status entry(helix_ctx* ctx, F&& body) {
 
 constexpr int kNormThreads = 256;
 
+// Kernel of rows of dim channels that are read once: "_w" + the chunks of 512 a wave holds, or "_g" + those of 2048 a
+// workgroup does; empty: the forms that read a row twice. A wave holds `most` chunks well (more would leave a SIMD
+// with one or two waves), and rows that would leave CUs without work (four to a workgroup) are a workgroup's each.
+std::string norm_form(long long rows, long long dim, bool vec, int most) {
+    if (!vec || dim > 8 * 2048) return "";
+    const bool wave = dim <= most * 512 && rows >= 4 * 256;
+    const long long chunks = ceil_div(dim, wave ? 512 : 2048);
+    for (const int n : {1, 2, 3, 4, 6, 8})
+        if (chunks <= n) return (wave ? "_w" : "_g") + std::to_string(n);
+    return "";
+}
+
+// Whether rows can be moved in pieces of 16 bytes.
+bool pieces(const void* p, long long rows, long long ld, size_t es) {
+    return !p || (aligned(p, 16) && (rows == 1 || ld * (long long)es % 16 == 0));
+}
+
 void norm(helix_ctx* ctx, void* stream, const helix_norm_args* a, bool quantize) {
     need(ctx && a, "NULL context or arguments");
     need(a->rows >= 0 && a->dim >= 1 && a->dim <= HELIX_LAYER_MAX_DIM, "rows or dim out of range",
@@ -152,42 +169,20 @@ void norm(helix_ctx* ctx, void* stream, const helix_norm_args* a, bool quantize)
     p.dim = a->dim;
     p.w_f32 = a->weight_dtype == HELIX_F32;
     p.eps = a->eps;
-    const unsigned gx = grid(a->rows);
-    const hipFunction_t f = kernel(ctx, std::string("helix_norm_") + kTags[a->io_dtype]);
+    const bool vec = a->dim % 8 == 0 && pieces(a->x, a->rows, a->ld_x, es) && pieces(a->residual, a->rows, a->ld_residual, es) &&
+                     pieces(a->weight, 1, 0, 1) && pieces(a->h, a->rows, a->ld_h, es) && pieces(a->y, a->rows, a->ld_y, es) &&
+                     (!a->q || (aligned(a->q, 8) && (a->rows == 1 || a->ld_q % 8 == 0)));
+    const std::string form = norm_form(a->rows, a->dim, vec, 4);
+    const unsigned gx = grid(form[0] && form[1] == 'w' ? ceil_div(a->rows, 4) : a->rows);
+    const hipFunction_t f = kernel(ctx, std::string("helix_norm_") + kTags[a->io_dtype] + form);
     const OnDevice on(ctx->device);
     launch(f, stream, gx, 1, kNormThreads, p);
 }
 
-// Parts that dweight's rows are summed in: as many as give every CU four
-// workgroups of 256 channels, of 16 rows at least.
-long long norm_parts(long long rows, long long dim) {
-    const long long most = ceil_div(1024, ceil_div(dim, kNormThreads));
-    return std::max(1LL, std::min(most, rows / 16));
-}
+// Parts that dweight's rows are summed in, a workgroup's each: three for every CU, of 16 rows at least.
+long long norm_parts(long long rows) { return std::max(1LL, std::min(3 * 256LL, rows / 16)); }
 
 }  // namespace
-
-namespace helix::rt {
-
-const std::vector<std::string>& layer_kernel_names() {
-    static const std::vector<std::string> names = [] {
-        std::vector<std::string> v{"helix_norm_dw", "helix_fp8_scales", "helix_gated_scan_fill"};
-        for (const char* t : kTags)
-            for (const char* k : {"helix_norm_", "helix_norm_bwd_", "helix_norm_dw_part_"})
-                v.push_back(std::string(k) + t);
-        for (const char* tag : kTags)
-            for (const char* k : {"_any", "_r1", "_r2", "_r4", "_r8", "_t88", "_t86", "_t84", "_t44", "_t42"})
-                if (tag != kTags[HELIX_F32] || k[1] != 't') v.push_back(std::string("helix_matmul_fp8_") + tag + k);
-        for (const char* t : kTags)
-            for (const char* k : {"helix_gated_scan_", "helix_gated_scan_bwd_"})
-                for (const char* x : {"_v_", "_s_"})
-                    for (const char* w : {"steps", "w4", "w8"}) v.push_back(std::string(k) + t + x + w);
-        return v;
-    }();
-    return names;
-}
-
-}  // namespace helix::rt
 
 extern "C" helix_status helix_norm_encode(helix_ctx* ctx, void* stream, const helix_norm_args* args) {
     return entry(ctx, [&] { norm(ctx, stream, args, false); });
@@ -199,7 +194,7 @@ extern "C" helix_status helix_quantize_fp8_encode(helix_ctx* ctx, void* stream, 
 
 extern "C" size_t helix_norm_backward_scratch_size(const helix_norm_backward_args* a) {
     if (!a || !a->dweight || a->rows <= 0 || a->dim <= 0) return 0;
-    return (size_t)norm_parts(a->rows, a->dim) * a->dim * sizeof(float);
+    return (size_t)norm_parts(a->rows) * a->dim * sizeof(float);
 }
 
 extern "C" helix_status helix_norm_backward_encode(helix_ctx* ctx, void* stream, const helix_norm_backward_args* a) {
@@ -243,19 +238,24 @@ extern "C" helix_status helix_norm_backward_encode(helix_ctx* ctx, void* stream,
         p.rows = a->rows;
         p.dim = a->dim;
         p.w_f32 = a->weight_dtype == HELIX_F32;
-        p.parts = a->rows ? (int)norm_parts(a->rows, a->dim) : 0;   // no rows: dweight is 0
+        p.parts = a->rows ? (int)norm_parts(a->rows) : 0;   // no rows: dweight is 0
         p.part_rows = p.parts ? ceil_div(a->rows, p.parts) : 0;
         const std::string tag = kTags[a->io_dtype];
+        const bool vec = a->dim % 8 == 0 && pieces(a->dy, a->rows, a->ld_dy, es) && pieces(a->h, a->rows, a->ld_h, es) &&
+                         pieces(a->weight, 1, 0, 1) && pieces(a->dh, a->rows, a->ld_dh, es) && pieces(a->dx, a->rows, a->ld_dx, es);
+        const std::string form = norm_form(a->rows, a->dim, vec, 2);
         const unsigned gx = grid(a->rows);
-        const unsigned gc = (unsigned)ceil_div(a->dim, kNormThreads);
-        const hipFunction_t dx = kernel(ctx, "helix_norm_bwd_" + tag), part = kernel(ctx, "helix_norm_dw_part_" + tag),
+        const unsigned gc = (unsigned)ceil_div(a->dim, kNormThreads), gd = (unsigned)ceil_div(a->dim, 64);
+        const hipFunction_t dx = kernel(ctx, "helix_norm_bwd_" + tag + form), part = kernel(ctx, "helix_norm_dw_part_" + tag),
                             dw = kernel(ctx, "helix_norm_dw");
         const OnDevice on(ctx->device);
-        if (p.dweight) {   // first: dx may be dy
-            if (p.parts) launch(part, stream, gc, (unsigned)p.parts, kNormThreads, p);
-            launch(dw, stream, gc, 1, kNormThreads, p);
+        if (a->rows && form.empty()) {   // dweight first: dx may be dy
+            if (p.dweight) launch(part, stream, gc, (unsigned)p.parts, kNormThreads, p);
+            launch(dx, stream, gx, 1, kNormThreads, p);
+        } else if (a->rows) {
+            launch(dx, stream, (unsigned)p.parts, 1, kNormThreads, p);
         }
-        if (a->rows) launch(dx, stream, gx, 1, kNormThreads, p);
+        if (p.dweight) launch(dw, stream, gd, 1, 1024, p);
     });
 }
 
@@ -358,7 +358,9 @@ extern "C" helix_status helix_matmul_fp8_encode(helix_ctx* ctx, void* stream, co
         p.m = a->m;
         p.n = a->n;
         p.k = a->k;
-        const hipFunction_t f = kernel(ctx, std::string("helix_matmul_fp8_") + kTags[a->out_dtype] + plan.kernel);
+        const hipFunction_t f =
+            kernel(ctx, plan.bm ? std::string("helix_matmul_fp8") + plan.kernel
+                                : std::string("helix_matmul_fp8_") + kTags[a->out_dtype] + plan.kernel);
         if (plan.rows) {
             const unsigned gx = grid(ceil_div(a->n, 16)), gy = (unsigned)ceil_div(a->m, plan.rows);
             const OnDevice on(ctx->device);
@@ -382,6 +384,7 @@ extern "C" helix_status helix_matmul_fp8_encode(helix_ctx* ctx, void* stream, co
         p.inv_gm = reciprocal(p.gm);
         p.inv_rest = reciprocal((unsigned)(mt % p.gm));
         p.stride = (int)std::min<long long>(tiles, 256LL * plan.per_cu);
+        p.f16 = a->out_dtype == HELIX_F16;
         p.wide = a->n % 8 == 0 && a->ld_c % 8 == 0 && aligned(a->c, 16);
         const unsigned ga = grid(ceil_div((long long)a->m * plan.pitch, 256)), gb = grid(ceil_div((long long)a->n * plan.pitch, 256));
         const hipFunction_t copy = kernel(ctx, "helix_fp8_scales");
@@ -579,3 +582,31 @@ extern "C" helix_status helix_gated_scan_backward_encode(helix_ctx* ctx, void* s
         run_scan(ctx, stream, *a, p, "helix_gated_scan_bwd_", HELIX_GS_RUN_BWD, vec, far);
     });
 }
+
+namespace helix::rt {
+
+const std::vector<std::string>& layer_kernel_names() {
+    static const std::vector<std::string> names = [] {
+        std::vector<std::string> v{"helix_norm_dw", "helix_fp8_scales", "helix_gated_scan_fill"};
+        for (const char* t : kTags)
+            for (const char* k : {"helix_norm_", "helix_norm_bwd_", "helix_norm_dw_part_"})
+                v.push_back(std::string(k) + t);
+        for (const char* tag : kTags)
+            for (const char* n : {"1", "2", "3", "4", "6", "8"}) {
+                for (const char* k : {"helix_norm_", "helix_norm_bwd_"}) v.push_back(std::string(k) + tag + "_g" + n);
+                if (n[0] <= '4') v.push_back(std::string("helix_norm_") + tag + "_w" + n);
+                if (n[0] <= '2') v.push_back(std::string("helix_norm_bwd_") + tag + "_w" + n);
+            }
+        for (const char* tag : kTags)
+            for (const char* k : {"_any", "_r1", "_r2", "_r4", "_r8"}) v.push_back(std::string("helix_matmul_fp8_") + tag + k);
+        for (const Tiling& t : kTilings) v.push_back(std::string("helix_matmul_fp8") + t.kernel);
+        for (const char* t : kTags)
+            for (const char* k : {"helix_gated_scan_", "helix_gated_scan_bwd_"})
+                for (const char* x : {"_v_", "_s_"})
+                    for (const char* w : {"steps", "w4", "w8"}) v.push_back(std::string(k) + t + x + w);
+        return v;
+    }();
+    return names;
+}
+
+}  // namespace helix::rt

@@ -79,7 +79,7 @@ def norm_args(rows=4, dim=200, io=2, w=0, eps=1e-5, x=P, r=0, weight=P, h=0, y=P
     (dict(ld=199), HELIX_ERR_INVALID_ARG, "overlap"),
     (dict(ld=-256), HELIX_ERR_INVALID_ARG, "stride"),
     (dict(rstd=P + 2), HELIX_ERR_INVALID_ARG, "rstd"),
-    (dict(rows=1 << 31), HELIX_ERR_INVALID_ARG, "grid"),
+    (dict(rows=1 << 34), HELIX_ERR_INVALID_ARG, "grid"),
 ])
 def test_norm_checks(host, change, status, word):
     assert call(host, "helix_norm_encode", norm_args(**change)) == status
@@ -263,9 +263,9 @@ def test_tiles_assembly_waits_for_its_operands():
     kernels = 0
     for block in re.split(r"\n(?=[0-9a-f]+ <)", out):
         name = re.match(r"[0-9a-f]+ <(\w+)>", block)
-        if not name or not re.match(r"helix_matmul_fp8_\w+_t\d", name.group(1)):
+        if not name or not re.match(r"helix_matmul_fp8_t\d", name.group(1)):
             continue
         kernels += 1
         lines = [re.sub(r"\s+", " ", ln.split("//")[0]).strip() for ln in block.splitlines()[1:]]
         assert _missing_waits([ln for ln in lines if ln]) == [], name.group(1)
-    assert kernels == 10
+    assert kernels == 5
