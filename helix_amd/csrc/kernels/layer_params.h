@@ -56,7 +56,9 @@ typedef struct {
      * 2^32 / d + 1 of band, gm and the last band's rows. */
     int            gm;
     unsigned       band, inv_band, inv_gm, inv_rest;
-    int            stride;  /* workgroups: tiles from one to a workgroup's next  */
+    int            stride;  /* tiles from a workgroup's one to its next          */
+    int            parts, part_blocks;   /* of the sum, and blocks of each but the last */
+    float*         part;    /* [parts][m][n to a multiple of 4]                */
 } HelixMatmulParams;
 
 /* Gated recurrence: tokens of a thread's run, forward and backward, chunks of a

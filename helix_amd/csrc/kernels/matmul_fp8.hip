@@ -107,16 +107,17 @@ __device__ void matmul_tile(const HelixMatmulParams& p) {
 
 // ---- few rows of a ------------------------------------------------------------
 //
-// A workgroup per 16 rows of b, its W waves each a stretch of the sum and all of up to
-// 16 MT rows of a; they meet in LDS, in the order of the waves. b is read once, straight
-// into registers, which is what bounds it; a comes from the caches.
+// A workgroup per 16 rows of b and up to 16 MT of a; its W waves each take a stretch of
+// the sum and meet in LDS, in their order. b comes from memory straight into
+// registers, all of a wave's loads of two blocks (four for up to 16 rows) before their
+// first product; a, read by every workgroup, comes from the caches.
 template <typename T, int MT, int W>
 __device__ void matmul_rows(const HelixMatmulParams& p) {
     __shared__ float sum[W][MT * 16][17];
     const int lane = lane_id(), wave = wave_uniform(), lo = lane & 15, kq = lane >> 4;
     const int j0 = blockIdx.x * 16, i0 = blockIdx.y * 16 * MT;
     const int nkb = (p.k + 127) >> 7, each = (nkb + W - 1) / W;
-    const int first = wave * each, last = min(first + each, nkb);
+    const int first = wave * each, last = min(first + each, nkb), whole = min(last, p.k >> 7);
     const long long rb = min(j0 + lo, p.n - 1);
     const uint8_t* b = p.b + rb * p.ld_b;
     const uint8_t* eb = p.b_scale + rb * p.ld_b_scale;
@@ -130,23 +131,53 @@ __device__ void matmul_rows(const HelixMatmulParams& p) {
     f32x4 acc[MT];
 #pragma unroll
     for (int t = 0; t < MT; ++t) acc[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    for (int kb = first; kb < last; ++kb) {
-        const i32x8 x = row_block(b, kb, kq, p.k);
-        const int ex = eb[kb];
+    auto block = [&](const uint8_t* row, int kb) {
+        const uint8_t* q = row + 128LL * kb + 16 * kq;
+        const i32x4 x = *reinterpret_cast<const i32x4*>(q), y = *reinterpret_cast<const i32x4*>(q + 64);
+        return __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
+    };
+    auto product = [&](int t, int kb, i32x8 x, i32x8 y, int ex, int ey) {
+        if constexpr (sizeof(T) == 4) {
+            const f32x4 s = block_sum(x, y);
 #pragma unroll
-        for (int t = 0; t < MT; ++t) {
-            const i32x8 y = row_block(a[t], kb, kq, p.k);
-            if constexpr (sizeof(T) == 4) {
-                const f32x4 s = block_sum(x, y);
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const long long row = min(j0 + 4 * kq + r, p.n - 1);
-                    acc[t][r] += scaled(s[r], p.b_scale[row * p.ld_b_scale + kb], ea[t][kb]);
-                }
-            } else {
-                acc[t] = mfma_fp8(x, y, acc[t], ex, ea[t][kb]);
+            for (int r = 0; r < 4; ++r) {
+                const long long row = min(j0 + 4 * kq + r, p.n - 1);
+                acc[t][r] += scaled(s[r], p.b_scale[row * p.ld_b_scale + kb], ey);
             }
+        } else {
+            acc[t] = mfma_fp8(x, y, acc[t], ex, ey);
         }
+    };
+    auto blocks = [&](auto count, int kb) {
+        constexpr int N = decltype(count)::value;
+        i32x8 x[N], y[N][MT];
+        int ex[N], ey[N][MT];
+#pragma unroll
+        for (int u = 0; u < N; ++u) {
+            x[u] = block(b, kb + u);
+            ex[u] = eb[kb + u];
+        }
+#pragma unroll
+        for (int u = 0; u < N; ++u)
+#pragma unroll
+            for (int t = 0; t < MT; ++t) {
+                y[u][t] = block(a[t], kb + u);
+                ey[u][t] = ea[t][kb + u];
+            }
+#pragma unroll
+        for (int u = 0; u < N; ++u)
+#pragma unroll
+            for (int t = 0; t < MT; ++t) product(t, kb + u, x[u], y[u][t], ex[u], ey[u][t]);
+    };
+    int kb = first;
+    if constexpr (MT == 1)
+        for (; kb + 4 <= whole; kb += 4) blocks(std::integral_constant<int, 4>{}, kb);
+    for (; kb + 2 <= whole; kb += 2) blocks(std::integral_constant<int, 2>{}, kb);
+    if (kb < whole) blocks(std::integral_constant<int, 1>{}, kb++);
+    if (kb < last) {   // the block that k ends in
+        const i32x8 x = row_block(b, kb, kq, p.k);
+#pragma unroll
+        for (int t = 0; t < MT; ++t) product(t, kb, x, row_block(a[t], kb, kq, p.k), eb[kb], ea[t][kb]);
     }
     // Register r of a lane: row 4 kq + r of b, row lo of a's tile.
 #pragma unroll
@@ -243,7 +274,7 @@ HELIX_DEV void repeat(F&& f) {
     }
 }
 
-template <int TM, int TN>
+template <int TM, int TN, bool PARTS>
 __device__ void matmul_tiles(const HelixMatmulParams& p) {
     constexpr int BN = 32 * TM, BM = 32 * TN, ROWS = BN + BM, STAGE = ROWS * 128, SLOT = ROWS * 4;
     constexpr int NX = BN / 32, NY = BM / 32;      // loads of a wave in a stage: 8 rows each
@@ -251,7 +282,10 @@ __device__ void matmul_tiles(const HelixMatmulParams& p) {
     __shared__ __attribute__((aligned(1024))) uint8_t lds[2 * STAGE + 4 * SLOT];
     const int lane = lane_id(), wave = wave_uniform();
     const int mt = (p.m + BM - 1) / BM, nt = (p.n + BN - 1) / BN, tiles = mt * nt;
-    const int nkb = (p.k + 127) >> 7, ngr = (nkb + 3) >> 2;
+    // This workgroup's stretch of the sum: all of it, or (PARTS) the blocks of part blockIdx.y.
+    const int k0 = PARTS ? blockIdx.y * p.part_blocks : 0;
+    const int k = PARTS ? ((int)blockIdx.y + 1 < p.parts ? (k0 + p.part_blocks) * 128 : p.k) - k0 * 128 : p.k;
+    const int nkb = (k + 127) >> 7, ngr = (nkb + 3) >> 2;
     // Tiles go down columns of GM tiles, a column beside the other, band by band: what runs on an XCD at a time shares rows of
     // both matrices. Divisions by products with reciprocals of the host's (mulhi of x with 2^32 / d + 1).
     auto tile_at = [&](int t) {
@@ -279,14 +313,14 @@ __device__ void matmul_tiles(const HelixMatmulParams& p) {
     // Rows and columns past the matrices are out of the resources' range and come as zeros.
     auto aim_data = [&](int t) {
         const TileAt at = tile_at(t);
-        const int k16 = (p.k + 15) & ~15;
-        rx = lds_rsrc(p.b + at.j * p.ld_b, (min(BN, p.n - at.j) - 1) * p.ld_b + k16);
-        ry = lds_rsrc(p.a + at.i * p.ld_a, (min(BM, p.m - at.i) - 1) * p.ld_a + k16);
+        const int k16 = (k + 15) & ~15;
+        rx = lds_rsrc(p.b + at.j * p.ld_b + k0 * 128, (min(BN, p.n - at.j) - 1) * p.ld_b + k16);
+        ry = lds_rsrc(p.a + at.i * p.ld_a + k0 * 128, (min(BM, p.m - at.i) - 1) * p.ld_a + k16);
     };
     auto aim_scales = [&](int t) {
         const TileAt at = tile_at(t);
-        rsx = lds_rsrc(p.b_scale + at.j * p.ld_b_scale, (min(BN, p.n - at.j) - 1) * p.ld_b_scale + 4 * ngr);
-        rsy = lds_rsrc(p.a_scale + at.i * p.ld_a_scale, (min(BM, p.m - at.i) - 1) * p.ld_a_scale + 4 * ngr);
+        rsx = lds_rsrc(p.b_scale + at.j * p.ld_b_scale + k0, (min(BN, p.n - at.j) - 1) * p.ld_b_scale + 4 * ngr);
+        rsy = lds_rsrc(p.a_scale + at.i * p.ld_a_scale + k0, (min(BM, p.m - at.i) - 1) * p.ld_a_scale + 4 * ngr);
     };
     // a row's 16-byte chunk c is kept at c ^ (what its row's number says)
 #pragma unroll
@@ -364,7 +398,7 @@ __device__ void matmul_tiles(const HelixMatmulParams& p) {
 
     int buf = 0, slot = 0;   // of the step at hand
     // A last block that k ends in: clears what a lane's 32 bytes (16 fq on, and 64 + 16 fq on) hold past it.
-    const int kt = p.k & 127;
+    const int kt = k & 127;
     auto cut = [&](i32x8& w) {
 #pragma unroll
         for (int d = 0; d < 8; ++d) {
@@ -489,34 +523,73 @@ __device__ void matmul_tiles(const HelixMatmulParams& p) {
         // Every store is issued, whatever its lanes may write: the waits of the next steps count them.
         const TileAt at = tile_at(t);
         const int left_n = p.n - at.j, left_m = p.m - at.i;
-        const helix_rsrc rc =
-            make_rsrc_u(static_cast<uint16_t*>(p.c) + at.i * p.ld_c + at.j,
-                        (unsigned)(((min(left_m, BM) - 1) * p.ld_c + min(left_n, BN)) * 2));
-        const int ldc = (int)p.ld_c * 2;
+        if constexpr (PARTS) {   // one tile a workgroup
+            const long long pitch = (p.n + 3) & ~3;
+            const helix_rsrc rp = make_rsrc_u(p.part + ((long long)blockIdx.y * p.m + at.i) * pitch + at.j,
+                                              (unsigned)(((min(left_m, BM) - 1) * pitch + min((left_n + 3) & ~3, BN)) * 4));
 #pragma unroll
-        for (int j = 0; j < TN; ++j) {
-            const int row = (wy + 16 * j + vgpr_fresh(fr)) * ldc;
+            for (int j = 0; j < TN; ++j)
 #pragma unroll
-            for (int i = 0; i < TM; i += 2) {
-                const int col = wx + 16 * i + 8 * vgpr_fresh(fq);
-                const f32x4 u = acc[i][j], v = acc[i + 1][j];
-                u32x4 w;
-                if (p.f16) w = u32x4{narrow2<_Float16>(u[0], u[1]), narrow2<_Float16>(u[2], u[3]), narrow2<_Float16>(v[0], v[1]), narrow2<_Float16>(v[2], v[3])};
-                else w = u32x4{narrow2<__bf16>(u[0], u[1]), narrow2<__bf16>(u[2], u[3]), narrow2<__bf16>(v[0], v[1]), narrow2<__bf16>(v[2], v[3])};
-                if (p.wide) {
-                    __builtin_amdgcn_raw_buffer_store_b128(w, rc, col < left_n ? row + 2 * col : (int)0x80000000, 0, 0);
-                } else {
+                for (int i = 0; i < TM; ++i) {
+                    const int col = wx + 32 * (i >> 1) + 8 * fq + 4 * (i & 1);
+                    const f32x4 u = acc[i][j];
+                    __builtin_amdgcn_raw_buffer_store_b128(u32x4{as_u32(u[0]), as_u32(u[1]), as_u32(u[2]), as_u32(u[3])}, rp,
+                                                           col < left_n ? ((wy + 16 * j + fr) * (int)pitch + col) * 4 : (int)0x80000000, 0, 0);
+                }
+        } else {
+            const helix_rsrc rc =
+                make_rsrc_u(static_cast<uint16_t*>(p.c) + at.i * p.ld_c + at.j,
+                            (unsigned)(((min(left_m, BM) - 1) * p.ld_c + min(left_n, BN)) * 2));
+            const int ldc = (int)p.ld_c * 2;
 #pragma unroll
-                    for (int r = 0; r < 8; ++r)
-                        __builtin_amdgcn_raw_buffer_store_b16((unsigned short)(w[r >> 1] >> (16 * (r & 1))), rc,
-                                                              col + r < left_n ? row + 2 * (col + r) : (int)0x80000000, 0, 0);
+            for (int j = 0; j < TN; ++j) {
+                const int row = (wy + 16 * j + vgpr_fresh(fr)) * ldc;
+#pragma unroll
+                for (int i = 0; i < TM; i += 2) {
+                    const int col = wx + 16 * i + 8 * vgpr_fresh(fq);
+                    const f32x4 u = acc[i][j], v = acc[i + 1][j];
+                    u32x4 w;
+                    if (p.f16) w = u32x4{narrow2<_Float16>(u[0], u[1]), narrow2<_Float16>(u[2], u[3]), narrow2<_Float16>(v[0], v[1]), narrow2<_Float16>(v[2], v[3])};
+                    else w = u32x4{narrow2<__bf16>(u[0], u[1]), narrow2<__bf16>(u[2], u[3]), narrow2<__bf16>(v[0], v[1]), narrow2<__bf16>(v[2], v[3])};
+                    if (p.wide) {
+                        __builtin_amdgcn_raw_buffer_store_b128(w, rc, col < left_n ? row + 2 * col : (int)0x80000000, 0, 0);
+                    } else {
+#pragma unroll
+                        for (int r = 0; r < 8; ++r)
+                            __builtin_amdgcn_raw_buffer_store_b16((unsigned short)(w[r >> 1] >> (16 * (r & 1))), rc,
+                                                                  col + r < left_n ? row + 2 * (col + r) : (int)0x80000000, 0, 0);
+                    }
                 }
             }
-        }
+            }
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 }
+// c from the parts of a divided sum, added in their order: four columns a thread.
+template <typename T>
+__device__ void matmul_join(const HelixMatmulParams& p) {
+    const int quads = (p.n + 3) >> 2;
+    const long long i = (long long)blockIdx.x * 256 + threadIdx.x, row = i / quads;
+    if (row >= p.m) return;
+    const int col = 4 * (int)(i % quads);
+    const f32x4* q = reinterpret_cast<const f32x4*>(p.part) + i;
+    f32x4 s = q[0];
+    for (int k = 1; k < p.parts; ++k) s += q[(long long)k * p.m * quads];
+    T* c = static_cast<T*>(p.c) + row * p.ld_c + col;
+    const float v[4] = {s[0], s[1], s[2], s[3]};
+    if (p.wide) {
+        *reinterpret_cast<typename Raw4<T>::type*>(c) = narrow4<T>(v);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (col + e < p.n) c[e] = (T)v[e];
+    }
+}
+
 }  // namespace
+
+extern "C" __global__ __launch_bounds__(256) void helix_matmul_fp8_join_f16(HelixMatmulParams p) { matmul_join<_Float16>(p); }
+extern "C" __global__ __launch_bounds__(256) void helix_matmul_fp8_join_bf16(HelixMatmulParams p) { matmul_join<__bf16>(p); }
 
 // Scales into rows of `pitch` bytes, a multiple of four, for the tiles' loads.
 extern "C" __global__ __launch_bounds__(256) void helix_fp8_scales(const uint8_t* from, uint8_t* to, long long ld,
@@ -527,25 +600,28 @@ extern "C" __global__ __launch_bounds__(256) void helix_fp8_scales(const uint8_t
     if (row < rows) to[i] = c < blocks ? from[row * ld + c] : 0;
 }
 
-#define MATMUL_TILES(TM, TN, BOUND)                                                                           \
-    extern "C" __global__ __launch_bounds__(256, BOUND) void helix_matmul_fp8_t##TM##TN(HelixMatmulParams p) { \
-        matmul_tiles<TM, TN>(p);                                                                              \
+#define MATMUL_TILES(NAME, TM, TN, PARTS, BOUND)                                                                \
+    extern "C" __global__ __launch_bounds__(256, BOUND) void helix_matmul_fp8_##NAME(HelixMatmulParams p) {     \
+        matmul_tiles<TM, TN, PARTS>(p);                                                                         \
     }
-MATMUL_TILES(8, 8, 1)
-MATMUL_TILES(8, 6, 1)
-MATMUL_TILES(8, 4, 1)
-MATMUL_TILES(4, 4, 2)
-MATMUL_TILES(4, 2, 2)
+MATMUL_TILES(t88, 8, 8, false, 1)
+MATMUL_TILES(t86, 8, 6, false, 1)
+MATMUL_TILES(t84, 8, 4, false, 1)
+MATMUL_TILES(t44, 4, 4, false, 2)
+MATMUL_TILES(t42, 4, 2, false, 2)
+MATMUL_TILES(t44p, 4, 4, true, 2)
+MATMUL_TILES(t42p, 4, 2, true, 2)
 
-#define MATMUL_ROWS(TAG, T, MT)                                                                              \
-    extern "C" __global__ __launch_bounds__(512) void helix_matmul_fp8_##TAG##_r##MT(HelixMatmulParams p) {  \
-        matmul_rows<T, MT, 8>(p);                                                                            \
+#define MATMUL_ROWS(TAG, T, MT, W)                                                                               \
+    extern "C" __global__ __launch_bounds__(64 * W) void helix_matmul_fp8_##TAG##_r##MT(HelixMatmulParams p)     { \
+        matmul_rows<T, MT, W>(p);                                                                                \
     }
 #define MATMUL_KERNELS(TAG, T)                                                                               \
-    MATMUL_ROWS(TAG, T, 1)                                                                                   \
-    MATMUL_ROWS(TAG, T, 2)                                                                                   \
-    MATMUL_ROWS(TAG, T, 4)                                                                                   \
-    MATMUL_ROWS(TAG, T, 8)                                                                                   \
+    MATMUL_ROWS(TAG, T, 1, 8)                                                                                \
+    extern "C" __global__ __launch_bounds__(256) void helix_matmul_fp8_##TAG##_r1w4(HelixMatmulParams p) { matmul_rows<T, 1, 4>(p); } \
+    MATMUL_ROWS(TAG, T, 2, 8)                                                                                \
+    MATMUL_ROWS(TAG, T, 3, 8)                                                                                \
+    MATMUL_ROWS(TAG, T, 4, 8)                                                                                \
     extern "C" __global__ __launch_bounds__(64) void helix_matmul_fp8_##TAG##_any(HelixMatmulParams p) {     \
         matmul_tile<T>(p);                                                                                   \
     }

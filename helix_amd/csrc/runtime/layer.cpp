@@ -4,6 +4,7 @@
 #include <algorithm>
 #include <cmath>
 #include <cstdint>
+#include <cstdlib>
 #include <exception>
 #include <string>
 
@@ -263,10 +264,13 @@ namespace {
 
 // How a product is computed (kernels/matmul_fp8.hip).
 struct MatmulPlan {
-    const char* kernel = "_any";
-    int rows = 0;                            // > 0: rows of a that a workgroup takes at once
-    int bm = 0, bn = 0, per_cu = 1;          // > 0: tiles
+    std::string kernel = "_any";
+    int rows = 0, waves = 8;                      // > 0: rows of a that a workgroup takes at once, and its waves
+    int bm = 0, bn = 0, per_cu = 1;               // > 0: tiles
+    int parts = 1, part_blocks = 0;               // of the sum, of which each tile has a workgroup each
     size_t pitch = 0, a_bytes = 0, b_bytes = 0;   // copies of the scales, in scratch
+    size_t part_bytes = 0;                        // and the parts, after them
+    size_t bytes() const { return a_bytes + b_bytes + part_bytes; }
 };
 
 struct Tiling {
@@ -280,37 +284,60 @@ const Tiling kTilings[] = {
     {"_t88", 256, 256, 1, 1.38, 6.4}, {"_t86", 192, 256, 1, 1.04, 6.4}, {"_t84", 128, 256, 1, 0.93, 2.2},
     {"_t44", 128, 128, 2, 1.10, 1.5}, {"_t42", 64, 128, 2, 0.75, 1.2},
 };
+// A step of a workgroup that has a CU to itself: the way of a load, which goes one and a half steps ahead. And a launch.
+constexpr double kLoneStep = 0.36, kLaunch = 2.5;
 
 MatmulPlan matmul_plan(const helix_matmul_fp8_args& a) {
     MatmulPlan p;
-    const long long blocks = ceil_div(a.k, HELIX_FP8_BLOCK);
-    // Few rows: b's bytes are what counts, and every wave reads all of a.
-    if (a.m <= 128) {
-        p.rows = a.m <= 16 ? 16 : a.m <= 32 ? 32 : a.m <= 64 ? 64 : 128;
-        p.kernel = a.m <= 16 ? "_r1" : a.m <= 32 ? "_r2" : a.m <= 64 ? "_r4" : "_r8";
-        return p;
+    const long long m = a.m, n = a.n, k = a.k, blocks = ceil_div(k, HELIX_FP8_BLOCK);
+    double best = 1e30;
+    // Rows: 4 us and 8 TB/s of what workgroups read, b once for each 64 rows of a and a for each 16 of b (17, 33 and 67 rows
+    // of 2048 x 4096: 7.5, 9.8, 11.6 us; of 10304 x 2048: 9.6, 13.0, 23.0).
+    if (m <= 128) {
+        const long long tiles = ceil_div(m, 16), ny = ceil_div(tiles, 4), each = ceil_div(tiles, ny);
+        p.rows = (int)(16 * each);
+        p.kernel = "_r" + std::to_string(each);
+        if (each == 1 && n >= 8192) p.kernel = "_r1w4", p.waves = 4;   // (10304 x 2048: 7.0 -> 6.3 us)
+        best = 4 + (double)ceil_div(n, 16) * k * 16 * (ny + tiles) / 8e6;
+        if (m <= 16) return p;
     }
     // The tiles' loads and stores reach a tile's rows by 32-bit offsets, and their loop is four steps long at least. fp32
     // results do not come from its instruction.
     const long long reach = (1LL << 31) / 256 / 2;
     if (a.out_dtype == HELIX_F32 || blocks < 4 || a.ld_a >= reach || a.ld_b >= reach || a.ld_c >= reach / 2 ||
-        a.ld_a_scale >= reach || a.ld_b_scale >= reach)
+        a.ld_a_scale >= reach || a.ld_b_scale >= reach || n >= reach / 4)
         return p;
-    double best = 0;
+    const MatmulPlan rows = p;
     for (const Tiling& t : kTilings) {
-        const long long tiles = ceil_div(a.m, t.bm) * ceil_div(a.n, t.bn);
-        const double us = ceil_div(tiles, 256 * t.per_cu) * (blocks * t.step + t.tile);
-        if (p.bm && us >= best) continue;
-        best = us;
-        p.kernel = t.kernel;
-        p.bm = t.bm;
-        p.bn = t.bn;
-        p.per_cu = t.per_cu;
+        const long long tiles = ceil_div(m, t.bm) * ceil_div(n, t.bn), slots = 256 * t.per_cu;
+        // The sum in parts (groups of four blocks) where small tiles leave CUs without work: another launch adds them up
+        // (67 and 256 rows of 2048 x 4096 in eight parts 12.5 and 21.5 us, in one 13.0 and 15.1; 67 of 2560 x 5120 in six
+        // 15.0, in one 17.6).
+        const long long most = t.bn > 128 ? 1 : std::max(1LL, slots / tiles);
+        for (long long each = blocks; each >= 4; each = each == blocks ? (blocks - 1) / 4 * 4 : each - 4) {
+            const long long rest = blocks % each, s = blocks / each + (rest >= 4), steps = rest && rest < 4 ? each + rest : each;
+            if (s > most) break;
+            const double busy = std::min(1.0, (double)tiles * s / slots);
+            double us = kLaunch + ceil_div(tiles, slots) * (steps * std::max(t.step * busy, kLoneStep) + t.tile);
+            if (s > 1) us += 5 + 4.0 * m * n * (s + 1) / 2e6;
+            if (us >= best) continue;
+            best = us;
+            p = MatmulPlan{};
+            p.kernel = std::string(t.kernel) + (s > 1 ? "p" : "");
+            p.bm = t.bm;
+            p.bn = t.bn;
+            p.per_cu = t.per_cu;
+            p.parts = (int)s;
+            p.part_blocks = s > 1 ? (int)each : (int)blocks;
+        }
     }
+    if (!p.bm) return rows;
+    auto up = [](size_t bytes) { return (bytes + 255) & ~(size_t)255; };
     p.pitch = (size_t)ceil_div(blocks, 4) * 4;
     // Scales are loaded as words of four.
-    if (a.ld_a_scale % 4 || !aligned(a.a_scale, 4)) p.a_bytes = ((size_t)a.m * p.pitch + 255) & ~(size_t)255;
-    if (a.ld_b_scale % 4 || !aligned(a.b_scale, 4)) p.b_bytes = ((size_t)a.n * p.pitch + 255) & ~(size_t)255;
+    if (a.ld_a_scale % 4 || !aligned(a.a_scale, 4)) p.a_bytes = up((size_t)m * p.pitch);
+    if (a.ld_b_scale % 4 || !aligned(a.b_scale, 4)) p.b_bytes = up((size_t)n * p.pitch);
+    if (p.parts > 1) p.part_bytes = (size_t)p.parts * m * ((n + 3) & ~3LL) * 4;
     return p;
 }
 
@@ -322,7 +349,7 @@ unsigned reciprocal(unsigned d) { return d > 1 ? (unsigned)((1ULL << 32) / d + 1
 extern "C" size_t helix_matmul_fp8_scratch_size(const helix_matmul_fp8_args* a) {
     if (!a || a->m <= 0 || a->n <= 0 || a->k <= 0) return 0;
     const MatmulPlan p = matmul_plan(*a);
-    return p.a_bytes + p.b_bytes;
+    return p.bytes();
 }
 
 extern "C" helix_status helix_matmul_fp8_encode(helix_ctx* ctx, void* stream, const helix_matmul_fp8_args* a) {
@@ -341,7 +368,7 @@ extern "C" helix_status helix_matmul_fp8_encode(helix_ctx* ctx, void* stream, co
         need((a->m == 1 || a->ld_a % 16 == 0) && (a->n == 1 || a->ld_b % 16 == 0),
              "ld_a and ld_b have to be multiples of 16");
         const MatmulPlan plan = matmul_plan(*a);
-        need(a->scratch_bytes >= plan.a_bytes + plan.b_bytes && (a->scratch || !(plan.a_bytes + plan.b_bytes)),
+        need(a->scratch_bytes >= plan.bytes() && (a->scratch || !plan.bytes()),
              "scratch smaller than helix_matmul_fp8_scratch_size()", HELIX_ERR_SCRATCH_TOO_SMALL);
         need(aligned(a->scratch, 16), "scratch is not 16-byte aligned");
         HelixMatmulParams p{};
@@ -364,7 +391,7 @@ extern "C" helix_status helix_matmul_fp8_encode(helix_ctx* ctx, void* stream, co
         if (plan.rows) {
             const unsigned gx = grid(ceil_div(a->n, 16)), gy = (unsigned)ceil_div(a->m, plan.rows);
             const OnDevice on(ctx->device);
-            launch(f, stream, gx, gy, 512, p);
+            launch(f, stream, gx, gy, 64 * plan.waves, p);
             return;
         }
         if (!plan.bm) {
@@ -387,7 +414,9 @@ extern "C" helix_status helix_matmul_fp8_encode(helix_ctx* ctx, void* stream, co
         p.f16 = a->out_dtype == HELIX_F16;
         p.wide = a->n % 8 == 0 && a->ld_c % 8 == 0 && aligned(a->c, 16);
         const unsigned ga = grid(ceil_div((long long)a->m * plan.pitch, 256)), gb = grid(ceil_div((long long)a->n * plan.pitch, 256));
-        const hipFunction_t copy = kernel(ctx, "helix_fp8_scales");
+        const unsigned gj = grid(ceil_div((long long)a->m * ceil_div(a->n, 4), 256));
+        const hipFunction_t copy = kernel(ctx, "helix_fp8_scales"),
+                            join = kernel(ctx, std::string("helix_matmul_fp8_join_") + kTags[a->out_dtype]);
         const OnDevice on(ctx->device);
         auto repack = [&](const uint8_t*& scale, long long& ld, long long rows, uint8_t* to, unsigned gx) {
             int nb = (int)blocks, pitch = (int)plan.pitch;
@@ -398,7 +427,13 @@ extern "C" helix_status helix_matmul_fp8_encode(helix_ctx* ctx, void* stream, co
         };
         if (plan.a_bytes) repack(p.a_scale, p.ld_a_scale, a->m, static_cast<uint8_t*>(a->scratch), ga);
         if (plan.b_bytes) repack(p.b_scale, p.ld_b_scale, a->n, static_cast<uint8_t*>(a->scratch) + plan.a_bytes, gb);
-        launch(f, stream, (unsigned)p.stride, 1, 256, p);
+        p.parts = plan.parts;
+        p.part_blocks = plan.part_blocks;
+        p.part = plan.parts > 1 ? reinterpret_cast<float*>(static_cast<uint8_t*>(a->scratch) + plan.a_bytes + plan.b_bytes) : nullptr;
+        launch(f, stream, (unsigned)p.stride, (unsigned)plan.parts, 256, p);
+        if (plan.parts == 1) return;
+        p.wide = a->n % 4 == 0 && a->ld_c % 4 == 0 && aligned(a->c, 8);
+        launch(join, stream, gj, 1, 256, p);
     });
 }
 
@@ -587,7 +622,8 @@ namespace helix::rt {
 
 const std::vector<std::string>& layer_kernel_names() {
     static const std::vector<std::string> names = [] {
-        std::vector<std::string> v{"helix_norm_dw", "helix_fp8_scales", "helix_gated_scan_fill"};
+        std::vector<std::string> v{"helix_norm_dw", "helix_fp8_scales", "helix_matmul_fp8_join_f16",
+                                   "helix_matmul_fp8_join_bf16", "helix_gated_scan_fill"};
         for (const char* t : kTags)
             for (const char* k : {"helix_norm_", "helix_norm_bwd_", "helix_norm_dw_part_"})
                 v.push_back(std::string(k) + t);
@@ -598,8 +634,10 @@ const std::vector<std::string>& layer_kernel_names() {
                 if (n[0] <= '2') v.push_back(std::string("helix_norm_bwd_") + tag + "_w" + n);
             }
         for (const char* tag : kTags)
-            for (const char* k : {"_any", "_r1", "_r2", "_r4", "_r8"}) v.push_back(std::string("helix_matmul_fp8_") + tag + k);
+            for (const char* k : {"_any", "_r1", "_r1w4", "_r2", "_r3", "_r4"})
+                v.push_back(std::string("helix_matmul_fp8_") + tag + k);
         for (const Tiling& t : kTilings) v.push_back(std::string("helix_matmul_fp8") + t.kernel);
+        for (const char* k : {"_t44p", "_t42p"}) v.push_back(std::string("helix_matmul_fp8") + k);
         for (const char* t : kTags)
             for (const char* k : {"helix_gated_scan_", "helix_gated_scan_bwd_"})
                 for (const char* x : {"_v_", "_s_"})

@@ -268,4 +268,4 @@ def test_tiles_assembly_waits_for_its_operands():
         kernels += 1
         lines = [re.sub(r"\s+", " ", ln.split("//")[0]).strip() for ln in block.splitlines()[1:]]
         assert _missing_waits([ln for ln in lines if ln]) == [], name.group(1)
-    assert kernels == 5
+    assert kernels == 7
