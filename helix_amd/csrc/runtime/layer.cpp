@@ -4,7 +4,6 @@
 #include <algorithm>
 #include <cmath>
 #include <cstdint>
-#include <cstdlib>
 #include <exception>
 #include <string>
 
@@ -264,7 +263,7 @@ namespace {
 
 // How a product is computed (kernels/matmul_fp8.hip).
 struct MatmulPlan {
-    std::string kernel = "_any";
+    std::string kernel = "_blocks";
     int rows = 0, waves = 8;                      // > 0: rows of a that a workgroup takes at once, and its waves
     int bm = 0, bn = 0, per_cu = 1;               // > 0: tiles
     int parts = 1, part_blocks = 0;               // of the sum, of which each tile has a workgroup each
@@ -395,9 +394,10 @@ extern "C" helix_status helix_matmul_fp8_encode(helix_ctx* ctx, void* stream, co
             return;
         }
         if (!plan.bm) {
-            const unsigned gx = grid(ceil_div(a->m, 16) * ceil_div(a->n, 16));
+            const unsigned gx = grid(ceil_div(a->m, 64) * ceil_div(a->n, 128));
+            p.wide = a->n % 4 == 0 && a->ld_c % 4 == 0 && aligned(a->c, 16);
             const OnDevice on(ctx->device);
-            launch(f, stream, gx, 1, 64, p);
+            launch(f, stream, gx, 1, 256, p);
             return;
         }
         const long long mt = ceil_div(a->m, plan.bm), nt = ceil_div(a->n, plan.bn), tiles = mt * nt;
@@ -634,7 +634,7 @@ const std::vector<std::string>& layer_kernel_names() {
                 if (n[0] <= '2') v.push_back(std::string("helix_norm_bwd_") + tag + "_w" + n);
             }
         for (const char* tag : kTags)
-            for (const char* k : {"_any", "_r1", "_r1w4", "_r2", "_r3", "_r4"})
+            for (const char* k : {"_blocks", "_r1", "_r1w4", "_r2", "_r3", "_r4"})
                 v.push_back(std::string("helix_matmul_fp8_") + tag + k);
         for (const Tiling& t : kTilings) v.push_back(std::string("helix_matmul_fp8") + t.kernel);
         for (const char* k : {"_t44p", "_t42p"}) v.push_back(std::string("helix_matmul_fp8") + k);

@@ -48,8 +48,36 @@ def test_rows(gpu, m, n, k):
 
 @pytest.mark.parametrize("m,n,k", [(1, 10304, 2048), (3, 2048, 4096), (16, 5184, 2000), (67, 2048, 4096),
                                    (300, 4104, 656), (1024, 1024, 512), (1500, 2600, 384), (2048, 2047, 256)])
-def test_larger(gpu, m, n, k):
-    check(*operands(m, n, k, seed=1))
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_larger(gpu, m, n, k, dtype):
+    check(*operands(m, n, k, seed=1), dtype)
+
+
+@pytest.mark.parametrize("m,n,k", [(40, 2048, 4096), (67, 2560, 5120), (100, 130, 9000), (150, 640, 2900)])
+def test_sum_in_parts(gpu, m, n, k):
+    check(*operands(m, n, k, seed=8), torch.float16)
+    a, sa, b, sb = operands(m, n, k, seed=9)
+    assert torch.equal(check(a, sa, b, sb), matmul_fp8(a, sa, b, sb))
+
+
+# More tiles than workgroups run at once, a last band of one row of tiles, rows and columns past the last tile.
+@pytest.mark.parametrize("m,n,k,dtype", [(4400, 4200, 600, torch.bfloat16), (2060, 8210, 704, torch.float16),
+                                         (700, 1003, 640, torch.bfloat16), (4500, 4300, 1200, torch.bfloat16)])
+def test_many_tiles(gpu, m, n, k, dtype):
+    check(*operands(m, n, k, seed=11), dtype)
+
+
+def test_scales_of_any_alignment(gpu):
+    # Rows of five scale bytes, one after the other, and from an odd address.
+    m, n, k = 400, 300, 600
+    a, sa, b, sb = operands(m, n, k, seed=10)
+    want = check(a, sa, b, sb)
+    flat = torch.empty((m + n) * 5 + 1, dtype=torch.uint8, device="cuda").view(torch.float8_e8m0fnu)
+    ta, tb = flat[1:1 + 5 * m].view(m, 5), flat[1 + 5 * m:].view(n, 5)
+    ta.copy_(sa)
+    tb.copy_(sb)
+    assert torch.equal(matmul_fp8(a, ta, b, tb), want)
+    assert torch.equal(matmul_fp8(a, sa, b, tb), want) and torch.equal(matmul_fp8(a, ta, b, sb), want)
 
 
 def test_leading_dimensions_strides_and_out(gpu):
@@ -109,13 +137,14 @@ def test_every_code_and_wide_scales(gpu):
     check(a, sa, b, sb, torch.float32)
 
 
-@pytest.mark.parametrize("m", [1, 40, 300])
-def test_nan_stays_in_its_row(gpu, m):
-    a, sa, b, sb = operands(m, 140, 300, seed=3)
-    want = matmul_fp8(a, sa, b, sb)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("m,k", [(1, 300), (40, 300), (300, 300), (300, 700), (50, 3000)])
+def test_nan_stays_in_its_row(gpu, m, k, dtype):
+    a, sa, b, sb = operands(m, 140, k, seed=3)
+    want = matmul_fp8(a, sa, b, sb, out_dtype=dtype)
     a.view(torch.uint8)[0, 299] = 0x7f
     sb.view(torch.uint8)[7, 1] = 255
-    got = matmul_fp8(a, sa, b, sb)
+    got = matmul_fp8(a, sa, b, sb, out_dtype=dtype)
     assert torch.isnan(got[0]).all() and torch.isnan(got[:, 7]).all()
     keep = torch.arange(140, device="cuda") != 7
     assert torch.equal(got[1:, keep], want[1:, keep])
@@ -127,7 +156,7 @@ def test_empty(gpu):
     assert matmul_fp8(a, sa, b[:0], sb[:0]).shape == (4, 0)
 
 
-@pytest.mark.parametrize("m", [1, 200, 600])
+@pytest.mark.parametrize("m", [1, 40, 200, 600])
 def test_other_stream_and_graph(gpu, m):
     a, sa, b, sb = operands(m, 300, 2048, seed=4)
     want = matmul_fp8(a, sa, b, sb)
