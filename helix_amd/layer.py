@@ -3,6 +3,8 @@ tensors, streams, scratch and errors. The arithmetic runs in the HIP kernels of 
 (include/helix/helix_layer.h)."""
 from __future__ import annotations
 
+import contextlib
+
 import torch
 
 from .abi import HelixError
@@ -56,13 +58,21 @@ def row_stride(name: str, t: torch.Tensor) -> int:
     return t.shape[-1] if ld is None else ld
 
 
+def rows_like(t: torch.Tensor) -> torch.Tensor:
+    """Uninitialised and contiguous, of t's shape and type."""
+    return torch.empty_like(t) if t.is_contiguous() else torch.empty(t.shape, dtype=t.dtype, device=t.device)
+
+
 def stream_handle(index: int, stream) -> int:
     return stream.cuda_stream if stream is not None else torch._C._cuda_getCurrentRawStream(index)
 
 
+_here = contextlib.nullcontext()
+
+
 def under(index: int, stream):
     """The context that outputs are allocated in, so that their memory is the stream's own."""
-    return _under(index, 0 if stream is None else stream.cuda_stream, stream)
+    return _here if stream is None else _under(index, stream.cuda_stream, stream)
 
 
 def scratch(index: int, st: int, stream, nbytes: int) -> torch.Tensor | None:

@@ -11,8 +11,8 @@ from __future__ import annotations
 import torch
 
 from . import abi
-from .layer import (FP8, FP8_BLOCK, FP8_SCALE, IO_DTYPES, device_index, expect, io_code, ptr, row_stride, run, scratch,
-                    stream_handle, under)
+from .layer import (FP8, FP8_BLOCK, FP8_SCALE, IO_DTYPES, device_index, expect, io_code, ptr, row_stride, rows_like, run,
+                    scratch, stream_handle, under)
 
 
 def _weight_code(weight: torch.Tensor, x: torch.Tensor) -> int:
@@ -54,11 +54,11 @@ def _norm(op, fn, x, weight, residual, eps, fp8, want_rstd, stream):
             expect("residual", residual, x.dtype, x.shape, x)
             ld_r = row_stride("residual", residual)
             if weight is not None:
-                h = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+                h = rows_like(x)
         if fp8:
             q, scale = fp8_rows(x.shape, x.device)
         else:
-            y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+            y = rows_like(x)
         if want_rstd:
             rstd = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
     pitch = -(-dim // 16) * 16
@@ -122,7 +122,7 @@ def rms_norm_backward(dy: torch.Tensor, h: torch.Tensor, weight: torch.Tensor, r
     w_code = _weight_code(weight, h)
     ld_dy, ld_h = row_stride("dy", dy), row_stride("h", h)
     with under(index, stream):
-        dx = torch.empty(h.shape, dtype=h.dtype, device=h.device)
+        dx = rows_like(h)
         dweight = torch.empty(dim, dtype=torch.float32, device=h.device)
     st = stream_handle(index, stream)
 
