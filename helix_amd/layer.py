@@ -19,10 +19,9 @@ FP8_BLOCK = 128
 
 
 def device_index(op: str, t: torch.Tensor) -> int:
-    dev = t.device
-    if dev.type != "cuda":
-        raise ValueError(f"{op} runs on a HIP device; got {dev}")
-    return dev.index if dev.index is not None else torch.cuda.current_device()
+    if not t.is_cuda:
+        raise ValueError(f"{op} runs on a HIP device; got {t.device}")
+    return t.get_device()
 
 
 def io_code(name: str, t: torch.Tensor) -> int:
@@ -33,7 +32,7 @@ def io_code(name: str, t: torch.Tensor) -> int:
 
 
 def expect(name: str, t: torch.Tensor, dtype: torch.dtype, shape, like: torch.Tensor) -> None:
-    if t.dtype != dtype or t.device != like.device:
+    if t.dtype != dtype or t.get_device() != like.get_device():
         raise ValueError(f"{name} must be {dtype} on {like.device}; got {t.dtype} on {t.device}")
     if t.shape != shape:
         raise ValueError(f"{name} must have shape {tuple(shape)}; got {tuple(t.shape)}")
@@ -58,9 +57,16 @@ def row_stride(name: str, t: torch.Tensor) -> int:
     return t.shape[-1] if ld is None else ld
 
 
-def rows_like(t: torch.Tensor) -> torch.Tensor:
-    """Uninitialised and contiguous, of t's shape and type."""
-    return torch.empty_like(t) if t.is_contiguous() else torch.empty(t.shape, dtype=t.dtype, device=t.device)
+def empty(shape, dtype: torch.dtype, device) -> torch.Tensor:
+    """Uninitialised. (Sizes one by one spare half of what torch.empty takes for a torch.Size.)"""
+    return torch.empty(*shape, dtype=dtype, device=device) if shape else torch.empty((), dtype=dtype, device=device)
+
+
+def rows_like(t: torch.Tensor, dtype: torch.dtype | None = None) -> torch.Tensor:
+    """Uninitialised and contiguous, of t's shape and, unless another is given, type."""
+    if t.is_contiguous():
+        return torch.empty_like(t, dtype=dtype)
+    return empty(t.shape, dtype or t.dtype, t.device)
 
 
 def stream_handle(index: int, stream) -> int:

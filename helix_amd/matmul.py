@@ -31,7 +31,7 @@ def matmul_fp8(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale:
         if out_dtype not in IO_DTYPES:
             raise ValueError(f"out_dtype must be float32, bfloat16 or float16; got {out_dtype}")
         with under(index, stream):
-            out = torch.empty((*lead, n), dtype=out_dtype, device=a.device)
+            out = torch.empty(*lead, n, dtype=out_dtype, device=a.device)
         ld_c = n
     else:
         if out.dtype not in IO_DTYPES:

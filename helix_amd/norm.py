@@ -11,7 +11,7 @@ from __future__ import annotations
 import torch
 
 from . import abi
-from .layer import (FP8, FP8_BLOCK, FP8_SCALE, IO_DTYPES, device_index, expect, io_code, ptr, row_stride, rows_like, run,
+from .layer import (FP8, FP8_BLOCK, FP8_SCALE, IO_DTYPES, device_index, empty, expect, io_code, ptr, row_stride, rows_like, run,
                     scratch, stream_handle, under)
 
 
@@ -20,7 +20,7 @@ def _weight_code(weight: torch.Tensor, x: torch.Tensor) -> int:
     if dtype != torch.float32 and dtype != x.dtype:
         raise ValueError(f"weight must be float32 or {x.dtype}; got {dtype}")
     expect("weight", weight, dtype, x.shape[-1:], x)
-    if weight.stride(0) != 1 and weight.shape[0] > 1:
+    if not weight.is_contiguous():
         raise ValueError("weight must be contiguous")
     return IO_DTYPES[dtype]
 
@@ -31,8 +31,9 @@ def fp8_rows(shape, device) -> tuple[torch.Tensor, torch.Tensor]:
     dim = shape[-1]
     blocks = -(-dim // FP8_BLOCK)
     pitch, s_pitch = -(-dim // 16) * 16, -(-blocks // 4) * 4
-    q = torch.empty((*shape[:-1], pitch), dtype=FP8, device=device)
-    scale = torch.empty((*shape[:-1], s_pitch), dtype=FP8_SCALE, device=device)
+    lead = shape[:-1]
+    q = torch.empty(*lead, pitch, dtype=FP8, device=device)
+    scale = torch.empty(*lead, s_pitch, dtype=FP8_SCALE, device=device)
     return q if pitch == dim else q[..., :dim], scale if s_pitch == blocks else scale[..., :blocks]
 
 
@@ -60,7 +61,7 @@ def _norm(op, fn, x, weight, residual, eps, fp8, want_rstd, stream):
         else:
             y = rows_like(x)
         if want_rstd:
-            rstd = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
+            rstd = empty(x.shape[:-1], torch.float32, x.device)
     pitch = -(-dim // 16) * 16
     args = abi.NORM_STRUCT.pack(x.numel() // dim, dim, io, w_code, eps, x.data_ptr(), ptr(residual), ptr(weight),
                                 0 if h is x else h.data_ptr(), ptr(y), ptr(q), ptr(scale), ptr(rstd), ld_x, ld_r, dim,

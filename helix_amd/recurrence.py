@@ -44,8 +44,8 @@ def gated_scan(g: torch.Tensor, v: torch.Tensor, h0: torch.Tensor | None = None,
     expect("v", v, g.dtype, g.shape, g)
     _state("h0", h0, g)
     with under(index, stream):
-        h = torch.empty((S, L, D), dtype=g.dtype, device=g.device)
-        last = torch.empty((S, D), dtype=torch.float32, device=g.device)
+        h = torch.empty(S, L, D, dtype=g.dtype, device=g.device)
+        last = torch.empty(S, D, dtype=torch.float32, device=g.device)
     st = stream_handle(index, stream)
     strides = (*_strides("g", g), *_strides("v", v), L * D, D)
 
@@ -73,9 +73,9 @@ def gated_scan_backward(dh: torch.Tensor, g: torch.Tensor, v: torch.Tensor, h: t
     _state("h0", h0, g)
     _state("dh_last", dh_last, g)
     with under(index, stream):
-        dg = torch.empty((S, L, D), dtype=g.dtype, device=g.device)
-        dv = torch.empty((S, L, D), dtype=g.dtype, device=g.device)
-        dh0 = torch.empty((S, D), dtype=torch.float32, device=g.device)
+        dg = torch.empty(S, L, D, dtype=g.dtype, device=g.device)
+        dv = torch.empty(S, L, D, dtype=g.dtype, device=g.device)
+        dh0 = torch.empty(S, D, dtype=torch.float32, device=g.device)
     st = stream_handle(index, stream)
     strides = (*_strides("dh", dh), *_strides("g", g), *_strides("v", v), *_strides("h", h), L * D, D, L * D, D)
 
