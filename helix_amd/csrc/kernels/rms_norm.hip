@@ -9,8 +9,13 @@
 // Accesses past a row's end are out of the resource's range: they read zeros, which add
 // nothing to a sum or a largest magnitude, and write nothing.
 //
-// Rows wider than that, or whose elements do not start at multiples of 16 bytes, go
-// through the forms below that read a row twice, element by element.
+// Rows that do not start at multiples of 16 bytes take the same way element by element
+// (8192 x 1001 in bf16 14 us where 8192 x 1024 take 11; in forms that read a row twice
+// 28). Only those wider than what registers hold go through the latter, below.
+//
+// 8192 x 2048 of bf16 with a residual into 8 bits: 21 us, 118 MB at 5.6 TB/s; 2871 x 5184
+// of f32 21 us, 5.7 TB/s; backward of 32768 x 2560 of bf16 145 us, 4.6 TB/s, as a copy
+// of 4 GiB (tensors that fit in the 256 MiB of cache go faster than those that do not).
 #include "layer_common.h"
 
 namespace {
@@ -39,14 +44,55 @@ HELIX_DEV helix_rsrc row_rsrc(const void* base, long long row, long long ld, int
     return make_rsrc_u(static_cast<const T*>(base) + row * ld, (unsigned)dim * (unsigned)sizeof(T));
 }
 
+// Chunk j of a lane's channels, eight of them from c on: neighbours (VEC), or in steps of
+// 64 in every W-th block of 128, where elements are moved one by one.
+template <int W, bool VEC>
+HELIX_DEV int first_channel(int j, int wave, int lane) {
+    if constexpr (VEC) return (W == 1 ? j : 4 * j + wave) * 512 + 8 * lane;
+    else return (4 * j * W + (W == 1 ? 0 : wave)) * HELIX_BLOCK + lane;
+}
+template <int W, bool VEC>
+HELIX_DEV int channel(int c, int i) {
+    return VEC ? c + i : c + (i >> 1) * W * HELIX_BLOCK + 64 * (i & 1);
+}
+template <typename T, int W, bool VEC>
+HELIX_DEV Raw8<T> load8(helix_rsrc r, int c) {
+    if constexpr (VEC) {
+        return buf_load8<T>(r, c * (int)sizeof(T));
+    } else {
+        Raw8<T> o;
+        if constexpr (sizeof(T) == 4) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                o.w[i >> 2][i & 3] = __builtin_amdgcn_raw_buffer_load_b32(r, channel<W, VEC>(c, i) * 4, 0, 0);
+        } else {
+            unsigned e[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) e[i] = (unsigned short)__builtin_amdgcn_raw_buffer_load_b16(r, channel<W, VEC>(c, i) * 2, 0, 0);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o.w[0][i] = e[2 * i] | e[2 * i + 1] << 16;
+        }
+        return o;
+    }
+}
+template <typename T, int W, bool VEC>
+HELIX_DEV void store8(helix_rsrc r, const float (&v)[8], int c) {
+    if constexpr (VEC) {
+        buf_store8<T>(r, v, c * (int)sizeof(T));
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) io_store<T, 0>(r, v[i], channel<W, VEC>(c, i) * (int)sizeof(T), 0);
+    }
+}
+
 // The weights of a lane's channels in fp32.
-template <typename T, int NC>
+template <typename T, int W, bool VEC, int NC>
 HELIX_DEV void load_weights(const void* w, int w_f32, int dim, const int (&c)[NC], float (&o)[NC][8]) {
     if (w_f32) {
         const helix_rsrc r = make_rsrc_u(w, dim * 4u);
 #pragma unroll
         for (int j = 0; j < NC; ++j) {
-            const Raw8<float> v = buf_load8<float>(r, c[j] * 4);
+            const Raw8<float> v = load8<float, W, VEC>(r, c[j]);
 #pragma unroll
             for (int i = 0; i < 8; ++i) o[j][i] = at8(v, i);
         }
@@ -54,7 +100,7 @@ HELIX_DEV void load_weights(const void* w, int w_f32, int dim, const int (&c)[NC
         const helix_rsrc r = make_rsrc_u(w, dim * (unsigned)sizeof(T));
 #pragma unroll
         for (int j = 0; j < NC; ++j) {
-            const Raw8<T> v = buf_load8<T>(r, c[j] * (int)sizeof(T));
+            const Raw8<T> v = load8<T, W, VEC>(r, c[j]);
 #pragma unroll
             for (int i = 0; i < 8; ++i) o[j][i] = at8(v, i);
         }
@@ -68,27 +114,26 @@ HELIX_DEV float row_sum(float v, float* red) {
     else return group_sum(v, red);
 }
 
-template <typename T, int W, int NC>
+template <typename T, int W, int NC, bool VEC>
 __device__ void norm_rows(const HelixNormParams& p) {
     __shared__ float red[NORM_THREADS / 64];
-    constexpr int ES = sizeof(T);
     const int lane = lane_id(), wave = wave_uniform();
     const long long row = W == 1 ? (long long)blockIdx.x * 4 + wave : blockIdx.x;
     if (W == 1 && row >= p.rows) return;
     int c[NC];
 #pragma unroll
-    for (int j = 0; j < NC; ++j) c[j] = (W == 1 ? j : 4 * j + wave) * 512 + 8 * lane;
+    for (int j = 0; j < NC; ++j) c[j] = first_channel<W, VEC>(j, wave, lane);
     Raw8<T> x[NC], r[NC];
     const helix_rsrc rx = row_rsrc<T>(p.x, row, p.ld_x, p.dim);
 #pragma unroll
-    for (int j = 0; j < NC; ++j) x[j] = buf_load8<T>(rx, c[j] * ES);
+    for (int j = 0; j < NC; ++j) x[j] = load8<T, W, VEC>(rx, c[j]);
     if (p.residual) {
         const helix_rsrc rr = row_rsrc<T>(p.residual, row, p.ld_residual, p.dim);
 #pragma unroll
-        for (int j = 0; j < NC; ++j) r[j] = buf_load8<T>(rr, c[j] * ES);
+        for (int j = 0; j < NC; ++j) r[j] = load8<T, W, VEC>(rr, c[j]);
     }
     float w[NC][8], v[NC][8];
-    if (p.weight) load_weights<T>(p.weight, p.w_f32, p.dim, c, w);
+    if (p.weight) load_weights<T, W, VEC>(p.weight, p.w_f32, p.dim, c, w);
     float ss = 0.0f;
 #pragma unroll
     for (int j = 0; j < NC; ++j)
@@ -103,7 +148,7 @@ __device__ void norm_rows(const HelixNormParams& p) {
     if (p.h) {
         const helix_rsrc rh = row_rsrc<T>(p.h, row, p.ld_h, p.dim);
 #pragma unroll
-        for (int j = 0; j < NC; ++j) buf_store8<T>(rh, v[j], c[j] * ES);
+        for (int j = 0; j < NC; ++j) store8<T, W, VEC>(rh, v[j], c[j]);
     }
     if (p.weight) {
 #pragma unroll
@@ -120,13 +165,26 @@ __device__ void norm_rows(const HelixNormParams& p) {
     if (p.y) {
         const helix_rsrc ry = row_rsrc<T>(p.y, row, p.ld_y, p.dim);
 #pragma unroll
-        for (int j = 0; j < NC; ++j) buf_store8<T>(ry, v[j], c[j] * ES);
+        for (int j = 0; j < NC; ++j) store8<T, W, VEC>(ry, v[j], c[j]);
         return;
     }
     const helix_rsrc rq = row_rsrc<uint8_t>(p.q, row, p.ld_q, p.dim);
     const helix_rsrc rs = row_rsrc<uint8_t>(p.scale, row, p.ld_scale, (p.dim + HELIX_BLOCK - 1) / HELIX_BLOCK);
 #pragma unroll
     for (int j = 0; j < NC; ++j) {
+        if constexpr (!VEC) {
+#pragma unroll
+            for (int i = 0; i < 8; i += 2) {   // a block of the wave's
+                const int e = block_exponent(wave_max(fmaxf(fabsf(v[j][i]), fabsf(v[j][i + 1]))));
+                const float inv = exponent_recip(e);
+                const int at = channel<W, VEC>(c[j], i);
+                const unsigned q = (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(v[j][i] * inv, v[j][i + 1] * inv, 0, false);
+                __builtin_amdgcn_raw_buffer_store_b8((unsigned char)q, rq, at, 0, 0);
+                __builtin_amdgcn_raw_buffer_store_b8((unsigned char)(q >> 8), rq, at + 64, 0, 0);
+                __builtin_amdgcn_raw_buffer_store_b8((unsigned char)e, rs, lane ? (int)0x80000000 : at >> 7, 0, 0);
+            }
+            continue;
+        }
         float top = 0.0f;
 #pragma unroll
         for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(v[j][i]));
@@ -145,17 +203,16 @@ __device__ void norm_rows(const HelixNormParams& p) {
 
 // dx, and dweight's sum over the rows of a part: a workgroup's, row by row in each of
 // its waves (W = 1) or in all of them (W = 4). The waves' sums are added in their order.
-template <typename T, int W, int NC>
+template <typename T, int W, int NC, bool VEC>
 __device__ void norm_bwd_rows(const HelixNormBwdParams& p) {
     __shared__ float red[2][NORM_THREADS / 64];
     __shared__ float sums[W == 1 ? 3 : 1][W == 1 ? NC * 512 : 1];
-    constexpr int ES = sizeof(T);
     const int lane = lane_id(), wave = wave_uniform();
     int c[NC];
 #pragma unroll
-    for (int j = 0; j < NC; ++j) c[j] = (W == 1 ? j : 4 * j + wave) * 512 + 8 * lane;
+    for (int j = 0; j < NC; ++j) c[j] = first_channel<W, VEC>(j, wave, lane);
     float w[NC][8], dw[NC][8];
-    load_weights<T>(p.weight, p.w_f32, p.dim, c, w);
+    load_weights<T, W, VEC>(p.weight, p.w_f32, p.dim, c, w);
 #pragma unroll
     for (int j = 0; j < NC; ++j)
 #pragma unroll
@@ -166,13 +223,13 @@ __device__ void norm_bwd_rows(const HelixNormBwdParams& p) {
         Raw8<T> dy[NC], h[NC], dh[NC];
         const helix_rsrc rd = row_rsrc<T>(p.dy, row, p.ld_dy, p.dim), rh = row_rsrc<T>(p.h, row, p.ld_h, p.dim);
 #pragma unroll
-        for (int j = 0; j < NC; ++j) dy[j] = buf_load8<T>(rd, c[j] * ES);
+        for (int j = 0; j < NC; ++j) dy[j] = load8<T, W, VEC>(rd, c[j]);
 #pragma unroll
-        for (int j = 0; j < NC; ++j) h[j] = buf_load8<T>(rh, c[j] * ES);
+        for (int j = 0; j < NC; ++j) h[j] = load8<T, W, VEC>(rh, c[j]);
         if (p.dh) {
             const helix_rsrc rg = row_rsrc<T>(p.dh, row, p.ld_dh, p.dim);
 #pragma unroll
-            for (int j = 0; j < NC; ++j) dh[j] = buf_load8<T>(rg, c[j] * ES);
+            for (int j = 0; j < NC; ++j) dh[j] = load8<T, W, VEC>(rg, c[j]);
         }
         const float rstd = p.rstd[row];
         float dot = 0.0f;
@@ -200,7 +257,7 @@ __device__ void norm_bwd_rows(const HelixNormBwdParams& p) {
 #pragma unroll
                 for (int i = 0; i < 8; ++i) o[i] += at8(dh[j], i);
             }
-            buf_store8<T>(rx, o, c[j] * ES);
+            store8<T, W, VEC>(rx, o, c[j]);
         }
     }
     if (!p.dweight) return;
@@ -222,7 +279,7 @@ __device__ void norm_bwd_rows(const HelixNormBwdParams& p) {
                 for (int o = 0; o < 3; ++o) dw[j][i] += sums[o][(j * 8 + i) * 64 + lane];
     }
 #pragma unroll
-    for (int j = 0; j < NC; ++j) buf_store8<float>(rp, dw[j], c[j] * 4);
+    for (int j = 0; j < NC; ++j) store8<float, W, VEC>(rp, dw[j], c[j]);
 }
 
 // One workgroup per row, which is read twice (the second time from the caches).
@@ -339,11 +396,11 @@ NORM_KERNELS(bf16, __bf16)
 
 #define NORM_FWD(TAG, T, KIND, W, NC)                                                                             \
     extern "C" __global__ __launch_bounds__(NORM_THREADS) void helix_norm_##TAG##_##KIND##NC(HelixNormParams p) { \
-        norm_rows<T, W, NC>(p);                                                                                   \
+        norm_rows<T, W, NC, #KIND[0] != 'e' && #KIND[0] != 'x'>(p);                                                                                   \
     }
 #define NORM_BWD(TAG, T, KIND, W, NC)                                                                                    \
     extern "C" __global__ __launch_bounds__(NORM_THREADS) void helix_norm_bwd_##TAG##_##KIND##NC(HelixNormBwdParams p) { \
-        norm_bwd_rows<T, W, NC>(p);                                                                                      \
+        norm_bwd_rows<T, W, NC, #KIND[0] != 'e' && #KIND[0] != 'x'>(p);                                                                                      \
     }
 #define NORM_ROWS(TAG, T)     \
     NORM_FWD(TAG, T, w, 1, 1) \
@@ -356,6 +413,16 @@ NORM_KERNELS(bf16, __bf16)
     NORM_FWD(TAG, T, g, 4, 4) \
     NORM_FWD(TAG, T, g, 4, 6) \
     NORM_FWD(TAG, T, g, 4, 8) \
+    NORM_FWD(TAG, T, x, 1, 1) \
+    NORM_FWD(TAG, T, x, 1, 2) \
+    NORM_BWD(TAG, T, x, 1, 1) \
+    NORM_BWD(TAG, T, x, 1, 2) \
+    NORM_FWD(TAG, T, e, 4, 1) \
+    NORM_FWD(TAG, T, e, 4, 2) \
+    NORM_FWD(TAG, T, e, 4, 4) \
+    NORM_BWD(TAG, T, e, 4, 1) \
+    NORM_BWD(TAG, T, e, 4, 2) \
+    NORM_BWD(TAG, T, e, 4, 4) \
     NORM_BWD(TAG, T, w, 1, 1) \
     NORM_BWD(TAG, T, w, 1, 2) \
     NORM_BWD(TAG, T, g, 4, 1) \

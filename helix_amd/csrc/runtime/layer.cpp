@@ -4,6 +4,7 @@
 #include <algorithm>
 #include <cmath>
 #include <cstdint>
+#include <cstring>
 #include <exception>
 #include <string>
 
@@ -105,13 +106,12 @@ helix_status entry(helix_ctx* ctx, F&& body) {
 
 constexpr int kNormThreads = 256;
 
-// Kernel of rows of dim channels that are read once: "_w" + the chunks of 512 a wave holds, or "_g" + those of 2048 a
-// workgroup does; empty: the forms that read a row twice. A wave holds `most` chunks well (more would leave a SIMD
-// with one or two waves), and rows that would leave CUs without work (four to a workgroup) are a workgroup's each.
-std::string norm_form(long long rows, long long dim, bool vec, int most) {
-    if (!vec || dim > 8 * 2048) return "";
-    const bool wave = dim <= most * 512 && rows >= 4 * 256;
+// Kernel of rows of dim channels that are read once: "_w" + the chunks of 512 a wave holds, where `wave`, or "_g" + those of
+// 2048 a workgroup does; element by element "_x" and "_e"; empty: the forms that read a row twice.
+std::string norm_form(long long dim, bool vec, bool wave) {
+    if (!vec) wave = wave && dim <= 2 * 512;
     const long long chunks = ceil_div(dim, wave ? 512 : 2048);
+    if (!vec) return wave ? (chunks <= 1 ? "_x1" : "_x2") : chunks <= 1 ? "_e1" : chunks <= 2 ? "_e2" : chunks <= 4 ? "_e4" : "";
     for (const int n : {1, 2, 3, 4, 6, 8})
         if (chunks <= n) return (wave ? "_w" : "_g") + std::to_string(n);
     return "";
@@ -172,15 +172,23 @@ void norm(helix_ctx* ctx, void* stream, const helix_norm_args* a, bool quantize)
     const bool vec = a->dim % 8 == 0 && pieces(a->x, a->rows, a->ld_x, es) && pieces(a->residual, a->rows, a->ld_residual, es) &&
                      pieces(a->weight, 1, 0, 1) && pieces(a->h, a->rows, a->ld_h, es) && pieces(a->y, a->rows, a->ld_y, es) &&
                      (!a->q || (aligned(a->q, 8) && (a->rows == 1 || a->ld_q % 8 == 0)));
-    const std::string form = norm_form(a->rows, a->dim, vec, 4);
-    const unsigned gx = grid(form[0] && form[1] == 'w' ? ceil_div(a->rows, 4) : a->rows);
+    // A wave each (four to a workgroup) where they give every CU four: 8192 rows of 512 and of 1024 6.8 and 10.9 us, as
+    // workgroups 12.3 and 13.8; 128 and 512 rows of 2048 4.0 and 4.3 us, as workgroups 3.4 and 3.9.
+    const std::string form = norm_form(a->dim, vec, a->dim <= 4 * 512 && a->rows >= 4 * 256);
+    const unsigned gx = grid(form[0] && (form[1] == 'w' || form[1] == 'x') ? ceil_div(a->rows, 4) : a->rows);
     const hipFunction_t f = kernel(ctx, std::string("helix_norm_") + kTags[a->io_dtype] + form);
     const OnDevice on(ctx->device);
     launch(f, stream, gx, 1, kNormThreads, p);
 }
 
-// Parts that dweight's rows are summed in, a workgroup's each: three for every CU, of 16 rows at least.
-long long norm_parts(long long rows) { return std::max(1LL, std::min(3 * 256LL, rows / 16)); }
+// Whether the backward pass gives a row to a wave: up to two chunks of 512, more would not fit in its registers with their
+// sums (512 rows of 1024 8.0 us, as workgroups 16.6; 32768 of them 53 and 78).
+bool norm_waves(long long dim) { return dim <= 2 * 512; }
+
+// Parts that dweight's rows are summed in, a workgroup's each: two for every CU, of four steps at least.
+long long norm_parts(long long rows, long long dim) {
+    return std::max(1LL, std::min(2 * 256LL, rows / (norm_waves(dim) ? 16 : 4)));
+}
 
 }  // namespace
 
@@ -194,7 +202,7 @@ extern "C" helix_status helix_quantize_fp8_encode(helix_ctx* ctx, void* stream, 
 
 extern "C" size_t helix_norm_backward_scratch_size(const helix_norm_backward_args* a) {
     if (!a || !a->dweight || a->rows <= 0 || a->dim <= 0) return 0;
-    return (size_t)norm_parts(a->rows) * a->dim * sizeof(float);
+    return (size_t)norm_parts(a->rows, a->dim) * a->dim * sizeof(float);
 }
 
 extern "C" helix_status helix_norm_backward_encode(helix_ctx* ctx, void* stream, const helix_norm_backward_args* a) {
@@ -238,12 +246,12 @@ extern "C" helix_status helix_norm_backward_encode(helix_ctx* ctx, void* stream,
         p.rows = a->rows;
         p.dim = a->dim;
         p.w_f32 = a->weight_dtype == HELIX_F32;
-        p.parts = a->rows ? (int)norm_parts(a->rows) : 0;   // no rows: dweight is 0
+        p.parts = a->rows ? (int)norm_parts(a->rows, a->dim) : 0;   // no rows: dweight is 0
         p.part_rows = p.parts ? ceil_div(a->rows, p.parts) : 0;
         const std::string tag = kTags[a->io_dtype];
         const bool vec = a->dim % 8 == 0 && pieces(a->dy, a->rows, a->ld_dy, es) && pieces(a->h, a->rows, a->ld_h, es) &&
                          pieces(a->weight, 1, 0, 1) && pieces(a->dh, a->rows, a->ld_dh, es) && pieces(a->dx, a->rows, a->ld_dx, es);
-        const std::string form = norm_form(a->rows, a->dim, vec, 2);
+        const std::string form = norm_form(a->dim, vec, norm_waves(a->dim));
         const unsigned gx = grid(a->rows);
         const unsigned gc = (unsigned)ceil_div(a->dim, kNormThreads), gd = (unsigned)ceil_div(a->dim, 64);
         const hipFunction_t dx = kernel(ctx, "helix_norm_bwd_" + tag + form), part = kernel(ctx, "helix_norm_dw_part_" + tag),
@@ -632,6 +640,9 @@ const std::vector<std::string>& layer_kernel_names() {
                 for (const char* k : {"helix_norm_", "helix_norm_bwd_"}) v.push_back(std::string(k) + tag + "_g" + n);
                 if (n[0] <= '4') v.push_back(std::string("helix_norm_") + tag + "_w" + n);
                 if (n[0] <= '2') v.push_back(std::string("helix_norm_bwd_") + tag + "_w" + n);
+                for (const char* k : {"helix_norm_", "helix_norm_bwd_"})
+                    for (const char* e : {"_x", "_e"})
+                        if (std::strchr(e[1] == 'x' ? "12" : "124", n[0])) v.push_back(std::string(k) + tag + e + n);
             }
         for (const char* tag : kTags)
             for (const char* k : {"_blocks", "_r1", "_r1w4", "_r2", "_r3", "_r4"})

@@ -44,8 +44,9 @@ def test_norm(gpu, dim, dtype):
 
 
 @pytest.mark.parametrize("rows", [1, 2, 3, 63, 257, 4099])
-def test_norm_rows(gpu, rows):
-    check_norm(normal(rows, 640, seed=4, dtype=torch.bfloat16), 1 + normal(640, seed=5), None)
+@pytest.mark.parametrize("dim,dtype", [(640, torch.bfloat16), (331, torch.float16), (1023, torch.bfloat16), (1025, torch.float32)])
+def test_norm_rows(gpu, rows, dim, dtype):
+    check_norm(normal(rows, dim, seed=4, dtype=dtype), 1 + normal(dim, seed=5), None)
 
 
 @pytest.mark.parametrize("dtype", TYPES)
@@ -139,7 +140,8 @@ def test_backward(gpu, dim, dtype):
         check_backward(dy, h, w.to(dtype), rstd, None)
 
 
-@pytest.mark.parametrize("rows,dim", [(3001, 96), (513, 1001), (20000, 40)])
+@pytest.mark.parametrize("rows,dim", [(3001, 96), (513, 1001), (20000, 40), (1500, 333), (700, 4099),
+                                      (2100, 2053), (130, 8191)])
 def test_backward_many_rows_strided(gpu, rows, dim):
     wide = normal(rows, 3 * dim + 7, seed=24, dtype=torch.bfloat16)
     w = 1 + 0.3 * normal(dim, seed=25)
