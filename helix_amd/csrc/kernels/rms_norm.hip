@@ -9,9 +9,9 @@
 // Accesses past a row's end are out of the resource's range: they read zeros, which add
 // nothing to a sum or a largest magnitude, and write nothing.
 //
-// Rows that do not start at multiples of 16 bytes take the same way element by element
-// (8192 x 1001 in bf16 14 us where 8192 x 1024 take 11; in forms that read a row twice
-// 28). Only those wider than what registers hold go through the latter, below.
+// Rows start anywhere (8192 x 1001 in bf16 12.7 us, 8192 x 1024 10.9; 2871 x 5183 27,
+// element by element 38). Those wider than what registers hold go through the forms below that read a row
+// twice.
 //
 // 8192 x 2048 of bf16 with a residual into 8 bits: 21 us, 118 MB at 5.6 TB/s; 2871 x 5184
 // of f32 21 us, 5.7 TB/s; backward of 32768 x 2560 of bf16 145 us, 4.6 TB/s, as a copy
@@ -44,66 +44,72 @@ HELIX_DEV helix_rsrc row_rsrc(const void* base, long long row, long long ld, int
     return make_rsrc_u(static_cast<const T*>(base) + row * ld, (unsigned)dim * (unsigned)sizeof(T));
 }
 
-// Chunk j of a lane's channels, eight of them from c on: neighbours (VEC), or in steps of
-// 64 in every W-th block of 128, where elements are moved one by one.
-template <int W, bool VEC>
-HELIX_DEV int first_channel(int j, int wave, int lane) {
-    if constexpr (VEC) return (W == 1 ? j : 4 * j + wave) * 512 + 8 * lane;
-    else return (4 * j * W + (W == 1 ? 0 : wave)) * HELIX_BLOCK + lane;
+// A row's eight channels from c on, at any address. A resource's range is checked word by
+// word, so a word that an odd last channel of 16 bits has half of is left out of it, and
+// that channel is moved by itself (Tail).
+template <typename T>
+HELIX_DEV helix_rsrc words_rsrc(const void* base, long long row, long long ld, int dim) {
+    return make_rsrc_u(static_cast<const T*>(base) + row * ld, (unsigned)dim * (unsigned)sizeof(T) & ~3u);
 }
-template <int W, bool VEC>
-HELIX_DEV int channel(int c, int i) {
-    return VEC ? c + i : c + (i >> 1) * W * HELIX_BLOCK + 64 * (i & 1);
-}
-template <typename T, int W, bool VEC>
-HELIX_DEV Raw8<T> load8(helix_rsrc r, int c) {
-    if constexpr (VEC) {
-        return buf_load8<T>(r, c * (int)sizeof(T));
-    } else {
-        Raw8<T> o;
-        if constexpr (sizeof(T) == 4) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-                o.w[i >> 2][i & 3] = __builtin_amdgcn_raw_buffer_load_b32(r, channel<W, VEC>(c, i) * 4, 0, 0);
-        } else {
-            unsigned e[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) e[i] = (unsigned short)__builtin_amdgcn_raw_buffer_load_b16(r, channel<W, VEC>(c, i) * 2, 0, 0);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) o.w[0][i] = e[2 * i] | e[2 * i + 1] << 16;
-        }
-        return o;
+template <typename T>
+struct Tail {
+    int last;      // the odd last channel, or -1
+    __device__ explicit Tail(int dim) : last(sizeof(T) == 2 && (dim & 1) ? dim - 1 : -1) {}
+    __device__ __forceinline__ unsigned load(const void* base, long long row, long long ld) const {
+        if (sizeof(T) == 4 || last < 0) return 0;
+        return reinterpret_cast<const uint16_t*>(base)[row * ld + last];
     }
-}
-template <typename T, int W, bool VEC>
-HELIX_DEV void store8(helix_rsrc r, const float (&v)[8], int c) {
-    if constexpr (VEC) {
-        buf_store8<T>(r, v, c * (int)sizeof(T));
-    } else {
+    // The channel in the lane and chunk that hold it.
+    __device__ __forceinline__ void put(unsigned x, Raw8<T>& v, int c) const {
+        if (sizeof(T) == 4 || last < 0) return;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) io_store<T, 0>(r, v[i], channel<W, VEC>(c, i) * (int)sizeof(T), 0);
+        for (int i = 0; i < 4; ++i) v.w[0][i] = c + 2 * i == last ? x : v.w[0][i];
+    }
+    __device__ __forceinline__ void store(void* base, long long row, long long ld, const float (&v)[8], int c) const {
+        if (sizeof(T) == 4 || last < 0) return;
+#pragma unroll
+        for (int i = 0; i < 8; i += 2)
+            if (c + i == last) static_cast<T*>(base)[row * ld + last] = (T)v[i];
+    }
+};
+template <typename T, int NC>
+HELIX_DEV void load_row(const void* base, long long row, long long ld, int dim, const int (&c)[NC], Raw8<T> (&o)[NC]) {
+    const helix_rsrc r = words_rsrc<T>(base, row, ld, dim);
+    const Tail<T> tail(dim);
+#pragma unroll
+    for (int j = 0; j < NC; ++j) o[j] = buf_load8<T>(r, c[j] * (int)sizeof(T));
+    const unsigned x = tail.load(base, row, ld);
+#pragma unroll
+    for (int j = 0; j < NC; ++j) tail.put(x, o[j], c[j]);
+}
+template <typename T, int NC>
+HELIX_DEV void store_row(void* base, long long row, long long ld, int dim, const int (&c)[NC], const float (&v)[NC][8]) {
+    const helix_rsrc r = words_rsrc<T>(base, row, ld, dim);
+    const Tail<T> tail(dim);
+#pragma unroll
+    for (int j = 0; j < NC; ++j) {
+        buf_store8<T>(r, v[j], c[j] * (int)sizeof(T));
+        tail.store(base, row, ld, v[j], c[j]);
     }
 }
 
 // The weights of a lane's channels in fp32.
-template <typename T, int W, bool VEC, int NC>
+template <typename T, int NC>
 HELIX_DEV void load_weights(const void* w, int w_f32, int dim, const int (&c)[NC], float (&o)[NC][8]) {
     if (w_f32) {
-        const helix_rsrc r = make_rsrc_u(w, dim * 4u);
+        Raw8<float> v[NC];
+        load_row<float>(w, 0, 0, dim, c, v);
 #pragma unroll
-        for (int j = 0; j < NC; ++j) {
-            const Raw8<float> v = load8<float, W, VEC>(r, c[j]);
+        for (int j = 0; j < NC; ++j)
 #pragma unroll
-            for (int i = 0; i < 8; ++i) o[j][i] = at8(v, i);
-        }
+            for (int i = 0; i < 8; ++i) o[j][i] = at8(v[j], i);
     } else {
-        const helix_rsrc r = make_rsrc_u(w, dim * (unsigned)sizeof(T));
+        Raw8<T> v[NC];
+        load_row<T>(w, 0, 0, dim, c, v);
 #pragma unroll
-        for (int j = 0; j < NC; ++j) {
-            const Raw8<T> v = load8<T, W, VEC>(r, c[j]);
+        for (int j = 0; j < NC; ++j)
 #pragma unroll
-            for (int i = 0; i < 8; ++i) o[j][i] = at8(v, i);
-        }
+            for (int i = 0; i < 8; ++i) o[j][i] = at8(v[j], i);
     }
 }
 
@@ -114,7 +120,7 @@ HELIX_DEV float row_sum(float v, float* red) {
     else return group_sum(v, red);
 }
 
-template <typename T, int W, int NC, bool VEC>
+template <typename T, int W, int NC>
 __device__ void norm_rows(const HelixNormParams& p) {
     __shared__ float red[NORM_THREADS / 64];
     const int lane = lane_id(), wave = wave_uniform();
@@ -122,18 +128,12 @@ __device__ void norm_rows(const HelixNormParams& p) {
     if (W == 1 && row >= p.rows) return;
     int c[NC];
 #pragma unroll
-    for (int j = 0; j < NC; ++j) c[j] = first_channel<W, VEC>(j, wave, lane);
+    for (int j = 0; j < NC; ++j) c[j] = (W == 1 ? j : 4 * j + wave) * 512 + 8 * lane;
     Raw8<T> x[NC], r[NC];
-    const helix_rsrc rx = row_rsrc<T>(p.x, row, p.ld_x, p.dim);
-#pragma unroll
-    for (int j = 0; j < NC; ++j) x[j] = load8<T, W, VEC>(rx, c[j]);
-    if (p.residual) {
-        const helix_rsrc rr = row_rsrc<T>(p.residual, row, p.ld_residual, p.dim);
-#pragma unroll
-        for (int j = 0; j < NC; ++j) r[j] = load8<T, W, VEC>(rr, c[j]);
-    }
+    load_row<T>(p.x, row, p.ld_x, p.dim, c, x);
+    if (p.residual) load_row<T>(p.residual, row, p.ld_residual, p.dim, c, r);
     float w[NC][8], v[NC][8];
-    if (p.weight) load_weights<T, W, VEC>(p.weight, p.w_f32, p.dim, c, w);
+    if (p.weight) load_weights<T>(p.weight, p.w_f32, p.dim, c, w);
     float ss = 0.0f;
 #pragma unroll
     for (int j = 0; j < NC; ++j)
@@ -145,11 +145,7 @@ __device__ void norm_rows(const HelixNormParams& p) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) v[j][i] += at8(r[j], i);
     }
-    if (p.h) {
-        const helix_rsrc rh = row_rsrc<T>(p.h, row, p.ld_h, p.dim);
-#pragma unroll
-        for (int j = 0; j < NC; ++j) store8<T, W, VEC>(rh, v[j], c[j]);
-    }
+    if (p.h) store_row<T>(p.h, row, p.ld_h, p.dim, c, v);
     if (p.weight) {
 #pragma unroll
         for (int j = 0; j < NC; ++j)
@@ -163,28 +159,13 @@ __device__ void norm_rows(const HelixNormParams& p) {
             for (int i = 0; i < 8; ++i) v[j][i] = v[j][i] * rstd * w[j][i];
     }
     if (p.y) {
-        const helix_rsrc ry = row_rsrc<T>(p.y, row, p.ld_y, p.dim);
-#pragma unroll
-        for (int j = 0; j < NC; ++j) store8<T, W, VEC>(ry, v[j], c[j]);
+        store_row<T>(p.y, row, p.ld_y, p.dim, c, v);
         return;
     }
-    const helix_rsrc rq = row_rsrc<uint8_t>(p.q, row, p.ld_q, p.dim);
+    const helix_rsrc rq = words_rsrc<uint8_t>(p.q, row, p.ld_q, p.dim);
     const helix_rsrc rs = row_rsrc<uint8_t>(p.scale, row, p.ld_scale, (p.dim + HELIX_BLOCK - 1) / HELIX_BLOCK);
 #pragma unroll
     for (int j = 0; j < NC; ++j) {
-        if constexpr (!VEC) {
-#pragma unroll
-            for (int i = 0; i < 8; i += 2) {   // a block of the wave's
-                const int e = block_exponent(wave_max(fmaxf(fabsf(v[j][i]), fabsf(v[j][i + 1]))));
-                const float inv = exponent_recip(e);
-                const int at = channel<W, VEC>(c[j], i);
-                const unsigned q = (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(v[j][i] * inv, v[j][i + 1] * inv, 0, false);
-                __builtin_amdgcn_raw_buffer_store_b8((unsigned char)q, rq, at, 0, 0);
-                __builtin_amdgcn_raw_buffer_store_b8((unsigned char)(q >> 8), rq, at + 64, 0, 0);
-                __builtin_amdgcn_raw_buffer_store_b8((unsigned char)e, rs, lane ? (int)0x80000000 : at >> 7, 0, 0);
-            }
-            continue;
-        }
         float top = 0.0f;
 #pragma unroll
         for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(v[j][i]));
@@ -197,22 +178,27 @@ __device__ void norm_rows(const HelixNormParams& p) {
             q[i] = (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(v[j][4 * i + 2] * inv, v[j][4 * i + 3] * inv, d, true);
         }
         __builtin_amdgcn_raw_buffer_store_b64(q, rq, c[j], 0, 0);
+        if (p.dim & 3) {   // the bytes of the last word
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (c[j] + i >= (p.dim & ~3) && c[j] + i < p.dim) p.q[row * p.ld_q + c[j] + i] = (uint8_t)(q[i >> 2] >> (8 * (i & 3)));
+        }
         __builtin_amdgcn_raw_buffer_store_b8((unsigned char)e, rs, lane & 15 ? (int)0x80000000 : c[j] >> 7, 0, 0);
     }
 }
 
 // dx, and dweight's sum over the rows of a part: a workgroup's, row by row in each of
 // its waves (W = 1) or in all of them (W = 4). The waves' sums are added in their order.
-template <typename T, int W, int NC, bool VEC>
+template <typename T, int W, int NC>
 __device__ void norm_bwd_rows(const HelixNormBwdParams& p) {
     __shared__ float red[2][NORM_THREADS / 64];
     __shared__ float sums[W == 1 ? 3 : 1][W == 1 ? NC * 512 : 1];
     const int lane = lane_id(), wave = wave_uniform();
     int c[NC];
 #pragma unroll
-    for (int j = 0; j < NC; ++j) c[j] = first_channel<W, VEC>(j, wave, lane);
+    for (int j = 0; j < NC; ++j) c[j] = (W == 1 ? j : 4 * j + wave) * 512 + 8 * lane;
     float w[NC][8], dw[NC][8];
-    load_weights<T, W, VEC>(p.weight, p.w_f32, p.dim, c, w);
+    load_weights<T>(p.weight, p.w_f32, p.dim, c, w);
 #pragma unroll
     for (int j = 0; j < NC; ++j)
 #pragma unroll
@@ -221,16 +207,9 @@ __device__ void norm_bwd_rows(const HelixNormBwdParams& p) {
     int turn = 0;
     for (long long row = first + (W == 1 ? wave : 0); row < end; row += W == 1 ? 4 : 1) {
         Raw8<T> dy[NC], h[NC], dh[NC];
-        const helix_rsrc rd = row_rsrc<T>(p.dy, row, p.ld_dy, p.dim), rh = row_rsrc<T>(p.h, row, p.ld_h, p.dim);
-#pragma unroll
-        for (int j = 0; j < NC; ++j) dy[j] = load8<T, W, VEC>(rd, c[j]);
-#pragma unroll
-        for (int j = 0; j < NC; ++j) h[j] = load8<T, W, VEC>(rh, c[j]);
-        if (p.dh) {
-            const helix_rsrc rg = row_rsrc<T>(p.dh, row, p.ld_dh, p.dim);
-#pragma unroll
-            for (int j = 0; j < NC; ++j) dh[j] = load8<T, W, VEC>(rg, c[j]);
-        }
+        load_row<T>(p.dy, row, p.ld_dy, p.dim, c, dy);
+        load_row<T>(p.h, row, p.ld_h, p.dim, c, h);
+        if (p.dh) load_row<T>(p.dh, row, p.ld_dh, p.dim, c, dh);
         const float rstd = p.rstd[row];
         float dot = 0.0f;
 #pragma unroll
@@ -244,24 +223,22 @@ __device__ void norm_bwd_rows(const HelixNormBwdParams& p) {
         // Two places in turn: a wave may be at the next row's sum while another reads this one's.
         const float mean = row_sum<W>(dot, red[turn]) / (float)p.dim;
         turn ^= 1;
-        const helix_rsrc rx = row_rsrc<T>(p.dx, row, p.ld_dx, p.dim);
+        float o[NC][8];
 #pragma unroll
         for (int j = 0; j < NC; ++j) {
-            float o[8];
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 const float n = at8(h[j], i) * rstd;
-                o[i] = rstd * (at8(dy[j], i) * w[j][i] - n * mean);
+                o[j][i] = rstd * (at8(dy[j], i) * w[j][i] - n * mean);
             }
             if (p.dh) {
 #pragma unroll
-                for (int i = 0; i < 8; ++i) o[i] += at8(dh[j], i);
+                for (int i = 0; i < 8; ++i) o[j][i] += at8(dh[j], i);
             }
-            store8<T, W, VEC>(rx, o, c[j]);
         }
+        store_row<T>(p.dx, row, p.ld_dx, p.dim, c, o);
     }
     if (!p.dweight) return;
-    const helix_rsrc rp = row_rsrc<float>(p.part, blockIdx.x, p.dim, p.dim);
     if constexpr (W == 1) {
         if (wave > 0) {
 #pragma unroll
@@ -278,8 +255,7 @@ __device__ void norm_bwd_rows(const HelixNormBwdParams& p) {
 #pragma unroll
                 for (int o = 0; o < 3; ++o) dw[j][i] += sums[o][(j * 8 + i) * 64 + lane];
     }
-#pragma unroll
-    for (int j = 0; j < NC; ++j) store8<float, W, VEC>(rp, dw[j], c[j]);
+    store_row<float>(p.part, blockIdx.x, p.dim, p.dim, c, dw);
 }
 
 // One workgroup per row, which is read twice (the second time from the caches).
@@ -396,11 +372,11 @@ NORM_KERNELS(bf16, __bf16)
 
 #define NORM_FWD(TAG, T, KIND, W, NC)                                                                             \
     extern "C" __global__ __launch_bounds__(NORM_THREADS) void helix_norm_##TAG##_##KIND##NC(HelixNormParams p) { \
-        norm_rows<T, W, NC, #KIND[0] != 'e' && #KIND[0] != 'x'>(p);                                                                                   \
+        norm_rows<T, W, NC>(p);                                                                                   \
     }
 #define NORM_BWD(TAG, T, KIND, W, NC)                                                                                    \
     extern "C" __global__ __launch_bounds__(NORM_THREADS) void helix_norm_bwd_##TAG##_##KIND##NC(HelixNormBwdParams p) { \
-        norm_bwd_rows<T, W, NC, #KIND[0] != 'e' && #KIND[0] != 'x'>(p);                                                                                      \
+        norm_bwd_rows<T, W, NC>(p);                                                                                      \
     }
 #define NORM_ROWS(TAG, T)     \
     NORM_FWD(TAG, T, w, 1, 1) \
@@ -413,16 +389,6 @@ NORM_KERNELS(bf16, __bf16)
     NORM_FWD(TAG, T, g, 4, 4) \
     NORM_FWD(TAG, T, g, 4, 6) \
     NORM_FWD(TAG, T, g, 4, 8) \
-    NORM_FWD(TAG, T, x, 1, 1) \
-    NORM_FWD(TAG, T, x, 1, 2) \
-    NORM_BWD(TAG, T, x, 1, 1) \
-    NORM_BWD(TAG, T, x, 1, 2) \
-    NORM_FWD(TAG, T, e, 4, 1) \
-    NORM_FWD(TAG, T, e, 4, 2) \
-    NORM_FWD(TAG, T, e, 4, 4) \
-    NORM_BWD(TAG, T, e, 4, 1) \
-    NORM_BWD(TAG, T, e, 4, 2) \
-    NORM_BWD(TAG, T, e, 4, 4) \
     NORM_BWD(TAG, T, w, 1, 1) \
     NORM_BWD(TAG, T, w, 1, 2) \
     NORM_BWD(TAG, T, g, 4, 1) \

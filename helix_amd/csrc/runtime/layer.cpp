@@ -4,7 +4,6 @@
 #include <algorithm>
 #include <cmath>
 #include <cstdint>
-#include <cstring>
 #include <exception>
 #include <string>
 
@@ -107,19 +106,12 @@ helix_status entry(helix_ctx* ctx, F&& body) {
 constexpr int kNormThreads = 256;
 
 // Kernel of rows of dim channels that are read once: "_w" + the chunks of 512 a wave holds, where `wave`, or "_g" + those of
-// 2048 a workgroup does; element by element "_x" and "_e"; empty: the forms that read a row twice.
-std::string norm_form(long long dim, bool vec, bool wave) {
-    if (!vec) wave = wave && dim <= 2 * 512;
+// 2048 a workgroup does; empty: the forms that read a row twice.
+std::string norm_form(long long dim, bool wave) {
     const long long chunks = ceil_div(dim, wave ? 512 : 2048);
-    if (!vec) return wave ? (chunks <= 1 ? "_x1" : "_x2") : chunks <= 1 ? "_e1" : chunks <= 2 ? "_e2" : chunks <= 4 ? "_e4" : "";
     for (const int n : {1, 2, 3, 4, 6, 8})
         if (chunks <= n) return (wave ? "_w" : "_g") + std::to_string(n);
     return "";
-}
-
-// Whether rows can be moved in pieces of 16 bytes.
-bool pieces(const void* p, long long rows, long long ld, size_t es) {
-    return !p || (aligned(p, 16) && (rows == 1 || ld * (long long)es % 16 == 0));
 }
 
 void norm(helix_ctx* ctx, void* stream, const helix_norm_args* a, bool quantize) {
@@ -169,13 +161,10 @@ void norm(helix_ctx* ctx, void* stream, const helix_norm_args* a, bool quantize)
     p.dim = a->dim;
     p.w_f32 = a->weight_dtype == HELIX_F32;
     p.eps = a->eps;
-    const bool vec = a->dim % 8 == 0 && pieces(a->x, a->rows, a->ld_x, es) && pieces(a->residual, a->rows, a->ld_residual, es) &&
-                     pieces(a->weight, 1, 0, 1) && pieces(a->h, a->rows, a->ld_h, es) && pieces(a->y, a->rows, a->ld_y, es) &&
-                     (!a->q || (aligned(a->q, 8) && (a->rows == 1 || a->ld_q % 8 == 0)));
     // A wave each (four to a workgroup) where they give every CU four: 8192 rows of 512 and of 1024 6.8 and 10.9 us, as
     // workgroups 12.3 and 13.8; 128 and 512 rows of 2048 4.0 and 4.3 us, as workgroups 3.4 and 3.9.
-    const std::string form = norm_form(a->dim, vec, a->dim <= 4 * 512 && a->rows >= 4 * 256);
-    const unsigned gx = grid(form[0] && (form[1] == 'w' || form[1] == 'x') ? ceil_div(a->rows, 4) : a->rows);
+    const std::string form = norm_form(a->dim, a->dim <= 4 * 512 && a->rows >= 4 * 256);
+    const unsigned gx = grid(form[0] && form[1] == 'w' ? ceil_div(a->rows, 4) : a->rows);
     const hipFunction_t f = kernel(ctx, std::string("helix_norm_") + kTags[a->io_dtype] + form);
     const OnDevice on(ctx->device);
     launch(f, stream, gx, 1, kNormThreads, p);
@@ -249,9 +238,7 @@ extern "C" helix_status helix_norm_backward_encode(helix_ctx* ctx, void* stream,
         p.parts = a->rows ? (int)norm_parts(a->rows, a->dim) : 0;   // no rows: dweight is 0
         p.part_rows = p.parts ? ceil_div(a->rows, p.parts) : 0;
         const std::string tag = kTags[a->io_dtype];
-        const bool vec = a->dim % 8 == 0 && pieces(a->dy, a->rows, a->ld_dy, es) && pieces(a->h, a->rows, a->ld_h, es) &&
-                         pieces(a->weight, 1, 0, 1) && pieces(a->dh, a->rows, a->ld_dh, es) && pieces(a->dx, a->rows, a->ld_dx, es);
-        const std::string form = norm_form(a->dim, vec, norm_waves(a->dim));
+        const std::string form = norm_form(a->dim, norm_waves(a->dim));
         const unsigned gx = grid(a->rows);
         const unsigned gc = (unsigned)ceil_div(a->dim, kNormThreads), gd = (unsigned)ceil_div(a->dim, 64);
         const hipFunction_t dx = kernel(ctx, "helix_norm_bwd_" + tag + form), part = kernel(ctx, "helix_norm_dw_part_" + tag),
@@ -479,18 +466,13 @@ ScanPlan scan_plan(long long n_seq, long long n_tok, long long n_chan, int run, 
     return p;
 }
 
-// Whether rows of four channels can be moved together.
-bool quads(const void* p, long long seq, long long tok, long long n_chan, size_t es) {
-    return !(n_chan % 4) && !(seq % 4) && !(tok % 4) && aligned(p, 4 * es);
-}
-
 // Whether a wave's rows (4 runs of 8 tokens at most, and one before them) reach
 // beyond 2^29 bytes.
 bool far_rows(long long tok, size_t es) { return tok >= (1LL << 29) / 33 / (long long)es; }
 
 // Fills in a plan, and runs it: P is HelixGatedScanParams or its backward form.
 template <typename A, typename P>
-void run_scan(helix_ctx* ctx, void* stream, const A& a, P& p, const char* name, int run, bool vec, bool far) {
+void run_scan(helix_ctx* ctx, void* stream, const A& a, P& p, const char* name, int run, bool far) {
     const ScanPlan plan = scan_plan(a.n_seq, a.n_tok, a.n_chan, run, far);
     need(plan.bytes == 0 || (a.scratch && a.scratch_bytes >= plan.bytes), "scratch smaller than its _scratch_size()",
          HELIX_ERR_SCRATCH_TOO_SMALL);
@@ -502,7 +484,7 @@ void run_scan(helix_ctx* ctx, void* stream, const A& a, P& p, const char* name, 
     p.join = HelixGatedScanJoin{};
     p.join.n_chunk = plan.n_chunk;
     p.join.n_group = plan.n_group;
-    const std::string base = std::string(name) + kTags[a.io_dtype] + (vec ? "_v" : "_s");
+    const std::string base = std::string(name) + kTags[a.io_dtype] + (a.n_chan % 4 ? "_s" : "_v");   // (channels that come in fours, or not)
     const unsigned gx = grid(plan.waves ? plan.streams * plan.n_chunk
                                         : ceil_div(a.n_seq * ceil_div(a.n_chan, 4), kScanThreads));
     const hipFunction_t f = kernel(ctx, plan.waves ? base + "_w" + std::to_string(plan.waves) : base + "_steps");
@@ -570,11 +552,9 @@ extern "C" helix_status helix_gated_scan_encode(helix_ctx* ctx, void* stream, co
         p.seq_h = a->seq_h;
         p.tok_h = a->tok_h;
         const size_t es = kBytes[a->io_dtype];
-        const long long D = a->n_chan;
-        const bool vec = quads(a->g, a->seq_g, a->tok_g, D, es) && quads(a->v, a->seq_v, a->tok_v, D, es) && quads(a->h, a->seq_h, a->tok_h, D, es);
         bool far = false;
         for (const long long tok : {(long long)a->tok_g, (long long)a->tok_v, (long long)a->tok_h}) far |= far_rows(tok, es);
-        run_scan(ctx, stream, *a, p, "helix_gated_scan_", HELIX_GS_RUN, vec, far);
+        run_scan(ctx, stream, *a, p, "helix_gated_scan_", HELIX_GS_RUN, far);
     });
 }
 
@@ -618,11 +598,9 @@ extern "C" helix_status helix_gated_scan_backward_encode(helix_ctx* ctx, void* s
         p.seq_dv = a->seq_dv;
         p.tok_dv = a->tok_dv;
         const size_t es = kBytes[a->io_dtype];
-        const long long D = a->n_chan;
-        const bool vec = quads(a->dh, a->seq_dh, a->tok_dh, D, es) && quads(a->g, a->seq_g, a->tok_g, D, es) && quads(a->v, a->seq_v, a->tok_v, D, es) && quads(a->h, a->seq_h, a->tok_h, D, es) && quads(a->dg, a->seq_dg, a->tok_dg, D, es) && quads(a->dv, a->seq_dv, a->tok_dv, D, es);
         bool far = false;
         for (const long long tok : {(long long)a->tok_dh, (long long)a->tok_g, (long long)a->tok_v, (long long)a->tok_h, (long long)a->tok_dg, (long long)a->tok_dv}) far |= far_rows(tok, es);
-        run_scan(ctx, stream, *a, p, "helix_gated_scan_bwd_", HELIX_GS_RUN_BWD, vec, far);
+        run_scan(ctx, stream, *a, p, "helix_gated_scan_bwd_", HELIX_GS_RUN_BWD, far);
     });
 }
 
@@ -640,9 +618,6 @@ const std::vector<std::string>& layer_kernel_names() {
                 for (const char* k : {"helix_norm_", "helix_norm_bwd_"}) v.push_back(std::string(k) + tag + "_g" + n);
                 if (n[0] <= '4') v.push_back(std::string("helix_norm_") + tag + "_w" + n);
                 if (n[0] <= '2') v.push_back(std::string("helix_norm_bwd_") + tag + "_w" + n);
-                for (const char* k : {"helix_norm_", "helix_norm_bwd_"})
-                    for (const char* e : {"_x", "_e"})
-                        if (std::strchr(e[1] == 'x' ? "12" : "124", n[0])) v.push_back(std::string(k) + tag + e + n);
             }
         for (const char* tag : kTags)
             for (const char* k : {"_blocks", "_r1", "_r1w4", "_r2", "_r3", "_r4"})

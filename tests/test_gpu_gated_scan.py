@@ -110,6 +110,8 @@ def test_strides(gpu):
     check(normal(1, 1, 70, seed=15).expand(2, 257, 70), normal(2, 257, 70, seed=16), normal(2, 70, seed=17))
     wide = normal(2, 260, 211, seed=18, dtype=torch.bfloat16)
     check(wide[:, :, 3:100], wide[:, :, 101:198], normal(2, 97, seed=19))
+    check(wide[:, :, 3:99], wide[:, :, 102:198], normal(2, 96, seed=19))
+    check(wide[:, :9, 1:129], wide[:, :9, 2:130], normal(2, 128, seed=19))
 
 
 def test_rows_far_apart(gpu):
