@@ -51,7 +51,6 @@ typedef struct {
     long long      ld_a, ld_a_scale, ld_b, ld_b_scale, ld_c;
     int            m, n, k;
     int            f16;     /* c is f16 (else bf16), in the tiled kernel       */
-    int            wide;    /* rows of c are 16-byte aligned (16-bit types)    */
     /* Tiled kernel: bands of gm rows of tiles, band = gm x columns of tiles, and
      * 2^32 / d + 1 of band, gm and the last band's rows. */
     int            gm;

@@ -390,7 +390,6 @@ extern "C" helix_status helix_matmul_fp8_encode(helix_ctx* ctx, void* stream, co
         }
         if (!plan.bm) {
             const unsigned gx = grid(ceil_div(a->m, 64) * ceil_div(a->n, 128));
-            p.wide = a->n % 4 == 0 && a->ld_c % 4 == 0 && aligned(a->c, 16);
             const OnDevice on(ctx->device);
             launch(f, stream, gx, 1, 256, p);
             return;
@@ -407,7 +406,6 @@ extern "C" helix_status helix_matmul_fp8_encode(helix_ctx* ctx, void* stream, co
         p.inv_rest = reciprocal((unsigned)(mt % p.gm));
         p.stride = (int)std::min<long long>(tiles, 256LL * plan.per_cu);
         p.f16 = a->out_dtype == HELIX_F16;
-        p.wide = a->n % 8 == 0 && a->ld_c % 8 == 0 && aligned(a->c, 16);
         const unsigned ga = grid(ceil_div((long long)a->m * plan.pitch, 256)), gb = grid(ceil_div((long long)a->n * plan.pitch, 256));
         const unsigned gj = grid(ceil_div((long long)a->m * ceil_div(a->n, 4), 256));
         const hipFunction_t copy = kernel(ctx, "helix_fp8_scales"),
@@ -427,7 +425,6 @@ extern "C" helix_status helix_matmul_fp8_encode(helix_ctx* ctx, void* stream, co
         p.part = plan.parts > 1 ? reinterpret_cast<float*>(static_cast<uint8_t*>(a->scratch) + plan.a_bytes + plan.b_bytes) : nullptr;
         launch(f, stream, (unsigned)p.stride, (unsigned)plan.parts, 256, p);
         if (plan.parts == 1) return;
-        p.wide = a->n % 4 == 0 && a->ld_c % 4 == 0 && aligned(a->c, 8);
         launch(join, stream, gj, 1, 256, p);
     });
 }
