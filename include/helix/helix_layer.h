@@ -120,9 +120,10 @@ typedef struct {
     const void* b;             /* (n, k) e4m3                                 */
     const void* b_scale;       /* (n, ceil(k / 128))                          */
     void*       c;             /* (m, n)                                      */
-    void*       scratch;       /* helix_matmul_fp8_scratch_size() bytes,
-                                  16-byte aligned; none is needed where rows of
-                                  scales start at multiples of four bytes     */
+    void*       scratch;       /* helix_matmul_fp8_scratch_size() bytes (for
+                                  parts of the sum where c is small, and for
+                                  scales whose rows do not start at multiples
+                                  of four bytes), 16-byte aligned             */
     uint64_t    scratch_bytes;
     int64_t     ld_a, ld_a_scale, ld_b, ld_b_scale, ld_c;
 } helix_matmul_fp8_args;
