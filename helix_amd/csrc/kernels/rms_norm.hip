@@ -14,8 +14,8 @@
 // twice.
 //
 // 8192 x 2048 of bf16 with a residual into 8 bits: 21 us, 118 MB at 5.6 TB/s; 2871 x 5184
-// of f32 21 us, 5.7 TB/s; backward of 32768 x 2560 of bf16 145 us, 4.6 TB/s, as a copy
-// of 4 GiB (tensors that fit in the 256 MiB of cache go faster than those that do not).
+// of f32 21 us, 5.7 TB/s; backward of 32768 x 2560 of bf16 138 us, 4.9 TB/s, where a
+// copy of 4 GiB reaches 4.65 (tensors that fit in the 256 MiB of cache go faster than those that do not).
 #include "layer_common.h"
 
 namespace {
@@ -340,19 +340,26 @@ __device__ void norm_dw_part(const HelixNormBwdParams& p) {
 
 }  // namespace
 
-// dweight from the parts: 64 channels a workgroup, a sixteenth of the parts a wave, the
-// sixteen added in their order.
+// dweight from the parts: 32 channels a workgroup, every 32nd part a half of a wave, eight
+// loads at a time; the 32 sums are added in their order (512 parts of 2560 channels 5 us; 64 channels a
+// workgroup and load by load 12).
 extern "C" __global__ __launch_bounds__(1024) void helix_norm_dw(HelixNormBwdParams p) {
-    __shared__ float sum[16][64];
-    const int lane = lane_id(), wave = wave_id(), c = blockIdx.x * 64 + lane;
+    __shared__ float sum[32][33];
+    const int half = threadIdx.x >> 5, lane = threadIdx.x & 31, c = blockIdx.x * 32 + lane;
     float s = 0.0f;
     if (c < p.dim)
-        for (int i = wave; i < p.parts; i += 16) s += p.part[(long long)i * p.dim + c];
-    sum[wave][lane] = s;
-    __syncthreads();
-    if (wave || c >= p.dim) return;
+        for (int i = half; i < p.parts; i += 32 * 8) {
+            float v[8];
 #pragma unroll
-    for (int w = 1; w < 16; ++w) s += sum[w][lane];
+            for (int u = 0; u < 8; ++u) v[u] = i + 32 * u < p.parts ? p.part[(i + 32LL * u) * p.dim + c] : 0.0f;
+#pragma unroll
+            for (int u = 0; u < 8; ++u) s += v[u];
+        }
+    sum[half][lane] = s;
+    __syncthreads();
+    if (half || c >= p.dim) return;
+#pragma unroll
+    for (int w = 1; w < 32; ++w) s += sum[w][lane];
     p.dweight[c] = s;
 }
 

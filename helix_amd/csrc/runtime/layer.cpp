@@ -240,7 +240,7 @@ extern "C" helix_status helix_norm_backward_encode(helix_ctx* ctx, void* stream,
         const std::string tag = kTags[a->io_dtype];
         const std::string form = norm_form(a->dim, norm_waves(a->dim));
         const unsigned gx = grid(a->rows);
-        const unsigned gc = (unsigned)ceil_div(a->dim, kNormThreads), gd = (unsigned)ceil_div(a->dim, 64);
+        const unsigned gc = (unsigned)ceil_div(a->dim, kNormThreads), gd = (unsigned)ceil_div(a->dim, 32);
         const hipFunction_t dx = kernel(ctx, "helix_norm_bwd_" + tag + form), part = kernel(ctx, "helix_norm_dw_part_" + tag),
                             dw = kernel(ctx, "helix_norm_dw");
         const OnDevice on(ctx->device);
