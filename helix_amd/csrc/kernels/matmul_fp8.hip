@@ -316,11 +316,11 @@ __device__ void matmul_rows(const HelixMatmulParams& p) {
 // so that the eight rows that are read together lie in different banks; the loads
 // write them there by reading the row's chunks in that order.
 //
-// The power limit binds it: 8192 x 8192 x 8192 take 392 us (2.81 PFLOP/s) at 2.0 GHz,
-// two thirds of the products' own rate at that clock. Smaller tiles: 192 rows 440 us,
+// The power limit binds it: 8192 x 8192 x 8192 take 364-392 us (2.8-3.0 PFLOP/s) at 2.0
+// GHz, two thirds of the products' own rate at that clock. Smaller tiles: 192 rows 440 us,
 // 128 rows 496, 128 x 128 in two workgroups per CU 573. Products of 32 x 32 x 64 run at
 // 3.5 PFLOP/s where those of 16 x 16 x 128 run at 4.1, and took 526 us in this loop's
-// first form, against 457.
+// first form, against 457. 8192 x 10304 x 2048 take 155 us, 32768 x 2560 x 5120 311.
 
 struct TileAt {
     int i, j;
