@@ -8,7 +8,7 @@ import contextlib
 import torch
 
 from .abi import HelixError
-from .desc import HELIX_BF16, HELIX_F16, HELIX_F32, HELIX_OK
+from .desc import HELIX_BF16, HELIX_ERR_SCRATCH_TOO_SMALL, HELIX_F16, HELIX_F32, HELIX_OK
 from .scan import _capturing, _contexts, _scratch_for, _under, context
 
 IO_DTYPES = {torch.float32: HELIX_F32, torch.bfloat16: HELIX_BF16, torch.float16: HELIX_F16}
@@ -94,6 +94,21 @@ def scratch(index: int, st: int, stream, nbytes: int) -> torch.Tensor | None:
 def run(fn, index: int, st: int, args: bytes) -> None:
     ctx = _contexts.get(index) or context(index)
     rc = fn(ctx.handle, st, args)
+    if rc != HELIX_OK:
+        raise HelixError(rc, ctx.last_error())
+
+
+def run_with_scratch(fn, size, index: int, st: int, stream, pack) -> None:
+    """run for an operator that may want scratch: pack(address, bytes) gives its arguments, size(arguments) the bytes.
+    It is asked for them once the call has been refused without (nothing is enqueued then): the small calls, whose time
+    on the host counts, want none."""
+    ctx = _contexts.get(index) or context(index)
+    args = pack(0, 0)
+    rc = fn(ctx.handle, st, args)
+    if rc == HELIX_ERR_SCRATCH_TOO_SMALL:
+        need = size(args)
+        buf = scratch(index, st, stream, need)
+        rc = fn(ctx.handle, st, pack(ptr(buf), need))
     if rc != HELIX_OK:
         raise HelixError(rc, ctx.last_error())
 

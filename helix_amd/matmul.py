@@ -4,7 +4,7 @@ from __future__ import annotations
 import torch
 
 from . import abi
-from .layer import (FP8, FP8_BLOCK, FP8_SCALE, IO_DTYPES, device_index, expect, ptr, row_stride, run, scratch,
+from .layer import (FP8, FP8_BLOCK, FP8_SCALE, IO_DTYPES, device_index, expect, row_stride, run_with_scratch,
                     stream_handle, under)
 
 
@@ -42,10 +42,10 @@ def matmul_fp8(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale:
     dims = (a.numel() // k, n, k, IO_DTYPES[out.dtype], a.data_ptr(), a_scale.data_ptr(), b.data_ptr(),
             b_scale.data_ptr(), out.data_ptr())
     strides = (row_stride("a", a), row_stride("a_scale", a_scale), row_stride("b", b), row_stride("b_scale", b_scale), ld_c)
+
+    def pack(buf, nbytes):
+        return abi.MATMUL_FP8_STRUCT.pack(*dims, buf, nbytes, *strides)
+
     lib = abi.lib()
-    args = abi.MATMUL_FP8_STRUCT.pack(*dims, 0, 0, *strides)
-    need = lib.helix_matmul_fp8_scratch_size(args)
-    if need:
-        args = abi.MATMUL_FP8_STRUCT.pack(*dims, ptr(scratch(index, st, stream, need)), need, *strides)
-    run(lib.helix_matmul_fp8_encode, index, st, args)
+    run_with_scratch(lib.helix_matmul_fp8_encode, lib.helix_matmul_fp8_scratch_size, index, st, stream, pack)
     return out

@@ -9,7 +9,7 @@ from __future__ import annotations
 import torch
 
 from . import abi
-from .layer import device_index, expect, io_code, ptr, run, scratch, stream_handle, under
+from .layer import device_index, expect, io_code, ptr, run_with_scratch, stream_handle, under
 
 
 def _strides(name: str, t: torch.Tensor) -> tuple[int, int]:
@@ -54,11 +54,7 @@ def gated_scan(g: torch.Tensor, v: torch.Tensor, h0: torch.Tensor | None = None,
                                           last.data_ptr(), buf, nbytes, *strides)
 
     lib = abi.lib()
-    args = pack(0, 0)
-    need = lib.helix_gated_scan_scratch_size(args)
-    if need:
-        args = pack(ptr(scratch(index, st, stream, need)), need)
-    run(lib.helix_gated_scan_encode, index, st, args)
+    run_with_scratch(lib.helix_gated_scan_encode, lib.helix_gated_scan_scratch_size, index, st, stream, pack)
     return h, last
 
 
@@ -85,9 +81,5 @@ def gated_scan_backward(dh: torch.Tensor, g: torch.Tensor, v: torch.Tensor, h: t
                                                    buf, nbytes, *strides)
 
     lib = abi.lib()
-    args = pack(0, 0)
-    need = lib.helix_gated_scan_backward_scratch_size(args)
-    if need:
-        args = pack(ptr(scratch(index, st, stream, need)), need)
-    run(lib.helix_gated_scan_backward_encode, index, st, args)
+    run_with_scratch(lib.helix_gated_scan_backward_encode, lib.helix_gated_scan_backward_scratch_size, index, st, stream, pack)
     return dg, dv, dh0
