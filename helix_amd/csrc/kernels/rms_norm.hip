@@ -9,13 +9,14 @@
 // Accesses past a row's end are out of the resource's range: they read zeros, which add
 // nothing to a sum or a largest magnitude, and write nothing.
 //
-// Rows start anywhere (8192 x 1001 in bf16 12.7 us, 8192 x 1024 10.9; 2871 x 5183 27,
-// element by element 38). Those wider than what registers hold go through the forms below that read a row
-// twice.
+// Rows start anywhere (8192 x 1001 in bf16 12.7 us, 8192 x 1024 10.9; 2871 x 5183 of
+// f32 27, element by element 38). Those wider than what registers hold go through the
+// forms below that read a row twice.
 //
 // 8192 x 2048 of bf16 with a residual into 8 bits: 21 us, 118 MB at 5.6 TB/s; 2871 x 5184
-// of f32 21 us, 5.7 TB/s; backward of 32768 x 2560 of bf16 138 us, 4.9 TB/s, where a
-// copy of 4 GiB reaches 4.65 (tensors that fit in the 256 MiB of cache go faster than those that do not).
+// of f32 21 us, 5.7 TB/s; backward of 32768 x 2560 of bf16 138 us, 4.9 TB/s, where a copy
+// of 4 GiB reaches 4.65 (tensors that fit in the 256 MiB of cache go faster than those
+// that do not).
 #include "layer_common.h"
 
 namespace {
