@@ -310,7 +310,10 @@ __device__ void matmul_rows(const HelixMatmulParams& p) {
 //    either of a step's two barriers.
 //  - Tiles follow each other without a pause: the loads of the next tile's first steps
 //    go out during the last steps of this one, and its first waits count this one's
-//    stores (vmcnt counts both, in order) instead of waiting for them.
+//    stores (vmcnt counts both, in order) instead of waiting for them. A workgroup's
+//    first tile follows none: it begins when both of its first steps have landed, so
+//    that nothing is left for these waits. tests/test_matmul_waits.py follows the
+//    counts through the built code.
 //
 // A row's eight 16-byte chunks lie exchanged in LDS (chunk c at c ^ its row's number),
 // so that the eight rows that are read together lie in different banks; the loads
@@ -483,7 +486,8 @@ __device__ void matmul_tiles(const HelixMatmulParams& p) {
         repeat<NX + NY>([&](auto e) { load(e, s * STAGE); });
         ++pkb;
     }
-    asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(WINDOW) : "memory");
+    // Both have landed: no stores have been issued that the first tile's waits could count.
+    asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
 #pragma unroll
     for (int i = 0; i < TM; ++i) { X[i] = frag_x(0, i); ex[i] = scale_x(0, i); }
 #pragma unroll
