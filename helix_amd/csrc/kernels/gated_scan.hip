@@ -186,8 +186,9 @@ HELIX_DEV unsigned tile_index(const HelixGatedScanJoin& j) {
 }
 
 // The tokens of a wave in one tensor, from its first token: a lane's own start at
-// `voff`, `tok` bytes apart. A lane without channels is out of range, as a token
-// past the sequence is: it reads zeros and writes nothing.
+// `voff`, `tok` bytes apart. A lane without channels is out of range: it reads zeros
+// and writes nothing. So is a token past the sequence where rows do not overlap, as
+// those that are written never do.
 struct WaveRows {
     helix_rsrc r;
     int voff, tok;
@@ -211,11 +212,16 @@ HELIX_DEV void not_earlier(W& w) {
     for (int i = 0; i < (int)(sizeof(w) / 4); ++i) w[i] = (unsigned)vgpr_fresh((int)w[i]);
 }
 
-// A token that does not exist has an infinite gate: the state passes through it.
+// A token that does not exist has an infinite gate and brings nothing (u: v, or backward
+// dh): the state passes through it. Where a tensor's tokens lie closer than a row is
+// long (all of them one row, say), its place is inside the resource's range.
 template <typename T>
-HELIX_DEV void shut_out(typename Raw4<T>::type& g, bool exists) {
+HELIX_DEV void shut_out(typename Raw4<T>::type& g, typename Raw4<T>::type& u, bool exists) {
 #pragma unroll
-    for (int i = 0; i < (int)(sizeof(g) / 4); ++i) g[i] = exists ? g[i] : inf_bits<T>;
+    for (int i = 0; i < (int)(sizeof(g) / 4); ++i) {
+        g[i] = exists ? g[i] : inf_bits<T>;
+        u[i] = exists ? u[i] : 0;
+    }
 }
 
 template <typename T, bool VEC, int NW>
@@ -237,7 +243,7 @@ HELIX_DEV void gated_scan_tile(const HelixGatedScanParams& p, unsigned tile) {
     for (int k = 0; k < R; ++k) vw[k] = buf_load4<T, VEC>(v.r, v.voff + k * v.tok, own);
     if (tokens < 4 * R) {
 #pragma unroll
-        for (int k = 0; k < R; ++k) shut_out<T>(gw[k], skip + k < tokens);
+        for (int k = 0; k < R; ++k) shut_out<T>(gw[k], vw[k], skip + k < tokens);
     }
     float f[R][4], b[R][4], ra[4], rb[4], s[4];
 #pragma unroll
@@ -325,7 +331,7 @@ HELIX_DEV void gated_scan_bwd_tile(const HelixGatedScanBwdParams& p, unsigned ti
     const WaveRows g = wave_rows<T>(p.g, seq * p.seq_g + t * p.tok_g + c0, p.tok_g, tokens, width, skip, any);
     const WaveRows d = wave_rows<T>(p.dh, seq * p.seq_dh + t * p.tok_dh + c0, p.tok_dh, tokens, width, skip, any);
     const WaveRows v = wave_rows<T>(p.v, seq * p.seq_v + t * p.tok_v + c0, p.tok_v, tokens, width, skip, any);
-    // h of the token before each; before token 0 there is none (zeros, and h0 below).
+    // h of the token before each; before token 0 there is none (h0 below).
     const int back = t > 0 ? 1 : 0;
     const WaveRows h = wave_rows<T>(p.h, seq * p.seq_h + (t - back) * p.tok_h + c0, p.tok_h, tokens - 1 + back, width,
                                     skip - 1 + back, any);
@@ -340,7 +346,7 @@ HELIX_DEV void gated_scan_bwd_tile(const HelixGatedScanBwdParams& p, unsigned ti
     for (int k = 0; k < R; ++k) hw[k] = buf_load4<T, VEC>(h.r, h.voff - k * h.tok, own);
     if (tokens < 4 * R) {
 #pragma unroll
-        for (int k = 0; k < R; ++k) shut_out<T>(gw[k], skip - k >= 0);
+        for (int k = 0; k < R; ++k) shut_out<T>(gw[k], dw[k], skip - k >= 0);
     }
     float f[R][4], u[R][4], ra[4], rb[4], s[4];
 #pragma unroll
@@ -371,10 +377,9 @@ HELIX_DEV void gated_scan_bwd_tile(const HelixGatedScanBwdParams& p, unsigned ti
         widen4<T>(dw[k], df);
         widen4<T>(vw[k], vf);
         widen4<T>(hw[k], past);
-        if (t == 0 && skip == k && p.h0) {   // token 0
+        if (t == 0 && skip == k) {   // token 0
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (i < own) past[i] = p.h0[at + 4 * (lane & 15) + i];
+            for (int i = 0; i < 4; ++i) past[i] = p.h0 && i < own ? p.h0[at + 4 * (lane & 15) + i] : 0.0f;
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
