@@ -112,16 +112,21 @@ HELIX_DEV float state_before(const HelixGatedScanJoin& j, long long stream, int 
     return state;
 }
 
+// v has been loaded before anything that follows reaches memory.
+HELIX_DEV void arrived(float& v) { asm volatile("" : "+v"(v)::"memory"); }
+
 // From the (A, B) of a thread's run of four channels to the state that enters it.
 // `start`, the state before the first chunk (64 channels; null: zero), and `end`,
-// where the last chunk leaves its state (null: nowhere), are of the tile's channels,
-// of which there are `width`.
+// where the last chunk leaves its state (null: nowhere; maybe start's memory), are of
+// the tile's channels, of which there are `width`.
 template <int NW>
 HELIX_DEV void entering(const HelixGatedScanJoin& j, long long stream, int chunk, const float* start, float* end,
                         int width, const float (&run_a)[4], const float (&run_b)[4], float (&state)[4]) {
     __shared__ float2 sum[NW][64];
     __shared__ float in[NW][64];
     const int lane = lane_id(), wave = wave_id(), q = lane >> 4, c4 = 4 * (lane & 15);
+    // Read before the chunk is published, and only by chunks that the last one waits for: `end` may be `start`.
+    float s = wave == 0 && start && chunk < HELIX_GS_GROUP && lane < width ? start[lane] : 0.0f;
     float a[4], b[4];   // of the wave's runs up to this one
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -145,6 +150,7 @@ HELIX_DEV void entering(const HelixGatedScanJoin& j, long long stream, int chunk
     if (wave == 0) {
         const int c = lane;
         const bool many = j.n_chunk > 1, final = chunk == j.n_chunk - 1;
+        arrived(s);
         if (many && !final) {
             float ca = 1.0f, cb = 0.0f;
 #pragma unroll
@@ -157,7 +163,6 @@ HELIX_DEV void entering(const HelixGatedScanJoin& j, long long stream, int chunk
             __hip_atomic_store(j.part + ((stream * j.n_chunk + chunk) * 64 + c), word, __ATOMIC_RELAXED,
                                __HIP_MEMORY_SCOPE_AGENT);
         }
-        float s = start && c < width ? start[c] : 0.0f;
         if (many && chunk) s = state_before(j, stream, chunk, s);
 #pragma unroll
         for (int w = 0; w < NW; ++w) {

@@ -4,15 +4,11 @@ A workgroup of matmul_tiles (kernels/matmul_fp8.hip) loads steps of the sum into
 its later accesses that may still be under way. A wave's accesses are followed here from the kernel's entry along every
 branch, and at each barrier the loads that the reads after it need have to be covered by a wait, in a workgroup's first
 tile as in those that follow one. Timing hides a wait that is too weak, so no result can show it."""
-import os
 import re
-import subprocess
 
 import pytest
 
-ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
-HSACO = os.path.join(ROOT, "helix_amd", "csrc", "_build", "helix_kernels.hsaco")
-OBJDUMP = "/opt/rocm/llvm/bin/llvm-objdump"
+import built_code
 
 # Kernels by the tiles of a wave, TM x TN: a step's loads are TM of X and TN of Y; X and the first half of Y are read after
 # a step's second barrier, the rest of Y after the next step's first.
@@ -22,19 +18,11 @@ KERNELS = {"helix_matmul_fp8_t88": (8, 8), "helix_matmul_fp8_t86": (8, 6), "heli
 COUNTED = 63   # the counter's largest value: an access that would pass it is not issued before the oldest is done
 
 
-def parse(text):
-    """[(what, argument)] of a kernel's disassembly, in order: ("load",) into LDS of a step's rows, ("other",) access,
-    ("wait", n), ("barrier",), ("go", index) and ("maybe", index) branches, ("end",)."""
-    lines = []
-    for line in text.splitlines():
-        m = re.match(r"\s+(\S+)\s*(.*?)\s*//\s*([0-9A-Fa-f]+):", line)
-        if m:
-            target = re.search(r"<\w+\+0x([0-9a-f]+)>", line)
-            lines.append((m.group(1), m.group(2), int(m.group(3), 16), int(target.group(1), 16) if target else None))
-    start = lines[0][2]
-    at, ops = {}, []
-    for name, rest, address, target in lines:
-        at[address - start] = len(ops)
+def accesses(code):
+    """[(what, argument)] of a kernel's instructions, in order: ("load",) into LDS of a step's rows, ("other",) access,
+    ("wait", n), ("barrier",), ("go", index) and ("maybe", index) branches, ("end",), ("",) for all else."""
+    ops = []
+    for name, rest, target in code:
         if name.startswith("s_branch"):
             ops.append(("go", target))
         elif name.startswith("s_cbranch"):
@@ -43,13 +31,13 @@ def parse(text):
             ops.append(("barrier",))
         elif name == "s_endpgm":
             ops.append(("end",))
-        elif name == "s_waitcnt":
-            m = re.search(r"vmcnt\((\d+)\)", rest)
-            if m:
-                ops.append(("wait", int(m.group(1))))
+        elif name == "s_waitcnt" and "vmcnt" in rest:
+            ops.append(("wait", int(re.search(r"vmcnt\((\d+)\)", rest).group(1))))
         elif re.match(r"(buffer|global|flat|scratch)_(load|store|atomic)", name):
             ops.append(("load",) if name == "buffer_load_dwordx4" and rest.endswith("lds") else ("other",))
-    return [(op[0], at[op[1]]) if op[0] in ("go", "maybe") else op for op in ops]
+        else:
+            ops.append(("",))
+    return ops
 
 
 def uncovered(ops, tm, tn):
@@ -64,10 +52,11 @@ def uncovered(ops, tm, tn):
     while todo:
         pc, turn, queue, issued = todo.pop()
         while True:
-            if (pc, turn, queue, issued) in seen:
-                break
-            seen.add((pc, turn, queue, issued))
             what = ops[pc]
+            if what[0] in ("maybe", "barrier"):
+                if (pc, turn, queue, issued) in seen:
+                    break
+                seen.add((pc, turn, queue, issued))
             if what[0] == "end":
                 break
             if what[0] == "go":
@@ -81,7 +70,7 @@ def uncovered(ops, tm, tn):
                 queue = (queue + "o")[-COUNTED:]
             elif what[0] == "wait":
                 queue = queue[max(0, len(queue) - what[1]):]
-            else:
+            elif what[0] == "barrier":
                 # Turn -1, the prologue's barrier: the first step's X and half of Y; 0: the rest of this step's Y;
                 # 1: the next step's X and half of Y.
                 needed = (first, each, each + first)[turn + 1]
@@ -119,20 +108,12 @@ def test_a_weak_wait_is_seen():
 
 @pytest.fixture(scope="module")
 def built():
-    if not (os.path.exists(HSACO) and os.path.exists(OBJDUMP)):
-        pytest.skip("needs the built code object and llvm-objdump")
-    out = subprocess.run([OBJDUMP, "-d", HSACO], check=True, capture_output=True, text=True).stdout
-    blocks = {}
-    for block in re.split(r"\n(?=[0-9a-f]+ <)", out):
-        name = re.match(r"[0-9a-f]+ <(\w+)>", block)
-        if name and name.group(1) in KERNELS:
-            blocks[name.group(1)] = block
-    return blocks
+    return built_code.kernels("|".join(KERNELS))
 
 
 @pytest.mark.parametrize("name", sorted(KERNELS))
 def test_tiles_wait_for_what_they_read(built, name):
     tm, tn = KERNELS[name]
-    ops = parse(built[name])
+    ops = accesses(built[name])
     assert sum(op[0] == "load" for op in ops) >= 4 * (tm + tn) and sum(op[0] == "barrier" for op in ops) >= 9
     assert uncovered(ops, tm, tn) == set()
