@@ -11,8 +11,11 @@ from .layer import (FP8, FP8_BLOCK, FP8_SCALE, IO_DTYPES, device_index, expect, 
 def matmul_fp8(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale: torch.Tensor, *,
                out_dtype: torch.dtype = torch.bfloat16, out: torch.Tensor | None = None,
                stream: torch.cuda.Stream | None = None) -> torch.Tensor:
-    """a [..., k] times b [n, k] transposed: [..., n], summed in float32 and rounded once to out_dtype (float32,
-    bfloat16 or float16), or into `out`.
+    """a [..., k] times b [n, k] transposed: [..., n] in out_dtype (float32, bfloat16 or float16), or into `out`.
+
+    Sums are float32. float32 results are sums of exact products; for the 16-bit ones, rounded once, the matrix
+    instruction cuts each of eight neighbouring products at 2^-13 of the largest of them (2e-5 of a result on ordinary
+    operands, and no less where products cancel: include/helix/helix_layer.h).
 
     a and b are float8_e4m3fn, a_scale [..., ceil(k / 128)] and b_scale [n, ceil(k / 128)] float8_e8m0fnu, as
     rms_norm_fp8 and quantize_fp8 leave them. Rows of a and b start at multiples of 16 bytes; k is any length."""
