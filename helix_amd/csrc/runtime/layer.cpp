@@ -81,12 +81,22 @@ void launch(hipFunction_t f, void* stream, unsigned gx, unsigned gy, unsigned th
     launch_args(f, stream, gx, gy, threads, args);
 }
 
-unsigned grid(long long n) {
-    need(n <= 0x7fffffffLL, "launch grid exceeds 2^31 workgroups");
+// A launch counts its threads along x in 32 bits, and one of more begins with as few as the lowest 32 bits say, without
+// an error: what may be more is launched in slices.
+constexpr long long most_groups(int threads) { return ((1LL << 32) - 1) / threads; }
+
+unsigned grid(long long n, int threads) {
+    need(n <= most_groups(threads), "launch grid exceeds 2^32 threads");
     return (unsigned)n;
 }
 
 long long ceil_div(long long a, long long b) { return (a + b - 1) / b; }
+
+// p, if there is one, `elements` of `size` bytes on.
+template <typename T>
+void advance(T*& p, long long elements, size_t size) {
+    if (p) p = (T*)((uintptr_t)p + elements * (long long)size);
+}
 
 // Runs an entry point's body: no exception leaves it.
 template <typename F>
@@ -164,10 +174,23 @@ void norm(helix_ctx* ctx, void* stream, const helix_norm_args* a, bool quantize)
     // A wave each (four to a workgroup) where they give every CU four: 8192 rows of 512 and of 1024 6.8 and 10.9 us, as
     // workgroups 12.3 and 13.8; 128 and 512 rows of 2048 4.0 and 4.3 us, as workgroups 3.4 and 3.9.
     const std::string form = norm_form(a->dim, a->dim <= 4 * 512 && a->rows >= 4 * 256);
-    const unsigned gx = grid(form[0] && form[1] == 'w' ? ceil_div(a->rows, 4) : a->rows);
+    const int each = form[0] && form[1] == 'w' ? 4 : 1;   // rows of a workgroup
+    need(ceil_div(a->rows, each) <= 0x7fffffffLL, "launch grid exceeds 2^31 workgroups");
     const hipFunction_t f = kernel(ctx, std::string("helix_norm_") + kTags[a->io_dtype] + form);
     const OnDevice on(ctx->device);
-    launch(f, stream, gx, 1, kNormThreads, p);
+    const long long most = each * most_groups(kNormThreads);
+    for (long long left = a->rows; left > 0; left -= most) {
+        p.rows = std::min(left, most);
+        launch(f, stream, grid(ceil_div(p.rows, each), kNormThreads), 1, kNormThreads, p);
+        if (left <= most) break;
+        advance(p.x, most * p.ld_x, es);
+        advance(p.residual, most * p.ld_residual, es);
+        advance(p.h, most * p.ld_h, es);
+        advance(p.y, most * p.ld_y, es);
+        advance(p.q, most * p.ld_q, 1);
+        advance(p.scale, most * p.ld_scale, 1);
+        advance(p.rstd, most, sizeof(float));
+    }
 }
 
 // Whether the backward pass gives a row to a wave: up to two chunks of 512, more would not fit in its registers with their
@@ -239,7 +262,7 @@ extern "C" helix_status helix_norm_backward_encode(helix_ctx* ctx, void* stream,
         p.part_rows = p.parts ? ceil_div(a->rows, p.parts) : 0;
         const std::string tag = kTags[a->io_dtype];
         const std::string form = norm_form(a->dim, norm_waves(a->dim));
-        const unsigned gx = grid(a->rows);
+        const unsigned gx = a->rows && form.empty() ? grid(a->rows, kNormThreads) : (unsigned)p.parts;
         const unsigned gc = (unsigned)ceil_div(a->dim, kNormThreads), gd = (unsigned)ceil_div(a->dim, 32);
         const hipFunction_t dx = kernel(ctx, "helix_norm_bwd_" + tag + form), part = kernel(ctx, "helix_norm_dw_part_" + tag),
                             dw = kernel(ctx, "helix_norm_dw");
@@ -248,7 +271,7 @@ extern "C" helix_status helix_norm_backward_encode(helix_ctx* ctx, void* stream,
             if (p.dweight) launch(part, stream, gc, (unsigned)p.parts, kNormThreads, p);
             launch(dx, stream, gx, 1, kNormThreads, p);
         } else if (a->rows) {
-            launch(dx, stream, (unsigned)p.parts, 1, kNormThreads, p);
+            launch(dx, stream, gx, 1, kNormThreads, p);
         }
         if (p.dweight) launch(dw, stream, gd, 1, 1024, p);
     });
@@ -383,13 +406,21 @@ extern "C" helix_status helix_matmul_fp8_encode(helix_ctx* ctx, void* stream, co
             kernel(ctx, plan.bm ? std::string("helix_matmul_fp8") + plan.kernel
                                 : std::string("helix_matmul_fp8_") + kTags[a->out_dtype] + plan.kernel);
         if (plan.rows) {
-            const unsigned gx = grid(ceil_div(a->n, 16)), gy = (unsigned)ceil_div(a->m, plan.rows);
+            const unsigned gy = (unsigned)ceil_div(a->m, plan.rows);
             const OnDevice on(ctx->device);
-            launch(f, stream, gx, gy, 64 * plan.waves, p);
+            const int threads = 64 * plan.waves, most = (int)(16 * most_groups(threads));
+            for (long long left = a->n; left > 0; left -= most) {
+                p.n = (int)std::min<long long>(left, most);
+                launch(f, stream, grid(ceil_div(p.n, 16), threads), gy, threads, p);
+                if (left <= most) break;
+                advance(p.b, most * p.ld_b, 1);
+                advance(p.b_scale, most * p.ld_b_scale, 1);
+                advance(p.c, most, kBytes[a->out_dtype]);
+            }
             return;
         }
         if (!plan.bm) {
-            const unsigned gx = grid(ceil_div(a->m, 64) * ceil_div(a->n, 128));
+            const unsigned gx = grid(ceil_div(a->m, 64) * ceil_div(a->n, 128), 256);
             const OnDevice on(ctx->device);
             launch(f, stream, gx, 1, 256, p);
             return;
@@ -406,8 +437,9 @@ extern "C" helix_status helix_matmul_fp8_encode(helix_ctx* ctx, void* stream, co
         p.inv_rest = reciprocal((unsigned)(mt % p.gm));
         p.stride = (int)std::min<long long>(tiles, 256LL * plan.per_cu);
         p.f16 = a->out_dtype == HELIX_F16;
-        const unsigned ga = grid(ceil_div((long long)a->m * plan.pitch, 256)), gb = grid(ceil_div((long long)a->n * plan.pitch, 256));
-        const unsigned gj = grid(ceil_div((long long)a->m * ceil_div(a->n, 4), 256));
+        const unsigned ga = grid(plan.a_bytes ? ceil_div((long long)a->m * plan.pitch, 256) : 0, 256),
+                       gb = grid(plan.b_bytes ? ceil_div((long long)a->n * plan.pitch, 256) : 0, 256),
+                       gj = grid(plan.parts > 1 ? ceil_div((long long)a->m * ceil_div(a->n, 4), 256) : 0, 256);
         const hipFunction_t copy = kernel(ctx, "helix_fp8_scales"),
                             join = kernel(ctx, std::string("helix_matmul_fp8_join_") + kTags[a->out_dtype]);
         const OnDevice on(ctx->device);
@@ -467,14 +499,13 @@ ScanPlan scan_plan(long long n_seq, long long n_tok, long long n_chan, int run, 
 // beyond 2^29 bytes.
 bool far_rows(long long tok, size_t es) { return tok >= (1LL << 29) / 33 / (long long)es; }
 
-// Fills in a plan, and runs it: P is HelixGatedScanParams or its backward form.
-template <typename A, typename P>
-void run_scan(helix_ctx* ctx, void* stream, const A& a, P& p, const char* name, int run, bool far) {
+// Fills in a plan, and runs it: P is HelixGatedScanParams or its backward form, ahead(p, n) takes p n sequences on.
+template <typename A, typename P, typename F>
+void run_scan(helix_ctx* ctx, void* stream, const A& a, P& p, const char* name, int run, bool far, F&& ahead) {
     const ScanPlan plan = scan_plan(a.n_seq, a.n_tok, a.n_chan, run, far);
     need(plan.bytes == 0 || (a.scratch && a.scratch_bytes >= plan.bytes), "scratch smaller than its _scratch_size()",
          HELIX_ERR_SCRATCH_TOO_SMALL);
     need(aligned(a.scratch, 16), "scratch is not 16-byte aligned");
-    p.n_seq = a.n_seq;
     p.n_tok = a.n_tok;
     p.n_chan = a.n_chan;
     p.n_slab = plan.n_slab;
@@ -482,28 +513,30 @@ void run_scan(helix_ctx* ctx, void* stream, const A& a, P& p, const char* name, 
     p.join.n_chunk = plan.n_chunk;
     p.join.n_group = plan.n_group;
     const std::string base = std::string(name) + kTags[a.io_dtype] + (a.n_chan % 4 ? "_s" : "_v");   // (channels that come in fours, or not)
-    const unsigned gx = grid(plan.waves ? plan.streams * plan.n_chunk
-                                        : ceil_div(a.n_seq * ceil_div(a.n_chan, 4), kScanThreads));
+    const int threads = plan.waves ? 64 * plan.waves : kScanThreads;
+    // Sequences of a launch.
+    const long long most = plan.waves ? most_groups(threads) / ((long long)plan.n_slab * plan.n_chunk)
+                                      : most_groups(threads) * threads / ceil_div(a.n_chan, 4);
+    need(most > 0, "launch grid exceeds 2^32 threads");
     const hipFunction_t f = kernel(ctx, plan.waves ? base + "_w" + std::to_string(plan.waves) : base + "_steps");
-    if (!plan.bytes) {
-        const OnDevice on(ctx->device);
-        launch(f, stream, gx, 1, plan.waves ? 64 * plan.waves : kScanThreads, p);
-        return;
-    }
+    const hipFunction_t ff = plan.bytes ? kernel(ctx, "helix_gated_scan_fill") : nullptr;
     char* sc = static_cast<char*>(a.scratch);
-    p.join.ticket = reinterpret_cast<unsigned*>(sc);
-    p.join.part = reinterpret_cast<unsigned long long*>(sc + plan.part_at);
-    p.join.left = reinterpret_cast<unsigned*>(sc + plan.left_at);
-    struct {
-        void* p;
-        long long n;
-    } fill{sc, (long long)(plan.bytes / 16)};
-    const hipFunction_t ff = kernel(ctx, "helix_gated_scan_fill");
-    const unsigned gf = grid(ceil_div(fill.n, kScanThreads));
     const OnDevice on(ctx->device);
-    void* args[] = {&fill.p, &fill.n};
-    launch_args(ff, stream, gf, 1, kScanThreads, args);
-    launch(f, stream, gx, 1, 64 * plan.waves, p);
+    for (long long left = a.n_seq; left > 0; left -= most) {
+        p.n_seq = (int)std::min(left, most);
+        const ScanPlan slice = scan_plan(p.n_seq, a.n_tok, a.n_chan, run, far);
+        if (slice.bytes) {
+            p.join.ticket = reinterpret_cast<unsigned*>(sc);
+            p.join.part = reinterpret_cast<unsigned long long*>(sc + slice.part_at);
+            p.join.left = reinterpret_cast<unsigned*>(sc + slice.left_at);
+            long long n = (long long)(slice.bytes / 16);
+            void* args[] = {&sc, &n};
+            launch_args(ff, stream, grid(ceil_div(n, kScanThreads), kScanThreads), 1, kScanThreads, args);
+        }
+        const long long groups = plan.waves ? slice.streams * plan.n_chunk : ceil_div(p.n_seq * ceil_div(a.n_chan, 4), kScanThreads);
+        launch(f, stream, grid(groups, threads), 1, threads, p);
+        if (left > most) ahead(p, most);
+    }
 }
 
 template <typename A>
@@ -551,7 +584,13 @@ extern "C" helix_status helix_gated_scan_encode(helix_ctx* ctx, void* stream, co
         const size_t es = kBytes[a->io_dtype];
         bool far = false;
         for (const long long tok : {(long long)a->tok_g, (long long)a->tok_v, (long long)a->tok_h}) far |= far_rows(tok, es);
-        run_scan(ctx, stream, *a, p, "helix_gated_scan_", HELIX_GS_RUN, far);
+        run_scan(ctx, stream, *a, p, "helix_gated_scan_", HELIX_GS_RUN, far, [&](HelixGatedScanParams& q, long long n) {
+            advance(q.g, n * q.seq_g, es);
+            advance(q.v, n * q.seq_v, es);
+            advance(q.h, n * q.seq_h, es);
+            advance(q.h0, n * a->n_chan, sizeof(float));
+            advance(q.last, n * a->n_chan, sizeof(float));
+        });
     });
 }
 
@@ -597,7 +636,17 @@ extern "C" helix_status helix_gated_scan_backward_encode(helix_ctx* ctx, void* s
         const size_t es = kBytes[a->io_dtype];
         bool far = false;
         for (const long long tok : {(long long)a->tok_dh, (long long)a->tok_g, (long long)a->tok_v, (long long)a->tok_h, (long long)a->tok_dg, (long long)a->tok_dv}) far |= far_rows(tok, es);
-        run_scan(ctx, stream, *a, p, "helix_gated_scan_bwd_", HELIX_GS_RUN_BWD, far);
+        run_scan(ctx, stream, *a, p, "helix_gated_scan_bwd_", HELIX_GS_RUN_BWD, far, [&](HelixGatedScanBwdParams& q, long long n) {
+            advance(q.dh, n * q.seq_dh, es);
+            advance(q.g, n * q.seq_g, es);
+            advance(q.v, n * q.seq_v, es);
+            advance(q.h, n * q.seq_h, es);
+            advance(q.dg, n * q.seq_dg, es);
+            advance(q.dv, n * q.seq_dv, es);
+            advance(q.h0, n * a->n_chan, sizeof(float));
+            advance(q.dh_last, n * a->n_chan, sizeof(float));
+            advance(q.dh0, n * a->n_chan, sizeof(float));
+        });
     });
 }
 
