@@ -4,6 +4,7 @@ tensors, streams, scratch and errors. The arithmetic runs in the HIP kernels of 
 from __future__ import annotations
 
 import contextlib
+import struct
 
 import torch
 
@@ -91,6 +92,14 @@ def scratch(index: int, st: int, stream, nbytes: int) -> torch.Tensor | None:
     return _scratch_for(index, st, nbytes, stream)
 
 
+def packed(pack, *fields) -> bytes:
+    """pack(*fields), an argument struct of helix_amd.abi; what its fields cannot hold is refused."""
+    try:
+        return pack(*fields)
+    except (struct.error, OverflowError) as e:
+        raise ValueError(f"a size, a stride or eps is out of range: {e}") from None
+
+
 def run(fn, index: int, st: int, args: bytes) -> None:
     ctx = _contexts.get(index) or context(index)
     rc = fn(ctx.handle, st, args)
@@ -103,7 +112,7 @@ def run_with_scratch(fn, size, index: int, st: int, stream, pack) -> None:
     It is asked for them once the call has been refused without (nothing is enqueued then): the small calls, whose time
     on the host counts, want none."""
     ctx = _contexts.get(index) or context(index)
-    args = pack(0, 0)
+    args = packed(pack, 0, 0)
     rc = fn(ctx.handle, st, args)
     if rc == HELIX_ERR_SCRATCH_TOO_SMALL:
         need = size(args)

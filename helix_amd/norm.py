@@ -11,8 +11,8 @@ from __future__ import annotations
 import torch
 
 from . import abi
-from .layer import (FP8, FP8_BLOCK, FP8_SCALE, IO_DTYPES, device_index, empty, expect, io_code, ptr, row_stride, rows_like, run,
-                    scratch, stream_handle, under)
+from .layer import (FP8, FP8_BLOCK, FP8_SCALE, IO_DTYPES, device_index, empty, expect, io_code, packed, ptr, row_stride,
+                    rows_like, run, scratch, stream_handle, under)
 
 
 def _weight_code(weight: torch.Tensor, x: torch.Tensor) -> int:
@@ -63,9 +63,9 @@ def _norm(op, fn, x, weight, residual, eps, fp8, want_rstd, stream):
         if want_rstd:
             rstd = empty(x.shape[:-1], torch.float32, x.device)
     pitch = -(-dim // 16) * 16
-    args = abi.NORM_STRUCT.pack(x.numel() // dim, dim, io, w_code, eps, x.data_ptr(), ptr(residual), ptr(weight),
-                                0 if h is x else h.data_ptr(), ptr(y), ptr(q), ptr(scale), ptr(rstd), ld_x, ld_r, dim,
-                                dim, pitch, -(-dim // (4 * FP8_BLOCK)) * 4)
+    args = packed(abi.NORM_STRUCT.pack, x.numel() // dim, dim, io, w_code, eps, x.data_ptr(), ptr(residual), ptr(weight),
+                  0 if h is x else h.data_ptr(), ptr(y), ptr(q), ptr(scale), ptr(rstd), ld_x, ld_r, dim, dim, pitch,
+                  -(-dim // (4 * FP8_BLOCK)) * 4)
     run(fn, index, stream_handle(index, stream), args)
     return y, q, scale, h, rstd
 
@@ -133,7 +133,7 @@ def rms_norm_backward(dy: torch.Tensor, h: torch.Tensor, weight: torch.Tensor, r
                                              ld_dy, ld_h, ld_dh, dim)
 
     L = abi.lib()
-    need = L.helix_norm_backward_scratch_size(pack(0, 0))
+    need = L.helix_norm_backward_scratch_size(packed(pack, 0, 0))
     buf = scratch(index, st, stream, need)
     run(L.helix_norm_backward_encode, index, st, pack(ptr(buf), need))
     return dx, dweight
