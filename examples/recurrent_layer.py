@@ -61,6 +61,30 @@ class Served:
         return matmul_fp8(q, scale, *self.w_out, out_dtype=x.dtype), residual, state
 
 
+class Decoder:
+    """Single tokens through a captured step: a replay takes the state that the one before left."""
+
+    def __init__(self, layer: Served, state, dtype=torch.bfloat16):
+        dim = layer.norm_in.shape[0]
+        self.state = state.clone()
+        self.x, self.residual = (torch.zeros(state.shape[0], 1, dim, dtype=dtype, device=state.device) for _ in range(2))
+        layer(self.x, self.residual, self.state)   # (what a first call does once is not captured)
+        self.graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(self.graph):
+            self.out, self.left, after = layer(self.x, self.residual, self.state)
+            self.state.copy_(after)
+
+    def __call__(self, x, residual=None):
+        """x, residual [sequences, 1, dim]: (out, residual) in memory that the next call writes again."""
+        self.x.copy_(x)
+        if residual is None:
+            self.residual.zero_()
+        else:
+            self.residual.copy_(residual)
+        self.graph.replay()
+        return self.out, self.left
+
+
 class Norm(torch.autograd.Function):
     """rms_norm of x + residual: (y, h)."""
 
@@ -146,18 +170,18 @@ def main() -> None:
     print(f"prompt of {a.prompt}: {clock(lambda: layer(x[:, :a.prompt]), 20):.0f} us a layer")
     token = x[:, :1].contiguous()
     print(f"one token: {clock(lambda: layer(token, token, state), 200):.0f} us a layer")
-    graph = torch.cuda.CUDAGraph()
-    with torch.cuda.graph(graph):
-        layer(token, token, state)
-    print(f"one token, captured: {clock(graph.replay, 200):.0f} us a layer")
-    steps = []
+    print(f"one token, captured, the state carried: {clock(Decoder(layer, state).graph.replay, 200):.0f} us a layer")
+    decoder = Decoder(layer, state)
+    steps, captured = [], []
     for t in range(a.prompt, a.prompt + a.tokens):
         out, _, state = layer(x[:, t:t + 1], None, state)
         steps.append(out)
+        captured.append(decoder(x[:, t:t + 1])[0].clone())
     whole = layer(x)[0][:, a.prompt:].float()
     if steps:
         error = (torch.cat(steps, 1).float() - whole).norm() / whole.norm()
         print(f"{a.tokens} tokens one by one against all at once: {error.item():.2e}")
+        print(f"captured and eager tokens are equal: {torch.equal(torch.cat(captured, 1), torch.cat(steps, 1))}")
     losses = train(w, x[:, :min(a.prompt, 1024)], torch.randn_like(x[:, :min(a.prompt, 1024)]), a.train_steps)
     print("training loss: " + ", ".join(f"{v:.4f}" for v in losses))
 
