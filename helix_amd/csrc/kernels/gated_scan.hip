@@ -28,9 +28,9 @@
 // scope, which go past the L2s of the XCDs. The parts are joined in the order of
 // time, whoever arrives first: results do not depend on it.
 //
-// Memory binds it. 8192 tokens of 4096 channels (bf16) take 52 us, 201 MB moved at
-// 3.9 TB/s; 3 x 1003 of 5184 (f32) 44 us, 4.3 TB/s; backward 8 x 4096 of 5120 (bf16)
-// 408 us, 4.9 TB/s, where a copy of 4 GiB reaches 4.6. Runs of 4 tokens instead of 8
+// Memory binds it. 8192 tokens of 4096 channels (bf16) take 51 us, 201 MB moved at
+// 4.0 TB/s; 3 x 1003 of 5184 (f32) 47 us, 4.0 TB/s; backward 8 x 4096 of 5120 (bf16)
+// 400 us, 5.0 TB/s, where a copy of 4 GiB reaches 4.6. Runs of 4 tokens instead of 8
 // took 62-66 us forward (twice the joins per value); backward, which holds twice the
 // words of a token, runs of 8 spill and took 422 us, of 2 532. Groups of 16 chunks
 // instead of 8 took 65 and 561 us: their words cost a wave of each SIMD. Stores that

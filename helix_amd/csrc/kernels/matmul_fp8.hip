@@ -326,7 +326,7 @@ __device__ void matmul_rows(const HelixMatmulParams& p) {
 // GHz, two thirds of the products' own rate at that clock. Smaller tiles: 192 rows 440 us,
 // 128 rows 496, 128 x 128 in two workgroups per CU 573. Products of 32 x 32 x 64 run at
 // 3.5 PFLOP/s where those of 16 x 16 x 128 run at 4.1, and took 526 us in this loop's
-// first form, against 457. 8192 x 10304 x 2048 take 155 us, 32768 x 2560 x 5120 311.
+// first form, against 457. 8192 x 10304 x 2048 take 156 us, 32768 x 2560 x 5120 314.
 
 struct TileAt {
     int i, j;
@@ -409,7 +409,8 @@ __device__ void matmul_tiles(const HelixMatmulParams& p) {
     int vx[NX], vy[NY], vsx, vsy;
     const int stride = p.stride;
     int pkb = 0, qt = blockIdx.x, qg = 0;   // where the data's and the scales' loads are
-    // Rows and columns past the matrices are out of the resources' range and come as zeros.
+    // Rows and columns past the matrices are out of the resources' range and come as zeros. The last row is read to the end
+    // of its last 16 bytes, and of its scales' last four, which lie in no other page than a byte of the row.
     auto aim_data = [&](int t) {
         const TileAt at = tile_at(t);
         const int k16 = (k + 15) & ~15;

@@ -296,7 +296,8 @@ struct Tiling {
     double step, tile;   // us of a step of 128 and of the rest of a tile, with every CU at work
 };
 // Fitted to 8192 x 8192 x 8192, 8192 x 10304 x 2048 and 32768 x 2560 x 5120: the large tiles take 20e-6 us per element
-// and step, the small ones up to 33e-6, but waste less of a last round.
+// and step, the small ones up to 33e-6, but waste less of a last round. Of one or two rounds it says too little (2871 x
+// 5183 x 2560: 36 us, measured 48).
 const Tiling kTilings[] = {
     {"_t88", 256, 256, 1, 1.38, 6.4}, {"_t86", 192, 256, 1, 1.04, 6.4}, {"_t84", 128, 256, 1, 0.93, 2.2},
     {"_t44", 128, 128, 2, 1.10, 1.5}, {"_t42", 64, 128, 2, 0.75, 1.2},
@@ -314,7 +315,10 @@ MatmulPlan matmul_plan(const helix_matmul_fp8_args& a) {
         const long long tiles = ceil_div(m, 16), ny = ceil_div(tiles, 4), each = ceil_div(tiles, ny);
         p.rows = (int)(16 * each);
         p.kernel = "_r" + std::to_string(each);
-        if (each == 1 && n >= 8192) p.kernel = "_r1w4", p.waves = 4;   // (10304 x 2048: 7.0 -> 6.3 us)
+        // Four waves where workgroups are many: eight and four for one row of 2048 x 8192, 16384 and 32768 5.6 and 5.4, 9.5
+        // and 8.3, 16.8 and 13.2 us, of 1024 x 10304 5.2 and 4.5, of 4096 x 10304 11.4 and 11.3 (16 rows 15.2 and 15.7); below
+        // within 0.2 us of each other (2048 x 4096: 3.9 and 3.9; 4096 x 4096: 6.0 and 6.2).
+        if (each == 1 && n >= 8192) p.kernel = "_r1w4", p.waves = 4;
         best = 4 + (double)ceil_div(n, 16) * k * 16 * (ny + tiles) / 8e6;
         if (m <= 16) return p;
     }
