@@ -148,6 +148,8 @@ helix_status helix_matmul_fp8_encode(helix_ctx* ctx, void* stream, const helix_m
 /* Per sequence and channel, with f_t = sigmoid(g_t) and the state in fp32:
  *   h_t = f_t h_(t-1) + (1 - f_t) v_t,   h_(-1) = h0
  * g = +inf keeps the state and takes no v (a finite v), g = -inf takes v alone.
+ * An infinite v or h0 leaves its channel infinite or NaN from its token on (NaN
+ * where the product of the gates since has reached zero in fp32).
  * n_tok = 1 is the step of a single token. h0, last, dh_last and dh0 are dense
  * fp32 (n_seq, n_chan); last may be h0. */
 typedef struct {
