@@ -48,29 +48,29 @@ def _norm_bwd(rows, dim, groups, store="bf16", gate=True):
 def listed():
     cases = [
         # The next token of one conversation: latency.
-        ("delta, one token", _delta(1, 1, 8, 64, 128, 64, carry=True)),
+        ("delta - one token", _delta(1, 1, 8, 64, 128, 64, carry=True)),
         # The next token of 64 conversations: every state is read and written.
-        ("delta, 64 single tokens", _delta(64, 1, 8, 64, 128, 64, carry=True)),
+        ("delta - 64 single tokens", _delta(64, 1, 8, 64, 128, 64, carry=True)),
         # A short user turn on a conversation's state.
-        ("delta, turn of 67 tokens", _delta(1, 67, 8, 64, 128, 64, carry=True)),
+        ("delta - turn of 67 tokens", _delta(1, 67, 8, 64, 128, 64, carry=True)),
         # A long prompt.
-        ("delta, 8k prompt", _delta(1, 8192, 8, 64, 128, 64)),
+        ("delta - 8k prompt", _delta(1, 8192, 8, 64, 128, 64)),
         # A ragged batch in 32 bits, heads of their own queries and keys, states carried in.
-        ("delta, ragged batch, f32", _delta(3, 1003, 27, 27, 64, 192, store="f32", carry=True, packed=False)),
+        ("delta - ragged batch f32", _delta(3, 1003, 27, 27, 64, 192, store="f32", carry=True, packed=False)),
         # A training step on four sequences: the rule's gradients.
-        ("delta backward, batch of 4", _delta(4, 2048, 8, 64, 128, 64, op="delta_bwd")),
+        ("delta backward - batch of 4", _delta(4, 2048, 8, 64, 128, 64, op="delta_bwd")),
         # A training step on short samples with few, odd heads.
-        ("delta backward, ragged, f16", _delta(2, 333, 5, 5, 40, 72, store="f16", carry=True, packed=False, op="delta_bwd")),
+        ("delta backward - ragged f16", _delta(2, 333, 5, 5, 40, 72, store="f16", carry=True, packed=False, op="delta_bwd")),
         # The next token of one conversation, before the layer's last projection in 8 bits: latency.
-        ("norm, one token", _norm(1, 4096, 64, fp8=True)),
+        ("norm - one token", _norm(1, 4096, 64, fp8=True)),
         # A long prompt, before the same projection.
-        ("norm, 8k prompt", _norm(8192, 4096, 64, fp8=True)),
+        ("norm - 8k prompt", _norm(8192, 4096, 64, fp8=True)),
         # A ragged batch through a layer kept in 32 bits, without a gate or an 8-bit output.
-        ("norm, ragged batch, f32", _norm(2871, 5184, 27, store="f32", gate=False)),
+        ("norm - ragged batch f32", _norm(2871, 5184, 27, store="f32", gate=False)),
         # A training step on eight sequences of an 80-head layer: the norm's gradients.
-        ("norm backward, batch of 8", _norm_bwd(32768, 5120, 80)),
+        ("norm backward - batch of 8", _norm_bwd(32768, 5120, 80)),
         # A training step on short samples with groups of an odd width.
-        ("norm backward, ragged, f16", _norm_bwd(1003, 2565, 27, store="f16")),
+        ("norm backward - ragged f16", _norm_bwd(1003, 2565, 27, store="f16")),
     ]
     return [dict(case, name=name) for name, case in cases]
 
