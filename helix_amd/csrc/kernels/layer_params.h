@@ -43,6 +43,47 @@ typedef struct {
 } HelixNormBwdParams;
 
 typedef struct {
+    const void* x;
+    const void* weight;
+    const void* bias;       /* may be null                                     */
+    const void* gate;       /* may be null                                     */
+    void*       y;          /* null: 8-bit output                              */
+    uint8_t*    q;
+    uint8_t*    scale;
+    float*      mean;       /* may be null                                     */
+    float*      rstd;       /* may be null                                     */
+    long long   ld_x, ld_gate, ld_y, ld_q, ld_scale;
+    long long   rows;
+    int         dim, groups, width;   /* width = dim / groups                  */
+    int         w_f32;      /* weight and bias are f32                         */
+    int         act;        /* helix_activation                                */
+    float       eps;
+} HelixGroupNormParams;
+
+typedef struct {
+    const void*  dy;
+    const void*  x;
+    const void*  weight;
+    const void*  bias;      /* may be null                                     */
+    const void*  gate;      /* may be null                                     */
+    const float* mean;
+    const float* rstd;
+    void*        dx;
+    void*        dgate;     /* null without a gate                             */
+    float*       dweight;   /* may be null                                     */
+    float*       dbias;     /* may be null                                     */
+    float*       part;      /* [parts x row slots][2 dim] sums; may be null    */
+    long long    ld_dy, ld_x, ld_gate, ld_dx, ld_dgate;
+    long long    rows;
+    long long    part_rows; /* rows of each part                               */
+    int          dim, groups, width;
+    int          w_f32;
+    int          act;
+    int          group_slots;   /* groups that a workgroup works on side by side */
+    int          parts;     /* parts x row slots: rows of `part`               */
+} HelixGroupNormBwdParams;
+
+typedef struct {
     const uint8_t* a;
     const uint8_t* a_scale;
     const uint8_t* b;

@@ -279,6 +279,186 @@ extern "C" helix_status helix_norm_backward_encode(helix_ctx* ctx, void* stream,
 
 namespace {
 
+// Lanes and vectors of eight of a group of `width` channels (kernels/group_norm.hip).
+struct GroupForm {
+    int lanes = 256, vectors = 4;
+    std::string name() const { return "_l" + std::to_string(lanes) + "_" + std::to_string(vectors); }
+};
+const GroupForm kGroupForms[] = {{4, 1}, {8, 1}, {16, 1}, {32, 1}, {64, 1}, {64, 2}, {256, 1}, {256, 2}, {256, 4}};
+GroupForm group_form(int width) {
+    for (const GroupForm& f : kGroupForms)
+        if (width <= 8 * f.lanes * f.vectors) return f;
+    return {};
+}
+
+bool group_shape(long long rows, int dim, int groups, int io, int weight, int act) {
+    need(rows >= 0 && dim >= 1 && dim <= HELIX_LAYER_MAX_DIM, "rows or dim out of range", HELIX_ERR_UNSUPPORTED_SHAPE);
+    need(groups >= 1 && dim % groups == 0 && dim / groups <= HELIX_GROUP_NORM_MAX_GROUP,
+         "groups does not divide dim, or its groups are too wide", HELIX_ERR_UNSUPPORTED_SHAPE);
+    need(dtype_ok(io), "io_dtype is none of HELIX_F32, HELIX_F16 and HELIX_BF16");
+    need(weight == HELIX_F32 || weight == io, "weight_dtype is neither HELIX_F32 nor io_dtype");
+    need(act == HELIX_ACT_NONE || act == HELIX_ACT_SILU || act == HELIX_ACT_SIGMOID, "activation is no helix_activation");
+    return rows > 0;
+}
+
+// How the backward pass of a group norm is spread.
+struct GroupBwdPlan {
+    GroupForm form;
+    int group_slots = 1, row_slots = 1;
+    long long gx = 0, parts = 0;   // workgroups along the groups and along the rows
+};
+// A workgroup has as many groups side by side as there are, up to its room, and rows in what is left of it. Along the
+// rows four workgroups a CU in all, of four rows a slot at least.
+GroupBwdPlan group_bwd_plan(long long rows, int dim, int groups) {
+    GroupBwdPlan p;
+    p.form = group_form(dim / groups);
+    const int room = kNormThreads / p.form.lanes;
+    while (p.group_slots < room && p.group_slots < groups) p.group_slots *= 2;
+    p.row_slots = room / p.group_slots;
+    p.gx = ceil_div(groups, p.group_slots);
+    p.parts = std::max(1LL, std::min(ceil_div(4 * 256, p.gx), rows / (4 * p.row_slots)));
+    return p;
+}
+
+}  // namespace
+
+extern "C" helix_status helix_group_norm_encode(helix_ctx* ctx, void* stream, const helix_group_norm_args* a) {
+    return entry(ctx, [&] {
+        need(ctx && a, "NULL context or arguments");
+        if (!group_shape(a->rows, a->dim, a->groups, a->io_dtype, a->weight_dtype, a->activation)) return;
+        need(!a->y != !a->q, "exactly one of y and q is wanted");
+        need(std::isfinite(a->eps) && a->eps >= 0, "eps is negative or not finite");
+        const int width = a->dim / a->groups;
+        const bool line_up = width % 128 == 0 || ((width == 32 || width == 64) && a->dim % 128 == 0);
+        need(!a->q || line_up || a->dim <= HELIX_GROUP_NORM_MAX_ROW, "dim too large for 8 bits in these groups",
+             HELIX_ERR_UNSUPPORTED_SHAPE);
+        const size_t es = kBytes[a->io_dtype], ws = kBytes[a->weight_dtype];
+        matrix("x", a->x, a->rows, a->dim, a->ld_x, es, false);
+        matrix("weight", a->weight, 1, a->dim, 0, ws, false);
+        if (a->bias) matrix("bias", a->bias, 1, a->dim, 0, ws, false);
+        if (a->gate) matrix("gate", a->gate, a->rows, a->dim, a->ld_gate, es, false);
+        if (a->y) matrix("y", a->y, a->rows, a->dim, a->ld_y, es, true);
+        if (a->q) {
+            matrix("q", a->q, a->rows, a->dim, a->ld_q, 1, true);
+            matrix("scale", a->scale, a->rows, ceil_div(a->dim, HELIX_FP8_BLOCK), a->ld_scale, 1, true);
+        }
+        need(aligned(a->mean, 4) && aligned(a->rstd, 4), "mean or rstd is not aligned to its elements");
+        HelixGroupNormParams p{};
+        p.x = a->x;
+        p.weight = a->weight;
+        p.bias = a->bias;
+        p.gate = a->gate;
+        p.y = a->y;
+        p.q = static_cast<uint8_t*>(a->q);
+        p.scale = static_cast<uint8_t*>(a->scale);
+        p.mean = a->mean;
+        p.rstd = a->rstd;
+        p.ld_x = a->ld_x;
+        p.ld_gate = a->ld_gate;
+        p.ld_y = a->ld_y;
+        p.ld_q = a->ld_q;
+        p.ld_scale = a->ld_scale;
+        p.dim = a->dim;
+        p.groups = a->groups;
+        p.width = width;
+        p.w_f32 = a->weight_dtype == HELIX_F32;
+        p.act = a->activation;
+        p.eps = a->eps;
+        const GroupForm form = group_form(width);
+        const bool any = a->q && !line_up;
+        const hipFunction_t f = kernel(ctx, std::string(a->q ? "helix_group_norm_fp8_" : "helix_group_norm_") +
+                                                kTags[a->io_dtype] + (any ? "_any" : form.name()));
+        const int units = kNormThreads / form.lanes;   // of a workgroup
+        // Units of a launch stay below 2^31 and its threads below 2^32.
+        const long long groups = any ? 1 : a->groups, each = any ? 1 : units;
+        const long long most = std::min((1LL << 31) - each, each * most_groups(kNormThreads)) / groups;
+        const OnDevice on(ctx->device);
+        for (long long left = a->rows; left > 0; left -= most) {
+            p.rows = std::min(left, most);
+            launch(f, stream, grid(ceil_div(p.rows * groups, each), kNormThreads), 1, kNormThreads, p);
+            if (left <= most) break;
+            advance(p.x, most * p.ld_x, es);
+            advance(p.gate, most * p.ld_gate, es);
+            advance(p.y, most * p.ld_y, es);
+            advance(p.q, most * p.ld_q, 1);
+            advance(p.scale, most * p.ld_scale, 1);
+            advance(p.mean, most * p.groups, sizeof(float));
+            advance(p.rstd, most * p.groups, sizeof(float));
+        }
+    });
+}
+
+extern "C" size_t helix_group_norm_backward_scratch_size(const helix_group_norm_backward_args* a) {
+    if (!a || (!a->dweight && !a->dbias) || a->rows <= 0 || a->dim <= 0 || a->groups <= 0 || a->dim % a->groups) return 0;
+    const GroupBwdPlan plan = group_bwd_plan(a->rows, a->dim, a->groups);
+    return (size_t)plan.parts * plan.row_slots * 2 * a->dim * sizeof(float);
+}
+
+extern "C" helix_status helix_group_norm_backward_encode(helix_ctx* ctx, void* stream,
+                                                         const helix_group_norm_backward_args* a) {
+    return entry(ctx, [&] {
+        need(ctx && a, "NULL context or arguments");
+        const bool some = group_shape(a->rows, a->dim, a->groups, a->io_dtype, a->weight_dtype, a->activation);
+        need(a->reserved == 0, "reserved is not 0");
+        need(aligned(a->dweight, 4) && aligned(a->dbias, 4), "dweight or dbias is not aligned to its elements");
+        const bool sums = a->dweight || a->dbias;
+        if (!some && !sums) return;
+        const size_t es = kBytes[a->io_dtype], ws = kBytes[a->weight_dtype];
+        if (some) {
+            matrix("dy", a->dy, a->rows, a->dim, a->ld_dy, es, false);
+            matrix("x", a->x, a->rows, a->dim, a->ld_x, es, false);
+            matrix("weight", a->weight, 1, a->dim, 0, ws, false);
+            if (a->bias) matrix("bias", a->bias, 1, a->dim, 0, ws, false);
+            if (a->gate) matrix("gate", a->gate, a->rows, a->dim, a->ld_gate, es, false);
+            need(!a->gate == !a->dgate, "dgate is wanted where there is a gate, and there alone");
+            matrix("mean", a->mean, a->rows, a->groups, a->groups, 4, false);
+            matrix("rstd", a->rstd, a->rows, a->groups, a->groups, 4, false);
+            matrix("dx", a->dx, a->rows, a->dim, a->ld_dx, es, true);
+            if (a->dgate) matrix("dgate", a->dgate, a->rows, a->dim, a->ld_dgate, es, true);
+            const size_t want = helix_group_norm_backward_scratch_size(a);
+            need(want == 0 || (a->scratch && a->scratch_bytes >= want),
+                 "scratch smaller than helix_group_norm_backward_scratch_size()", HELIX_ERR_SCRATCH_TOO_SMALL);
+            need(aligned(a->scratch, 16), "scratch is not 16-byte aligned");
+        }
+        const GroupBwdPlan plan = group_bwd_plan(a->rows, a->dim, a->groups);
+        HelixGroupNormBwdParams p{};
+        p.dy = a->dy;
+        p.x = a->x;
+        p.weight = a->weight;
+        p.bias = a->bias;
+        p.gate = a->gate;
+        p.mean = a->mean;
+        p.rstd = a->rstd;
+        p.dx = a->dx;
+        p.dgate = a->dgate;
+        p.dweight = a->dweight;
+        p.dbias = a->dbias;
+        p.part = sums ? static_cast<float*>(a->scratch) : nullptr;
+        p.ld_dy = a->ld_dy;
+        p.ld_x = a->ld_x;
+        p.ld_gate = a->ld_gate;
+        p.ld_dx = a->ld_dx;
+        p.ld_dgate = a->ld_dgate;
+        p.rows = a->rows;
+        p.part_rows = some ? ceil_div(a->rows, plan.parts) : 0;
+        p.dim = a->dim;
+        p.groups = a->groups;
+        p.width = a->dim / a->groups;
+        p.w_f32 = a->weight_dtype == HELIX_F32;
+        p.act = a->activation;
+        p.group_slots = plan.group_slots;
+        p.parts = some ? (int)(plan.parts * plan.row_slots) : 0;   // no rows: the sums are 0
+        const hipFunction_t f = kernel(ctx, std::string("helix_group_norm_bwd_") + kTags[a->io_dtype] + plan.form.name()),
+                            dw = kernel(ctx, "helix_group_norm_dw");
+        const unsigned gd = (unsigned)ceil_div(2LL * a->dim, 32);
+        const OnDevice on(ctx->device);
+        if (some) launch(f, stream, grid(plan.gx, kNormThreads), (unsigned)plan.parts, kNormThreads, p);
+        if (sums) launch(dw, stream, gd, 1, 1024, p);
+    });
+}
+
+namespace {
+
 // How a product is computed (kernels/matmul_fp8.hip).
 struct MatmulPlan {
     std::string kernel = "_blocks";
@@ -669,6 +849,13 @@ const std::vector<std::string>& layer_kernel_names() {
                 if (n[0] <= '4') v.push_back(std::string("helix_norm_") + tag + "_w" + n);
                 if (n[0] <= '2') v.push_back(std::string("helix_norm_bwd_") + tag + "_w" + n);
             }
+        v.push_back("helix_group_norm_dw");
+        for (const char* tag : kTags) {
+            v.push_back(std::string("helix_group_norm_fp8_") + tag + "_any");
+            for (const GroupForm& f : kGroupForms)
+                for (const char* k : {"helix_group_norm_", "helix_group_norm_bwd_", "helix_group_norm_fp8_"})
+                    v.push_back(k + (tag + f.name()));
+        }
         for (const char* tag : kTags)
             for (const char* k : {"_blocks", "_r1", "_r1w4", "_r2", "_r3", "_r4"})
                 v.push_back(std::string("helix_matmul_fp8_") + tag + k);

@@ -3,6 +3,9 @@
  *   helix_norm_*         root-mean-square norm with the residual's addition,
  *                        stored as it is or in 8 bits with scales, and its
  *                        backward pass
+ *   helix_group_norm_*   norm of the groups of a token's channels (a head's, say)
+ *                        with an activation or a gate, stored as it is or in 8
+ *                        bits, and its backward pass
  *   helix_matmul_fp8_*   product of two 8-bit matrices with a scale for each
  *                        block of 128 along the sum
  *   helix_gated_scan_*   gated linear recurrence per channel, and its backward
@@ -104,6 +107,87 @@ typedef struct {
 /* From rows, dim and dweight (NULL: 0); the other fields are not read. */
 size_t       helix_norm_backward_scratch_size(const helix_norm_backward_args* args);
 helix_status helix_norm_backward_encode(helix_ctx* ctx, void* stream, const helix_norm_backward_args* args);
+
+/* ------------------------------------------------------------------------- */
+/* Group norm                                                                */
+/* ------------------------------------------------------------------------- */
+
+/* The activation a: of the gate where there is one, else of the norm itself. */
+typedef enum {
+    HELIX_ACT_NONE    = 0,   /* a(u) = u                                      */
+    HELIX_ACT_SILU    = 1,   /* u / (1 + exp(-u))                             */
+    HELIX_ACT_SIGMOID = 2    /* 1 / (1 + exp(-u))                             */
+} helix_activation;
+
+/* Largest group of helix_group_norm_*, and largest row of it in 8 bits where
+ * blocks of 128 do not line up with the groups. */
+#define HELIX_GROUP_NORM_MAX_GROUP 8192
+#define HELIX_GROUP_NORM_MAX_ROW   16384
+
+/* A row's channels are `groups` groups of dim / groups neighbours. Per group:
+ *   mean, rstd = 1 / sqrt(mean((x - mean)^2) + eps),  n = (x - mean) rstd
+ *   z = n weight + bias
+ *   out = z a(gate) with a gate, a(z) without
+ * in fp32 throughout, rounded once; with q, out is stored in 8 bits as
+ * helix_norm_encode stores it. Blocks line up with the groups where dim / groups
+ * is a multiple of 128, or 32 or 64 and dim a multiple of 128. */
+typedef struct {
+    int64_t     rows;         /* 0: nothing is done                           */
+    int32_t     dim;          /* 1 .. HELIX_LAYER_MAX_DIM                     */
+    int32_t     groups;       /* divides dim; dim / groups is at most
+                                 HELIX_GROUP_NORM_MAX_GROUP                   */
+    int32_t     io_dtype;     /* helix_dtype of x, gate and y                 */
+    int32_t     weight_dtype; /* HELIX_F32 or io_dtype: of weight and bias    */
+    int32_t     activation;   /* helix_activation                             */
+    float       eps;
+    const void* x;
+    const void* weight;       /* dim                                          */
+    const void* bias;         /* dim; NULL: none                              */
+    const void* gate;         /* NULL: none                                   */
+    void*       y;            /* out (may be x or gate, at their strides);
+                                 exactly one of y and q                       */
+    void*       q;            /* out in e4m3                                  */
+    void*       scale;        /* its scales                                   */
+    float*      mean;         /* rows x groups, dense; NULL: not stored       */
+    float*      rstd;         /* the same                                     */
+    int64_t     ld_x, ld_gate, ld_y, ld_q, ld_scale;
+} helix_group_norm_args;
+
+helix_status helix_group_norm_encode(helix_ctx* ctx, void* stream, const helix_group_norm_args* args);
+
+/* Gradients, from dy (of y). With dz = dy a(gate), or dy a'(z) without a gate:
+ *   dgate = dy z a'(gate)
+ *   t = dz weight,  dx = rstd (t - mean(t) - n mean(t n))    (means of a group)
+ *   dweight = sum over rows of dz n,  dbias = sum over rows of dz  (fp32)
+ * The rows of these sums are added in an order that depends on the shape alone. */
+typedef struct {
+    int64_t      rows;         /* 0: dweight and dbias are 0                  */
+    int32_t      dim, groups;
+    int32_t      io_dtype;     /* of dy, x, gate, dx and dgate                */
+    int32_t      weight_dtype;
+    int32_t      activation;
+    int32_t      reserved;     /* 0                                           */
+    const void*  dy;
+    const void*  x;
+    const void*  weight;
+    const void*  bias;         /* NULL: none                                  */
+    const void*  gate;         /* NULL: none                                  */
+    const float* mean;         /* as helix_group_norm_encode stored them      */
+    const float* rstd;
+    void*        dx;           /* may be dy or x, at their strides            */
+    void*        dgate;        /* NULL without a gate, else wanted            */
+    float*       dweight;      /* dim; NULL: not wanted                       */
+    float*       dbias;        /* dim; NULL: not wanted                       */
+    void*        scratch;      /* helix_group_norm_backward_scratch_size()
+                                  bytes, 16-byte aligned; none is needed
+                                  without dweight and dbias                   */
+    uint64_t     scratch_bytes;
+    int64_t      ld_dy, ld_x, ld_gate, ld_dx, ld_dgate;
+} helix_group_norm_backward_args;
+
+/* From rows, dim, groups, dweight and dbias (NULL: not wanted). */
+size_t       helix_group_norm_backward_scratch_size(const helix_group_norm_backward_args* args);
+helix_status helix_group_norm_backward_encode(helix_ctx* ctx, void* stream, const helix_group_norm_backward_args* args);
 
 /* ------------------------------------------------------------------------- */
 /* Product of 8-bit matrices                                                 */
