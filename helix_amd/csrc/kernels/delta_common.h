@@ -1,0 +1,152 @@
+// delta_common.h -- what the delta rule's kernels share: operands of 16 x 16 x 32
+// matrix instructions in bf16 parts, rows of tokens, decays.
+//
+// v_mfma_f32_16x16x32_bf16, lane = 16 q + c:  A[i][k]: lane holds A[c][8 q + e], e = 0..7;
+// B[k][j]: B[8 q + e][c];  D[i][j]: register r holds D[4 q + r][c].
+//
+// An fp32 value is three bf16 parts, and a product of two the six products of parts i, j
+// with i + j <= 2: fp32's own accuracy (helix_common.h). A bf16 element is one part, an f16
+// one two, exactly.
+#ifndef HELIX_DELTA_COMMON_H
+#define HELIX_DELTA_COMMON_H
+
+#include "layer_common.h"
+
+namespace {
+
+constexpr int DR_C = HELIX_DR_CHUNK;
+
+template <typename T> constexpr int dr_planes = __is_same(T, float) ? 3 : __is_same(T, _Float16) ? 2 : 1;
+// Parts of operands that meet outputs of the storage type alone: two (2^-18) where that has 16 bits.
+template <typename T> constexpr int dr_out_planes = __is_same(T, float) ? 3 : 2;
+
+// Products of the parts i, j with i + j < MAX, smallest first.
+template <int NA, int NB, int MAX = 3>
+HELIX_DEV f32x4 dr_mfma(const bf16x8 (&a)[NA], const bf16x8 (&b)[NB], f32x4 acc) {
+#pragma unroll
+    for (int sum = MAX - 1; sum >= 0; --sum)
+#pragma unroll
+        for (int i = sum; i >= 0; --i)
+            if (i < NA && sum - i < NB) acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[i], b[sum - i], acc, 0, 0, 0);
+    return acc;
+}
+
+template <int NPL>
+HELIX_DEV void dr_split2(float a, float b, unsigned (&w)[NPL]) {
+    if constexpr (NPL == 3) split3_pair(a, b, w[0], w[1], w[2]);
+    else if constexpr (NPL == 2) split2_pair(a, b, w[0], w[1]);
+    else w[0] = pk_bf16(a, b);
+}
+template <int NPL>
+HELIX_DEV void dr_split8(const float (&v)[8], bf16x8 (&o)[NPL]) {
+    u32x4 q[NPL];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        unsigned w[NPL];
+        dr_split2<NPL>(v[2 * e], v[2 * e + 1], w);
+#pragma unroll
+        for (int k = 0; k < NPL; ++k) q[k][e] = w[k];
+    }
+#pragma unroll
+    for (int k = 0; k < NPL; ++k) o[k] = __builtin_bit_cast(bf16x8, q[k]);
+}
+
+// Eight stored elements as an operand's parts, those from n on cleared.
+template <typename T>
+HELIX_DEV void dr_operand(const Raw8<T>& v, int n, bf16x8 (&o)[dr_planes<T>]) {
+    if constexpr (__is_same(T, __bf16)) {
+        u32x4 w = v.w[0];
+        if (n < 8) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) w[e] &= (2 * e < n ? 0xffffu : 0u) | (2 * e + 1 < n ? 0xffff0000u : 0u);
+        }
+        o[0] = __builtin_bit_cast(bf16x8, w);
+    } else {
+        float f[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) f[e] = e < n ? at8(v, e) : 0.0f;
+        dr_split8<dr_planes<T>>(f, o);
+    }
+}
+
+// The rows of a chunk's tokens of one head: `len` of them of `width` elements, `tok` elements apart.
+template <typename T>
+struct Rows {
+    helix_rsrc r;
+    int tok, len, width;
+    bool whole;   // rows end at whole words
+    __device__ Rows(const void* base, long long at, long long tok_, int len_, int width_) : tok((int)tok_), len(len_), width(width_) {
+        whole = sizeof(T) == 4 || !(width & 1);
+        r = make_rsrc_u(static_cast<const T*>(base) + at, len > 0 ? (unsigned)(((len - 1) * tok_ + width) * (long long)sizeof(T)) : 0u);
+    }
+    // Eight elements from (row, col) on; what lies outside is unspecified past the row's end and 0 past the tokens.
+    __device__ __forceinline__ Raw8<T> load8(int row, int col) const {
+        const int off = row < len && col < width ? (row * tok + col) * (int)sizeof(T) : (int)0x80000000;
+        if (whole) return buf_load8<T>(r, off);
+        Raw8<T> o;
+        if constexpr (sizeof(T) == 2) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const unsigned a = (unsigned short)__builtin_amdgcn_raw_buffer_load_b16(r, col + 2 * e < width ? off + 4 * e : (int)0x80000000, 0, 0);
+                const unsigned b = (unsigned short)__builtin_amdgcn_raw_buffer_load_b16(r, col + 2 * e + 1 < width ? off + 4 * e + 2 : (int)0x80000000, 0, 0);
+                o.w[0][e] = a | b << 16;
+            }
+        }
+        return o;
+    }
+    __device__ __forceinline__ unsigned raw(int row, int col) const {
+        const int off = row < len && col < width ? (row * tok + col) * (int)sizeof(T) : (int)0x80000000;
+        if constexpr (sizeof(T) == 4) return (unsigned)__builtin_amdgcn_raw_buffer_load_b32(r, off, 0, 0);
+        else return (unsigned short)__builtin_amdgcn_raw_buffer_load_b16(r, off, 0, 0);
+    }
+    __device__ __forceinline__ void store(int row, int col, float v) const {
+        const int off = row < len && col < width ? (row * tok + col) * (int)sizeof(T) : (int)0x80000000;
+        io_store<T, 0>(r, v, off, 0);
+    }
+};
+template <typename T>
+HELIX_DEV float raw_f32(unsigned w) {
+    if constexpr (sizeof(T) == 4) return as_f32(w);
+    else return io_f32<T>((unsigned short)w);
+}
+
+// Four values of a result's registers (rows 4 q .. 4 q + 3 of a column) as parts in LDS, the rows side by side: to[k * stride + 0..3].
+template <int NPL>
+HELIX_DEV void dr_put4(__bf16* to, int stride, float a, float b, float c, float d) {
+    unsigned lo[NPL], hi[NPL];
+    dr_split2<NPL>(a, b, lo);
+    dr_split2<NPL>(c, d, hi);
+#pragma unroll
+    for (int k = 0; k < NPL; ++k) *reinterpret_cast<u32x2*>(to + k * stride) = u32x2{lo[k], hi[k]};
+}
+template <int NPL>
+HELIX_DEV void dr_get8(const __bf16* from, int stride, bf16x8 (&o)[NPL]) {
+#pragma unroll
+    for (int k = 0; k < NPL; ++k) o[k] = *reinterpret_cast<const bf16x8*>(from + k * stride);
+}
+// Rows t .. t + 7 of column c0 + c, from parts stored by rows of `pitch` elements, by transposed reads: the operand of a
+// product that sums over the rows. `from` is row t, column c0; all sixteen lanes of a group name the same t.
+template <int NPL>
+HELIX_DEV void dr_get8_t(const __bf16* from, int pitch, int stride, int c, bf16x8 (&o)[NPL]) {
+    const __bf16* at = from + (c >> 2) * pitch + 4 * (c & 3);
+#pragma unroll
+    for (int k = 0; k < NPL; ++k) {
+        const u32x2 a = lds_read_tr16(at + k * stride), b = lds_read_tr16(at + k * stride + 4 * pitch);
+        o[k] = __builtin_bit_cast(bf16x8, u32x4{a[0], a[1], b[0], b[1]});
+    }
+}
+
+HELIX_DEV f32x4 zero4() { return f32x4{0.0f, 0.0f, 0.0f, 0.0f}; }
+
+// Sums of g from a chunk's start, lane = token, in fp64 (differences of neighbouring ones count). Tokens past the end have
+// g = 0. What e^g cannot tell from e^-100000, infinity among it, counts as that: differences of infinities would be NaN.
+HELIX_DEV double dr_log_decay(float g) { return wave_incl_sum(g < -1e5f ? -1e5 : (double)g); }
+
+// Fragment of the block in row tile w, columns 32 ks .., of a lower triangle (ks = 0 for w < 2), or of an upper one (ks = 1
+// alone for w > 1).
+HELIX_DEV int dr_low(int w, int ks) { return w < 2 ? w : 2 * w - 2 + ks; }
+HELIX_DEV int dr_up(int w, int ks) { return w < 2 ? 2 * w + ks : w + 2; }
+
+}  // namespace
+
+#endif

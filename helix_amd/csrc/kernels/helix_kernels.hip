@@ -13,3 +13,4 @@
 #include "group_norm.hip"
 #include "matmul_fp8.hip"
 #include "gated_scan.hip"
+#include "delta_rule.hip"

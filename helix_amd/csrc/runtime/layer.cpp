@@ -5,7 +5,10 @@
 #include <cmath>
 #include <cstdint>
 #include <exception>
+#include <initializer_list>
 #include <string>
+#include <utility>
+#include <vector>
 
 #include "helix/helix_layer.h"
 #include "helix_internal.h"
@@ -834,6 +837,167 @@ extern "C" helix_status helix_gated_scan_backward_encode(helix_ctx* ctx, void* s
     });
 }
 
+namespace {
+
+constexpr int kDeltaThreads = 256;
+
+// Elements of strides that do not overlap: each dimension's stride reaches past what the ones below it span.
+bool disjoint(std::initializer_list<std::pair<long long, long long>> dims) {   // (size, stride)
+    std::vector<std::pair<long long, long long>> d;   // (stride, size)
+    for (const auto& x : dims)
+        if (x.first > 1) d.push_back({x.second, x.first});
+    std::sort(d.begin(), d.end());
+    long long span = 1;
+    for (const auto& x : d) {
+        if (x.first < span) return false;
+        span = x.first * (x.second - 1) + span;
+    }
+    return true;
+}
+
+// A tensor (n_seq, n_tok, heads, width) with contiguous last dimension: present, aligned, and within the kernels' reach.
+void heads(const char* name, const void* p, long long n_seq, long long n_tok, long long n_head, long long width, long long seq,
+           long long tok, long long head, size_t es, bool written) {
+    if (!n_tok) return;
+    const std::string n = name;
+    if (!p) throw Bad{HELIX_ERR_INVALID_ARG, n + " is NULL"};
+    if (!aligned(p, es)) throw Bad{HELIX_ERR_INVALID_ARG, n + " is not aligned to its elements"};
+    if (seq < 0 || tok < 0 || head < 0) throw Bad{HELIX_ERR_INVALID_ARG, n + ": negative stride"};
+    if (n_tok > 1 && tok >= (1LL << 31) / 64 / (long long)es)
+        throw Bad{HELIX_ERR_UNSUPPORTED_SHAPE, n + ": 64 tokens span 2^31 bytes or more"};
+    if (written && !disjoint({{n_seq, seq}, {n_tok, tok}, {n_head, head}, {width, 1}}))
+        throw Bad{HELIX_ERR_INVALID_ARG, n + ": elements overlap"};
+}
+
+// Checks of what both passes have; whether there is anything to do.
+template <typename A>
+bool delta_shape(const A& a) {
+    need(a.n_seq >= 0 && a.n_tok >= 0 && a.n_qk_head >= 0 && a.n_head >= 0, "n_seq, n_tok, n_qk_head or n_head is negative",
+         HELIX_ERR_UNSUPPORTED_SHAPE);
+    need(a.n_key >= 1 && a.n_key <= HELIX_DELTA_MAX_KEY && a.n_val >= 1 && a.n_val <= HELIX_DELTA_MAX_VAL,
+         "n_key or n_val out of range", HELIX_ERR_UNSUPPORTED_SHAPE);
+    need(dtype_ok(a.io_dtype), "io_dtype is none of HELIX_F32, HELIX_F16 and HELIX_BF16");
+    need(std::isfinite(a.scale), "scale is not finite");
+    if (!a.n_seq || !a.n_head) return false;
+    need(a.n_qk_head >= 1 && a.n_head % a.n_qk_head == 0, "n_qk_head does not divide n_head", HELIX_ERR_UNSUPPORTED_SHAPE);
+    return true;
+}
+
+int delta_keys(int n_key) { return n_key <= 64 ? 64 : 128; }   // of the kernels
+
+// How the rule is cut: segments of `chunks` chunks of every sequence, whose operands scratch holds at a time.
+struct DeltaPlan {
+    int n_chunk = 0, chunks = 0, n_slice = 0;
+    size_t x_at = 0, p_at = 0, decay_at = 0, bytes = 0;
+};
+// Scratch of a segment: up to a gigabyte, and one chunk of every sequence where that is more.
+constexpr size_t kDeltaScratch = (size_t)1 << 30;
+
+DeltaPlan delta_plan(const helix_delta_rule_args& a) {
+    DeltaPlan p;
+    if (a.n_seq <= 0 || a.n_head <= 0 || a.n_tok <= HELIX_DR_STEPS || a.n_key <= 0 || a.n_val <= 0) return p;
+    const size_t sh = (size_t)a.n_seq * a.n_head, out = a.io_dtype == HELIX_F32 ? 3 : 2;
+    const size_t x = 6 * 3 * HELIX_DR_FRAG, pp = 6 * out * HELIX_DR_FRAG, each = sh * (x + pp + HELIX_DR_DECAY);
+    p.n_chunk = (int)ceil_div(a.n_tok, HELIX_DR_CHUNK);
+    p.chunks = (int)std::min<size_t>(p.n_chunk, std::max<size_t>(1, kDeltaScratch / each));
+    p.n_slice = (int)ceil_div(a.n_val, HELIX_DR_SLICE);
+    p.p_at = p.x_at + sh * p.chunks * x;
+    p.decay_at = p.p_at + sh * p.chunks * pp;
+    p.bytes = p.decay_at + sh * p.chunks * HELIX_DR_DECAY;
+    return p;
+}
+
+// What both passes' arguments have alike.
+template <typename A>
+HelixDeltaParams delta_params(const A& a) {
+    HelixDeltaParams p{};
+    p.q = a.q;
+    p.k = a.k;
+    p.v = a.v;
+    p.g = a.g;
+    p.beta = a.beta;
+    p.s0 = a.s0;
+    p.seq_q = a.seq_q;
+    p.tok_q = a.tok_q;
+    p.head_q = a.head_q;
+    p.seq_k = a.seq_k;
+    p.tok_k = a.tok_k;
+    p.head_k = a.head_k;
+    p.seq_v = a.seq_v;
+    p.tok_v = a.tok_v;
+    p.head_v = a.head_v;
+    p.seq_g = a.seq_g;
+    p.tok_g = a.tok_g;
+    p.seq_b = a.seq_beta;
+    p.tok_b = a.tok_beta;
+    p.n_seq = a.n_seq;
+    p.n_tok = a.n_tok;
+    p.n_qk = a.n_qk_head;
+    p.n_head = a.n_head;
+    p.share = a.n_head / a.n_qk_head;
+    p.n_key = a.n_key;
+    p.n_val = a.n_val;
+    p.scale = a.scale;
+    return p;
+}
+template <typename A>
+void delta_inputs(const A& a, size_t es) {
+    heads("q", a.q, a.n_seq, a.n_tok, a.n_qk_head, a.n_key, a.seq_q, a.tok_q, a.head_q, es, false);
+    heads("k", a.k, a.n_seq, a.n_tok, a.n_qk_head, a.n_key, a.seq_k, a.tok_k, a.head_k, es, false);
+    heads("v", a.v, a.n_seq, a.n_tok, a.n_head, a.n_val, a.seq_v, a.tok_v, a.head_v, es, false);
+    heads("g", a.g, a.n_seq, a.n_tok, 1, a.n_head, a.seq_g, a.tok_g, 0, 4, false);
+    heads("beta", a.beta, a.n_seq, a.n_tok, 1, a.n_head, a.seq_beta, a.tok_beta, 0, 4, false);
+    need(aligned(a.s0, 4), "s0 is not aligned to its elements");
+}
+
+}  // namespace
+
+extern "C" size_t helix_delta_rule_scratch_size(const helix_delta_rule_args* a) { return a ? delta_plan(*a).bytes : 0; }
+
+extern "C" helix_status helix_delta_rule_encode(helix_ctx* ctx, void* stream, const helix_delta_rule_args* a) {
+    return entry(ctx, [&] {
+        need(ctx && a, "NULL context or arguments");
+        if (!delta_shape(*a)) return;
+        const size_t es = kBytes[a->io_dtype];
+        delta_inputs(*a, es);
+        heads("o", a->o, a->n_seq, a->n_tok, a->n_head, a->n_val, a->seq_o, a->tok_o, a->head_o, es, true);
+        need(a->s != nullptr && aligned(a->s, 4), "s is NULL or not aligned to its elements");
+        const DeltaPlan plan = delta_plan(*a);
+        need(plan.bytes == 0 || (a->scratch && a->scratch_bytes >= plan.bytes),
+             "scratch smaller than helix_delta_rule_scratch_size()", HELIX_ERR_SCRATCH_TOO_SMALL);
+        need(aligned(a->scratch, 16), "scratch is not 16-byte aligned");
+        HelixDeltaParams p = delta_params(*a);
+        p.o = a->o;
+        p.s = a->s;
+        p.seq_o = a->seq_o;
+        p.tok_o = a->tok_o;
+        p.head_o = a->head_o;
+        const std::string form = std::string(kTags[a->io_dtype]) + "_" + std::to_string(delta_keys(a->n_key));
+        const long long sh = (long long)a->n_seq * a->n_head;
+        if (!plan.bytes) {
+            const hipFunction_t f = kernel(ctx, "helix_delta_steps_" + form);
+            const unsigned gx = grid(sh * ceil_div(a->n_val, 64), kDeltaThreads);
+            const OnDevice on(ctx->device);
+            launch(f, stream, gx, 1, kDeltaThreads, p);
+            return;
+        }
+        const hipFunction_t prep = kernel(ctx, "helix_delta_prep_" + form), walk = kernel(ctx, "helix_delta_walk_" + form);
+        const unsigned gp = grid(sh * plan.chunks, kDeltaThreads), gw = grid(sh * plan.n_slice, kDeltaThreads);
+        char* sc = static_cast<char*>(a->scratch);
+        p.x = sc + plan.x_at;
+        p.p = sc + plan.p_at;
+        p.decay = reinterpret_cast<float*>(sc + plan.decay_at);
+        p.n_slice = plan.n_slice;
+        const OnDevice on(ctx->device);
+        for (p.chunk0 = 0; p.chunk0 < plan.n_chunk; p.chunk0 += plan.chunks) {
+            p.n_chunk = std::min(plan.chunks, plan.n_chunk - p.chunk0);
+            launch(prep, stream, p.n_chunk == plan.chunks ? gp : (unsigned)(sh * p.n_chunk), 1, kDeltaThreads, p);
+            launch(walk, stream, gw, 1, kDeltaThreads, p);
+            p.s0 = p.s;   // the next segment starts where this one ends
+        }
+    });
+}
+
 namespace helix::rt {
 
 const std::vector<std::string>& layer_kernel_names() {
@@ -849,6 +1013,9 @@ const std::vector<std::string>& layer_kernel_names() {
                 if (n[0] <= '4') v.push_back(std::string("helix_norm_") + tag + "_w" + n);
                 if (n[0] <= '2') v.push_back(std::string("helix_norm_bwd_") + tag + "_w" + n);
             }
+        for (const char* tag : kTags)
+            for (const char* n : {"_64", "_128"})
+                for (const char* k : {"steps_", "prep_", "walk_"}) v.push_back(std::string("helix_delta_") + k + tag + n);
         v.push_back("helix_group_norm_dw");
         for (const char* tag : kTags) {
             v.push_back(std::string("helix_group_norm_fp8_") + tag + "_any");

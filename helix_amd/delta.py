@@ -1,0 +1,79 @@
+"""Gated delta rule: a recurrence whose state is a matrix per head (include/helix/helix_layer.h).
+
+    S_t = e^(g_t) S_(t-1) + beta_t k_t (v_t - e^(g_t) S_(t-1)' k_t)',  o_t = scale S_t' q_t,  S_(-1) = s0
+
+The state, keys x values, is float32 throughout. Keys are taken as they are: a layer norms them (and the queries) to
+length one, rms_norm with a weight of keys ** -0.5, say. A token that is to leave the state as it is has g = 0 and beta = 0.
+"""
+from __future__ import annotations
+
+import torch
+
+from . import abi
+from .layer import device_index, expect, io_code, ptr, run_with_scratch, stream_handle, under
+
+
+def _strides(name: str, t: torch.Tensor) -> tuple[int, int, int]:
+    if t.stride(3) != 1 and t.shape[3] > 1:
+        raise ValueError(f"{name}: the channels must be contiguous")
+    return t.stride(0), t.stride(1), t.stride(2)
+
+
+def _gate_strides(name: str, t: torch.Tensor) -> tuple[int, int]:
+    if t.stride(2) != 1 and t.shape[2] > 1:
+        raise ValueError(f"{name}: the heads must be contiguous")
+    return t.stride(0), t.stride(1)
+
+
+def _state(name: str, t: torch.Tensor | None, like: torch.Tensor, shape) -> None:
+    if t is None:
+        return
+    expect(name, t, torch.float32, shape, like)
+    if not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous")
+
+
+def _inputs(op, q, k, v, g, beta, s0, scale):
+    """Checks: (device, io, the sizes' fields of the arguments, the inputs' strides)."""
+    index = device_index(op, q)
+    io = io_code("q", q)
+    if q.dim() != 4 or v.dim() != 4:
+        raise ValueError("q must be [sequences, tokens, heads, keys] and v [sequences, tokens, heads, values]")
+    S, L, Hk, N = q.shape
+    H, P = v.shape[2:]
+    if N < 1 or P < 1:
+        raise ValueError("heads must have at least one key and one value channel")
+    if (Hk and H % Hk) or (H and not Hk):
+        raise ValueError(f"the {Hk} heads of q and k must divide the {H} heads of v")
+    expect("k", k, q.dtype, q.shape, q)
+    expect("v", v, q.dtype, (S, L, H, P), q)
+    expect("g", g, torch.float32, (S, L, H), q)
+    expect("beta", beta, torch.float32, (S, L, H), q)
+    _state("s0", s0, q, (S, H, N, P))
+    sizes = (S, L, Hk, H, N, P, io, N ** -0.5 if scale is None else scale)
+    strides = (*_strides("q", q), *_strides("k", k), *_strides("v", v), *_gate_strides("g", g), *_gate_strides("beta", beta))
+    return index, sizes, strides
+
+
+def delta_rule(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Tensor, beta: torch.Tensor,
+               s0: torch.Tensor | None = None, *, scale: float | None = None, stream: torch.cuda.Stream | None = None):
+    """The rule over q and k [S, L, Hk, N], v [S, L, H, P], g and beta [S, L, H]: returns (o, s).
+
+    q, k and v are float32, bfloat16 or float16 (one type), of any strides but the last (column ranges of one projected
+    row per token, say); Hk divides H, and H / Hk neighbouring heads of v share a head of q and k. N is at most 128. g, the
+    logarithm of the decay, and beta are float32. o [S, L, H, P] has v's type; s0 and s, the states before and after, are
+    float32 [S, H, N, P] (s0 zeros when None). scale is N ** -0.5 when None. L = 1 is the step of a single token."""
+    index, sizes, strides = _inputs("delta_rule", q, k, v, g, beta, s0, scale)
+    S, L, _, H, N, P = sizes[:6]
+    with under(index, stream):
+        o = torch.empty(S, L, H, P, dtype=v.dtype, device=v.device)
+        s = torch.empty(S, H, N, P, dtype=torch.float32, device=v.device)
+    st = stream_handle(index, stream)
+
+    def pack(buf, nbytes):
+        return abi.DELTA_RULE_STRUCT.pack(*sizes, q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(), beta.data_ptr(),
+                                          ptr(s0), o.data_ptr(), s.data_ptr(), buf, nbytes, *strides, L * H * P, H * P, P)
+
+    lib = abi.lib()
+    run_with_scratch(lib.helix_delta_rule_encode, lib.helix_delta_rule_scratch_size, index, st, stream, pack)
+    return o, s

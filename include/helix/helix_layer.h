@@ -10,6 +10,8 @@
  *                        block of 128 along the sum
  *   helix_gated_scan_*   gated linear recurrence per channel, and its backward
  *                        pass
+ *   helix_delta_rule_*   gated delta rule: a recurrence whose state is a matrix
+ *                        per head, and its backward pass
  *
  * The reference has no counterpart of them. They keep helix.h's manner: they
  * enqueue kernels on the caller's stream and never allocate, synchronize or
@@ -281,6 +283,58 @@ typedef struct {
 size_t       helix_gated_scan_backward_scratch_size(const helix_gated_scan_backward_args* args);
 helix_status helix_gated_scan_backward_encode(helix_ctx* ctx, void* stream,
                                               const helix_gated_scan_backward_args* args);
+
+/* ------------------------------------------------------------------------- */
+/* Gated delta rule                                                          */
+/* ------------------------------------------------------------------------- */
+
+/* Largest n_key and n_val. */
+#define HELIX_DELTA_MAX_KEY 128
+#define HELIX_DELTA_MAX_VAL (1 << 16)
+
+/* Per sequence and value head, with the state S (n_key x n_val) in fp32:
+ *   S_t = e^(g_t) S_(t-1) + beta_t k_t (v_t - e^(g_t) S_(t-1)' k_t)'
+ *   o_t = scale S_t' q_t,   S_(-1) = s0
+ * Value head h has the queries and keys of head h / (n_head / n_qk_head). g is the
+ * logarithm of the decay: 0 keeps the state, -inf forgets it; a token with g = 0
+ * and beta = 0 leaves the state as it is. Keys are taken as they are: of length
+ * one at most, with beta up to 2, they keep the state bounded.
+ *
+ * Products keep fp32 accuracy (operands in three bf16 parts, fp32 sums); with
+ * 16-bit storage what only o takes is in two parts, 2^-18, below its rounding.
+ * Where an element of v is infinite or NaN, its column of the state and of o is
+ * from the chunk of 64 tokens on that it lies in; where one of q, k, g or beta
+ * is, its heads are. Other heads and sequences are not touched.
+ *
+ * n_tok = 1 is the step of a single token; s may be s0. Strides are any that are
+ * not negative (o's elements do not overlap); 64 tokens of q, k, v or o span
+ * less than 2^31 bytes. g and beta are fp32 with dense heads; s0 and s are dense
+ * (n_seq, n_head, n_key, n_val). */
+typedef struct {
+    int32_t      n_seq, n_tok;       /* n_seq or n_head 0: nothing is done;
+                                        n_tok 0: s = s0                       */
+    int32_t      n_qk_head, n_head;  /* the first divides the second          */
+    int32_t      n_key, n_val;
+    int32_t      io_dtype;           /* of q, k, v and o                      */
+    float        scale;
+    const void*  q;                  /* (n_seq, n_tok, n_qk_head, n_key)      */
+    const void*  k;                  /* the same                              */
+    const void*  v;                  /* (n_seq, n_tok, n_head, n_val)         */
+    const float* g;                  /* (n_seq, n_tok, n_head)                */
+    const float* beta;               /* the same                              */
+    const float* s0;                 /* NULL: zero                            */
+    void*        o;                  /* as v                                  */
+    float*       s;                  /* the state after the last token        */
+    void*        scratch;            /* helix_delta_rule_scratch_size() bytes,
+                                        16-byte aligned                       */
+    uint64_t     scratch_bytes;
+    int64_t      seq_q, tok_q, head_q, seq_k, tok_k, head_k, seq_v, tok_v, head_v;
+    int64_t      seq_g, tok_g, seq_beta, tok_beta, seq_o, tok_o, head_o;
+} helix_delta_rule_args;
+
+/* From the sizes and io_dtype; the other fields are not read. */
+size_t       helix_delta_rule_scratch_size(const helix_delta_rule_args* args);
+helix_status helix_delta_rule_encode(helix_ctx* ctx, void* stream, const helix_delta_rule_args* args);
 
 #ifdef __cplusplus
 }
