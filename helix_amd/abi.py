@@ -34,7 +34,8 @@ LAYER_SYMBOLS = ("helix_norm_encode", "helix_quantize_fp8_encode", "helix_norm_b
                  "helix_norm_backward_encode", "helix_group_norm_encode", "helix_group_norm_backward_scratch_size",
                  "helix_group_norm_backward_encode", "helix_matmul_fp8_scratch_size", "helix_matmul_fp8_encode", "helix_gated_scan_scratch_size",
                  "helix_gated_scan_encode", "helix_gated_scan_backward_scratch_size",
-                 "helix_gated_scan_backward_encode", "helix_delta_rule_scratch_size", "helix_delta_rule_encode")
+                 "helix_gated_scan_backward_encode", "helix_delta_rule_scratch_size", "helix_delta_rule_encode",
+                 "helix_delta_rule_backward_scratch_size", "helix_delta_rule_backward_encode")
 # include/helix/helix_host.h HELIX_PASS_B_*: where Pass B's segment scan runs
 PASS_B_LAUNCHED, PASS_B_IN_C = 0, 1
 # include/helix/helix_host.h HELIX_NOALLOC_SCRATCH_BYTES
@@ -97,6 +98,7 @@ MATMUL_FP8_STRUCT = struct.Struct("=4i7Q5q")
 GATED_SCAN_STRUCT = struct.Struct("=4i7Q6q")
 GATED_SCAN_BACKWARD_STRUCT = struct.Struct("=4i11Q12q")
 DELTA_RULE_STRUCT = struct.Struct("=7if10Q16q")
+DELTA_RULE_BACKWARD_STRUCT = struct.Struct("=7if16Q16q")
 assert DESC_STRUCT.size == ctypes.sizeof(HelixScanDesc)
 
 

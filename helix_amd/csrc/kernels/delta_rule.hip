@@ -141,12 +141,12 @@ constexpr int DR_LD = DR_C + 4;   // fp32 rows of a chunk's square matrices in L
 // A workgroup a chunk of a head. Wave w: rows 16 w .. of K K' and Q K'; the inverse of A's diagonal block w by forward
 // substitution, a column a lane; then block column w of the inverse, from the diagonal down:
 //     T_iw = -T_ii (sum over j of A_ij T_jw),  w <= j < i
-// on fp32 matrix instructions, T_jw staying in the registers it was formed in. BWD: X' and P' as well, without P.
+// on fp32 matrix instructions, T_jw staying in the registers it was formed in. BWD: T' and P' with X, without P.
 template <typename T, int NK, bool BWD>
 __device__ void delta_prep(const HelixDeltaParams& p) {
     constexpr int NPL = dr_planes<T>, NO = dr_out_planes<T>, KP = NK + 8;
     __shared__ __bf16 sK[NPL][DR_C][KP];
-    __shared__ float sA[DR_C][DR_LD], sX[DR_C][DR_LD], sP[DR_C][DR_LD];
+    __shared__ float sA[DR_C][DR_LD], sT[DR_C][DR_LD], sP[DR_C][DR_LD];
     __shared__ float sD[4][16][20];
     __shared__ double sG[DR_C];
     __shared__ float sB[DR_C];
@@ -176,6 +176,7 @@ __device__ void delta_prep(const HelixDeltaParams& p) {
         float* dec = p.decay + id * (HELIX_DR_DECAY / 4ll);
         dec[lane] = exp_diff(G, 0.0);
         dec[64 + lane] = exp_diff(end, G);
+        dec[128 + lane] = bl;
     }
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
@@ -215,7 +216,7 @@ __device__ void delta_prep(const HelixDeltaParams& p) {
             const float e = j <= w && jj <= i ? exp_diff(sG[i], Gj) : 0.0f;
             sA[i][jj] = jj < i && j <= w ? sB[i] * (e * kk[j][r]) : 0.0f;
             sP[i][jj] = jj <= i && j <= w ? p.scale * (e * qk[j][r]) : 0.0f;
-            if (j > w) sX[i][jj] = 0.0f;
+            if (j > w) sT[i][jj] = 0.0f;
         }
     }
     __syncthreads();
@@ -240,10 +241,9 @@ __device__ void delta_prep(const HelixDeltaParams& p) {
         f32x4 t[4];
 #pragma unroll
         for (int r = 0; r < 4; ++r) t[0][r] = sD[w][4 * q + r][c];
-        const float b = sB[16 * w + c];
         auto put = [&](int i, const f32x4& v) {
 #pragma unroll
-            for (int r = 0; r < 4; ++r) sX[16 * i + 4 * q + r][16 * w + c] = v[r] * b;
+            for (int r = 0; r < 4; ++r) sT[16 * i + 4 * q + r][16 * w + c] = v[r];
         };
         put(w, t[0]);
 #pragma unroll
@@ -276,7 +276,7 @@ __device__ void delta_prep(const HelixDeltaParams& p) {
         const int row = 16 * w + c, col = 32 * ks + 8 * q;
         if (ks == 0 || w > 1) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = sX[row][col + e];
+            for (int e = 0; e < 8; ++e) v[e] = sT[row][col + e] * sB[col + e];
             emit(p.x, dr_low(w, ks), v, std::integral_constant<int, 3>{});
             if constexpr (!BWD) {
 #pragma unroll
@@ -287,8 +287,8 @@ __device__ void delta_prep(const HelixDeltaParams& p) {
         if constexpr (BWD) {
             if (ks == 1 || w < 2) {
 #pragma unroll
-                for (int e = 0; e < 8; ++e) v[e] = sX[col + e][row];
-                emit(p.xt, dr_up(w, ks), v, std::integral_constant<int, 3>{});
+                for (int e = 0; e < 8; ++e) v[e] = sT[col + e][row];
+                emit(p.tt, dr_up(w, ks), v, std::integral_constant<int, 3>{});
 #pragma unroll
                 for (int e = 0; e < 8; ++e) v[e] = sP[col + e][row];
                 emit(p.pt, dr_up(w, ks), v, std::integral_constant<int, 3>{});
@@ -484,6 +484,496 @@ __device__ void delta_walk(const HelixDeltaParams& p) {
     }
 }
 
+// ---- backward -----------------------------------------------------------------------------
+//
+// With dO, and E the gradient of the state after a chunk (dS of the one before it, or the
+// caller's):
+//     dD = P' dO + (e^(G_63 - G) K) E,   Z = T' dD,   dV = beta Z
+//     dS = e^(G_63) E + scale (e^G Q)' dO - (e^G K)' dV
+// from the last chunk to the first: helix_delta_back_*, spread and laid out as the walk, dO
+// and e^G dO in V's place. It leaves E and Z for helix_delta_grad_*.
+template <typename T, int NK>
+__device__ void delta_back(const HelixDeltaParams& p) {
+    constexpr int NPL = dr_planes<T>, KP = NK + 8, TP = DR_C + 8, NT = NK / 64, KS = NK / 32;
+    __shared__ __bf16 sK[NPL][DR_C][KP], sQ[NPL][DR_C][KP];
+    __shared__ __bf16 sE[3][16][KP];
+    __shared__ __bf16 sO[NPL][16][TP], sW[3][16][TP], sR[3][16][TP], sU[3][16][TP];
+    const int tid = threadIdx.x, lane = lane_id(), w = wave_uniform(), c = lane & 15, q = lane >> 4;
+    const unsigned id = xcd_logical_id(blockIdx.x, gridDim.x);
+    const int slice = (int)(id % (unsigned)p.n_slice);
+    const unsigned sh = id / (unsigned)p.n_slice;
+    const int seq = (int)(sh / (unsigned)p.n_head), h = (int)(sh % (unsigned)p.n_head), hk = h / p.share;
+    const int p0 = 16 * slice, P = p.n_val, N = p.n_key;
+    const unsigned state_bytes = (unsigned)N * (unsigned)P * 4u;
+    const int row0 = 16 * w + 4 * q;
+    auto state_off = [&](int i, int r) {
+        const int n = NT * 16 * w + 16 * i + 4 * q + r;
+        return n < N && p0 + c < P ? (n * P + p0 + c) * 4 : (int)0x80000000;
+    };
+    auto put_state = [&](const f32x4 (&S)[NT], helix_rsrc r0) {
+#pragma unroll
+        for (int i = 0; i < NT; ++i)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) __builtin_amdgcn_raw_buffer_store_b32(as_u32(S[i][r]), r0, state_off(i, r), 0, 0);
+    };
+    f32x4 E[NT];
+    {
+        const helix_rsrc r0 = make_rsrc_u(p.d_s + (long long)sh * N * P, p.d_s ? state_bytes : 0u);   // none: reads 0
+#pragma unroll
+        for (int i = 0; i < NT; ++i)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) E[i][r] = buf_f32(r0, state_off(i, r), 0);
+    }
+    constexpr int PER = DR_C * (NK / 8) / 256;
+    struct Ahead {
+        Raw8<T> k[PER], q[PER];
+        bf16x8 t[2][3], p[2][3];
+        unsigned o[4];
+        f32x4 start, left, beta;
+        float all;
+    } next;
+    auto load = [&](int ch) {
+        const long long t0 = (long long)(p.chunk0 + ch) * DR_C;
+        const int len = (int)min((long long)DR_C, p.n_tok - t0);
+        const Rows<T> rk(p.k, seq * p.seq_k + hk * p.head_k + t0 * p.tok_k, p.tok_k, len, N);
+        const Rows<T> rq(p.q, seq * p.seq_q + hk * p.head_q + t0 * p.tok_q, p.tok_q, len, N);
+        const Rows<T> ro(p.d_o, seq * p.seq_o + h * p.head_o + t0 * p.tok_o, p.tok_o, len, P);
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            const int row = (tid + 256 * i) / (NK / 8), col = 8 * ((tid + 256 * i) % (NK / 8));
+            next.k[i] = rk.load8(row, col);
+            next.q[i] = rq.load8(row, col);
+        }
+        const long long at = (long long)sh * p.n_chunk + ch;
+        const char* tt = p.tt + at * (6 * 3 * HELIX_DR_FRAG) + 16 * lane;
+        const char* pt = p.pt + at * (6 * 3 * HELIX_DR_FRAG) + 16 * lane;
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks) {
+            if (ks == 0 && w > 1) continue;
+#pragma unroll
+            for (int k = 0; k < 3; ++k) {
+                next.t[ks][k] = *reinterpret_cast<const bf16x8*>(tt + (dr_up(w, ks) * 3 + k) * HELIX_DR_FRAG);
+                next.p[ks][k] = *reinterpret_cast<const bf16x8*>(pt + (dr_up(w, ks) * 3 + k) * HELIX_DR_FRAG);
+            }
+        }
+#pragma unroll
+        for (int r = 0; r < 4; ++r) next.o[r] = ro.raw(row0 + r, p0 + c);
+        const float* dec = p.decay + at * (HELIX_DR_DECAY / 4);
+        next.start = *reinterpret_cast<const f32x4*>(dec + row0);
+        next.left = *reinterpret_cast<const f32x4*>(dec + 64 + row0);
+        next.beta = *reinterpret_cast<const f32x4*>(dec + 128 + row0);
+        next.all = dec[63];
+    };
+    if (p.n_chunk) load(p.n_chunk - 1);
+    for (int ch = p.n_chunk - 1; ch >= 0; --ch) {
+        const Ahead now = next;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            const int row = (tid + 256 * i) / (NK / 8), col = 8 * ((tid + 256 * i) % (NK / 8));
+            bf16x8 k[NPL], qq[NPL];
+            dr_operand<T>(now.k[i], N - col, k);
+            dr_operand<T>(now.q[i], N - col, qq);
+#pragma unroll
+            for (int j = 0; j < NPL; ++j) {
+                *reinterpret_cast<bf16x8*>(&sK[j][row][col]) = k[j];
+                *reinterpret_cast<bf16x8*>(&sQ[j][row][col]) = qq[j];
+            }
+        }
+        {
+            float o[4];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) o[r] = raw_f32<T>(now.o[r]);
+            dr_put4<NPL>(&sO[0][c][row0], 16 * TP, o[0], o[1], o[2], o[3]);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) o[r] *= p.scale * now.start[r];
+            dr_put4<3>(&sW[0][c][row0], 16 * TP, o[0], o[1], o[2], o[3]);
+        }
+#pragma unroll
+        for (int i = 0; i < NT; ++i)
+            dr_put4<3>(&sE[0][c][NT * 16 * w + 16 * i + 4 * q], 16 * KP, E[i][0], E[i][1], E[i][2], E[i][3]);
+        if (ch) load(ch - 1);
+        const long long at = (long long)sh * p.n_chunk + ch;
+        const long long t0 = (long long)(p.chunk0 + ch) * DR_C;
+        const int len = (int)min((long long)DR_C, p.n_tok - t0);
+        __syncthreads();
+        put_state(E, make_rsrc_u(p.keep_e + at * N * P, state_bytes));
+        f32x4 ke = zero4();
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+            const int col = 32 * s + 8 * q;
+            bf16x8 a[NPL], b[3];
+            dr_get8<NPL>(&sK[0][16 * w + c][col], DR_C * KP, a);
+            dr_get8<3>(&sE[0][c][col], 16 * KP, b);
+            ke = dr_mfma<NPL, 3>(a, b, ke);
+        }
+        f32x4 dd = ke * now.left;
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks) {
+            if (ks == 0 && w > 1) continue;
+            bf16x8 b[NPL];
+            dr_get8<NPL>(&sO[0][c][32 * ks + 8 * q], 16 * TP, b);
+            dd = dr_mfma<3, NPL>(now.p[ks], b, dd);
+        }
+        dr_put4<3>(&sR[0][c][row0], 16 * TP, dd[0], dd[1], dd[2], dd[3]);
+        __syncthreads();
+        f32x4 Z = zero4();
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks) {
+            if (ks == 0 && w > 1) continue;
+            bf16x8 b[3];
+            dr_get8<3>(&sR[0][c][32 * ks + 8 * q], 16 * TP, b);
+            Z = dr_mfma<3, 3>(now.t[ks], b, Z);
+        }
+        const f32x4 dv = Z * now.beta;
+        const f32x4 u = -(dv * now.start);
+        dr_put4<3>(&sU[0][c][row0], 16 * TP, u[0], u[1], u[2], u[3]);
+        const Rows<float> rz(p.keep_z, at * DR_C * P, P, DR_C, P);
+        const Rows<T> rv(p.dv, (((long long)seq * p.n_tok + t0) * p.n_head + h) * P, (long long)p.n_head * P, len, P);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            rz.store(row0 + r, p0 + c, Z[r]);
+            rv.store(row0 + r, p0 + c, dv[r]);
+        }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < NT; ++i) E[i] *= now.all;
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks) {
+            bf16x8 bw[3], bu[3];
+            dr_get8<3>(&sW[0][c][32 * ks + 8 * q], 16 * TP, bw);
+            dr_get8<3>(&sU[0][c][32 * ks + 8 * q], 16 * TP, bu);
+#pragma unroll
+            for (int i = 0; i < NT; ++i) {
+                bf16x8 a[NPL];
+                dr_get8_t<NPL>(&sQ[0][32 * ks + 8 * q][NT * 16 * w + 16 * i], KP, DR_C * KP, c, a);
+                E[i] = dr_mfma<NPL, 3>(a, bw, E[i]);
+                dr_get8_t<NPL>(&sK[0][32 * ks + 8 * q][NT * 16 * w + 16 * i], KP, DR_C * KP, c, a);
+                E[i] = dr_mfma<NPL, 3>(a, bu, E[i]);
+            }
+        }
+        __syncthreads();   // K, Q and the operands are written again
+    }
+    put_state(E, make_rsrc_u(p.ds0 + (long long)sh * N * P, state_bytes));
+}
+
+// The other gradients, a chunk of a head of queries and keys a workgroup, its value heads one
+// after another. With D, Z, E and the state S before the chunk:
+//     U = dO S',  B = Z S',  L = D E';   dP = dO D' for j <= i,  dA = -Z D' below the diagonal
+//     M_P = scale dP . E_ij,  M_A = beta_i dA . E_ij       (summed over the heads that share)
+//     dQ = scale e^G U + M_P K
+//     dK = e^(G_63 - G) L - e^G beta B + M_P' Q + (M_A + M_A') K
+//     dbeta = Z . V - e^G (K . B) + sum_j dA . E_ij . K K'
+// and g_t has the sum over i >= t of what G_i has: M_P . Q K' + M_A . K K' by rows less by
+// columns, scale e^G (Q . U) - e^G beta (K . B) - e^(G_63 - G) (K . L), and for the last one the
+// sum of e^(G_63 - G) (K . L) and e^(G_63) (S . E); in fp64, as neighbours nearly cancel.
+// A wave has 16 of the keys' columns (U, B, L, dQ, dK for all tokens; its rows of S and E
+// straight from memory) and blocks of the triangles. Operands that waves share are in LDS, by
+// parts: dO, Z and D 64 columns at a time; K and Q before and after.
+template <typename T, int NK>
+__device__ void delta_grad(const HelixDeltaParams& p) {
+    constexpr int NPL = dr_planes<T>, NO = dr_out_planes<T>, KP = NK + 8, TP = DR_C + 8, W = NK / 16, TH = 64 * W;
+    constexpr int TILES = (10 + W - 1) / W, ROWS = DR_C * 8 / TH;
+    constexpr int kKQ = 2 * NPL * DR_C * KP, kOZD = (NPL + 6) * DR_C * TP;
+    __shared__ __bf16 sBig[kKQ > kOZD ? kKQ : kOZD];
+    struct Sums {   // of a head; the triangles' parts take their place at the end
+        double G[DR_C];
+        float row[4][DR_C], col[4][DR_C], beta[4][DR_C], dot[3][W][DR_C], zv[DR_C], se[W];
+    };
+    __shared__ __attribute__((aligned(16))) __bf16 sM[2][NO][DR_C][TP];
+    static_assert(sizeof(Sums) <= sizeof(sM), "the sums fit in the triangles' place");
+    Sums& sums = *reinterpret_cast<Sums*>(&sM[0][0][0][0]);
+    __bf16* const sK = sBig;
+    __bf16* const sQ = sBig + NPL * DR_C * KP;
+    __bf16* const sO = sBig;
+    __bf16* const sZ = sBig + NPL * DR_C * TP;
+    __bf16* const sD = sZ + 3 * DR_C * TP;
+    const int tid = threadIdx.x, lane = lane_id(), w = wave_uniform(), c = lane & 15, q = lane >> 4;
+    const unsigned id = blockIdx.x;
+    const int ch = (int)(id % (unsigned)p.n_chunk);
+    const unsigned sk = id / (unsigned)p.n_chunk;
+    const int seq = (int)(sk / (unsigned)p.n_qk), hk = (int)(sk % (unsigned)p.n_qk);
+    const long long t0 = (long long)(p.chunk0 + ch) * DR_C;
+    const int len = (int)min((long long)DR_C, p.n_tok - t0), P = p.n_val, N = p.n_key;
+    const int n0 = 16 * w;
+    const Rows<T> rk(p.k, seq * p.seq_k + hk * p.head_k + t0 * p.tok_k, p.tok_k, len, N);
+    const Rows<T> rq(p.q, seq * p.seq_q + hk * p.head_q + t0 * p.tok_q, p.tok_q, len, N);
+    auto stage_kq = [&] {
+#pragma unroll
+        for (int i = 0; i < DR_C * (NK / 8) / TH; ++i) {
+            const int row = (tid + TH * i) / (NK / 8), col = 8 * ((tid + TH * i) % (NK / 8));
+            const Raw8<T> kr = rk.load8(row, col), qr = rq.load8(row, col);
+            bf16x8 k[NPL], qq[NPL];
+            dr_operand<T>(kr, N - col, k);
+            dr_operand<T>(qr, N - col, qq);
+#pragma unroll
+            for (int j = 0; j < NPL; ++j) {
+                *reinterpret_cast<bf16x8*>(&sK[(j * DR_C + row) * KP + col]) = k[j];
+                *reinterpret_cast<bf16x8*>(&sQ[(j * DR_C + row) * KP + col]) = qq[j];
+            }
+        }
+    };
+    // The wave's blocks (tb, jb) of the lower triangle: K K' and Q K'.
+    auto tb_of = [&](int k) { const int x = w + W * k; return (x >= 1) + (x >= 3) + (x >= 6); };
+    auto jb_of = [&](int k) { const int x = w + W * k, t = tb_of(k); return x - t * (t + 1) / 2; };
+    f32x4 kk[TILES], qk[TILES], mp[TILES], ma[TILES];
+    f32x4 kv[4], qv[4], dq[4], dk[4];   // k, q at (16 i + 4 q + r, n0 + c), and their gradients
+    stage_kq();
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < TILES; ++k) {
+        kk[k] = qk[k] = mp[k] = ma[k] = zero4();
+        if (w + W * k > 9) continue;
+        const int tb = tb_of(k), jb = jb_of(k);
+#pragma unroll
+        for (int s = 0; s < NK / 32; ++s) {
+            const int col = 32 * s + 8 * q;
+            bf16x8 a[NPL], b[NPL];
+            dr_get8<NPL>(&sK[(16 * jb + c) * KP + col], DR_C * KP, b);
+            dr_get8<NPL>(&sK[(16 * tb + c) * KP + col], DR_C * KP, a);
+            kk[k] = dr_mfma<NPL, NPL>(a, b, kk[k]);
+            dr_get8<NPL>(&sQ[(16 * tb + c) * KP + col], DR_C * KP, a);
+            qk[k] = dr_mfma<NPL, NPL>(a, b, qk[k]);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        dq[i] = dk[i] = zero4();
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const int at = (16 * i + 4 * q + r) * KP + n0 + c;
+            float a = 0.0f, b = 0.0f;
+#pragma unroll
+            for (int j = NPL - 1; j >= 0; --j) {
+                a += (float)sK[j * DR_C * KP + at];
+                b += (float)sQ[j * DR_C * KP + at];
+            }
+            kv[i][r] = a;
+            qv[i][r] = b;
+        }
+    }
+    for (int hs = 0; hs < p.share; ++hs) {
+        const int h = hk * p.share + hs;
+        const long long at = ((long long)seq * p.n_head + h) * p.n_chunk + ch;
+        const Rows<T> ro(p.d_o, seq * p.seq_o + h * p.head_o + t0 * p.tok_o, p.tok_o, len, P);
+        const Rows<T> rv(p.v, seq * p.seq_v + h * p.head_v + t0 * p.tok_v, p.tok_v, len, P);
+        const Rows<float> rz(p.keep_z, at * DR_C * P, P, DR_C, P), rd(p.keep_d, at * DR_C * P, P, DR_C, P);
+        const Rows<float> rs(p.keep_s, at * N * P, P, N, P), re(p.keep_e, at * N * P, P, N, P);
+        f32x4 U[4], B[4], L[4], dP[TILES], dA[TILES];
+        float zv[ROWS], se = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) U[i] = B[i] = L[i] = zero4();
+#pragma unroll
+        for (int k = 0; k < TILES; ++k) dP[k] = dA[k] = zero4();
+#pragma unroll
+        for (int i = 0; i < ROWS; ++i) zv[i] = 0.0f;
+        for (int pb = 0; pb < P; pb += 64) {
+            __syncthreads();   // what these overwrite has been read
+#pragma unroll
+            for (int i = 0; i < ROWS; ++i) {
+                const int row = (tid + TH * i) / 8, col = 8 * (tid % 8), n = P - pb - col;
+                const Raw8<T> orow = ro.load8(row, pb + col), vr = rv.load8(row, pb + col);
+                const Raw8<float> zr = rz.load8(row, pb + col), dr = rd.load8(row, pb + col);
+                bf16x8 o[NPL], z[3], d[3];
+                dr_operand<T>(orow, n, o);
+                dr_operand<float>(zr, n, z);
+                dr_operand<float>(dr, n, d);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) zv[i] += e < n ? at8(zr, e) * at8(vr, e) : 0.0f;
+#pragma unroll
+                for (int j = 0; j < NPL; ++j) *reinterpret_cast<bf16x8*>(&sO[(j * DR_C + row) * TP + col]) = o[j];
+#pragma unroll
+                for (int j = 0; j < 3; ++j) {
+                    *reinterpret_cast<bf16x8*>(&sZ[(j * DR_C + row) * TP + col]) = z[j];
+                    *reinterpret_cast<bf16x8*>(&sD[(j * DR_C + row) * TP + col]) = d[j];
+                }
+            }
+            Raw8<float> sr[2], er[2];
+#pragma unroll
+            for (int ks = 0; ks < 2; ++ks) {
+                sr[ks] = rs.load8(n0 + c, pb + 32 * ks + 8 * q);
+                er[ks] = re.load8(n0 + c, pb + 32 * ks + 8 * q);
+            }
+            __syncthreads();
+#pragma unroll
+            for (int ks = 0; ks < 2; ++ks) {
+                const int col = 32 * ks + 8 * q, n = P - pb - col;
+                bf16x8 bs[3], be[3];
+                dr_operand<float>(sr[ks], n, bs);
+                dr_operand<float>(er[ks], n, be);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) se += e < n ? at8(sr[ks], e) * at8(er[ks], e) : 0.0f;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int a_at = (16 * i + c) * TP + col;
+                    bf16x8 ao[NPL], az[3], ad[3];
+                    dr_get8<NPL>(&sO[a_at], DR_C * TP, ao);
+                    U[i] = dr_mfma<NPL, 3>(ao, bs, U[i]);
+                    dr_get8<3>(&sZ[a_at], DR_C * TP, az);
+                    B[i] = dr_mfma<3, 3>(az, bs, B[i]);
+                    dr_get8<3>(&sD[a_at], DR_C * TP, ad);
+                    L[i] = dr_mfma<3, 3>(ad, be, L[i]);
+                }
+#pragma unroll
+                for (int k = 0; k < TILES; ++k) {
+                    if (w + W * k > 9) continue;
+                    const int tb = tb_of(k), jb = jb_of(k);
+                    bf16x8 ao[NPL], az[3], bd[3];
+                    dr_get8<3>(&sD[(16 * jb + c) * TP + col], DR_C * TP, bd);
+                    dr_get8<NPL>(&sO[(16 * tb + c) * TP + col], DR_C * TP, ao);
+                    dP[k] = dr_mfma<NPL, 3>(ao, bd, dP[k]);
+                    dr_get8<3>(&sZ[(16 * tb + c) * TP + col], DR_C * TP, az);
+                    dA[k] = dr_mfma<3, 3>(az, bd, dA[k]);
+                }
+            }
+        }
+        const float gl = lane < len ? p.g[seq * p.seq_g + (t0 + lane) * p.tok_g + h] : 0.0f;
+        const double G = dr_log_decay(gl);
+        const float* dec = p.decay + at * (HELIX_DR_DECAY / 4);
+        if (w == 0) sums.G[lane] = G;
+#pragma unroll
+        for (int i = 0; i < ROWS; ++i) {
+            // Eight lanes a row.
+            float z = zv[i];
+            z += __shfl_xor(z, 1, 64);
+            z += __shfl_xor(z, 2, 64);
+            z += __shfl_xor(z, 4, 64);
+            if ((tid & 7) == 0) sums.zv[(tid + TH * i) / 8] = z;
+        }
+        se = wave_sum(se);
+        if (lane == 0) sums.se[w] = se;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int row = 16 * i + 4 * q;
+            const f32x4 start = *reinterpret_cast<const f32x4*>(dec + row), left = *reinterpret_cast<const f32x4*>(dec + 64 + row),
+                        beta = *reinterpret_cast<const f32x4*>(dec + 128 + row);
+            dq[i] += p.scale * start * U[i];
+            dk[i] += left * L[i] - start * beta * B[i];
+            const f32x4 x = qv[i] * U[i], y = kv[i] * B[i], z = kv[i] * L[i];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const float a = row16_sum(x[r]), b = row16_sum(y[r]), l = row16_sum(z[r]);
+                if (c == 0) {
+                    sums.dot[0][w][row + r] = a;
+                    sums.dot[1][w][row + r] = b;
+                    sums.dot[2][w][row + r] = l;
+                }
+            }
+        }
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < TILES; ++k) {
+            if (w + W * k > 9) continue;
+            const int tb = tb_of(k), jb = jb_of(k), j = 16 * jb + c;
+            const double Gj = sums.G[j];
+            const f32x4 beta = *reinterpret_cast<const f32x4*>(dec + 128 + 16 * tb + 4 * q);
+            float col = 0.0f;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int i = 16 * tb + 4 * q + r;
+                const float e = j <= i ? exp_diff(sums.G[i], Gj) : 0.0f, ea = j < i ? -(e * dA[k][r]) : 0.0f;
+                const float m = j <= i ? p.scale * (e * dP[k][r]) : 0.0f, n = beta[r] * ea;
+                mp[k][r] += m;
+                ma[k][r] += n;
+                const float b = ea * kk[k][r], pair = m * qk[k][r] + beta[r] * b;
+                col += pair;
+                const float row = row16_sum(pair), bs = row16_sum(b);
+                if (c == 0) {
+                    sums.row[jb][i] = row;
+                    sums.beta[jb][i] = bs;
+                }
+            }
+            col += __shfl_xor(col, 16, 64);
+            col += __shfl_xor(col, 32, 64);
+            if (q == 0) sums.col[tb][j] = col;
+        }
+        __syncthreads();
+        if (w == 0) {
+            // Lane = token.
+            float dots[3];
+#pragma unroll
+            for (int j = 0; j < 3; ++j) {
+                dots[j] = 0.0f;
+#pragma unroll
+                for (int x = 0; x < W; ++x) dots[j] += sums.dot[j][x][lane];
+            }
+            float sse = 0.0f;
+#pragma unroll
+            for (int x = 0; x < W; ++x) sse += sums.se[x];
+            const float start = dec[lane], left = dec[64 + lane], beta = dec[128 + lane];
+            const int tile = lane >> 4;
+            double own = 0.0;
+            float db = 0.0f;
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+                if (x <= tile) {
+                    own += sums.row[x][lane];
+                    db += sums.beta[x][lane];
+                }
+                if (x >= tile) own -= sums.col[x][lane];
+            }
+            const double tail = (double)left * dots[2];
+            own += (double)(p.scale * start) * dots[0] - (double)(start * beta) * dots[1] - tail;
+            const double tails = __shfl(wave_incl_sum(tail), 63, 64);
+            if (lane == 63) own += tails + (double)dec[63] * sse;
+            const double incl = wave_incl_sum(own);
+            const double dg = __shfl(incl, 63, 64) - incl + own;
+            if (lane < len) {
+                const long long to = ((long long)seq * p.n_tok + t0 + lane) * p.n_head + h;
+                p.dg[to] = (float)dg;
+                p.dbeta[to] = sums.zv[lane] - start * dots[1] + db;
+            }
+        }
+    }
+    // The triangles' products, once for all heads.
+    __syncthreads();
+    stage_kq();
+#pragma unroll
+    for (int k = 0; k < TILES; ++k) {
+        if (w + W * k > 9) continue;
+        const int tb = tb_of(k), jb = jb_of(k);
+        // Stored by columns: M[j][i].
+        dr_put4<NO>(&sM[0][0][16 * jb + c][16 * tb + 4 * q], DR_C * TP, mp[k][0], mp[k][1], mp[k][2], mp[k][3]);
+        dr_put4<NO>(&sM[1][0][16 * jb + c][16 * tb + 4 * q], DR_C * TP, ma[k][0], ma[k][1], ma[k][2], ma[k][3]);
+        if (tb != jb) {   // 0 above the diagonal
+            dr_put4<NO>(&sM[0][0][16 * tb + c][16 * jb + 4 * q], DR_C * TP, 0.0f, 0.0f, 0.0f, 0.0f);
+            dr_put4<NO>(&sM[1][0][16 * tb + c][16 * jb + 4 * q], DR_C * TP, 0.0f, 0.0f, 0.0f, 0.0f);
+        }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks) {
+        bf16x8 bk[NPL], bq[NPL];
+        dr_get8_t<NPL>(&sK[(32 * ks + 8 * q) * KP + n0], KP, DR_C * KP, c, bk);
+        dr_get8_t<NPL>(&sQ[(32 * ks + 8 * q) * KP + n0], KP, DR_C * KP, c, bq);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            bf16x8 a[NO];
+            // M[i][j] over j: columns of what is stored; M'[j][i] over i: its rows.
+            if (2 * ks <= i) {
+                dr_get8_t<NO>(&sM[0][0][32 * ks + 8 * q][16 * i], TP, DR_C * TP, c, a);
+                dq[i] = dr_mfma<NO, NPL, NO>(a, bk, dq[i]);
+                dr_get8_t<NO>(&sM[1][0][32 * ks + 8 * q][16 * i], TP, DR_C * TP, c, a);
+                dk[i] = dr_mfma<NO, NPL, NO>(a, bk, dk[i]);
+            }
+            if (2 * ks + 1 >= i) {
+                dr_get8<NO>(&sM[0][0][16 * i + c][32 * ks + 8 * q], DR_C * TP, a);
+                dk[i] = dr_mfma<NO, NPL, NO>(a, bq, dk[i]);
+                dr_get8<NO>(&sM[1][0][16 * i + c][32 * ks + 8 * q], DR_C * TP, a);
+                dk[i] = dr_mfma<NO, NPL, NO>(a, bk, dk[i]);
+            }
+        }
+    }
+    const long long to = (((long long)seq * p.n_tok + t0) * p.n_qk + hk) * N;
+    const Rows<T> oq(p.dq, to, (long long)p.n_qk * N, len, N), ok(p.dk, to, (long long)p.n_qk * N, len, N);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            oq.store(16 * i + 4 * q + r, n0 + c, dq[i][r]);
+            ok.store(16 * i + 4 * q + r, n0 + c, dk[i][r]);
+        }
+}
+
 }  // namespace
 
 #define DR_KERNELS(TAG, T, NK)                                                                                              \
@@ -495,6 +985,18 @@ __device__ void delta_walk(const HelixDeltaParams& p) {
     }                                                                                                                       \
     extern "C" __global__ __launch_bounds__(256) void helix_delta_walk_##TAG##_##NK(HelixDeltaParams p) {                   \
         delta_walk<T, NK, false>(p);                                                                                        \
+    }                                                                                                                       \
+    extern "C" __global__ __launch_bounds__(256) void helix_delta_prep_bwd_##TAG##_##NK(HelixDeltaParams p) {               \
+        delta_prep<T, NK, true>(p);                                                                                         \
+    }                                                                                                                       \
+    extern "C" __global__ __launch_bounds__(256) void helix_delta_keep_##TAG##_##NK(HelixDeltaParams p) {                   \
+        delta_walk<T, NK, true>(p);                                                                                         \
+    }                                                                                                                       \
+    extern "C" __global__ __launch_bounds__(256) void helix_delta_back_##TAG##_##NK(HelixDeltaParams p) {                   \
+        delta_back<T, NK>(p);                                                                                               \
+    }                                                                                                                       \
+    extern "C" __global__ __launch_bounds__(4 * NK) void helix_delta_grad_##TAG##_##NK(HelixDeltaParams p) {                \
+        delta_grad<T, NK>(p);                                                                                               \
     }
 DR_KERNELS(f32, float, 64)
 DR_KERNELS(f32, float, 128)

@@ -67,10 +67,6 @@ HELIX_DEV void gn_weights(const void* w, int w_f32, int c, int n, float (&o)[8])
     }
 }
 
-template <int CTRL>
-HELIX_DEV float add_dpp(float v) {
-    return v + as_f32((unsigned)__builtin_amdgcn_update_dpp(0, (int)as_u32(v), CTRL, 0xf, 0xf, true));
-}
 // The sum over LP neighbouring lanes; all of them have it. 256: over the workgroup,
 // through red (one float per wave), which the next call does not use.
 template <int LP>

@@ -163,4 +163,16 @@ HELIX_DEV float row16_max(float v) {
     return max_dpp<0x140>(v);   // mirrored in sixteen
 }
 
+// The sum over each sixteen lanes, the same way.
+template <int CTRL>
+HELIX_DEV float add_dpp(float v) {
+    return v + as_f32((unsigned)__builtin_amdgcn_update_dpp(0, (int)as_u32(v), CTRL, 0xf, 0xf, true));
+}
+HELIX_DEV float row16_sum(float v) {
+    v = add_dpp<0xb1>(v);
+    v = add_dpp<0x4e>(v);
+    v = add_dpp<0x141>(v);
+    return add_dpp<0x140>(v);
+}
+
 #endif

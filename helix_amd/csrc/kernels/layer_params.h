@@ -153,9 +153,10 @@ typedef struct {
 
 /* Bytes, per chunk of a head, of the operands that the first kernel leaves for
  * the walks: fragments (16 bytes a lane) of six 16 x 32 blocks of a triangle, by
- * bf16 parts. And of its decays: exp(G_t) and exp(G_63 - G_t). */
+ * bf16 parts. And of 64 floats each of its decays exp(G_t) and exp(G_63 - G_t),
+ * and of beta. */
 #define HELIX_DR_FRAG 1024
-#define HELIX_DR_DECAY 512
+#define HELIX_DR_DECAY 768
 
 typedef struct {
     const void*  q;
@@ -176,14 +177,13 @@ typedef struct {
     float*       ds0;
     long long    seq_q, tok_q, head_q, seq_k, tok_k, head_k, seq_v, tok_v, head_v;
     long long    seq_g, tok_g, seq_b, tok_b, seq_o, tok_o, head_o;   /* (o, or its gradient) */
-    long long    seq_dq, tok_dq, seq_dk, tok_dk, seq_dv, tok_dv, seq_dg;   /* outputs' heads are dense */
     int          n_seq, n_tok, n_qk, n_head, share, n_key, n_val;   /* share = n_head / n_qk */
     float        scale;
     /* Chunked: the chunks chunk0 .. chunk0 + n_chunk - 1 of every sequence. */
     int          chunk0, n_chunk, n_slice;
     char*        x;         /* [sequence x head][chunk] fragments of X         */
     char*        p;         /* of scale P                                      */
-    char*        xt;        /* of X^T and P^T (backward)                       */
+    char*        tt;        /* of T^T and scale P^T (backward)                 */
     char*        pt;
     float*       decay;
     float*       keep_s;    /* [sequence x head][chunk][n_key][n_val] states before the chunks */

@@ -998,6 +998,126 @@ extern "C" helix_status helix_delta_rule_encode(helix_ctx* ctx, void* stream, co
     });
 }
 
+namespace {
+
+// The backward pass: what a segment's chunks leave for its kernels, and the states that the segments start from.
+struct DeltaBwdPlan {
+    int n_chunk = 0, chunks = 0, n_seg = 0, n_slice = 0;
+    size_t x_at = 0, tt_at = 0, pt_at = 0, decay_at = 0, s_at = 0, e_at = 0, d_at = 0, z_at = 0, start_at = 0, bytes = 0;
+};
+// Scratch of a segment: up to two gigabytes, and one chunk of every sequence where that is more. More than one segment forms
+// its states twice.
+constexpr size_t kDeltaBwdScratch = (size_t)2 << 30;
+
+DeltaBwdPlan delta_bwd_plan(const helix_delta_rule_backward_args& a) {
+    DeltaBwdPlan p;
+    if (a.n_seq <= 0 || a.n_head <= 0 || a.n_tok <= 0 || a.n_key <= 0 || a.n_val <= 0) return p;
+    const size_t sh = (size_t)a.n_seq * a.n_head, x = 6 * 3 * HELIX_DR_FRAG;
+    auto up = [](size_t bytes) { return (bytes + 255) & ~(size_t)255; };
+    const size_t state = (size_t)a.n_key * a.n_val * 4, rows = (size_t)HELIX_DR_CHUNK * a.n_val * 4;
+    p.n_chunk = (int)ceil_div(a.n_tok, HELIX_DR_CHUNK);
+    p.chunks = (int)std::min<size_t>(p.n_chunk,
+                                     std::max<size_t>(1, kDeltaBwdScratch / (sh * (3 * x + HELIX_DR_DECAY + 2 * state + 2 * rows))));
+    p.n_seg = (int)ceil_div(p.n_chunk, p.chunks);
+    p.n_slice = (int)ceil_div(a.n_val, HELIX_DR_SLICE);
+    const size_t each = sh * p.chunks;
+    p.tt_at = p.x_at + each * x;
+    p.pt_at = p.tt_at + each * x;
+    p.decay_at = p.pt_at + each * x;
+    p.s_at = p.decay_at + up(each * HELIX_DR_DECAY);
+    p.e_at = p.s_at + up(each * state);
+    p.d_at = p.e_at + up(each * state);
+    p.z_at = p.d_at + up(each * rows);
+    p.start_at = p.z_at + up(each * rows);
+    p.bytes = p.start_at + (size_t)(p.n_seg - 1) * up(sh * state);
+    return p;
+}
+
+}  // namespace
+
+extern "C" size_t helix_delta_rule_backward_scratch_size(const helix_delta_rule_backward_args* a) {
+    return a ? delta_bwd_plan(*a).bytes : 0;
+}
+
+extern "C" helix_status helix_delta_rule_backward_encode(helix_ctx* ctx, void* stream,
+                                                         const helix_delta_rule_backward_args* a) {
+    return entry(ctx, [&] {
+        need(ctx && a, "NULL context or arguments");
+        if (!delta_shape(*a)) return;
+        const size_t es = kBytes[a->io_dtype];
+        delta_inputs(*a, es);
+        heads("d_o", a->d_o, a->n_seq, a->n_tok, a->n_head, a->n_val, a->seq_do, a->tok_do, a->head_do, es, false);
+        for (const void* o : {(const void*)a->dq, (const void*)a->dk, (const void*)a->dv})
+            need(!a->n_tok || (o && aligned(o, es)), "dq, dk or dv is NULL or not aligned to its elements");
+        for (const float* o : {a->dg, a->dbeta})
+            need(!a->n_tok || (o && aligned(o, 4)), "dg or dbeta is NULL or not aligned to its elements");
+        need(a->ds0 != nullptr && aligned(a->ds0, 4) && aligned(a->d_s, 4),
+             "ds0 is NULL, or it or d_s not aligned to its elements");
+        need((long long)a->n_head * a->n_val < (1LL << 31) / 64 / (long long)es && (long long)a->n_qk_head * a->n_key < (1LL << 31) / 64 / (long long)es,
+             "64 tokens of dq, dk or dv span 2^31 bytes or more", HELIX_ERR_UNSUPPORTED_SHAPE);
+        const DeltaBwdPlan plan = delta_bwd_plan(*a);
+        need(plan.bytes == 0 || (a->scratch && a->scratch_bytes >= plan.bytes),
+             "scratch smaller than helix_delta_rule_backward_scratch_size()", HELIX_ERR_SCRATCH_TOO_SMALL);
+        need(aligned(a->scratch, 16), "scratch is not 16-byte aligned");
+        HelixDeltaParams p = delta_params(*a);
+        p.d_o = a->d_o;
+        p.d_s = a->d_s;
+        p.seq_o = a->seq_do;
+        p.tok_o = a->tok_do;
+        p.head_o = a->head_do;
+        p.dq = a->dq;
+        p.dk = a->dk;
+        p.dv = a->dv;
+        p.dg = a->dg;
+        p.dbeta = a->dbeta;
+        p.ds0 = a->ds0;
+        char* sc = static_cast<char*>(a->scratch);
+        p.x = sc + plan.x_at;
+        p.tt = sc + plan.tt_at;
+        p.pt = sc + plan.pt_at;
+        p.decay = reinterpret_cast<float*>(sc + plan.decay_at);
+        p.keep_s = reinterpret_cast<float*>(sc + plan.s_at);
+        p.keep_e = reinterpret_cast<float*>(sc + plan.e_at);
+        p.keep_d = reinterpret_cast<float*>(sc + plan.d_at);
+        p.keep_z = reinterpret_cast<float*>(sc + plan.z_at);
+        p.n_slice = (int)ceil_div(a->n_val, HELIX_DR_SLICE);
+        const int keys = delta_keys(a->n_key);
+        const std::string form = std::string(kTags[a->io_dtype]) + "_" + std::to_string(keys);
+        const hipFunction_t prep = kernel(ctx, "helix_delta_prep_bwd_" + form), keep = kernel(ctx, "helix_delta_keep_" + form),
+                            back = kernel(ctx, "helix_delta_back_" + form), grad = kernel(ctx, "helix_delta_grad_" + form);
+        const long long sh = (long long)a->n_seq * a->n_head, sk = (long long)a->n_seq * a->n_qk_head;
+        const unsigned gw = grid(sh * p.n_slice, kDeltaThreads);
+        grid(sh * plan.chunks, kDeltaThreads);
+        grid(sk * plan.chunks, 4 * keys);
+        const OnDevice on(ctx->device);
+        if (!a->n_tok) {
+            launch(back, stream, gw, 1, kDeltaThreads, p);
+            return;
+        }
+        const size_t state = ((size_t)sh * a->n_key * a->n_val * 4 + 255) & ~(size_t)255;
+        // The state before segment i (i > 0).
+        auto start = [&](int i) { return reinterpret_cast<float*>(sc + plan.start_at + (size_t)(i - 1) * state); };
+        auto states = [&](int i) {
+            p.chunk0 = i * plan.chunks;
+            p.n_chunk = std::min(plan.chunks, plan.n_chunk - p.chunk0);
+            p.s0 = i ? start(i) : a->s0;
+            launch(prep, stream, (unsigned)(sh * p.n_chunk), 1, kDeltaThreads, p);
+            launch(keep, stream, gw, 1, kDeltaThreads, p);
+        };
+        for (int i = 0; i + 1 < plan.n_seg; ++i) {
+            p.s = start(i + 1);
+            states(i);
+        }
+        p.s = nullptr;
+        for (int i = plan.n_seg - 1; i >= 0; --i) {
+            states(i);
+            launch(back, stream, gw, 1, kDeltaThreads, p);
+            launch(grad, stream, (unsigned)(sk * p.n_chunk), 1, (unsigned)(4 * keys), p);
+            p.d_s = p.ds0;   // the segment before goes on from here
+        }
+    });
+}
+
 namespace helix::rt {
 
 const std::vector<std::string>& layer_kernel_names() {
@@ -1015,7 +1135,7 @@ const std::vector<std::string>& layer_kernel_names() {
             }
         for (const char* tag : kTags)
             for (const char* n : {"_64", "_128"})
-                for (const char* k : {"steps_", "prep_", "walk_"}) v.push_back(std::string("helix_delta_") + k + tag + n);
+                for (const char* k : {"steps_", "prep_", "walk_", "prep_bwd_", "keep_", "back_", "grad_"}) v.push_back(std::string("helix_delta_") + k + tag + n);
         v.push_back("helix_group_norm_dw");
         for (const char* tag : kTags) {
             v.push_back(std::string("helix_group_norm_fp8_") + tag + "_any");

@@ -1,4 +1,4 @@
-"""Gated delta rule: a recurrence whose state is a matrix per head (include/helix/helix_layer.h).
+"""Gated delta rule, a recurrence whose state is a matrix per head, and its backward pass (include/helix/helix_layer.h).
 
     S_t = e^(g_t) S_(t-1) + beta_t k_t (v_t - e^(g_t) S_(t-1)' k_t)',  o_t = scale S_t' q_t,  S_(-1) = s0
 
@@ -10,7 +10,7 @@ from __future__ import annotations
 import torch
 
 from . import abi
-from .layer import device_index, expect, io_code, ptr, run_with_scratch, stream_handle, under
+from .layer import device_index, expect, io_code, packed, ptr, run, run_with_scratch, scratch, stream_handle, under
 
 
 def _strides(name: str, t: torch.Tensor) -> tuple[int, int, int]:
@@ -77,3 +77,34 @@ def delta_rule(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Tenso
     lib = abi.lib()
     run_with_scratch(lib.helix_delta_rule_encode, lib.helix_delta_rule_scratch_size, index, st, stream, pack)
     return o, s
+
+
+def delta_rule_backward(do: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Tensor,
+                        beta: torch.Tensor, s0: torch.Tensor | None = None, ds: torch.Tensor | None = None, *,
+                        scale: float | None = None, stream: torch.cuda.Stream | None = None):
+    """Gradients of delta_rule from do [S, L, H, P] and ds [S, H, N, P] (None: s is not used further): returns
+    (dq, dk, dv, dg, dbeta, ds0), dq, dk and dv of q's type, the others float32. The inputs are delta_rule's; its states
+    are formed again. dq and dk of a head that several heads of v share are the sums over them."""
+    index, sizes, strides = _inputs("delta_rule_backward", q, k, v, g, beta, s0, scale)
+    S, L, Hk, H, N, P = sizes[:6]
+    expect("do", do, q.dtype, (S, L, H, P), q)
+    _state("ds", ds, q, (S, H, N, P))
+    with under(index, stream):
+        dq, dk = (torch.empty(S, L, Hk, N, dtype=q.dtype, device=q.device) for _ in range(2))
+        dv = torch.empty(S, L, H, P, dtype=q.dtype, device=q.device)
+        dg, dbeta = (torch.empty(S, L, H, dtype=torch.float32, device=q.device) for _ in range(2))
+        ds0 = torch.empty(S, H, N, P, dtype=torch.float32, device=q.device)
+    st = stream_handle(index, stream)
+    strides = (*_strides("do", do), *strides)
+
+    def pack(buf, nbytes):
+        return abi.DELTA_RULE_BACKWARD_STRUCT.pack(*sizes, do.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(),
+                                                   g.data_ptr(), beta.data_ptr(), ptr(s0), ptr(ds), dq.data_ptr(),
+                                                   dk.data_ptr(), dv.data_ptr(), dg.data_ptr(), dbeta.data_ptr(),
+                                                   ds0.data_ptr(), buf, nbytes, *strides)
+
+    lib = abi.lib()
+    need = lib.helix_delta_rule_backward_scratch_size(packed(pack, 0, 0))
+    buf = scratch(index, st, stream, need)
+    run(lib.helix_delta_rule_backward_encode, index, st, pack(ptr(buf), need))
+    return dq, dk, dv, dg, dbeta, ds0

@@ -336,6 +336,43 @@ typedef struct {
 size_t       helix_delta_rule_scratch_size(const helix_delta_rule_args* args);
 helix_status helix_delta_rule_encode(helix_ctx* ctx, void* stream, const helix_delta_rule_args* args);
 
+/* Gradients, from d_o (of every o) and d_s (of s). The states are formed again.
+ * dq and dk of a head that value heads share are the sums over them, in fp32 and in
+ * the heads' order. Of a non-finite input the gradients of its heads (of its column,
+ * for v and d_o: also dq, dk, dg and dbeta of the head) are not finite either. */
+typedef struct {
+    int32_t      n_seq, n_tok;       /* n_seq or n_head 0: nothing is done;
+                                        n_tok 0: ds0 = d_s                    */
+    int32_t      n_qk_head, n_head;
+    int32_t      n_key, n_val;
+    int32_t      io_dtype;           /* of d_o, q, k, v, dq, dk and dv        */
+    float        scale;
+    const void*  d_o;                /* (n_seq, n_tok, n_head, n_val)         */
+    const void*  q;
+    const void*  k;
+    const void*  v;
+    const float* g;
+    const float* beta;
+    const float* s0;                 /* NULL: zero                            */
+    const float* d_s;                /* dense (n_seq, n_head, n_key, n_val);
+                                        NULL: zero                            */
+    void*        dq;                 /* the outputs are dense                 */
+    void*        dk;
+    void*        dv;
+    float*       dg;
+    float*       dbeta;
+    float*       ds0;                /* may be d_s                            */
+    void*        scratch;            /* helix_delta_rule_backward_scratch_size()
+                                        bytes, 16-byte aligned                */
+    uint64_t     scratch_bytes;
+    int64_t      seq_do, tok_do, head_do, seq_q, tok_q, head_q, seq_k, tok_k, head_k, seq_v, tok_v, head_v;
+    int64_t      seq_g, tok_g, seq_beta, tok_beta;
+} helix_delta_rule_backward_args;
+
+/* From the sizes; the other fields are not read. */
+size_t       helix_delta_rule_backward_scratch_size(const helix_delta_rule_backward_args* args);
+helix_status helix_delta_rule_backward_encode(helix_ctx* ctx, void* stream, const helix_delta_rule_backward_args* args);
+
 #ifdef __cplusplus
 }
 #endif
