@@ -15,6 +15,8 @@
 namespace {
 
 constexpr int DR_C = HELIX_DR_CHUNK;
+// Elements between the keys' rows in LDS: sixteen rows' 16 bytes, and the four rows of transposed reads, on banks of their own.
+template <int NK> constexpr int dr_pitch = NK + 24;
 
 template <typename T> constexpr int dr_planes = __is_same(T, float) ? 3 : __is_same(T, _Float16) ? 2 : 1;
 // Parts of operands that meet outputs of the storage type alone: two (2^-18) where that has 16 bits.
@@ -29,6 +31,22 @@ HELIX_DEV f32x4 dr_mfma(const bf16x8 (&a)[NA], const bf16x8 (&b)[NB], f32x4 acc)
         for (int i = sum; i >= 0; --i)
             if (i < NA && sum - i < NB) acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[i], b[sum - i], acc, 0, 0, 0);
     return acc;
+}
+
+// The same into a sum of its own for each i + j: three chains, so that none of the products waits for the one before it.
+struct DrAcc {
+    f32x4 s[3];
+    __device__ __forceinline__ DrAcc() { s[0] = s[1] = s[2] = f32x4{0.0f, 0.0f, 0.0f, 0.0f}; }
+    __device__ __forceinline__ f32x4 sum() const { return (s[2] + s[1]) + s[0]; }
+};
+template <int NA, int NB, int MAX = 3>
+HELIX_DEV void dr_mfma(const bf16x8 (&a)[NA], const bf16x8 (&b)[NB], DrAcc& acc) {
+#pragma unroll
+    for (int i = 0; i < NA; ++i)
+#pragma unroll
+        for (int sum = MAX - 1; sum >= 0; --sum)
+            if (sum - i >= 0 && sum - i < NB)
+                acc.s[sum] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[i], b[sum - i], acc.s[sum], 0, 0, 0);
 }
 
 template <int NPL>
@@ -69,30 +87,30 @@ HELIX_DEV void dr_operand(const Raw8<T>& v, int n, bf16x8 (&o)[dr_planes<T>]) {
     }
 }
 
-// The rows of a chunk's tokens of one head: `len` of them of `width` elements, `tok` elements apart.
-template <typename T>
+// The rows of a chunk's tokens of one head: `len` of them of `width` elements, `tok` elements apart. ODD: of 16 bits and an
+// odd width, whose last element is half of a word that a wide load finds out of the resource's range.
+template <typename T, bool ODD = false>
 struct Rows {
     helix_rsrc r;
     int tok, len, width;
-    bool whole;   // rows end at whole words
     __device__ Rows(const void* base, long long at, long long tok_, int len_, int width_) : tok((int)tok_), len(len_), width(width_) {
-        whole = sizeof(T) == 4 || !(width & 1);
         r = make_rsrc_u(static_cast<const T*>(base) + at, len > 0 ? (unsigned)(((len - 1) * tok_ + width) * (long long)sizeof(T)) : 0u);
     }
     // Eight elements from (row, col) on; what lies outside is unspecified past the row's end and 0 past the tokens.
     __device__ __forceinline__ Raw8<T> load8(int row, int col) const {
         const int off = row < len && col < width ? (row * tok + col) * (int)sizeof(T) : (int)0x80000000;
-        if (whole) return buf_load8<T>(r, off);
-        Raw8<T> o;
-        if constexpr (sizeof(T) == 2) {
+        if constexpr (!ODD || sizeof(T) == 4) {
+            return buf_load8<T>(r, off);
+        } else {
+            Raw8<T> o;
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const unsigned a = (unsigned short)__builtin_amdgcn_raw_buffer_load_b16(r, col + 2 * e < width ? off + 4 * e : (int)0x80000000, 0, 0);
                 const unsigned b = (unsigned short)__builtin_amdgcn_raw_buffer_load_b16(r, col + 2 * e + 1 < width ? off + 4 * e + 2 : (int)0x80000000, 0, 0);
                 o.w[0][e] = a | b << 16;
             }
+            return o;
         }
-        return o;
     }
     __device__ __forceinline__ unsigned raw(int row, int col) const {
         const int off = row < len && col < width ? (row * tok + col) * (int)sizeof(T) : (int)0x80000000;
@@ -134,6 +152,13 @@ HELIX_DEV void dr_get8_t(const __bf16* from, int pitch, int stride, int c, bf16x
         const u32x2 a = lds_read_tr16(at + k * stride), b = lds_read_tr16(at + k * stride + 4 * pitch);
         o[k] = __builtin_bit_cast(bf16x8, u32x4{a[0], a[1], b[0], b[1]});
     }
+}
+
+// A barrier that the waves of a workgroup may meet in different places of the program (as many times each).
+HELIX_DEV void dr_barrier() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup");
 }
 
 HELIX_DEV f32x4 zero4() { return f32x4{0.0f, 0.0f, 0.0f, 0.0f}; }

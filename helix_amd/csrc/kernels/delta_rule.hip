@@ -142,7 +142,7 @@ constexpr int DR_LD = DR_C + 4;   // fp32 rows of a chunk's square matrices in L
 // substitution, a column a lane; then block column w of the inverse, from the diagonal down:
 //     T_iw = -T_ii (sum over j of A_ij T_jw),  w <= j < i
 // on fp32 matrix instructions, T_jw staying in the registers it was formed in. BWD: T' and P' with X, without P.
-template <typename T, int NK, bool BWD>
+template <typename T, int NK, bool ODD, bool BWD>
 __device__ void delta_prep(const HelixDeltaParams& p) {
     constexpr int NPL = dr_planes<T>, NO = dr_out_planes<T>, KP = NK + 8;
     __shared__ __bf16 sK[NPL][DR_C][KP];
@@ -157,8 +157,8 @@ __device__ void delta_prep(const HelixDeltaParams& p) {
     const int seq = (int)(sh / (unsigned)p.n_head), h = (int)(sh % (unsigned)p.n_head), hk = h / p.share;
     const long long t0 = (long long)(p.chunk0 + ch) * DR_C;
     const int len = (int)min((long long)DR_C, p.n_tok - t0);
-    const Rows<T> rk(p.k, seq * p.seq_k + hk * p.head_k + t0 * p.tok_k, p.tok_k, len, p.n_key);
-    const Rows<T> rq(p.q, seq * p.seq_q + hk * p.head_q + t0 * p.tok_q, p.tok_q, len, p.n_key);
+    const Rows<T, ODD> rk(p.k, seq * p.seq_k + hk * p.head_k + t0 * p.tok_k, p.tok_k, len, p.n_key);
+    const Rows<T, ODD> rq(p.q, seq * p.seq_q + hk * p.head_q + t0 * p.tok_q, p.tok_q, len, p.n_key);
     // K's parts into LDS; the wave's rows of Q in registers.
     constexpr int PER = DR_C * (NK / 8) / 256;
     Raw8<T> kr[PER], qr[NK / 32];
@@ -299,33 +299,145 @@ __device__ void delta_prep(const HelixDeltaParams& p) {
 
 // ---- the walk -----------------------------------------------------------------------------
 //
-// Sixteen columns of a state, four waves. Wave w forms rows 16 w .. of K S and Q S, of
-// R = V - e^G K S and of D = X R, and keeps the rows NK / 4 w .. of S in registers. S, R, D and
-// e^(G_63 - G) D go from wave to wave through LDS, in bf16 parts and with the index that the
-// next product sums over running inside a row. A chunk is three barriers; everything that does
-// not depend on the state (K's rows, the fragments of X and P, the wave's rows of Q and V) is
-// loaded a chunk ahead.
-// KEEP: no outputs; the states before the chunks and D are stored (fp32) for the backward pass.
-template <typename T, int NK, bool KEEP>
+// Sixteen columns of a state, and two kinds of waves. The first four carry the state: wave w
+// forms rows 16 w .. of K S, of R = V - e^G K S and of D = X R, and keeps the rows NK / 4 w ..
+// of S in registers. The other four do what nothing waits for: they bring K's rows into LDS
+// and form the outputs, a phase behind. S, R, D and e^(G_63 - G) D go from wave to wave
+// through LDS, in bf16 parts and with the index that the next product sums over running inside
+// a row. A chunk is three barriers; what does not depend on the state is loaded as soon as the
+// chunk before has used its registers. K is read in the first phase alone (K' as operands of
+// the third is kept in registers), so that its next rows can take its place.
+// What bounds it is the chain of a chunk, with the latencies of LDS and of three products that
+// wait for one another.
+// KEEP: no outputs and no waves for them; the states before the chunks and D are stored (fp32)
+// for the backward pass.
+template <typename T, int NK, bool ODD, bool KEEP>
 __device__ void delta_walk(const HelixDeltaParams& p) {
-    constexpr int NPL = dr_planes<T>, NO = dr_out_planes<T>, KP = NK + 8, TP = DR_C + 8, NT = NK / 64, KS = NK / 32;
-    __shared__ __bf16 sK[2][NPL][DR_C][KP];
-    __shared__ __bf16 sS[3][16][KP];
-    __shared__ __bf16 sR[3][16][TP], sU[3][16][TP], sD[KEEP ? 1 : NO][KEEP ? 1 : 16][TP];
-    const int tid = threadIdx.x, lane = lane_id(), w = wave_uniform(), c = lane & 15, q = lane >> 4;
+    constexpr int NPL = dr_planes<T>, NO = dr_out_planes<T>, KP = dr_pitch<NK>, TP = DR_C + 8, NT = NK / 64, KS = NK / 32;
+    __shared__ __attribute__((aligned(16))) __bf16 sK[NPL][DR_C][KP];
+    __shared__ __attribute__((aligned(16))) __bf16 sS[3][16][KP];
+    __shared__ __attribute__((aligned(16))) __bf16 sR[3][16][TP], sU[3][16][TP], sD[KEEP ? 1 : NO][KEEP ? 1 : 16][TP];
+    const int tid = threadIdx.x & 255, lane = lane_id(), w = wave_uniform() & 3, c = lane & 15, q = lane >> 4;
     const unsigned id = xcd_logical_id(blockIdx.x, gridDim.x);   // a head's slices share an XCD's cache
     const int slice = (int)(id % (unsigned)p.n_slice);
     const unsigned sh = id / (unsigned)p.n_slice;
     const int seq = (int)(sh / (unsigned)p.n_head), h = (int)(sh % (unsigned)p.n_head), hk = h / p.share;
     const int p0 = 16 * slice, P = p.n_val, N = p.n_key;
     const unsigned state_bytes = (unsigned)N * (unsigned)P * 4u;
-    const int row0 = 16 * w + 4 * q;
+    const int row0 = 16 * w + 4 * q, last = p.n_chunk - 1;
+    auto first = [&](int ch) { return (long long)(p.chunk0 + ch) * DR_C; };
+    auto tokens = [&](int ch) { return (int)min((long long)DR_C, p.n_tok - first(ch)); };
+    const float* const decay = p.decay + (long long)sh * p.n_chunk * (HELIX_DR_DECAY / 4);
+    // K's rows, by 256 threads: loaded, and laid out in LDS.
+    constexpr int PER = DR_C * (NK / 8) / 256;
+    Raw8<T> kr[PER];
+    auto load_k = [&](int ch) {
+        ch = min(ch, last);
+        const Rows<T, ODD> rk(p.k, seq * p.seq_k + hk * p.head_k + first(ch) * p.tok_k, p.tok_k, tokens(ch), N);
+#pragma unroll
+        for (int i = 0; i < PER; ++i) kr[i] = rk.load8((tid + 256 * i) / (NK / 8), 8 * ((tid + 256 * i) % (NK / 8)));
+    };
+    auto put_k = [&] {
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            const int row = (tid + 256 * i) / (NK / 8), col = 8 * ((tid + 256 * i) % (NK / 8));
+            bf16x8 o[NPL];
+            dr_operand<T>(kr[i], N - col, o);
+#pragma unroll
+            for (int k = 0; k < NPL; ++k) *reinterpret_cast<bf16x8*>(&sK[k][row][col]) = o[k];
+        }
+    };
+
+    if (!KEEP && wave_uniform() >= 4) {
+        Raw8<T> qr[KS];
+        bf16x8 pf[2][NO];
+        f32x4 start;
+        auto load_q = [&](int ch) {
+            ch = min(ch, last);
+            const Rows<T, ODD> rq(p.q, seq * p.seq_q + hk * p.head_q + first(ch) * p.tok_q, p.tok_q, tokens(ch), N);
+#pragma unroll
+            for (int s = 0; s < KS; ++s) qr[s] = rq.load8(16 * w + c, 32 * s + 8 * q);
+            start = *reinterpret_cast<const f32x4*>(decay + ch * (HELIX_DR_DECAY / 4) + row0);
+        };
+        auto load_p = [&](int ch) {
+            const char* pp = p.p + ((long long)sh * p.n_chunk + min(ch, last)) * (6 * NO * HELIX_DR_FRAG) + 16 * lane;
+#pragma unroll
+            for (int ks = 0; ks < 2; ++ks) {
+                if (ks && w < 2) break;
+#pragma unroll
+                for (int k = 0; k < NO; ++k) pf[ks][k] = *reinterpret_cast<const bf16x8*>(pp + (dr_low(w, ks) * NO + k) * HELIX_DR_FRAG);
+            }
+        };
+        load_k(0);
+        load_q(0);
+        load_p(0);
+        put_k();
+        load_k(1);
+        for (int ch = 0; ch <= last; ++ch) {
+            dr_barrier();   // K and S are there
+            DrAcc qs;
+#pragma unroll
+            for (int s = 0; s < KS; ++s) {
+                const int col = 32 * s + 8 * q;
+                bf16x8 a[NPL], b[NO];
+                dr_operand<T>(qr[s], N - col, a);
+                dr_get8<NO>(&sS[0][c][col], 16 * KP, b);
+                dr_mfma<NPL, NO, NO>(a, b, qs);
+            }
+            f32x4 o = qs.sum() * (p.scale * start);
+            load_q(ch + 1);
+            dr_barrier();   // R is there; K has been read
+            put_k();
+            load_k(ch + 2);
+            dr_barrier();   // D is there
+#pragma unroll
+            for (int ks = 0; ks < 2; ++ks) {
+                if (ks && w < 2) break;
+                bf16x8 b[NO];
+                dr_get8<NO>(&sD[0][c][32 * ks + 8 * q], 16 * TP, b);
+                o = dr_mfma<NO, NO, NO>(pf[ks], b, o);
+            }
+            load_p(ch + 1);
+            const Rows<T> ro(p.o, seq * p.seq_o + h * p.head_o + first(ch) * p.tok_o, p.tok_o, tokens(ch), P);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) ro.store(row0 + r, p0 + c, o[r]);
+        }
+        return;
+    }
+
     // Register r of tile i: S[n = NT 16 w + 16 i + 4 q + r][p0 + c].
     auto state_off = [&](int i, int r) {
         const int n = NT * 16 * w + 16 * i + 4 * q + r;
         return n < N && p0 + c < P ? (n * P + p0 + c) * 4 : (int)0x80000000;
     };
-    f32x4 S[NT];
+    f32x4 S[NT], start, left;
+    bf16x8 xf[2][3];
+    unsigned vr[4];
+    float all;
+    auto load_v = [&](int ch) {
+        ch = min(ch, last);
+        const Rows<T> rv(p.v, seq * p.seq_v + h * p.head_v + first(ch) * p.tok_v, p.tok_v, tokens(ch), P);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) vr[r] = rv.raw(row0 + r, p0 + c);
+        start = *reinterpret_cast<const f32x4*>(decay + ch * (HELIX_DR_DECAY / 4) + row0);
+    };
+    auto load_x = [&](int ch) {
+        ch = min(ch, last);
+        const char* x = p.x + ((long long)sh * p.n_chunk + ch) * (6 * 3 * HELIX_DR_FRAG) + 16 * lane;
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks) {
+            if (ks && w < 2) break;
+#pragma unroll
+            for (int k = 0; k < 3; ++k) xf[ks][k] = *reinterpret_cast<const bf16x8*>(x + (dr_low(w, ks) * 3 + k) * HELIX_DR_FRAG);
+        }
+        left = *reinterpret_cast<const f32x4*>(decay + ch * (HELIX_DR_DECAY / 4) + 64 + row0);
+    };
+    auto load_all = [&](int ch) { all = decay[min(ch, last) * (HELIX_DR_DECAY / 4) + 63]; };
+    auto put_s = [&] {
+#pragma unroll
+        for (int i = 0; i < NT; ++i)
+            dr_put4<3>(&sS[0][c][NT * 16 * w + 16 * i + 4 * q], 16 * KP, S[i][0], S[i][1], S[i][2], S[i][3]);
+    };
     {
         const helix_rsrc r0 = make_rsrc_u(p.s0 + (long long)sh * N * P, p.s0 ? state_bytes : 0u);   // none: reads 0
 #pragma unroll
@@ -333,147 +445,79 @@ __device__ void delta_walk(const HelixDeltaParams& p) {
 #pragma unroll
             for (int r = 0; r < 4; ++r) S[i][r] = buf_f32(r0, state_off(i, r), 0);
     }
-    constexpr int PER = DR_C * (NK / 8) / 256;
-    struct Ahead {
-        Raw8<T> k[PER], q[KEEP ? 1 : KS];
-        bf16x8 x[2][3], p[KEEP ? 1 : 2][KEEP ? 1 : NO];
-        unsigned v[4];
-        f32x4 start, left;
-        float all;
-    } next;
-    auto load = [&](int ch) {
-        const long long t0 = (long long)(p.chunk0 + ch) * DR_C;
-        const int len = (int)min((long long)DR_C, p.n_tok - t0);
-        const Rows<T> rk(p.k, seq * p.seq_k + hk * p.head_k + t0 * p.tok_k, p.tok_k, len, N);
-        const Rows<T> rv(p.v, seq * p.seq_v + h * p.head_v + t0 * p.tok_v, p.tok_v, len, P);
-#pragma unroll
-        for (int i = 0; i < PER; ++i) next.k[i] = rk.load8((tid + 256 * i) / (NK / 8), 8 * ((tid + 256 * i) % (NK / 8)));
-        const long long at = (long long)sh * p.n_chunk + ch;
-        const char* x = p.x + at * (6 * 3 * HELIX_DR_FRAG) + 16 * lane;
-#pragma unroll
-        for (int ks = 0; ks < 2; ++ks) {
-            if (ks && w < 2) break;
-#pragma unroll
-            for (int k = 0; k < 3; ++k) next.x[ks][k] = *reinterpret_cast<const bf16x8*>(x + (dr_low(w, ks) * 3 + k) * HELIX_DR_FRAG);
-        }
-        if constexpr (!KEEP) {
-            const Rows<T> rq(p.q, seq * p.seq_q + hk * p.head_q + t0 * p.tok_q, p.tok_q, len, N);
-#pragma unroll
-            for (int s = 0; s < KS; ++s) next.q[s] = rq.load8(16 * w + c, 32 * s + 8 * q);
-            const char* pp = p.p + at * (6 * NO * HELIX_DR_FRAG) + 16 * lane;
-#pragma unroll
-            for (int ks = 0; ks < 2; ++ks) {
-                if (ks && w < 2) break;
-#pragma unroll
-                for (int k = 0; k < NO; ++k) next.p[ks][k] = *reinterpret_cast<const bf16x8*>(pp + (dr_low(w, ks) * NO + k) * HELIX_DR_FRAG);
-            }
-        }
-#pragma unroll
-        for (int r = 0; r < 4; ++r) next.v[r] = rv.raw(row0 + r, p0 + c);
-        const float* dec = p.decay + at * (HELIX_DR_DECAY / 4);
-        next.start = *reinterpret_cast<const f32x4*>(dec + row0);
-        next.left = *reinterpret_cast<const f32x4*>(dec + 64 + row0);
-        next.all = dec[63];
-    };
-    auto put_k = [&](int buf) {
-#pragma unroll
-        for (int i = 0; i < PER; ++i) {
-            const int row = (tid + 256 * i) / (NK / 8), col = 8 * ((tid + 256 * i) % (NK / 8));
-            bf16x8 o[NPL];
-            dr_operand<T>(next.k[i], N - col, o);
-#pragma unroll
-            for (int k = 0; k < NPL; ++k) *reinterpret_cast<bf16x8*>(&sK[buf][k][row][col]) = o[k];
-        }
-    };
-    auto put_s = [&] {
-#pragma unroll
-        for (int i = 0; i < NT; ++i)
-            dr_put4<3>(&sS[0][c][NT * 16 * w + 16 * i + 4 * q], 16 * KP, S[i][0], S[i][1], S[i][2], S[i][3]);
-    };
-    load(0);
-    put_k(0);
+    if constexpr (KEEP) load_k(0);
+    load_v(0);
+    load_x(0);
+    load_all(0);
+    if constexpr (KEEP) {
+        put_k();
+        load_k(1);
+    }
     put_s();
-    for (int ch = 0; ch < p.n_chunk; ++ch) {
-        const int buf = ch & 1;
-        const Ahead now = next;
-        if (ch + 1 < p.n_chunk) load(ch + 1);
-        const long long at = (long long)sh * p.n_chunk + ch;
-        const long long t0 = (long long)(p.chunk0 + ch) * DR_C;
-        const int len = (int)min((long long)DR_C, p.n_tok - t0);
-        __syncthreads();
+    for (int ch = 0; ch <= last; ++ch) {
+        dr_barrier();   // K and S are there
         if constexpr (KEEP) {
-            const helix_rsrc rs = make_rsrc_u(p.keep_s + at * N * P, state_bytes);
+            const helix_rsrc rs = make_rsrc_u(p.keep_s + ((long long)sh * p.n_chunk + ch) * N * P, state_bytes);
 #pragma unroll
             for (int i = 0; i < NT; ++i)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) __builtin_amdgcn_raw_buffer_store_b32(as_u32(S[i][r]), rs, state_off(i, r), 0, 0);
         }
-        f32x4 ks_ = zero4(), qs = zero4();
+        DrAcc ks_;
 #pragma unroll
         for (int s = 0; s < KS; ++s) {
             const int col = 32 * s + 8 * q;
             bf16x8 a[NPL], b[3];
-            dr_get8<NPL>(&sK[buf][0][16 * w + c][col], DR_C * KP, a);
+            dr_get8<NPL>(&sK[0][16 * w + c][col], DR_C * KP, a);
             dr_get8<3>(&sS[0][c][col], 16 * KP, b);
-            ks_ = dr_mfma<NPL, 3>(a, b, ks_);
-            if constexpr (!KEEP) {
-                bf16x8 aq[NPL];
-                dr_operand<T>(now.q[s], N - col, aq);
-                qs = dr_mfma<NPL, 3, NO>(aq, b, qs);
-            }
+            dr_mfma<NPL, 3>(a, b, ks_);
         }
-        f32x4 R;
+        bf16x8 kt[2][NT][NPL];
 #pragma unroll
-        for (int r = 0; r < 4; ++r) R[r] = raw_f32<T>(now.v[r]) - now.start[r] * ks_[r];
+        for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+            for (int i = 0; i < NT; ++i) dr_get8_t<NPL>(&sK[0][32 * ks + 8 * q][NT * 16 * w + 16 * i], KP, DR_C * KP, c, kt[ks][i]);
+        f32x4 R = ks_.sum();
+#pragma unroll
+        for (int r = 0; r < 4; ++r) R[r] = raw_f32<T>(vr[r]) - start[r] * R[r];
         dr_put4<3>(&sR[0][c][row0], 16 * TP, R[0], R[1], R[2], R[3]);
-        __syncthreads();
-        f32x4 D = zero4();
+        load_v(ch + 1);
+        dr_barrier();   // R is there; K has been read
+        if constexpr (KEEP) {
+            put_k();
+            load_k(ch + 2);
+        }
+        DrAcc ds;
 #pragma unroll
         for (int ks = 0; ks < 2; ++ks) {
             if (ks && w < 2) break;
             bf16x8 b[3];
             dr_get8<3>(&sR[0][c][32 * ks + 8 * q], 16 * TP, b);
-            D = dr_mfma<3, 3>(now.x[ks], b, D);
+            dr_mfma<3, 3>(xf[ks], b, ds);
         }
-        dr_put4<3>(&sU[0][c][row0], 16 * TP, D[0] * now.left[0], D[1] * now.left[1], D[2] * now.left[2], D[3] * now.left[3]);
+        const f32x4 D = ds.sum();
+        dr_put4<3>(&sU[0][c][row0], 16 * TP, D[0] * left[0], D[1] * left[1], D[2] * left[2], D[3] * left[3]);
+        load_x(ch + 1);
         if constexpr (KEEP) {
-            const Rows<float> rd(p.keep_d, at * DR_C * P, P, DR_C, P);
+            const Rows<float> rd(p.keep_d, ((long long)sh * p.n_chunk + ch) * DR_C * P, P, DR_C, P);
 #pragma unroll
             for (int r = 0; r < 4; ++r) rd.store(row0 + r, p0 + c, D[r]);
         } else {
             dr_put4<NO>(&sD[0][c][row0], 16 * TP, D[0], D[1], D[2], D[3]);
         }
-        __syncthreads();
-        if constexpr (!KEEP) {
-            f32x4 o;
-#pragma unroll
-            for (int r = 0; r < 4; ++r) o[r] = p.scale * now.start[r] * qs[r];
-#pragma unroll
-            for (int ks = 0; ks < 2; ++ks) {
-                if (ks && w < 2) break;
-                bf16x8 b[NO];
-                dr_get8<NO>(&sD[0][c][32 * ks + 8 * q], 16 * TP, b);
-                o = dr_mfma<NO, NO, NO>(now.p[ks], b, o);
-            }
-            const Rows<T> ro(p.o, seq * p.seq_o + h * p.head_o + t0 * p.tok_o, p.tok_o, len, P);
-#pragma unroll
-            for (int r = 0; r < 4; ++r) ro.store(row0 + r, p0 + c, o[r]);
-        }
-#pragma unroll
-        for (int i = 0; i < NT; ++i) S[i] *= now.all;
+        dr_barrier();   // D is there
+        DrAcc up[NT];
 #pragma unroll
         for (int ks = 0; ks < 2; ++ks) {
             bf16x8 b[3];
             dr_get8<3>(&sU[0][c][32 * ks + 8 * q], 16 * TP, b);
 #pragma unroll
-            for (int i = 0; i < NT; ++i) {
-                bf16x8 a[NPL];
-                dr_get8_t<NPL>(&sK[buf][0][32 * ks + 8 * q][NT * 16 * w + 16 * i], KP, DR_C * KP, c, a);
-                S[i] = dr_mfma<NPL, 3>(a, b, S[i]);
-            }
+            for (int i = 0; i < NT; ++i) dr_mfma<NPL, 3>(kt[ks][i], b, up[i]);
         }
+#pragma unroll
+        for (int i = 0; i < NT; ++i) S[i] = all * S[i] + up[i].sum();
+        load_all(ch + 1);
         put_s();
-        if (ch + 1 < p.n_chunk) put_k(buf ^ 1);
     }
     if (p.s) {
         const helix_rsrc r1 = make_rsrc_u(p.s + (long long)sh * N * P, state_bytes);
@@ -492,7 +536,7 @@ __device__ void delta_walk(const HelixDeltaParams& p) {
 //     dS = e^(G_63) E + scale (e^G Q)' dO - (e^G K)' dV
 // from the last chunk to the first: helix_delta_back_*, spread and laid out as the walk, dO
 // and e^G dO in V's place. It leaves E and Z for helix_delta_grad_*.
-template <typename T, int NK>
+template <typename T, int NK, bool ODD>
 __device__ void delta_back(const HelixDeltaParams& p) {
     constexpr int NPL = dr_planes<T>, KP = NK + 8, TP = DR_C + 8, NT = NK / 64, KS = NK / 32;
     __shared__ __bf16 sK[NPL][DR_C][KP], sQ[NPL][DR_C][KP];
@@ -535,8 +579,8 @@ __device__ void delta_back(const HelixDeltaParams& p) {
     auto load = [&](int ch) {
         const long long t0 = (long long)(p.chunk0 + ch) * DR_C;
         const int len = (int)min((long long)DR_C, p.n_tok - t0);
-        const Rows<T> rk(p.k, seq * p.seq_k + hk * p.head_k + t0 * p.tok_k, p.tok_k, len, N);
-        const Rows<T> rq(p.q, seq * p.seq_q + hk * p.head_q + t0 * p.tok_q, p.tok_q, len, N);
+        const Rows<T, ODD> rk(p.k, seq * p.seq_k + hk * p.head_k + t0 * p.tok_k, p.tok_k, len, N);
+        const Rows<T, ODD> rq(p.q, seq * p.seq_q + hk * p.head_q + t0 * p.tok_q, p.tok_q, len, N);
         const Rows<T> ro(p.d_o, seq * p.seq_o + h * p.head_o + t0 * p.tok_o, p.tok_o, len, P);
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
@@ -669,7 +713,7 @@ __device__ void delta_back(const HelixDeltaParams& p) {
 // A wave has 16 of the keys' columns (U, B, L, dQ, dK for all tokens; its rows of S and E
 // straight from memory) and blocks of the triangles. Operands that waves share are in LDS, by
 // parts: dO, Z and D 64 columns at a time; K and Q before and after.
-template <typename T, int NK>
+template <typename T, int NK, bool ODD>
 __device__ void delta_grad(const HelixDeltaParams& p) {
     constexpr int NPL = dr_planes<T>, NO = dr_out_planes<T>, KP = NK + 8, TP = DR_C + 8, W = NK / 16, TH = 64 * W;
     constexpr int TILES = (10 + W - 1) / W, ROWS = DR_C * 8 / TH;
@@ -695,8 +739,8 @@ __device__ void delta_grad(const HelixDeltaParams& p) {
     const long long t0 = (long long)(p.chunk0 + ch) * DR_C;
     const int len = (int)min((long long)DR_C, p.n_tok - t0), P = p.n_val, N = p.n_key;
     const int n0 = 16 * w;
-    const Rows<T> rk(p.k, seq * p.seq_k + hk * p.head_k + t0 * p.tok_k, p.tok_k, len, N);
-    const Rows<T> rq(p.q, seq * p.seq_q + hk * p.head_q + t0 * p.tok_q, p.tok_q, len, N);
+    const Rows<T, ODD> rk(p.k, seq * p.seq_k + hk * p.head_k + t0 * p.tok_k, p.tok_k, len, N);
+    const Rows<T, ODD> rq(p.q, seq * p.seq_q + hk * p.head_q + t0 * p.tok_q, p.tok_q, len, N);
     auto stage_kq = [&] {
 #pragma unroll
         for (int i = 0; i < DR_C * (NK / 8) / TH; ++i) {
@@ -754,8 +798,8 @@ __device__ void delta_grad(const HelixDeltaParams& p) {
     for (int hs = 0; hs < p.share; ++hs) {
         const int h = hk * p.share + hs;
         const long long at = ((long long)seq * p.n_head + h) * p.n_chunk + ch;
-        const Rows<T> ro(p.d_o, seq * p.seq_o + h * p.head_o + t0 * p.tok_o, p.tok_o, len, P);
-        const Rows<T> rv(p.v, seq * p.seq_v + h * p.head_v + t0 * p.tok_v, p.tok_v, len, P);
+        const Rows<T, ODD> ro(p.d_o, seq * p.seq_o + h * p.head_o + t0 * p.tok_o, p.tok_o, len, P);
+        const Rows<T, ODD> rv(p.v, seq * p.seq_v + h * p.head_v + t0 * p.tok_v, p.tok_v, len, P);
         const Rows<float> rz(p.keep_z, at * DR_C * P, P, DR_C, P), rd(p.keep_d, at * DR_C * P, P, DR_C, P);
         const Rows<float> rs(p.keep_s, at * N * P, P, N, P), re(p.keep_e, at * N * P, P, N, P);
         f32x4 U[4], B[4], L[4], dP[TILES], dA[TILES];
@@ -976,31 +1020,29 @@ __device__ void delta_grad(const HelixDeltaParams& p) {
 
 }  // namespace
 
-#define DR_KERNELS(TAG, T, NK)                                                                                              \
-    extern "C" __global__ __launch_bounds__(256) void helix_delta_steps_##TAG##_##NK(HelixDeltaParams p) {                  \
-        delta_steps<T, NK / 16>(p);                                                                                         \
-    }                                                                                                                       \
-    extern "C" __global__ __launch_bounds__(256) void helix_delta_prep_##TAG##_##NK(HelixDeltaParams p) {                   \
-        delta_prep<T, NK, false>(p);                                                                                        \
-    }                                                                                                                       \
-    extern "C" __global__ __launch_bounds__(256) void helix_delta_walk_##TAG##_##NK(HelixDeltaParams p) {                   \
-        delta_walk<T, NK, false>(p);                                                                                        \
-    }                                                                                                                       \
-    extern "C" __global__ __launch_bounds__(256) void helix_delta_prep_bwd_##TAG##_##NK(HelixDeltaParams p) {               \
-        delta_prep<T, NK, true>(p);                                                                                         \
-    }                                                                                                                       \
-    extern "C" __global__ __launch_bounds__(256) void helix_delta_keep_##TAG##_##NK(HelixDeltaParams p) {                   \
-        delta_walk<T, NK, true>(p);                                                                                         \
-    }                                                                                                                       \
-    extern "C" __global__ __launch_bounds__(256) void helix_delta_back_##TAG##_##NK(HelixDeltaParams p) {                   \
-        delta_back<T, NK>(p);                                                                                               \
-    }                                                                                                                       \
-    extern "C" __global__ __launch_bounds__(4 * NK) void helix_delta_grad_##TAG##_##NK(HelixDeltaParams p) {                \
-        delta_grad<T, NK>(p);                                                                                               \
-    }
-DR_KERNELS(f32, float, 64)
-DR_KERNELS(f32, float, 128)
-DR_KERNELS(f16, _Float16, 64)
-DR_KERNELS(f16, _Float16, 128)
-DR_KERNELS(bf16, __bf16, 64)
-DR_KERNELS(bf16, __bf16, 128)
+#define DR_STEPS(TAG, T, NK)                                                                                                             \
+    extern "C" __global__ __launch_bounds__(256) void helix_delta_steps_##TAG##_##NK(HelixDeltaParams p) { delta_steps<T, NK / 16>(p); }
+// _s: rows of an odd width.
+#define DR_KERNELS(TAG, T, NK, SUF, ODD)                                                                                                              \
+    extern "C" __global__ __launch_bounds__(256) void helix_delta_prep_##TAG##_##NK##SUF(HelixDeltaParams p) { delta_prep<T, NK, ODD, false>(p); }    \
+    extern "C" __global__ __launch_bounds__(512) void helix_delta_walk_##TAG##_##NK##SUF(HelixDeltaParams p) { delta_walk<T, NK, ODD, false>(p); }    \
+    extern "C" __global__ __launch_bounds__(256) void helix_delta_prep_bwd_##TAG##_##NK##SUF(HelixDeltaParams p) { delta_prep<T, NK, ODD, true>(p); } \
+    extern "C" __global__ __launch_bounds__(256) void helix_delta_keep_##TAG##_##NK##SUF(HelixDeltaParams p) { delta_walk<T, NK, ODD, true>(p); }     \
+    extern "C" __global__ __launch_bounds__(256) void helix_delta_back_##TAG##_##NK##SUF(HelixDeltaParams p) { delta_back<T, NK, ODD>(p); }           \
+    extern "C" __global__ __launch_bounds__(4 * NK) void helix_delta_grad_##TAG##_##NK##SUF(HelixDeltaParams p) { delta_grad<T, NK, ODD>(p); }
+DR_STEPS(f32, float, 64)
+DR_KERNELS(f32, float, 64, , false)
+DR_STEPS(f32, float, 128)
+DR_KERNELS(f32, float, 128, , false)
+DR_STEPS(f16, _Float16, 64)
+DR_KERNELS(f16, _Float16, 64, , false)
+DR_KERNELS(f16, _Float16, 64, _s, true)
+DR_STEPS(f16, _Float16, 128)
+DR_KERNELS(f16, _Float16, 128, , false)
+DR_KERNELS(f16, _Float16, 128, _s, true)
+DR_STEPS(bf16, __bf16, 64)
+DR_KERNELS(bf16, __bf16, 64, , false)
+DR_KERNELS(bf16, __bf16, 64, _s, true)
+DR_STEPS(bf16, __bf16, 128)
+DR_KERNELS(bf16, __bf16, 128, , false)
+DR_KERNELS(bf16, __bf16, 128, _s, true)

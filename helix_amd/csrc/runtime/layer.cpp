@@ -884,6 +884,12 @@ bool delta_shape(const A& a) {
 }
 
 int delta_keys(int n_key) { return n_key <= 64 ? 64 : 128; }   // of the kernels
+// Type and keys of a kernel; "_s": for rows of 16 bits and an odd width (the steps go element by element anyway).
+template <typename A>
+std::string delta_form(const A& a, bool steps = false) {
+    const bool odd = !steps && a.io_dtype != HELIX_F32 && ((a.n_key | a.n_val) & 1);
+    return std::string(kTags[a.io_dtype]) + "_" + std::to_string(delta_keys(a.n_key)) + (odd ? "_s" : "");
+}
 
 // How the rule is cut: segments of `chunks` chunks of every sequence, whose operands scratch holds at a time.
 struct DeltaPlan {
@@ -972,7 +978,7 @@ extern "C" helix_status helix_delta_rule_encode(helix_ctx* ctx, void* stream, co
         p.seq_o = a->seq_o;
         p.tok_o = a->tok_o;
         p.head_o = a->head_o;
-        const std::string form = std::string(kTags[a->io_dtype]) + "_" + std::to_string(delta_keys(a->n_key));
+        const std::string form = delta_form(*a, !plan.bytes);
         const long long sh = (long long)a->n_seq * a->n_head;
         if (!plan.bytes) {
             const hipFunction_t f = kernel(ctx, "helix_delta_steps_" + form);
@@ -982,7 +988,7 @@ extern "C" helix_status helix_delta_rule_encode(helix_ctx* ctx, void* stream, co
             return;
         }
         const hipFunction_t prep = kernel(ctx, "helix_delta_prep_" + form), walk = kernel(ctx, "helix_delta_walk_" + form);
-        const unsigned gp = grid(sh * plan.chunks, kDeltaThreads), gw = grid(sh * plan.n_slice, kDeltaThreads);
+        const unsigned gp = grid(sh * plan.chunks, kDeltaThreads), gw = grid(sh * plan.n_slice, 2 * kDeltaThreads);
         char* sc = static_cast<char*>(a->scratch);
         p.x = sc + plan.x_at;
         p.p = sc + plan.p_at;
@@ -992,7 +998,7 @@ extern "C" helix_status helix_delta_rule_encode(helix_ctx* ctx, void* stream, co
         for (p.chunk0 = 0; p.chunk0 < plan.n_chunk; p.chunk0 += plan.chunks) {
             p.n_chunk = std::min(plan.chunks, plan.n_chunk - p.chunk0);
             launch(prep, stream, p.n_chunk == plan.chunks ? gp : (unsigned)(sh * p.n_chunk), 1, kDeltaThreads, p);
-            launch(walk, stream, gw, 1, kDeltaThreads, p);
+            launch(walk, stream, gw, 1, 2 * kDeltaThreads, p);
             p.s0 = p.s;   // the next segment starts where this one ends
         }
     });
@@ -1082,7 +1088,7 @@ extern "C" helix_status helix_delta_rule_backward_encode(helix_ctx* ctx, void* s
         p.keep_z = reinterpret_cast<float*>(sc + plan.z_at);
         p.n_slice = (int)ceil_div(a->n_val, HELIX_DR_SLICE);
         const int keys = delta_keys(a->n_key);
-        const std::string form = std::string(kTags[a->io_dtype]) + "_" + std::to_string(keys);
+        const std::string form = delta_form(*a);
         const hipFunction_t prep = kernel(ctx, "helix_delta_prep_bwd_" + form), keep = kernel(ctx, "helix_delta_keep_" + form),
                             back = kernel(ctx, "helix_delta_back_" + form), grad = kernel(ctx, "helix_delta_grad_" + form);
         const long long sh = (long long)a->n_seq * a->n_head, sk = (long long)a->n_seq * a->n_qk_head;
@@ -1134,8 +1140,12 @@ const std::vector<std::string>& layer_kernel_names() {
                 if (n[0] <= '2') v.push_back(std::string("helix_norm_bwd_") + tag + "_w" + n);
             }
         for (const char* tag : kTags)
-            for (const char* n : {"_64", "_128"})
-                for (const char* k : {"steps_", "prep_", "walk_", "prep_bwd_", "keep_", "back_", "grad_"}) v.push_back(std::string("helix_delta_") + k + tag + n);
+            for (const char* n : {"_64", "_128"}) {
+                v.push_back(std::string("helix_delta_steps_") + tag + n);
+                for (const char* k : {"prep_", "walk_", "prep_bwd_", "keep_", "back_", "grad_"})
+                    for (const char* s : {"", "_s"})
+                        if (!*s || tag != kTags[HELIX_F32]) v.push_back(std::string("helix_delta_") + k + tag + n + s);
+            }
         v.push_back("helix_group_norm_dw");
         for (const char* tag : kTags) {
             v.push_back(std::string("helix_group_norm_fp8_") + tag + "_any");
