@@ -15,8 +15,15 @@
 namespace {
 
 constexpr int DR_C = HELIX_DR_CHUNK;
-// Elements between the keys' rows in LDS: sixteen rows' 16 bytes, and the four rows of transposed reads, on banks of their own.
-template <int NK> constexpr int dr_pitch = NK + 24;
+
+// Rows of W = 64 or 128 elements in LDS, without padding: the place of a row's chunk of eight (16 bytes), turned by its row so
+// that the sixteen rows' chunks which lanes read together, in whichever groups the hardware takes them, are on banks of
+// their own.
+template <int W>
+HELIX_DEV int dr_at(int row, int chunk) {
+    static_assert(W == 64 || W == 128, "rows of 64 or 128");
+    return row * W + 8 * (W == 128 ? chunk ^ (row & 15) : chunk ^ (row >> 1 & 7));
+}
 
 template <typename T> constexpr int dr_planes = __is_same(T, float) ? 3 : __is_same(T, _Float16) ? 2 : 1;
 // Parts of operands that meet outputs of the storage type alone: two (2^-18) where that has 16 bits.
@@ -39,6 +46,9 @@ struct DrAcc {
     __device__ __forceinline__ DrAcc() { s[0] = s[1] = s[2] = f32x4{0.0f, 0.0f, 0.0f, 0.0f}; }
     __device__ __forceinline__ f32x4 sum() const { return (s[2] + s[1]) + s[0]; }
 };
+// Of products with NPL parts on both sides; one part's have one sum.
+template <int NPL>
+HELIX_DEV f32x4 dr_sum(const DrAcc& a) { return NPL == 1 ? a.s[0] : a.sum(); }
 template <int NA, int NB, int MAX = 3>
 HELIX_DEV void dr_mfma(const bf16x8 (&a)[NA], const bf16x8 (&b)[NB], DrAcc& acc) {
 #pragma unroll
@@ -128,28 +138,40 @@ HELIX_DEV float raw_f32(unsigned w) {
     else return io_f32<T>((unsigned short)w);
 }
 
-// Four values of a result's registers (rows 4 q .. 4 q + 3 of a column) as parts in LDS, the rows side by side: to[k * stride + 0..3].
-template <int NPL>
-HELIX_DEV void dr_put4(__bf16* to, int stride, float a, float b, float c, float d) {
+// Four values of a result's registers (rows i .. i + 3, i a multiple of 4, of a column) as parts, side by side in row `row`
+// of planes of ROWS rows of W.
+template <int NPL, int W, int ROWS>
+HELIX_DEV void dr_put4(__bf16* planes, int row, int i, float a, float b, float c, float d) {
     unsigned lo[NPL], hi[NPL];
     dr_split2<NPL>(a, b, lo);
     dr_split2<NPL>(c, d, hi);
+    __bf16* to = planes + dr_at<W>(row, i >> 3) + (i & 4);
 #pragma unroll
-    for (int k = 0; k < NPL; ++k) *reinterpret_cast<u32x2*>(to + k * stride) = u32x2{lo[k], hi[k]};
+    for (int k = 0; k < NPL; ++k) *reinterpret_cast<u32x2*>(to + k * ROWS * W) = u32x2{lo[k], hi[k]};
 }
-template <int NPL>
-HELIX_DEV void dr_get8(const __bf16* from, int stride, bf16x8 (&o)[NPL]) {
+// An operand's eight elements: columns col .. col + 7 (a multiple of 8) of row `row`.
+template <int NPL, int W, int ROWS>
+HELIX_DEV void dr_get8(const __bf16* planes, int row, int col, bf16x8 (&o)[NPL]) {
+    const __bf16* from = planes + dr_at<W>(row, col >> 3);
 #pragma unroll
-    for (int k = 0; k < NPL; ++k) o[k] = *reinterpret_cast<const bf16x8*>(from + k * stride);
+    for (int k = 0; k < NPL; ++k) o[k] = *reinterpret_cast<const bf16x8*>(from + k * ROWS * W);
 }
-// Rows t .. t + 7 of column c0 + c, from parts stored by rows of `pitch` elements, by transposed reads: the operand of a
-// product that sums over the rows. `from` is row t, column c0; all sixteen lanes of a group name the same t.
-template <int NPL>
-HELIX_DEV void dr_get8_t(const __bf16* from, int pitch, int stride, int c, bf16x8 (&o)[NPL]) {
-    const __bf16* at = from + (c >> 2) * pitch + 4 * (c & 3);
+template <int NPL, int W, int ROWS>
+HELIX_DEV void dr_put8(__bf16* planes, int row, int col, const bf16x8 (&v)[NPL]) {
+    __bf16* to = planes + dr_at<W>(row, col >> 3);
+#pragma unroll
+    for (int k = 0; k < NPL; ++k) *reinterpret_cast<bf16x8*>(to + k * ROWS * W) = v[k];
+}
+// Rows row .. row + 7 of column col + c, by transposed reads: the operand of a product that sums over the rows. All sixteen
+// lanes of a group name the same row (a multiple of 8) and col (of 16).
+template <int NPL, int W, int ROWS>
+HELIX_DEV void dr_get8_t(const __bf16* planes, int row, int col, int c, bf16x8 (&o)[NPL]) {
+    const int r = row + (c >> 2), at = col + 4 * (c & 3);
+    const __bf16* p0 = planes + dr_at<W>(r, at >> 3) + (at & 4);
+    const __bf16* p1 = planes + dr_at<W>(r + 4, at >> 3) + (at & 4);
 #pragma unroll
     for (int k = 0; k < NPL; ++k) {
-        const u32x2 a = lds_read_tr16(at + k * stride), b = lds_read_tr16(at + k * stride + 4 * pitch);
+        const u32x2 a = lds_read_tr16(p0 + k * ROWS * W), b = lds_read_tr16(p1 + k * ROWS * W);
         o[k] = __builtin_bit_cast(bf16x8, u32x4{a[0], a[1], b[0], b[1]});
     }
 }

@@ -141,17 +141,23 @@ constexpr int DR_LD = DR_C + 4;   // fp32 rows of a chunk's square matrices in L
 // A workgroup a chunk of a head. Wave w: rows 16 w .. of K K' and Q K'; the inverse of A's diagonal block w by forward
 // substitution, a column a lane; then block column w of the inverse, from the diagonal down:
 //     T_iw = -T_ii (sum over j of A_ij T_jw),  w <= j < i
-// on fp32 matrix instructions, T_jw staying in the registers it was formed in. BWD: T' and P' with X, without P.
+// on fp32 matrix instructions, T_jw staying in the registers it was formed in. (Products of powers of A would be fewer steps,
+// but keys that repeat make the powers large, and they cancel.) BWD: T' and P' with X, without P.
+// Four workgroups a CU hide one another's chains: P takes the place of K's parts in LDS, T that of A.
 template <typename T, int NK, bool ODD, bool BWD>
 __device__ void delta_prep(const HelixDeltaParams& p) {
-    constexpr int NPL = dr_planes<T>, NO = dr_out_planes<T>, KP = NK + 8;
-    __shared__ __bf16 sK[NPL][DR_C][KP];
-    __shared__ float sA[DR_C][DR_LD], sT[DR_C][DR_LD], sP[DR_C][DR_LD];
-    __shared__ float sD[4][16][20];
+    constexpr int NPL = dr_planes<T>, NO = dr_out_planes<T>;
+    constexpr int kK = NPL * DR_C * NK * 2, kP = DR_C * DR_LD * 4;
+    __shared__ __attribute__((aligned(16))) char sKP[kK > kP ? kK : kP];
+    __shared__ __attribute__((aligned(16))) float sA[DR_C][DR_LD];
+    __shared__ __attribute__((aligned(16))) float sD[4][16][20];
     __shared__ double sG[DR_C];
-    __shared__ float sB[DR_C];
-    const int tid = threadIdx.x, lane = lane_id(), w = wave_uniform(), c = lane & 15, q = lane >> 4;
+    __shared__ __attribute__((aligned(16))) float sB[DR_C];
+    __bf16* const sK = reinterpret_cast<__bf16*>(sKP);
+    float (*const sP)[DR_LD] = reinterpret_cast<float (*)[DR_LD]>(sKP);
     const unsigned id = blockIdx.x;
+    // (Wave w has w + 1 blocks of the products: turned from workgroup to workgroup, every SIMD gets each.)
+    const int tid = threadIdx.x, lane = lane_id(), w = (wave_uniform() + (int)id) & 3, c = lane & 15, q = lane >> 4;
     const int ch = (int)(id % (unsigned)p.n_chunk);
     const unsigned sh = id / (unsigned)p.n_chunk;
     const int seq = (int)(sh / (unsigned)p.n_head), h = (int)(sh % (unsigned)p.n_head), hk = h / p.share;
@@ -166,12 +172,12 @@ __device__ void delta_prep(const HelixDeltaParams& p) {
     for (int i = 0; i < PER; ++i) kr[i] = rk.load8((tid + 256 * i) / (NK / 8), 8 * ((tid + 256 * i) % (NK / 8)));
 #pragma unroll
     for (int s = 0; s < NK / 32; ++s) qr[s] = rq.load8(16 * w + c, 32 * s + 8 * q);
-    const float gl = lane < len ? p.g[seq * p.seq_g + (t0 + lane) * p.tok_g + h] : 0.0f;
-    const float bl = lane < len ? p.beta[seq * p.seq_b + (t0 + lane) * p.tok_b + h] : 0.0f;
-    const double G = dr_log_decay(gl);
-    const double end = __shfl(G, 63, 64);
     if (w == 0) {
-        sG[lane] = G;
+        const float gl = lane < len ? p.g[seq * p.seq_g + (t0 + lane) * p.tok_g + h] : 0.0f;
+        const float bl = lane < len ? p.beta[seq * p.seq_b + (t0 + lane) * p.tok_b + h] : 0.0f;
+        const double G = dr_log_decay(gl);
+        const double end = __shfl(G, 63, 64);
+        sG[lane] = G * 1.4426950408889634074;
         sB[lane] = bl;
         float* dec = p.decay + id * (HELIX_DR_DECAY / 4ll);
         dec[lane] = exp_diff(G, 0.0);
@@ -183,53 +189,71 @@ __device__ void delta_prep(const HelixDeltaParams& p) {
         const int row = (tid + 256 * i) / (NK / 8), col = 8 * ((tid + 256 * i) % (NK / 8));
         bf16x8 o[NPL];
         dr_operand<T>(kr[i], p.n_key - col, o);
-#pragma unroll
-        for (int k = 0; k < NPL; ++k) *reinterpret_cast<bf16x8*>(&sK[k][row][col]) = o[k];
+        dr_put8<NPL, NK, DR_C>(sK, row, col, o);
     }
     __syncthreads();
-    f32x4 kk[4], qk[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) kk[j] = qk[j] = zero4();
+    DrAcc kk[4], qk[4];
 #pragma unroll
     for (int s = 0; s < NK / 32; ++s) {
         const int col = 32 * s + 8 * q;
         bf16x8 ak[NPL], aq[NPL];
-        dr_get8<NPL>(&sK[0][16 * w + c][col], DR_C * KP, ak);
+        dr_get8<NPL, NK, DR_C>(sK, 16 * w + c, col, ak);
         dr_operand<T>(qr[s], p.n_key - col, aq);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            if (j > w) continue;
+            if (j > w) break;
             bf16x8 b[NPL];
-            dr_get8<NPL>(&sK[0][16 * j + c][col], DR_C * KP, b);
-            kk[j] = dr_mfma<NPL, NPL>(ak, b, kk[j]);
-            qk[j] = dr_mfma<NPL, NPL>(aq, b, qk[j]);
+            dr_get8<NPL, NK, DR_C>(sK, 16 * j + c, col, b);
+            dr_mfma<NPL, NPL>(ak, b, kk[j]);
+            dr_mfma<NPL, NPL>(aq, b, qk[j]);
         }
     }
-    // (Blocks above the diagonal that fragments reach are 0.)
+    f32x4 pv[4];
+    {
+        double Gi[4];
+        const f32x4 beta = *reinterpret_cast<const f32x4*>(&sB[16 * w + 4 * q]);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        const int jj = 16 * j + c;
-        const double Gj = sG[jj];
+        for (int r = 0; r < 4; ++r) Gi[r] = sG[16 * w + 4 * q + r];
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const int i = 16 * w + 4 * q + r;
-            const float e = j <= w && jj <= i ? exp_diff(sG[i], Gj) : 0.0f;
-            sA[i][jj] = jj < i && j <= w ? sB[i] * (e * kk[j][r]) : 0.0f;
-            sP[i][jj] = jj <= i && j <= w ? p.scale * (e * qk[j][r]) : 0.0f;
-            if (j > w) sT[i][jj] = 0.0f;
+        for (int j = 0; j < 4; ++j) {
+            if (j > w) break;
+            const double Gj = sG[16 * j + c];
+            const f32x4 k = dr_sum<NPL>(kk[j]), x = dr_sum<NPL>(qk[j]);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                float e = __builtin_amdgcn_exp2f((float)(Gi[r] - Gj));
+                float a = beta[r] * (e * k[r]);
+                if (j == w) {
+                    if (c > 4 * q + r) e = 0.0f;
+                    if (c >= 4 * q + r) a = 0.0f;
+                }
+                pv[j][r] = j == w && c > 4 * q + r ? 0.0f : p.scale * (e * x[r]);
+                sA[16 * w + 4 * q + r][16 * j + c] = a;
+            }
         }
     }
     __syncthreads();
-    // Diagonal block w: lane c its column c (the four groups alike).
+    // P by rows, 0 above the diagonal where fragments reach.
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        if (j > (w | 1)) break;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) sP[16 * w + 4 * q + r][16 * j + c] = j <= w ? pv[j][r] : 0.0f;
+    }
+    // Diagonal block w: lane c its column c (the four groups alike), four rows at a time.
     {
         float x[16];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            float s = i == c ? 1.0f : 0.0f;
+        for (int i = 0; i < 16; ++i) x[i] = i == c ? 1.0f : 0.0f;
 #pragma unroll
-            for (int j = 0; j < 16; ++j)
-                if (j < i) s = fmaf(-sA[16 * w + i][16 * w + j], x[j], s);
-            x[i] = s;
+        for (int jb = 0; jb < 16; jb += 4) {
+#pragma unroll
+            for (int i = jb + 1; i < 16; ++i) {
+                const f32x4 a = *reinterpret_cast<const f32x4*>(&sA[16 * w + i][16 * w + jb]);
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (jb + j < i) x[i] = fmaf(-a[j], x[jb + j], x[i]);
+            }
         }
         if (q == 0) {
 #pragma unroll
@@ -237,38 +261,38 @@ __device__ void delta_prep(const HelixDeltaParams& p) {
         }
     }
     __syncthreads();
-    {
-        f32x4 t[4];
+    f32x4 t[4];
 #pragma unroll
-        for (int r = 0; r < 4; ++r) t[0][r] = sD[w][4 * q + r][c];
-        auto put = [&](int i, const f32x4& v) {
+    for (int r = 0; r < 4; ++r) t[0][r] = sD[w][4 * q + r][c];
 #pragma unroll
-            for (int r = 0; r < 4; ++r) sT[16 * i + 4 * q + r][16 * w + c] = v[r];
-        };
-        put(w, t[0]);
+    for (int step = 1; step < 4; ++step) {
+        const int i = w + step;
+        if (i > 3) break;
+        f32x4 m = zero4();
 #pragma unroll
-        for (int step = 1; step < 4; ++step) {
-            const int i = w + step;
-            if (i > 3) break;
-            f32x4 m = zero4();
-#pragma unroll
-            for (int j = 0; j < step; ++j)
-                m = dr_mfma_f32(*reinterpret_cast<const f32x4*>(&sA[16 * i + c][16 * (w + j) + 4 * q]), t[j], m);
-            f32x4 a = *reinterpret_cast<const f32x4*>(&sD[i][c][4 * q]);
-            a = -a;
-            t[step] = dr_mfma_f32(a, m, zero4());
-            put(i, t[step]);
-        }
+        for (int j = 0; j < step; ++j)
+            m = dr_mfma_f32(*reinterpret_cast<const f32x4*>(&sA[16 * i + c][16 * (w + j) + 4 * q]), t[j], m);
+        const f32x4 a = *reinterpret_cast<const f32x4*>(&sD[i][c][4 * q]);
+        t[step] = dr_mfma_f32(-a, m, zero4());
     }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            // (t[i - w], by a choice of constants.)
+            const float v = i < w ? 0.0f : i == w ? t[0][r] : i == w + 1 ? t[1][r] : i == w + 2 ? t[2][r] : t[3][r];
+            sA[16 * i + 4 * q + r][16 * w + c] = v;
+        }
     __syncthreads();
     // Fragments: row 16 w + c, columns 32 ks + 8 q ..
     auto emit = [&](char* to, int frag, const float (&v)[8], auto parts) {
-        constexpr int N = decltype(parts)::value;
-        bf16x8 o[N];
-        dr_split8<N>(v, o);
+        constexpr int M = decltype(parts)::value;
+        bf16x8 o[M];
+        dr_split8<M>(v, o);
 #pragma unroll
-        for (int k = 0; k < N; ++k)
-            *reinterpret_cast<bf16x8*>(to + ((long long)id * 6 * N + frag * N + k) * HELIX_DR_FRAG + 16 * lane) = o[k];
+        for (int k = 0; k < M; ++k)
+            *reinterpret_cast<bf16x8*>(to + ((long long)id * 6 * M + frag * M + k) * HELIX_DR_FRAG + 16 * lane) = o[k];
     };
 #pragma unroll
     for (int ks = 0; ks < 2; ++ks) {
@@ -276,7 +300,7 @@ __device__ void delta_prep(const HelixDeltaParams& p) {
         const int row = 16 * w + c, col = 32 * ks + 8 * q;
         if (ks == 0 || w > 1) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = sT[row][col + e] * sB[col + e];
+            for (int e = 0; e < 8; ++e) v[e] = sA[row][col + e] * sB[col + e];
             emit(p.x, dr_low(w, ks), v, std::integral_constant<int, 3>{});
             if constexpr (!BWD) {
 #pragma unroll
@@ -287,7 +311,7 @@ __device__ void delta_prep(const HelixDeltaParams& p) {
         if constexpr (BWD) {
             if (ks == 1 || w < 2) {
 #pragma unroll
-                for (int e = 0; e < 8; ++e) v[e] = sT[col + e][row];
+                for (int e = 0; e < 8; ++e) v[e] = sA[col + e][row];
                 emit(p.tt, dr_up(w, ks), v, std::integral_constant<int, 3>{});
 #pragma unroll
                 for (int e = 0; e < 8; ++e) v[e] = sP[col + e][row];
@@ -313,10 +337,15 @@ __device__ void delta_prep(const HelixDeltaParams& p) {
 // for the backward pass.
 template <typename T, int NK, bool ODD, bool KEEP>
 __device__ void delta_walk(const HelixDeltaParams& p) {
-    constexpr int NPL = dr_planes<T>, NO = dr_out_planes<T>, KP = dr_pitch<NK>, TP = DR_C + 8, NT = NK / 64, KS = NK / 32;
-    __shared__ __attribute__((aligned(16))) __bf16 sK[NPL][DR_C][KP];
-    __shared__ __attribute__((aligned(16))) __bf16 sS[3][16][KP];
-    __shared__ __attribute__((aligned(16))) __bf16 sR[3][16][TP], sU[3][16][TP], sD[KEEP ? 1 : NO][KEEP ? 1 : 16][TP];
+    constexpr int NPL = dr_planes<T>, NO = dr_out_planes<T>, NT = NK / 64, KS = NK / 32;
+    constexpr int VP = 16 + 16 / sizeof(T);   // rows of V and of outputs in LDS
+    __shared__ __attribute__((aligned(16))) __bf16 sK[NPL * DR_C * NK];
+    __shared__ __attribute__((aligned(16))) __bf16 sS[3 * 16 * NK];
+    __shared__ __attribute__((aligned(16))) __bf16 sR[3 * 16 * DR_C], sU[3 * 16 * DR_C], sD[KEEP ? 8 : NO * 16 * DR_C];
+    __shared__ __attribute__((aligned(16))) T sV[DR_C][VP];
+    __shared__ __attribute__((aligned(16))) float sDec[2][HELIX_DR_DECAY / 4];
+    typedef typename std::conditional<KEEP, float, T>::type Out;   // D, or o
+    __shared__ __attribute__((aligned(16))) Out sOut[DR_C][16 + 16 / sizeof(Out)];
     const int tid = threadIdx.x & 255, lane = lane_id(), w = wave_uniform() & 3, c = lane & 15, q = lane >> 4;
     const unsigned id = xcd_logical_id(blockIdx.x, gridDim.x);   // a head's slices share an XCD's cache
     const int slice = (int)(id % (unsigned)p.n_slice);
@@ -325,42 +354,58 @@ __device__ void delta_walk(const HelixDeltaParams& p) {
     const int p0 = 16 * slice, P = p.n_val, N = p.n_key;
     const unsigned state_bytes = (unsigned)N * (unsigned)P * 4u;
     const int row0 = 16 * w + 4 * q, last = p.n_chunk - 1;
+    const long long base = (long long)sh * p.n_chunk;
     auto first = [&](int ch) { return (long long)(p.chunk0 + ch) * DR_C; };
     auto tokens = [&](int ch) { return (int)min((long long)DR_C, p.n_tok - first(ch)); };
-    const float* const decay = p.decay + (long long)sh * p.n_chunk * (HELIX_DR_DECAY / 4);
-    // K's rows, by 256 threads: loaded, and laid out in LDS.
-    constexpr int PER = DR_C * (NK / 8) / 256;
-    Raw8<T> kr[PER];
-    auto load_k = [&](int ch) {
-        ch = min(ch, last);
-        const Rows<T, ODD> rk(p.k, seq * p.seq_k + hk * p.head_k + first(ch) * p.tok_k, p.tok_k, tokens(ch), N);
-#pragma unroll
-        for (int i = 0; i < PER; ++i) kr[i] = rk.load8((tid + 256 * i) / (NK / 8), 8 * ((tid + 256 * i) % (NK / 8)));
-    };
-    auto put_k = [&] {
-#pragma unroll
-        for (int i = 0; i < PER; ++i) {
-            const int row = (tid + 256 * i) / (NK / 8), col = 8 * ((tid + 256 * i) % (NK / 8));
-            bf16x8 o[NPL];
-            dr_operand<T>(kr[i], N - col, o);
-#pragma unroll
-            for (int k = 0; k < NPL; ++k) *reinterpret_cast<bf16x8*>(&sK[k][row][col]) = o[k];
-        }
-    };
 
-    if (!KEEP && wave_uniform() >= 4) {
+    if (wave_uniform() >= 4) {
+        // K's rows, 16 columns of V's (two lanes a row) and the decays: loaded, and laid out in LDS.
+        constexpr int PER = DR_C * (NK / 8) / 256;
+        Raw8<T> kr[PER], vr;
+        f32x4 dec;
+        const int vrow = (tid >> 1) & 63, vcol = 8 * (tid & 1);
+        auto load_k = [&](int ch) {
+            ch = min(ch, last);
+            const Rows<T, ODD> rk(p.k, seq * p.seq_k + hk * p.head_k + first(ch) * p.tok_k, p.tok_k, tokens(ch), N);
+            const Rows<T, ODD> rv(p.v, seq * p.seq_v + h * p.head_v + first(ch) * p.tok_v, p.tok_v, tokens(ch), P);
+#pragma unroll
+            for (int i = 0; i < PER; ++i) kr[i] = rk.load8((tid + 256 * i) / (NK / 8), 8 * ((tid + 256 * i) % (NK / 8)));
+            if (tid < 128) vr = rv.load8(vrow, p0 + vcol);
+            else if (tid < 128 + HELIX_DR_DECAY / 16)
+                dec = *reinterpret_cast<const f32x4*>(p.decay + (base + ch) * (HELIX_DR_DECAY / 4) + 4 * (tid - 128));
+        };
+        auto put_k = [&](int ch) {
+#pragma unroll
+            for (int i = 0; i < PER; ++i) {
+                const int row = (tid + 256 * i) / (NK / 8), col = 8 * ((tid + 256 * i) % (NK / 8));
+                bf16x8 o[NPL];
+                dr_operand<T>(kr[i], N - col, o);
+                dr_put8<NPL, NK, DR_C>(sK, row, col, o);
+            }
+            if (tid < 128) *reinterpret_cast<Raw8<T>*>(&sV[vrow][vcol]) = vr;
+            else if (tid < 128 + HELIX_DR_DECAY / 16) *reinterpret_cast<f32x4*>(&sDec[ch & 1][4 * (tid - 128)]) = dec;
+        };
+        // What a chunk left in sOut, by the lanes that have V's places.
+        auto store_out = [&](int ch) {
+            if (tid >= 128) return;
+            const Raw8<Out> v = *reinterpret_cast<const Raw8<Out>*>(&sOut[vrow][vcol]);
+            if constexpr (KEEP) {
+                store8_at<float>(p.keep_d + ((base + ch) * DR_C + vrow) * P + p0 + vcol, v, P - p0 - vcol);
+            } else if (vrow < tokens(ch)) {
+                store8_at<T>(static_cast<T*>(p.o) + seq * p.seq_o + h * p.head_o + (first(ch) + vrow) * p.tok_o + p0 + vcol, v,
+                             P - p0 - vcol);
+            }
+        };
         Raw8<T> qr[KS];
         bf16x8 pf[2][NO];
-        f32x4 start;
         auto load_q = [&](int ch) {
             ch = min(ch, last);
             const Rows<T, ODD> rq(p.q, seq * p.seq_q + hk * p.head_q + first(ch) * p.tok_q, p.tok_q, tokens(ch), N);
 #pragma unroll
             for (int s = 0; s < KS; ++s) qr[s] = rq.load8(16 * w + c, 32 * s + 8 * q);
-            start = *reinterpret_cast<const f32x4*>(decay + ch * (HELIX_DR_DECAY / 4) + row0);
         };
         auto load_p = [&](int ch) {
-            const char* pp = p.p + ((long long)sh * p.n_chunk + min(ch, last)) * (6 * NO * HELIX_DR_FRAG) + 16 * lane;
+            const char* pp = p.p + (base + min(ch, last)) * (6 * NO * HELIX_DR_FRAG) + 16 * lane;
 #pragma unroll
             for (int ks = 0; ks < 2; ++ks) {
                 if (ks && w < 2) break;
@@ -369,39 +414,48 @@ __device__ void delta_walk(const HelixDeltaParams& p) {
             }
         };
         load_k(0);
-        load_q(0);
-        load_p(0);
-        put_k();
+        if constexpr (!KEEP) {
+            load_q(0);
+            load_p(0);
+        }
+        put_k(0);
         load_k(1);
         for (int ch = 0; ch <= last; ++ch) {
-            dr_barrier();   // K and S are there
-            DrAcc qs;
+            dr_barrier();   // K, V and S are there
+            f32x4 o;
+            if constexpr (!KEEP) {
+                DrAcc qs;
 #pragma unroll
-            for (int s = 0; s < KS; ++s) {
-                const int col = 32 * s + 8 * q;
-                bf16x8 a[NPL], b[NO];
-                dr_operand<T>(qr[s], N - col, a);
-                dr_get8<NO>(&sS[0][c][col], 16 * KP, b);
-                dr_mfma<NPL, NO, NO>(a, b, qs);
+                for (int s = 0; s < KS; ++s) {
+                    const int col = 32 * s + 8 * q;
+                    bf16x8 a[NPL], b[NO];
+                    dr_operand<T>(qr[s], N - col, a);
+                    dr_get8<NO, NK, 16>(sS, c, col, b);
+                    dr_mfma<NPL, NO, NO>(a, b, qs);
+                }
+                o = qs.sum() * (p.scale * *reinterpret_cast<const f32x4*>(&sDec[ch & 1][row0]));
+                load_q(ch + 1);
             }
-            f32x4 o = qs.sum() * (p.scale * start);
-            load_q(ch + 1);
-            dr_barrier();   // R is there; K has been read
-            put_k();
+            if (ch) store_out(ch - 1);
+            dr_barrier();   // R is there; K and V have been read
+            put_k(ch + 1);
             load_k(ch + 2);
             dr_barrier();   // D is there
+            if constexpr (!KEEP) {
 #pragma unroll
-            for (int ks = 0; ks < 2; ++ks) {
-                if (ks && w < 2) break;
-                bf16x8 b[NO];
-                dr_get8<NO>(&sD[0][c][32 * ks + 8 * q], 16 * TP, b);
-                o = dr_mfma<NO, NO, NO>(pf[ks], b, o);
+                for (int ks = 0; ks < 2; ++ks) {
+                    if (ks && w < 2) break;
+                    bf16x8 b[NO];
+                    dr_get8<NO, DR_C, 16>(sD, c, 32 * ks + 8 * q, b);
+                    o = dr_mfma<NO, NO, NO>(pf[ks], b, o);
+                }
+                load_p(ch + 1);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) sOut[row0 + r][c] = (T)o[r];
             }
-            load_p(ch + 1);
-            const Rows<T> ro(p.o, seq * p.seq_o + h * p.head_o + first(ch) * p.tok_o, p.tok_o, tokens(ch), P);
-#pragma unroll
-            for (int r = 0; r < 4; ++r) ro.store(row0 + r, p0 + c, o[r]);
         }
+        dr_barrier();   // the last outputs are there
+        if (last >= 0) store_out(last);
         return;
     }
 
@@ -410,33 +464,21 @@ __device__ void delta_walk(const HelixDeltaParams& p) {
         const int n = NT * 16 * w + 16 * i + 4 * q + r;
         return n < N && p0 + c < P ? (n * P + p0 + c) * 4 : (int)0x80000000;
     };
-    f32x4 S[NT], start, left;
+    f32x4 S[NT];
     bf16x8 xf[2][3];
-    unsigned vr[4];
-    float all;
-    auto load_v = [&](int ch) {
-        ch = min(ch, last);
-        const Rows<T> rv(p.v, seq * p.seq_v + h * p.head_v + first(ch) * p.tok_v, p.tok_v, tokens(ch), P);
-#pragma unroll
-        for (int r = 0; r < 4; ++r) vr[r] = rv.raw(row0 + r, p0 + c);
-        start = *reinterpret_cast<const f32x4*>(decay + ch * (HELIX_DR_DECAY / 4) + row0);
-    };
     auto load_x = [&](int ch) {
-        ch = min(ch, last);
-        const char* x = p.x + ((long long)sh * p.n_chunk + ch) * (6 * 3 * HELIX_DR_FRAG) + 16 * lane;
+        const char* x = p.x + (base + min(ch, last)) * (6 * 3 * HELIX_DR_FRAG) + 16 * lane;
 #pragma unroll
         for (int ks = 0; ks < 2; ++ks) {
             if (ks && w < 2) break;
 #pragma unroll
             for (int k = 0; k < 3; ++k) xf[ks][k] = *reinterpret_cast<const bf16x8*>(x + (dr_low(w, ks) * 3 + k) * HELIX_DR_FRAG);
         }
-        left = *reinterpret_cast<const f32x4*>(decay + ch * (HELIX_DR_DECAY / 4) + 64 + row0);
     };
-    auto load_all = [&](int ch) { all = decay[min(ch, last) * (HELIX_DR_DECAY / 4) + 63]; };
     auto put_s = [&] {
 #pragma unroll
         for (int i = 0; i < NT; ++i)
-            dr_put4<3>(&sS[0][c][NT * 16 * w + 16 * i + 4 * q], 16 * KP, S[i][0], S[i][1], S[i][2], S[i][3]);
+            dr_put4<3, NK, 16>(sS, c, NT * 16 * w + 16 * i + 4 * q, S[i][0], S[i][1], S[i][2], S[i][3]);
     };
     {
         const helix_rsrc r0 = make_rsrc_u(p.s0 + (long long)sh * N * P, p.s0 ? state_bytes : 0u);   // none: reads 0
@@ -445,80 +487,71 @@ __device__ void delta_walk(const HelixDeltaParams& p) {
 #pragma unroll
             for (int r = 0; r < 4; ++r) S[i][r] = buf_f32(r0, state_off(i, r), 0);
     }
-    if constexpr (KEEP) load_k(0);
-    load_v(0);
     load_x(0);
-    load_all(0);
-    if constexpr (KEEP) {
-        put_k();
-        load_k(1);
-    }
     put_s();
     for (int ch = 0; ch <= last; ++ch) {
-        dr_barrier();   // K and S are there
+        dr_barrier();   // K, V and S are there
         if constexpr (KEEP) {
-            const helix_rsrc rs = make_rsrc_u(p.keep_s + ((long long)sh * p.n_chunk + ch) * N * P, state_bytes);
+            const helix_rsrc rs = make_rsrc_u(p.keep_s + (base + ch) * N * P, state_bytes);
 #pragma unroll
             for (int i = 0; i < NT; ++i)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) __builtin_amdgcn_raw_buffer_store_b32(as_u32(S[i][r]), rs, state_off(i, r), 0, 0);
         }
+        const float* const dec = sDec[ch & 1];
         DrAcc ks_;
 #pragma unroll
         for (int s = 0; s < KS; ++s) {
             const int col = 32 * s + 8 * q;
             bf16x8 a[NPL], b[3];
-            dr_get8<NPL>(&sK[0][16 * w + c][col], DR_C * KP, a);
-            dr_get8<3>(&sS[0][c][col], 16 * KP, b);
+            dr_get8<NPL, NK, DR_C>(sK, 16 * w + c, col, a);
+            dr_get8<3, NK, 16>(sS, c, col, b);
             dr_mfma<NPL, 3>(a, b, ks_);
         }
         bf16x8 kt[2][NT][NPL];
 #pragma unroll
         for (int ks = 0; ks < 2; ++ks)
 #pragma unroll
-            for (int i = 0; i < NT; ++i) dr_get8_t<NPL>(&sK[0][32 * ks + 8 * q][NT * 16 * w + 16 * i], KP, DR_C * KP, c, kt[ks][i]);
+            for (int i = 0; i < NT; ++i) dr_get8_t<NPL, NK, DR_C>(sK, 32 * ks + 8 * q, NT * 16 * w + 16 * i, c, kt[ks][i]);
+        const f32x4 start = *reinterpret_cast<const f32x4*>(dec + row0);
         f32x4 R = ks_.sum();
 #pragma unroll
-        for (int r = 0; r < 4; ++r) R[r] = raw_f32<T>(vr[r]) - start[r] * R[r];
-        dr_put4<3>(&sR[0][c][row0], 16 * TP, R[0], R[1], R[2], R[3]);
-        load_v(ch + 1);
-        dr_barrier();   // R is there; K has been read
-        if constexpr (KEEP) {
-            put_k();
-            load_k(ch + 2);
-        }
+        for (int r = 0; r < 4; ++r) R[r] = (float)sV[row0 + r][c] - start[r] * R[r];
+        dr_put4<3, DR_C, 16>(sR, c, row0, R[0], R[1], R[2], R[3]);
+        dr_barrier();   // R is there; K and V have been read
         DrAcc ds;
 #pragma unroll
         for (int ks = 0; ks < 2; ++ks) {
             if (ks && w < 2) break;
             bf16x8 b[3];
-            dr_get8<3>(&sR[0][c][32 * ks + 8 * q], 16 * TP, b);
+            dr_get8<3, DR_C, 16>(sR, c, 32 * ks + 8 * q, b);
             dr_mfma<3, 3>(xf[ks], b, ds);
         }
+        const f32x4 left = *reinterpret_cast<const f32x4*>(dec + 64 + row0);
         const f32x4 D = ds.sum();
-        dr_put4<3>(&sU[0][c][row0], 16 * TP, D[0] * left[0], D[1] * left[1], D[2] * left[2], D[3] * left[3]);
-        load_x(ch + 1);
+        dr_put4<3, DR_C, 16>(sU, c, row0, D[0] * left[0], D[1] * left[1], D[2] * left[2], D[3] * left[3]);
         if constexpr (KEEP) {
-            const Rows<float> rd(p.keep_d, ((long long)sh * p.n_chunk + ch) * DR_C * P, P, DR_C, P);
 #pragma unroll
-            for (int r = 0; r < 4; ++r) rd.store(row0 + r, p0 + c, D[r]);
+            for (int r = 0; r < 4; ++r) sOut[row0 + r][c] = D[r];
         } else {
-            dr_put4<NO>(&sD[0][c][row0], 16 * TP, D[0], D[1], D[2], D[3]);
+            dr_put4<NO, DR_C, 16>(sD, c, row0, D[0], D[1], D[2], D[3]);
         }
+        load_x(ch + 1);
+        const float all = dec[63];
         dr_barrier();   // D is there
         DrAcc up[NT];
 #pragma unroll
         for (int ks = 0; ks < 2; ++ks) {
             bf16x8 b[3];
-            dr_get8<3>(&sU[0][c][32 * ks + 8 * q], 16 * TP, b);
+            dr_get8<3, DR_C, 16>(sU, c, 32 * ks + 8 * q, b);
 #pragma unroll
             for (int i = 0; i < NT; ++i) dr_mfma<NPL, 3>(kt[ks][i], b, up[i]);
         }
 #pragma unroll
         for (int i = 0; i < NT; ++i) S[i] = all * S[i] + up[i].sum();
-        load_all(ch + 1);
         put_s();
     }
+    dr_barrier();
     if (p.s) {
         const helix_rsrc r1 = make_rsrc_u(p.s + (long long)sh * N * P, state_bytes);
 #pragma unroll
@@ -538,10 +571,9 @@ __device__ void delta_walk(const HelixDeltaParams& p) {
 // and e^G dO in V's place. It leaves E and Z for helix_delta_grad_*.
 template <typename T, int NK, bool ODD>
 __device__ void delta_back(const HelixDeltaParams& p) {
-    constexpr int NPL = dr_planes<T>, KP = NK + 8, TP = DR_C + 8, NT = NK / 64, KS = NK / 32;
-    __shared__ __bf16 sK[NPL][DR_C][KP], sQ[NPL][DR_C][KP];
-    __shared__ __bf16 sE[3][16][KP];
-    __shared__ __bf16 sO[NPL][16][TP], sW[3][16][TP], sR[3][16][TP], sU[3][16][TP];
+    constexpr int NPL = dr_planes<T>, NT = NK / 64, KS = NK / 32;
+    __shared__ __attribute__((aligned(16))) __bf16 sK[NPL * DR_C * NK], sQ[NPL * DR_C * NK], sE[3 * 16 * NK];
+    __shared__ __attribute__((aligned(16))) __bf16 sO[NPL * 16 * DR_C], sW[3 * 16 * DR_C], sR[3 * 16 * DR_C], sU[3 * 16 * DR_C];
     const int tid = threadIdx.x, lane = lane_id(), w = wave_uniform(), c = lane & 15, q = lane >> 4;
     const unsigned id = xcd_logical_id(blockIdx.x, gridDim.x);
     const int slice = (int)(id % (unsigned)p.n_slice);
@@ -617,24 +649,21 @@ __device__ void delta_back(const HelixDeltaParams& p) {
             bf16x8 k[NPL], qq[NPL];
             dr_operand<T>(now.k[i], N - col, k);
             dr_operand<T>(now.q[i], N - col, qq);
-#pragma unroll
-            for (int j = 0; j < NPL; ++j) {
-                *reinterpret_cast<bf16x8*>(&sK[j][row][col]) = k[j];
-                *reinterpret_cast<bf16x8*>(&sQ[j][row][col]) = qq[j];
-            }
+            dr_put8<NPL, NK, DR_C>(sK, row, col, k);
+            dr_put8<NPL, NK, DR_C>(sQ, row, col, qq);
         }
         {
             float o[4];
 #pragma unroll
             for (int r = 0; r < 4; ++r) o[r] = raw_f32<T>(now.o[r]);
-            dr_put4<NPL>(&sO[0][c][row0], 16 * TP, o[0], o[1], o[2], o[3]);
+            dr_put4<NPL, DR_C, 16>(sO, c, row0, o[0], o[1], o[2], o[3]);
 #pragma unroll
             for (int r = 0; r < 4; ++r) o[r] *= p.scale * now.start[r];
-            dr_put4<3>(&sW[0][c][row0], 16 * TP, o[0], o[1], o[2], o[3]);
+            dr_put4<3, DR_C, 16>(sW, c, row0, o[0], o[1], o[2], o[3]);
         }
 #pragma unroll
         for (int i = 0; i < NT; ++i)
-            dr_put4<3>(&sE[0][c][NT * 16 * w + 16 * i + 4 * q], 16 * KP, E[i][0], E[i][1], E[i][2], E[i][3]);
+            dr_put4<3, NK, 16>(sE, c, NT * 16 * w + 16 * i + 4 * q, E[i][0], E[i][1], E[i][2], E[i][3]);
         if (ch) load(ch - 1);
         const long long at = (long long)sh * p.n_chunk + ch;
         const long long t0 = (long long)(p.chunk0 + ch) * DR_C;
@@ -646,8 +675,8 @@ __device__ void delta_back(const HelixDeltaParams& p) {
         for (int s = 0; s < KS; ++s) {
             const int col = 32 * s + 8 * q;
             bf16x8 a[NPL], b[3];
-            dr_get8<NPL>(&sK[0][16 * w + c][col], DR_C * KP, a);
-            dr_get8<3>(&sE[0][c][col], 16 * KP, b);
+            dr_get8<NPL, NK, DR_C>(sK, 16 * w + c, col, a);
+            dr_get8<3, NK, 16>(sE, c, col, b);
             ke = dr_mfma<NPL, 3>(a, b, ke);
         }
         f32x4 dd = ke * now.left;
@@ -655,22 +684,22 @@ __device__ void delta_back(const HelixDeltaParams& p) {
         for (int ks = 0; ks < 2; ++ks) {
             if (ks == 0 && w > 1) continue;
             bf16x8 b[NPL];
-            dr_get8<NPL>(&sO[0][c][32 * ks + 8 * q], 16 * TP, b);
+            dr_get8<NPL, DR_C, 16>(sO, c, 32 * ks + 8 * q, b);
             dd = dr_mfma<3, NPL>(now.p[ks], b, dd);
         }
-        dr_put4<3>(&sR[0][c][row0], 16 * TP, dd[0], dd[1], dd[2], dd[3]);
+        dr_put4<3, DR_C, 16>(sR, c, row0, dd[0], dd[1], dd[2], dd[3]);
         __syncthreads();
         f32x4 Z = zero4();
 #pragma unroll
         for (int ks = 0; ks < 2; ++ks) {
             if (ks == 0 && w > 1) continue;
             bf16x8 b[3];
-            dr_get8<3>(&sR[0][c][32 * ks + 8 * q], 16 * TP, b);
+            dr_get8<3, DR_C, 16>(sR, c, 32 * ks + 8 * q, b);
             Z = dr_mfma<3, 3>(now.t[ks], b, Z);
         }
         const f32x4 dv = Z * now.beta;
         const f32x4 u = -(dv * now.start);
-        dr_put4<3>(&sU[0][c][row0], 16 * TP, u[0], u[1], u[2], u[3]);
+        dr_put4<3, DR_C, 16>(sU, c, row0, u[0], u[1], u[2], u[3]);
         const Rows<float> rz(p.keep_z, at * DR_C * P, P, DR_C, P);
         const Rows<T> rv(p.dv, (((long long)seq * p.n_tok + t0) * p.n_head + h) * P, (long long)p.n_head * P, len, P);
 #pragma unroll
@@ -684,14 +713,14 @@ __device__ void delta_back(const HelixDeltaParams& p) {
 #pragma unroll
         for (int ks = 0; ks < 2; ++ks) {
             bf16x8 bw[3], bu[3];
-            dr_get8<3>(&sW[0][c][32 * ks + 8 * q], 16 * TP, bw);
-            dr_get8<3>(&sU[0][c][32 * ks + 8 * q], 16 * TP, bu);
+            dr_get8<3, DR_C, 16>(sW, c, 32 * ks + 8 * q, bw);
+            dr_get8<3, DR_C, 16>(sU, c, 32 * ks + 8 * q, bu);
 #pragma unroll
             for (int i = 0; i < NT; ++i) {
                 bf16x8 a[NPL];
-                dr_get8_t<NPL>(&sQ[0][32 * ks + 8 * q][NT * 16 * w + 16 * i], KP, DR_C * KP, c, a);
+                dr_get8_t<NPL, NK, DR_C>(sQ, 32 * ks + 8 * q, NT * 16 * w + 16 * i, c, a);
                 E[i] = dr_mfma<NPL, 3>(a, bw, E[i]);
-                dr_get8_t<NPL>(&sK[0][32 * ks + 8 * q][NT * 16 * w + 16 * i], KP, DR_C * KP, c, a);
+                dr_get8_t<NPL, NK, DR_C>(sK, 32 * ks + 8 * q, NT * 16 * w + 16 * i, c, a);
                 E[i] = dr_mfma<NPL, 3>(a, bu, E[i]);
             }
         }
@@ -715,22 +744,22 @@ __device__ void delta_back(const HelixDeltaParams& p) {
 // parts: dO, Z and D 64 columns at a time; K and Q before and after.
 template <typename T, int NK, bool ODD>
 __device__ void delta_grad(const HelixDeltaParams& p) {
-    constexpr int NPL = dr_planes<T>, NO = dr_out_planes<T>, KP = NK + 8, TP = DR_C + 8, W = NK / 16, TH = 64 * W;
+    constexpr int NPL = dr_planes<T>, NO = dr_out_planes<T>, W = NK / 16, TH = 64 * W;
     constexpr int TILES = (10 + W - 1) / W, ROWS = DR_C * 8 / TH;
-    constexpr int kKQ = 2 * NPL * DR_C * KP, kOZD = (NPL + 6) * DR_C * TP;
-    __shared__ __bf16 sBig[kKQ > kOZD ? kKQ : kOZD];
+    constexpr int kKQ = 2 * NPL * DR_C * NK, kOZD = (NPL + 6) * DR_C * DR_C;
+    __shared__ __attribute__((aligned(16))) __bf16 sBig[kKQ > kOZD ? kKQ : kOZD];
     struct Sums {   // of a head; the triangles' parts take their place at the end
         double G[DR_C];
         float row[4][DR_C], col[4][DR_C], beta[4][DR_C], dot[3][W][DR_C], zv[DR_C], se[W];
     };
-    __shared__ __attribute__((aligned(16))) __bf16 sM[2][NO][DR_C][TP];
+    __shared__ __attribute__((aligned(16))) __bf16 sM[2 * NO * DR_C * DR_C];
     static_assert(sizeof(Sums) <= sizeof(sM), "the sums fit in the triangles' place");
-    Sums& sums = *reinterpret_cast<Sums*>(&sM[0][0][0][0]);
+    Sums& sums = *reinterpret_cast<Sums*>(&sM[0]);
     __bf16* const sK = sBig;
-    __bf16* const sQ = sBig + NPL * DR_C * KP;
+    __bf16* const sQ = sBig + NPL * DR_C * NK;
     __bf16* const sO = sBig;
-    __bf16* const sZ = sBig + NPL * DR_C * TP;
-    __bf16* const sD = sZ + 3 * DR_C * TP;
+    __bf16* const sZ = sBig + NPL * DR_C * DR_C;
+    __bf16* const sD = sZ + 3 * DR_C * DR_C;
     const int tid = threadIdx.x, lane = lane_id(), w = wave_uniform(), c = lane & 15, q = lane >> 4;
     const unsigned id = blockIdx.x;
     const int ch = (int)(id % (unsigned)p.n_chunk);
@@ -749,11 +778,8 @@ __device__ void delta_grad(const HelixDeltaParams& p) {
             bf16x8 k[NPL], qq[NPL];
             dr_operand<T>(kr, N - col, k);
             dr_operand<T>(qr, N - col, qq);
-#pragma unroll
-            for (int j = 0; j < NPL; ++j) {
-                *reinterpret_cast<bf16x8*>(&sK[(j * DR_C + row) * KP + col]) = k[j];
-                *reinterpret_cast<bf16x8*>(&sQ[(j * DR_C + row) * KP + col]) = qq[j];
-            }
+            dr_put8<NPL, NK, DR_C>(sK, row, col, k);
+            dr_put8<NPL, NK, DR_C>(sQ, row, col, qq);
         }
     };
     // The wave's blocks (tb, jb) of the lower triangle: K K' and Q K'.
@@ -772,10 +798,10 @@ __device__ void delta_grad(const HelixDeltaParams& p) {
         for (int s = 0; s < NK / 32; ++s) {
             const int col = 32 * s + 8 * q;
             bf16x8 a[NPL], b[NPL];
-            dr_get8<NPL>(&sK[(16 * jb + c) * KP + col], DR_C * KP, b);
-            dr_get8<NPL>(&sK[(16 * tb + c) * KP + col], DR_C * KP, a);
+            dr_get8<NPL, NK, DR_C>(sK, 16 * jb + c, col, b);
+            dr_get8<NPL, NK, DR_C>(sK, 16 * tb + c, col, a);
             kk[k] = dr_mfma<NPL, NPL>(a, b, kk[k]);
-            dr_get8<NPL>(&sQ[(16 * tb + c) * KP + col], DR_C * KP, a);
+            dr_get8<NPL, NK, DR_C>(sQ, 16 * tb + c, col, a);
             qk[k] = dr_mfma<NPL, NPL>(a, b, qk[k]);
         }
     }
@@ -784,12 +810,12 @@ __device__ void delta_grad(const HelixDeltaParams& p) {
         dq[i] = dk[i] = zero4();
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-            const int at = (16 * i + 4 * q + r) * KP + n0 + c;
+            const int row = 16 * i + 4 * q + r, at = dr_at<NK>(row, (n0 + c) >> 3) + (c & 7);
             float a = 0.0f, b = 0.0f;
 #pragma unroll
             for (int j = NPL - 1; j >= 0; --j) {
-                a += (float)sK[j * DR_C * KP + at];
-                b += (float)sQ[j * DR_C * KP + at];
+                a += (float)sK[j * DR_C * NK + at];
+                b += (float)sQ[j * DR_C * NK + at];
             }
             kv[i][r] = a;
             qv[i][r] = b;
@@ -823,13 +849,9 @@ __device__ void delta_grad(const HelixDeltaParams& p) {
                 dr_operand<float>(dr, n, d);
 #pragma unroll
                 for (int e = 0; e < 8; ++e) zv[i] += e < n ? at8(zr, e) * at8(vr, e) : 0.0f;
-#pragma unroll
-                for (int j = 0; j < NPL; ++j) *reinterpret_cast<bf16x8*>(&sO[(j * DR_C + row) * TP + col]) = o[j];
-#pragma unroll
-                for (int j = 0; j < 3; ++j) {
-                    *reinterpret_cast<bf16x8*>(&sZ[(j * DR_C + row) * TP + col]) = z[j];
-                    *reinterpret_cast<bf16x8*>(&sD[(j * DR_C + row) * TP + col]) = d[j];
-                }
+                dr_put8<NPL, DR_C, DR_C>(sO, row, col, o);
+                dr_put8<3, DR_C, DR_C>(sZ, row, col, z);
+                dr_put8<3, DR_C, DR_C>(sD, row, col, d);
             }
             Raw8<float> sr[2], er[2];
 #pragma unroll
@@ -848,13 +870,12 @@ __device__ void delta_grad(const HelixDeltaParams& p) {
                 for (int e = 0; e < 8; ++e) se += e < n ? at8(sr[ks], e) * at8(er[ks], e) : 0.0f;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const int a_at = (16 * i + c) * TP + col;
                     bf16x8 ao[NPL], az[3], ad[3];
-                    dr_get8<NPL>(&sO[a_at], DR_C * TP, ao);
+                    dr_get8<NPL, DR_C, DR_C>(sO, 16 * i + c, col, ao);
                     U[i] = dr_mfma<NPL, 3>(ao, bs, U[i]);
-                    dr_get8<3>(&sZ[a_at], DR_C * TP, az);
+                    dr_get8<3, DR_C, DR_C>(sZ, 16 * i + c, col, az);
                     B[i] = dr_mfma<3, 3>(az, bs, B[i]);
-                    dr_get8<3>(&sD[a_at], DR_C * TP, ad);
+                    dr_get8<3, DR_C, DR_C>(sD, 16 * i + c, col, ad);
                     L[i] = dr_mfma<3, 3>(ad, be, L[i]);
                 }
 #pragma unroll
@@ -862,10 +883,10 @@ __device__ void delta_grad(const HelixDeltaParams& p) {
                     if (w + W * k > 9) continue;
                     const int tb = tb_of(k), jb = jb_of(k);
                     bf16x8 ao[NPL], az[3], bd[3];
-                    dr_get8<3>(&sD[(16 * jb + c) * TP + col], DR_C * TP, bd);
-                    dr_get8<NPL>(&sO[(16 * tb + c) * TP + col], DR_C * TP, ao);
+                    dr_get8<3, DR_C, DR_C>(sD, 16 * jb + c, col, bd);
+                    dr_get8<NPL, DR_C, DR_C>(sO, 16 * tb + c, col, ao);
                     dP[k] = dr_mfma<NPL, 3>(ao, bd, dP[k]);
-                    dr_get8<3>(&sZ[(16 * tb + c) * TP + col], DR_C * TP, az);
+                    dr_get8<3, DR_C, DR_C>(sZ, 16 * tb + c, col, az);
                     dA[k] = dr_mfma<3, 3>(az, bd, dA[k]);
                 }
             }
@@ -976,33 +997,33 @@ __device__ void delta_grad(const HelixDeltaParams& p) {
         if (w + W * k > 9) continue;
         const int tb = tb_of(k), jb = jb_of(k);
         // Stored by columns: M[j][i].
-        dr_put4<NO>(&sM[0][0][16 * jb + c][16 * tb + 4 * q], DR_C * TP, mp[k][0], mp[k][1], mp[k][2], mp[k][3]);
-        dr_put4<NO>(&sM[1][0][16 * jb + c][16 * tb + 4 * q], DR_C * TP, ma[k][0], ma[k][1], ma[k][2], ma[k][3]);
+        dr_put4<NO, DR_C, DR_C>(sM + 0 * NO * DR_C * DR_C, 16 * jb + c, 16 * tb + 4 * q, mp[k][0], mp[k][1], mp[k][2], mp[k][3]);
+        dr_put4<NO, DR_C, DR_C>(sM + 1 * NO * DR_C * DR_C, 16 * jb + c, 16 * tb + 4 * q, ma[k][0], ma[k][1], ma[k][2], ma[k][3]);
         if (tb != jb) {   // 0 above the diagonal
-            dr_put4<NO>(&sM[0][0][16 * tb + c][16 * jb + 4 * q], DR_C * TP, 0.0f, 0.0f, 0.0f, 0.0f);
-            dr_put4<NO>(&sM[1][0][16 * tb + c][16 * jb + 4 * q], DR_C * TP, 0.0f, 0.0f, 0.0f, 0.0f);
+            dr_put4<NO, DR_C, DR_C>(sM + 0 * NO * DR_C * DR_C, 16 * tb + c, 16 * jb + 4 * q, 0.0f, 0.0f, 0.0f, 0.0f);
+            dr_put4<NO, DR_C, DR_C>(sM + 1 * NO * DR_C * DR_C, 16 * tb + c, 16 * jb + 4 * q, 0.0f, 0.0f, 0.0f, 0.0f);
         }
     }
     __syncthreads();
 #pragma unroll
     for (int ks = 0; ks < 2; ++ks) {
         bf16x8 bk[NPL], bq[NPL];
-        dr_get8_t<NPL>(&sK[(32 * ks + 8 * q) * KP + n0], KP, DR_C * KP, c, bk);
-        dr_get8_t<NPL>(&sQ[(32 * ks + 8 * q) * KP + n0], KP, DR_C * KP, c, bq);
+        dr_get8_t<NPL, NK, DR_C>(sK, 32 * ks + 8 * q, n0, c, bk);
+        dr_get8_t<NPL, NK, DR_C>(sQ, 32 * ks + 8 * q, n0, c, bq);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             bf16x8 a[NO];
             // M[i][j] over j: columns of what is stored; M'[j][i] over i: its rows.
             if (2 * ks <= i) {
-                dr_get8_t<NO>(&sM[0][0][32 * ks + 8 * q][16 * i], TP, DR_C * TP, c, a);
+                dr_get8_t<NO, DR_C, DR_C>(sM + 0 * NO * DR_C * DR_C, 32 * ks + 8 * q, 16 * i, c, a);
                 dq[i] = dr_mfma<NO, NPL, NO>(a, bk, dq[i]);
-                dr_get8_t<NO>(&sM[1][0][32 * ks + 8 * q][16 * i], TP, DR_C * TP, c, a);
+                dr_get8_t<NO, DR_C, DR_C>(sM + 1 * NO * DR_C * DR_C, 32 * ks + 8 * q, 16 * i, c, a);
                 dk[i] = dr_mfma<NO, NPL, NO>(a, bk, dk[i]);
             }
             if (2 * ks + 1 >= i) {
-                dr_get8<NO>(&sM[0][0][16 * i + c][32 * ks + 8 * q], DR_C * TP, a);
+                dr_get8<NO, DR_C, DR_C>(sM + 0 * NO * DR_C * DR_C, 16 * i + c, 32 * ks + 8 * q, a);
                 dk[i] = dr_mfma<NO, NPL, NO>(a, bq, dk[i]);
-                dr_get8<NO>(&sM[1][0][16 * i + c][32 * ks + 8 * q], DR_C * TP, a);
+                dr_get8<NO, DR_C, DR_C>(sM + 1 * NO * DR_C * DR_C, 16 * i + c, 32 * ks + 8 * q, a);
                 dk[i] = dr_mfma<NO, NPL, NO>(a, bk, dk[i]);
             }
         }
@@ -1027,7 +1048,7 @@ __device__ void delta_grad(const HelixDeltaParams& p) {
     extern "C" __global__ __launch_bounds__(256) void helix_delta_prep_##TAG##_##NK##SUF(HelixDeltaParams p) { delta_prep<T, NK, ODD, false>(p); }    \
     extern "C" __global__ __launch_bounds__(512) void helix_delta_walk_##TAG##_##NK##SUF(HelixDeltaParams p) { delta_walk<T, NK, ODD, false>(p); }    \
     extern "C" __global__ __launch_bounds__(256) void helix_delta_prep_bwd_##TAG##_##NK##SUF(HelixDeltaParams p) { delta_prep<T, NK, ODD, true>(p); } \
-    extern "C" __global__ __launch_bounds__(256) void helix_delta_keep_##TAG##_##NK##SUF(HelixDeltaParams p) { delta_walk<T, NK, ODD, true>(p); }     \
+    extern "C" __global__ __launch_bounds__(512) void helix_delta_keep_##TAG##_##NK##SUF(HelixDeltaParams p) { delta_walk<T, NK, ODD, true>(p); }     \
     extern "C" __global__ __launch_bounds__(256) void helix_delta_back_##TAG##_##NK##SUF(HelixDeltaParams p) { delta_back<T, NK, ODD>(p); }           \
     extern "C" __global__ __launch_bounds__(4 * NK) void helix_delta_grad_##TAG##_##NK##SUF(HelixDeltaParams p) { delta_grad<T, NK, ODD>(p); }
 DR_STEPS(f32, float, 64)

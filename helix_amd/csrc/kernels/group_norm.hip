@@ -14,54 +14,15 @@ namespace {
 
 constexpr int GN_THREADS = 256;
 
-// Eight elements at p, at any alignment: the first n of them (all where n >= 8).
-template <typename T>
-HELIX_DEV Raw8<T> gn_load(const T* p, int n) {
-    Raw8<T> o;
-    if (n >= 8) {
-        __builtin_memcpy(&o, p, 8 * sizeof(T));
-        return o;
-    }
-#pragma unroll
-    for (int i = 0; i < (int)sizeof(T) / 2; ++i) o.w[i] = u32x4{0, 0, 0, 0};
-#pragma unroll
-    for (int i = 0; i < 7; ++i) {
-        if (i >= n) break;
-        if constexpr (sizeof(T) == 4) o.w[i >> 2][i & 3] = as_u32(p[i]);
-        else o.w[0][i >> 1] |= (unsigned)reinterpret_cast<const uint16_t*>(p)[i] << (16 * (i & 1));
-    }
-    return o;
-}
-template <typename T>
-HELIX_DEV void gn_store(T* p, const float (&v)[8], int n) {
-    T e[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) e[i] = (T)v[i];
-    if (n >= 8) {
-        __builtin_memcpy(p, e, 8 * sizeof(T));
-        return;
-    }
-    int at = 0;
-    if (n & 4) {
-        __builtin_memcpy(p, e, 4 * sizeof(T));
-        at = 4;
-    }
-    if (n & 2) {
-        const T two[2] = {at ? e[4] : e[0], at ? e[5] : e[1]};
-        __builtin_memcpy(p + at, two, 2 * sizeof(T));
-        at += 2;
-    }
-    if (n & 1) p[at] = at == 6 ? e[6] : at == 4 ? e[4] : at == 2 ? e[2] : e[0];
-}
 // Weights or biases of a vector in fp32.
 template <typename T>
 HELIX_DEV void gn_weights(const void* w, int w_f32, int c, int n, float (&o)[8]) {
     if (w_f32) {
-        const Raw8<float> v = gn_load<float>(static_cast<const float*>(w) + c, n);
+        const Raw8<float> v = load8_at<float>(static_cast<const float*>(w) + c, n);
 #pragma unroll
         for (int i = 0; i < 8; ++i) o[i] = at8(v, i);
     } else {
-        const Raw8<T> v = gn_load<T>(static_cast<const T*>(w) + c, n);
+        const Raw8<T> v = load8_at<T>(static_cast<const T*>(w) + c, n);
 #pragma unroll
         for (int i = 0; i < 8; ++i) o[i] = at8(v, i);
     }
@@ -136,8 +97,8 @@ __device__ void group_norm(const HelixGroupNormParams& p) {
         const int c = 8 * (l + LP * j);
         n[j] = here ? min(8, p.width - c) : 0;
         const int wide = n[j] > 0 && first + c + 8 <= p.dim ? 8 : n[j];   // what may be read
-        xr[j] = gn_load<T>(x + c, wide);
-        if (p.gate) gr[j] = gn_load<T>(gt + c, wide);
+        xr[j] = load8_at<T>(x + c, wide);
+        if (p.gate) gr[j] = load8_at<T>(gt + c, wide);
         gn_weights<T>(p.weight, p.w_f32, first + c, wide, w[j]);
         if (p.bias) gn_weights<T>(p.bias, p.w_f32, first + c, wide, b[j]);
     }
@@ -184,7 +145,7 @@ __device__ void group_norm(const HelixGroupNormParams& p) {
                 if ((c & 127) == 0) p.scale[row * p.ld_scale + (c >> 7)] = (uint8_t)e;
             }
         } else if (n[j] > 0) {
-            gn_store<T>(static_cast<T*>(p.y) + row * p.ld_y + c, v[j], n[j]);
+            store8_at<T>(static_cast<T*>(p.y) + row * p.ld_y + c, v[j], n[j]);
         }
     }
 }
@@ -273,9 +234,9 @@ __device__ void group_norm_bwd(const HelixGroupNormBwdParams& p) {
 #pragma unroll
         for (int j = 0; j < NC; ++j) {
             const int c = first + 8 * (l + LP * j);
-            xr[j] = gn_load<T>(static_cast<const T*>(p.x) + row * p.ld_x + c, wide[j]);
-            yr[j] = gn_load<T>(static_cast<const T*>(p.dy) + row * p.ld_dy + c, wide[j]);
-            if (p.gate) gr[j] = gn_load<T>(static_cast<const T*>(p.gate) + row * p.ld_gate + c, wide[j]);
+            xr[j] = load8_at<T>(static_cast<const T*>(p.x) + row * p.ld_x + c, wide[j]);
+            yr[j] = load8_at<T>(static_cast<const T*>(p.dy) + row * p.ld_dy + c, wide[j]);
+            if (p.gate) gr[j] = load8_at<T>(static_cast<const T*>(p.gate) + row * p.ld_gate + c, wide[j]);
         }
         const float mean = mine ? p.mean[row * p.groups + g] : 0.0f, rstd = mine ? p.rstd[row * p.groups + g] : 0.0f;
         float t[NC][8], s = 0.0f, st = 0.0f;
@@ -299,7 +260,7 @@ __device__ void group_norm_bwd(const HelixGroupNormBwdParams& p) {
                 }
             }
             if (p.gate && n[j] > 0)
-                gn_store<T>(static_cast<T*>(p.dgate) + row * p.ld_dgate + first + 8 * (l + LP * j), dg, n[j]);
+                store8_at<T>(static_cast<T*>(p.dgate) + row * p.ld_dgate + first + 8 * (l + LP * j), dg, n[j]);
         }
         // Two places in turn: a wave may be at the next row's sums while another reads this one's.
         const float ms = lanes_sum<LP>(s, red[turn][0]) / (float)p.width;
@@ -310,7 +271,7 @@ __device__ void group_norm_bwd(const HelixGroupNormBwdParams& p) {
             float o[8];
 #pragma unroll
             for (int i = 0; i < 8; ++i) o[i] = rstd * (t[j][i] - ms - (at8(xr[j], i) - mean) * rstd * mt);
-            if (n[j] > 0) gn_store<T>(static_cast<T*>(p.dx) + row * p.ld_dx + first + 8 * (l + LP * j), o, n[j]);
+            if (n[j] > 0) store8_at<T>(static_cast<T*>(p.dx) + row * p.ld_dx + first + 8 * (l + LP * j), o, n[j]);
         }
     }
     if (!p.part || !mine) return;
@@ -319,8 +280,8 @@ __device__ void group_norm_bwd(const HelixGroupNormBwdParams& p) {
     for (int j = 0; j < NC; ++j)
         if (n[j] > 0) {
             const int c = 8 * (l + LP * j);
-            gn_store<float>(to + c, dw[j], n[j]);
-            gn_store<float>(to + p.dim + c, db[j], n[j]);
+            store8_at<float>(to + c, dw[j], n[j]);
+            store8_at<float>(to + p.dim + c, db[j], n[j]);
         }
 }
 

@@ -151,6 +151,56 @@ HELIX_DEV void buf_store8(helix_rsrc r, const float (&v)[8], int voff) {
     }
 }
 
+// Eight elements at p, at any alignment: the first n of them (all where n >= 8).
+template <typename T>
+HELIX_DEV Raw8<T> load8_at(const T* p, int n) {
+    Raw8<T> o;
+    if (n >= 8) {
+        __builtin_memcpy(&o, p, 8 * sizeof(T));
+        return o;
+    }
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) o.w[i] = u32x4{0, 0, 0, 0};
+#pragma unroll
+    for (int i = 0; i < 7; ++i) {
+        if (i >= n) break;
+        if constexpr (sizeof(T) == 4) o.w[i >> 2][i & 3] = as_u32(p[i]);
+        else o.w[0][i >> 1] |= (unsigned)reinterpret_cast<const uint16_t*>(p)[i] << (16 * (i & 1));
+    }
+    return o;
+}
+template <typename T>
+HELIX_DEV void store8_at(T* p, const float (&v)[8], int n) {
+    T e[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) e[i] = (T)v[i];
+    if (n >= 8) {
+        __builtin_memcpy(p, e, 8 * sizeof(T));
+        return;
+    }
+    int at = 0;
+    if (n & 4) {
+        __builtin_memcpy(p, e, 4 * sizeof(T));
+        at = 4;
+    }
+    if (n & 2) {
+        const T two[2] = {at ? e[4] : e[0], at ? e[5] : e[1]};
+        __builtin_memcpy(p + at, two, 2 * sizeof(T));
+        at += 2;
+    }
+    if (n & 1) p[at] = at == 6 ? e[6] : at == 4 ? e[4] : at == 2 ? e[2] : e[0];
+}
+template <typename T>
+HELIX_DEV void store8_at(T* p, const Raw8<T>& v, int n) {
+    if (n >= 8) {
+        __builtin_memcpy(p, &v, 8 * sizeof(T));
+    } else {
+#pragma unroll
+        for (int i = 0; i < 7; ++i)
+            if (i < n) p[i] = (T)at8(v, i);
+    }
+}
+
 // The largest over each sixteen lanes, by moves within a row of lanes; all have it.
 template <int CTRL>
 HELIX_DEV float max_dpp(float v) {

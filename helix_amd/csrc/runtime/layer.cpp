@@ -1092,7 +1092,7 @@ extern "C" helix_status helix_delta_rule_backward_encode(helix_ctx* ctx, void* s
         const hipFunction_t prep = kernel(ctx, "helix_delta_prep_bwd_" + form), keep = kernel(ctx, "helix_delta_keep_" + form),
                             back = kernel(ctx, "helix_delta_back_" + form), grad = kernel(ctx, "helix_delta_grad_" + form);
         const long long sh = (long long)a->n_seq * a->n_head, sk = (long long)a->n_seq * a->n_qk_head;
-        const unsigned gw = grid(sh * p.n_slice, kDeltaThreads);
+        const unsigned gw = grid(sh * p.n_slice, 2 * kDeltaThreads);
         grid(sh * plan.chunks, kDeltaThreads);
         grid(sk * plan.chunks, 4 * keys);
         const OnDevice on(ctx->device);
@@ -1108,7 +1108,7 @@ extern "C" helix_status helix_delta_rule_backward_encode(helix_ctx* ctx, void* s
             p.n_chunk = std::min(plan.chunks, plan.n_chunk - p.chunk0);
             p.s0 = i ? start(i) : a->s0;
             launch(prep, stream, (unsigned)(sh * p.n_chunk), 1, kDeltaThreads, p);
-            launch(keep, stream, gw, 1, kDeltaThreads, p);
+            launch(keep, stream, gw, 1, 2 * kDeltaThreads, p);
         };
         for (int i = 0; i + 1 < plan.n_seg; ++i) {
             p.s = start(i + 1);
