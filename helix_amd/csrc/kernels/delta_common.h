@@ -176,6 +176,21 @@ HELIX_DEV void dr_get8_t(const __bf16* planes, int row, int col, int c, bf16x8 (
     }
 }
 
+// Four raw elements side by side, as widen4 takes them.
+template <typename T>
+HELIX_DEV typename Raw4<T>::type pack4(const unsigned (&e)[4]) {
+    if constexpr (sizeof(T) == 4) return u32x4{e[0], e[1], e[2], e[3]};
+    else return u32x2{e[0] | e[1] << 16, e[2] | e[3] << 16};
+}
+
+// The same elements, to be widened where they are used: a loop would keep them in twice the registers.
+template <typename T>
+HELIX_DEV typename Raw4<T>::type fresh4(typename Raw4<T>::type v) {
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T); ++i) v[i] = (unsigned)vgpr_fresh((int)v[i]);
+    return v;
+}
+
 // A barrier that the waves of a workgroup may meet in different places of the program (as many times each).
 HELIX_DEV void dr_barrier() {
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");

@@ -739,22 +739,16 @@ __device__ void delta_back(const HelixDeltaParams& p) {
 // and g_t has the sum over i >= t of what G_i has: M_P . Q K' + M_A . K K' by rows less by
 // columns, scale e^G (Q . U) - e^G beta (K . B) - e^(G_63 - G) (K . L), and for the last one the
 // sum of e^(G_63 - G) (K . L) and e^(G_63) (S . E); in fp64, as neighbours nearly cancel.
-// A wave has 16 of the keys' columns (U, B, L, dQ, dK for all tokens; its rows of S and E
-// straight from memory) and blocks of the triangles. Operands that waves share are in LDS, by
-// parts: dO, Z and D 64 columns at a time; K and Q before and after.
+// Two kernels, as the registers do not hold both: the triangles first (helix_delta_pairs_*, a
+// wave a block of 16 x 16), which read dO, Z, D and V, then the products with the states
+// (helix_delta_grad_*), which read dO, Z and D again, S and E.
 template <typename T, int NK, bool ODD>
-__device__ void delta_grad(const HelixDeltaParams& p) {
-    constexpr int NPL = dr_planes<T>, NO = dr_out_planes<T>, W = NK / 16, TH = 64 * W;
-    constexpr int TILES = (10 + W - 1) / W, ROWS = DR_C * 8 / TH;
+__device__ void delta_pairs(const HelixDeltaParams& p) {
+    constexpr int NPL = dr_planes<T>, TH = 640;
     constexpr int kKQ = 2 * NPL * DR_C * NK, kOZD = (NPL + 6) * DR_C * DR_C;
     __shared__ __attribute__((aligned(16))) __bf16 sBig[kKQ > kOZD ? kKQ : kOZD];
-    struct Sums {   // of a head; the triangles' parts take their place at the end
-        double G[DR_C];
-        float row[4][DR_C], col[4][DR_C], beta[4][DR_C], dot[3][W][DR_C], zv[DR_C], se[W];
-    };
-    __shared__ __attribute__((aligned(16))) __bf16 sM[2 * NO * DR_C * DR_C];
-    static_assert(sizeof(Sums) <= sizeof(sM), "the sums fit in the triangles' place");
-    Sums& sums = *reinterpret_cast<Sums*>(&sM[0]);
+    __shared__ double sG[DR_C];
+    __shared__ float sRow[4][DR_C], sCol[4][DR_C], sBeta[4][DR_C], sZV[DR_C];
     __bf16* const sK = sBig;
     __bf16* const sQ = sBig + NPL * DR_C * NK;
     __bf16* const sO = sBig;
@@ -767,242 +761,334 @@ __device__ void delta_grad(const HelixDeltaParams& p) {
     const int seq = (int)(sk / (unsigned)p.n_qk), hk = (int)(sk % (unsigned)p.n_qk);
     const long long t0 = (long long)(p.chunk0 + ch) * DR_C;
     const int len = (int)min((long long)DR_C, p.n_tok - t0), P = p.n_val, N = p.n_key;
-    const int n0 = 16 * w;
-    const Rows<T, ODD> rk(p.k, seq * p.seq_k + hk * p.head_k + t0 * p.tok_k, p.tok_k, len, N);
-    const Rows<T, ODD> rq(p.q, seq * p.seq_q + hk * p.head_q + t0 * p.tok_q, p.tok_q, len, N);
-    auto stage_kq = [&] {
-#pragma unroll
-        for (int i = 0; i < DR_C * (NK / 8) / TH; ++i) {
-            const int row = (tid + TH * i) / (NK / 8), col = 8 * ((tid + TH * i) % (NK / 8));
-            const Raw8<T> kr = rk.load8(row, col), qr = rq.load8(row, col);
+    const int tb = (w >= 1) + (w >= 3) + (w >= 6), jb = w - tb * (tb + 1) / 2;   // the wave's block
+    {
+        const Rows<T, ODD> rk(p.k, seq * p.seq_k + hk * p.head_k + t0 * p.tok_k, p.tok_k, len, N);
+        const Rows<T, ODD> rq(p.q, seq * p.seq_q + hk * p.head_q + t0 * p.tok_q, p.tok_q, len, N);
+        for (int i = tid; i < DR_C * (NK / 8); i += TH) {
+            const int row = i / (NK / 8), col = 8 * (i % (NK / 8));
             bf16x8 k[NPL], qq[NPL];
-            dr_operand<T>(kr, N - col, k);
-            dr_operand<T>(qr, N - col, qq);
+            dr_operand<T>(rk.load8(row, col), N - col, k);
+            dr_operand<T>(rq.load8(row, col), N - col, qq);
             dr_put8<NPL, NK, DR_C>(sK, row, col, k);
             dr_put8<NPL, NK, DR_C>(sQ, row, col, qq);
         }
+    }
+    // A pass over 64 columns of a head's values, loaded while the one before is at work: a row's eight by the first 512 threads.
+    const int srow = tid / 8, scol = 8 * (tid % 8);
+    Raw8<T> no, nv;
+    Raw8<float> nz, nd;
+    float ng;
+    auto load = [&](int hs, int pb) {
+        if (hs >= p.share) return;
+        const int h = hk * p.share + hs;
+        const long long at = ((long long)seq * p.n_head + h) * p.n_chunk + ch;
+        const Rows<T, ODD> ro(p.d_o, seq * p.seq_o + h * p.head_o + t0 * p.tok_o, p.tok_o, len, P);
+        const Rows<T, ODD> rv(p.v, seq * p.seq_v + h * p.head_v + t0 * p.tok_v, p.tok_v, len, P);
+        const Rows<float> rz(p.keep_z, at * DR_C * P, P, DR_C, P), rd(p.keep_d, at * DR_C * P, P, DR_C, P);
+        if (tid < 512) {
+            no = ro.load8(srow, pb + scol);
+            nz = rz.load8(srow, pb + scol);
+            nd = rd.load8(srow, pb + scol);
+            nv = rv.load8(srow, pb + scol);
+        }
+        ng = lane < len ? p.g[seq * p.seq_g + (t0 + lane) * p.tok_g + h] : 0.0f;
     };
-    // The wave's blocks (tb, jb) of the lower triangle: K K' and Q K'.
-    auto tb_of = [&](int k) { const int x = w + W * k; return (x >= 1) + (x >= 3) + (x >= 6); };
-    auto jb_of = [&](int k) { const int x = w + W * k, t = tb_of(k); return x - t * (t + 1) / 2; };
-    f32x4 kk[TILES], qk[TILES], mp[TILES], ma[TILES];
-    f32x4 kv[4], qv[4], dq[4], dk[4];   // k, q at (16 i + 4 q + r, n0 + c), and their gradients
-    stage_kq();
+    load(0, 0);
     __syncthreads();
-#pragma unroll
-    for (int k = 0; k < TILES; ++k) {
-        kk[k] = qk[k] = mp[k] = ma[k] = zero4();
-        if (w + W * k > 9) continue;
-        const int tb = tb_of(k), jb = jb_of(k);
+    f32x4 kk, qk, mp = zero4(), ma = zero4();
+    {
+        DrAcc x, y;
 #pragma unroll
         for (int s = 0; s < NK / 32; ++s) {
             const int col = 32 * s + 8 * q;
             bf16x8 a[NPL], b[NPL];
             dr_get8<NPL, NK, DR_C>(sK, 16 * jb + c, col, b);
             dr_get8<NPL, NK, DR_C>(sK, 16 * tb + c, col, a);
-            kk[k] = dr_mfma<NPL, NPL>(a, b, kk[k]);
+            dr_mfma<NPL, NPL>(a, b, x);
             dr_get8<NPL, NK, DR_C>(sQ, 16 * tb + c, col, a);
-            qk[k] = dr_mfma<NPL, NPL>(a, b, qk[k]);
+            dr_mfma<NPL, NPL>(a, b, y);
         }
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        dq[i] = dk[i] = zero4();
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const int row = 16 * i + 4 * q + r, at = dr_at<NK>(row, (n0 + c) >> 3) + (c & 7);
-            float a = 0.0f, b = 0.0f;
-#pragma unroll
-            for (int j = NPL - 1; j >= 0; --j) {
-                a += (float)sK[j * DR_C * NK + at];
-                b += (float)sQ[j * DR_C * NK + at];
-            }
-            kv[i][r] = a;
-            qv[i][r] = b;
-        }
+        kk = dr_sum<NPL>(x);
+        qk = dr_sum<NPL>(y);
     }
     for (int hs = 0; hs < p.share; ++hs) {
-        const int h = hk * p.share + hs;
-        const long long at = ((long long)seq * p.n_head + h) * p.n_chunk + ch;
-        const Rows<T, ODD> ro(p.d_o, seq * p.seq_o + h * p.head_o + t0 * p.tok_o, p.tok_o, len, P);
-        const Rows<T, ODD> rv(p.v, seq * p.seq_v + h * p.head_v + t0 * p.tok_v, p.tok_v, len, P);
-        const Rows<float> rz(p.keep_z, at * DR_C * P, P, DR_C, P), rd(p.keep_d, at * DR_C * P, P, DR_C, P);
-        const Rows<float> rs(p.keep_s, at * N * P, P, N, P), re(p.keep_e, at * N * P, P, N, P);
-        f32x4 U[4], B[4], L[4], dP[TILES], dA[TILES];
-        float zv[ROWS], se = 0.0f;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) U[i] = B[i] = L[i] = zero4();
-#pragma unroll
-        for (int k = 0; k < TILES; ++k) dP[k] = dA[k] = zero4();
-#pragma unroll
-        for (int i = 0; i < ROWS; ++i) zv[i] = 0.0f;
+        const long long at = ((long long)seq * p.n_head + hk * p.share + hs) * p.n_chunk + ch;
+        const float* dec = p.decay + at * (HELIX_DR_DECAY / 4);
+        const double G = dr_log_decay(ng) * 1.4426950408889634074;
+        DrAcc dP, dA;
+        float zv = 0.0f;
         for (int pb = 0; pb < P; pb += 64) {
             __syncthreads();   // what these overwrite has been read
-#pragma unroll
-            for (int i = 0; i < ROWS; ++i) {
-                const int row = (tid + TH * i) / 8, col = 8 * (tid % 8), n = P - pb - col;
-                const Raw8<T> orow = ro.load8(row, pb + col), vr = rv.load8(row, pb + col);
-                const Raw8<float> zr = rz.load8(row, pb + col), dr = rd.load8(row, pb + col);
+            if (tid < 512) {
+                const int n = P - pb - scol;
                 bf16x8 o[NPL], z[3], d[3];
-                dr_operand<T>(orow, n, o);
-                dr_operand<float>(zr, n, z);
-                dr_operand<float>(dr, n, d);
+                dr_operand<T>(no, n, o);
+                dr_operand<float>(nz, n, z);
+                dr_operand<float>(nd, n, d);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) zv[i] += e < n ? at8(zr, e) * at8(vr, e) : 0.0f;
+                for (int e = 0; e < 8; ++e) zv += e < n ? at8(nz, e) * at8(nv, e) : 0.0f;
+                dr_put8<NPL, DR_C, DR_C>(sO, srow, scol, o);
+                dr_put8<3, DR_C, DR_C>(sZ, srow, scol, z);
+                dr_put8<3, DR_C, DR_C>(sD, srow, scol, d);
+            }
+            load(pb + 64 < P ? hs : hs + 1, pb + 64 < P ? pb + 64 : 0);
+            __syncthreads();
+#pragma unroll
+            for (int ks = 0; ks < 2; ++ks) {
+                const int col = 32 * ks + 8 * q;
+                bf16x8 ao[NPL], az[3], bd[3];
+                dr_get8<3, DR_C, DR_C>(sD, 16 * jb + c, col, bd);
+                dr_get8<NPL, DR_C, DR_C>(sO, 16 * tb + c, col, ao);
+                dr_mfma<NPL, 3>(ao, bd, dP);
+                dr_get8<3, DR_C, DR_C>(sZ, 16 * tb + c, col, az);
+                dr_mfma<3, 3>(az, bd, dA);
+            }
+        }
+        if (w == 0) sG[lane] = G;
+        if (tid < 512) {
+            zv = add_dpp<0xb1>(zv);   // eight lanes a row
+            zv = add_dpp<0x4e>(zv);
+            zv = add_dpp<0x141>(zv);
+            if ((tid & 7) == 0) sZV[srow] = zv;
+        }
+        __syncthreads();
+        {
+            const f32x4 x = dP.sum(), y = dA.sum();
+            const int j = 16 * jb + c;
+            const double Gj = sG[j];
+            const f32x4 beta = *reinterpret_cast<const f32x4*>(dec + 128 + 16 * tb + 4 * q);
+            float pair[4], bs[4];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int i = 16 * tb + 4 * q + r;
+                const float e = __builtin_amdgcn_exp2f((float)(sG[i] - Gj));
+                const bool in = tb > jb || j <= i, below = tb > jb || j < i;
+                const float m = in ? p.scale * (e * x[r]) : 0.0f, a = below ? -(e * y[r]) : 0.0f;
+                mp[r] += m;
+                ma[r] += beta[r] * a;
+                bs[r] = below ? a * kk[r] : 0.0f;
+                pair[r] = in ? m * qk[r] + beta[r] * bs[r] : 0.0f;
+            }
+            const float row = row16_sum4(pair[0], pair[1], pair[2], pair[3], lane), b = row16_sum4(bs[0], bs[1], bs[2], bs[3], lane);
+            float col = (pair[0] + pair[1]) + (pair[2] + pair[3]);
+            col += __shfl_xor(col, 16, 64);
+            col += __shfl_xor(col, 32, 64);
+            if (c < 4) {
+                sRow[jb][16 * tb + 4 * q + c] = row;
+                sBeta[jb][16 * tb + 4 * q + c] = b;
+            }
+            if (q == 0) sCol[tb][j] = col;
+        }
+        __syncthreads();
+        if (w == 9) {
+            // Lane = token: what G and beta have of the triangles, and Z . V.
+            const int tile = lane >> 4;
+            double own = 0.0;
+            float db = sZV[lane];
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+                if (x <= tile) {
+                    own += sRow[x][lane];
+                    db += sBeta[x][lane];
+                }
+                if (x >= tile) own -= sCol[x][lane];
+            }
+            p.pair_g[at * DR_C + lane] = own;
+            p.pair_b[at * DR_C + lane] = db;
+        }
+    }
+    float* to = p.tri + (long long)id * (2 * 10 * 256) + 4 * lane;
+    *reinterpret_cast<f32x4*>(to + 256 * w) = mp;
+    *reinterpret_cast<f32x4*>(to + 256 * (10 + w)) = ma;
+}
+
+// A wave has 16 of the keys' columns (U, B, L, dQ, dK for its tokens; its rows of S and E straight
+// from memory), of all tokens or, with 64 keys, half of them. dO, Z and D are in LDS, by parts,
+// 64 columns at a time; K, Q and the triangles at the end.
+template <typename T, int NK, bool ODD>
+__device__ void delta_grad(const HelixDeltaParams& p) {
+    constexpr int NPL = dr_planes<T>, NO = dr_out_planes<T>, W = NK / 16, TH = 512;
+    constexpr int RG = 8 / W, RT = 4 / RG;   // groups of waves along the tokens, and row tiles of a wave
+    constexpr int kKQ = 2 * NPL * DR_C * NK, kM = 2 * NO * DR_C * DR_C, kOZD = (NPL + 6) * DR_C * DR_C;
+    __shared__ __attribute__((aligned(16))) __bf16 sBig[kKQ + kM > kOZD ? kKQ + kM : kOZD];
+    __shared__ __attribute__((aligned(16))) float sDec[HELIX_DR_DECAY / 4];
+    __shared__ float sDot[3][W][DR_C], sSE[W];
+    __bf16* const sK = sBig;
+    __bf16* const sQ = sBig + NPL * DR_C * NK;
+    __bf16* const sM = sBig + kKQ;
+    __bf16* const sO = sBig;
+    __bf16* const sZ = sBig + NPL * DR_C * DR_C;
+    __bf16* const sD = sZ + 3 * DR_C * DR_C;
+    const int tid = threadIdx.x, lane = lane_id(), w = wave_uniform(), c = lane & 15, q = lane >> 4;
+    const unsigned id = blockIdx.x;
+    const int ch = (int)(id % (unsigned)p.n_chunk);
+    const unsigned sk = id / (unsigned)p.n_chunk;
+    const int seq = (int)(sk / (unsigned)p.n_qk), hk = (int)(sk % (unsigned)p.n_qk);
+    const long long t0 = (long long)(p.chunk0 + ch) * DR_C;
+    const int len = (int)min((long long)DR_C, p.n_tok - t0), P = p.n_val, N = p.n_key;
+    const int cw = RG == 1 ? w : w % W, n0 = 16 * cw, i0 = RG == 1 ? 0 : w / W * RT;   // the wave's columns, and first row tile
+    const Rows<T, ODD> rk(p.k, seq * p.seq_k + hk * p.head_k + t0 * p.tok_k, p.tok_k, len, N);
+    const Rows<T, ODD> rq(p.q, seq * p.seq_q + hk * p.head_q + t0 * p.tok_q, p.tok_q, len, N);
+    f32x4 dq[RT], dk[RT];
+    typename Raw4<T>::type kv[RT], qv[RT];   // k and q at (16 (i0 + i) + 4 q + r, n0 + c), as they are stored
+#pragma unroll
+    for (int i = 0; i < RT; ++i) {
+        dq[i] = dk[i] = zero4();
+        unsigned k4[4], q4[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            k4[r] = rk.raw(16 * (i0 + i) + 4 * q + r, n0 + c);
+            q4[r] = rq.raw(16 * (i0 + i) + 4 * q + r, n0 + c);
+        }
+        kv[i] = pack4<T>(k4);
+        qv[i] = pack4<T>(q4);
+    }
+    // A pass over 64 columns of a head's values, loaded while the one before is at work: the thread's row of dO, Z and D, and
+    // the wave's rows of S and E.
+    struct Ahead {
+        Raw8<T> o;
+        Raw8<float> z, d, s[2], e[2];
+        f32x4 dec;
+    } next;
+    auto load = [&](int hs, int pb) {
+        if (hs >= p.share) return;
+        const int tid = vgpr_fresh(threadIdx.x), c = tid & 15, q = (tid & 63) >> 4, h = hk * p.share + hs;
+        const long long at = ((long long)seq * p.n_head + h) * p.n_chunk + ch;
+        const Rows<T, ODD> ro(p.d_o, seq * p.seq_o + h * p.head_o + t0 * p.tok_o, p.tok_o, len, P);
+        const Rows<float> rz(p.keep_z, at * DR_C * P, P, DR_C, P), rd(p.keep_d, at * DR_C * P, P, DR_C, P);
+        const Rows<float> rs(p.keep_s, at * N * P, P, N, P), re(p.keep_e, at * N * P, P, N, P);
+        const int row = tid / 8, col = pb + 8 * (tid % 8);
+        next.o = ro.load8(row, col);
+        next.z = rz.load8(row, col);
+        next.d = rd.load8(row, col);
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks) {
+            next.s[ks] = rs.load8(n0 + c, pb + 32 * ks + 8 * q);
+            next.e[ks] = re.load8(n0 + c, pb + 32 * ks + 8 * q);
+        }
+        if (tid < HELIX_DR_DECAY / 16) next.dec = *reinterpret_cast<const f32x4*>(p.decay + at * (HELIX_DR_DECAY / 4) + 4 * tid);
+    };
+    load(0, 0);
+    for (int hs = 0; hs < p.share; ++hs) {
+        float se = 0.0f, dots[3][RT];   // (of row 16 (i0 + i) + 4 q + c % 4)
+#pragma unroll
+        for (int i = 0; i < RT; ++i) dots[0][i] = dots[1][i] = dots[2][i] = 0.0f;
+        for (int pb = 0; pb < P; pb += 64) {
+            // (Addresses formed from these are formed here, not kept over the loop.)
+            const int fresh = vgpr_fresh(tid), lane = fresh & 63, c = lane & 15, q = lane >> 4;
+            __syncthreads();   // what these overwrite has been read
+            {
+                const int row = fresh / 8, col = 8 * (fresh % 8), n = P - pb - col;
+                bf16x8 o[NPL], z[3], d[3];
+                dr_operand<T>(next.o, n, o);
+                dr_operand<float>(next.z, n, z);
+                dr_operand<float>(next.d, n, d);
                 dr_put8<NPL, DR_C, DR_C>(sO, row, col, o);
                 dr_put8<3, DR_C, DR_C>(sZ, row, col, z);
                 dr_put8<3, DR_C, DR_C>(sD, row, col, d);
             }
-            Raw8<float> sr[2], er[2];
+            if (tid < HELIX_DR_DECAY / 16) *reinterpret_cast<f32x4*>(&sDec[4 * tid]) = next.dec;
+            bf16x8 bs[2][3], be[2][3];
 #pragma unroll
             for (int ks = 0; ks < 2; ++ks) {
-                sr[ks] = rs.load8(n0 + c, pb + 32 * ks + 8 * q);
-                er[ks] = re.load8(n0 + c, pb + 32 * ks + 8 * q);
+                const int n = P - pb - 32 * ks - 8 * q;
+                dr_operand<float>(next.s[ks], n, bs[ks]);
+                dr_operand<float>(next.e[ks], n, be[ks]);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) se += e < n ? at8(next.s[ks], e) * at8(next.e[ks], e) : 0.0f;
             }
+            load(pb + 64 < P ? hs : hs + 1, pb + 64 < P ? pb + 64 : 0);
             __syncthreads();
+            // Row tile by row tile: each product goes into the gradients (and its dot with q or k) at once.
 #pragma unroll
-            for (int ks = 0; ks < 2; ++ks) {
-                const int col = 32 * ks + 8 * q, n = P - pb - col;
-                bf16x8 bs[3], be[3];
-                dr_operand<float>(sr[ks], n, bs);
-                dr_operand<float>(er[ks], n, be);
+            for (int i = 0; i < RT; ++i) {
+                const int tile = 16 * (i0 + i), row = tile + 4 * q;
+                DrAcc U, B, L;
 #pragma unroll
-                for (int e = 0; e < 8; ++e) se += e < n ? at8(sr[ks], e) * at8(er[ks], e) : 0.0f;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
+                for (int ks = 0; ks < 2; ++ks) {
+                    const int col = 32 * ks + 8 * q;
                     bf16x8 ao[NPL], az[3], ad[3];
-                    dr_get8<NPL, DR_C, DR_C>(sO, 16 * i + c, col, ao);
-                    U[i] = dr_mfma<NPL, 3>(ao, bs, U[i]);
-                    dr_get8<3, DR_C, DR_C>(sZ, 16 * i + c, col, az);
-                    B[i] = dr_mfma<3, 3>(az, bs, B[i]);
-                    dr_get8<3, DR_C, DR_C>(sD, 16 * i + c, col, ad);
-                    L[i] = dr_mfma<3, 3>(ad, be, L[i]);
+                    dr_get8<NPL, DR_C, DR_C>(sO, tile + c, col, ao);
+                    dr_mfma<NPL, 3>(ao, bs[ks], U);
+                    dr_get8<3, DR_C, DR_C>(sZ, tile + c, col, az);
+                    dr_mfma<3, 3>(az, bs[ks], B);
+                    dr_get8<3, DR_C, DR_C>(sD, tile + c, col, ad);
+                    dr_mfma<3, 3>(ad, be[ks], L);
                 }
-#pragma unroll
-                for (int k = 0; k < TILES; ++k) {
-                    if (w + W * k > 9) continue;
-                    const int tb = tb_of(k), jb = jb_of(k);
-                    bf16x8 ao[NPL], az[3], bd[3];
-                    dr_get8<3, DR_C, DR_C>(sD, 16 * jb + c, col, bd);
-                    dr_get8<NPL, DR_C, DR_C>(sO, 16 * tb + c, col, ao);
-                    dP[k] = dr_mfma<NPL, 3>(ao, bd, dP[k]);
-                    dr_get8<3, DR_C, DR_C>(sZ, 16 * tb + c, col, az);
-                    dA[k] = dr_mfma<3, 3>(az, bd, dA[k]);
-                }
+                const f32x4 start = *reinterpret_cast<const f32x4*>(&sDec[row]), left = *reinterpret_cast<const f32x4*>(&sDec[64 + row]),
+                            beta = *reinterpret_cast<const f32x4*>(&sDec[128 + row]);
+                const f32x4 u = U.sum(), b = B.sum(), l = L.sum();
+                dq[i] += p.scale * start * u;
+                dk[i] += left * l - start * beta * b;
+                float x[4];
+                widen4<T>(fresh4<T>(qv[i]), x);
+                dots[0][i] += row16_sum4(x[0] * u[0], x[1] * u[1], x[2] * u[2], x[3] * u[3], lane);
+                widen4<T>(fresh4<T>(kv[i]), x);
+                dots[1][i] += row16_sum4(x[0] * b[0], x[1] * b[1], x[2] * b[2], x[3] * b[3], lane);
+                dots[2][i] += row16_sum4(x[0] * l[0], x[1] * l[1], x[2] * l[2], x[3] * l[3], lane);
+                __builtin_amdgcn_sched_barrier(0);   // (the next tile's reads would not fit in the registers)
             }
-        }
-        const float gl = lane < len ? p.g[seq * p.seq_g + (t0 + lane) * p.tok_g + h] : 0.0f;
-        const double G = dr_log_decay(gl);
-        const float* dec = p.decay + at * (HELIX_DR_DECAY / 4);
-        if (w == 0) sums.G[lane] = G;
-#pragma unroll
-        for (int i = 0; i < ROWS; ++i) {
-            // Eight lanes a row.
-            float z = zv[i];
-            z += __shfl_xor(z, 1, 64);
-            z += __shfl_xor(z, 2, 64);
-            z += __shfl_xor(z, 4, 64);
-            if ((tid & 7) == 0) sums.zv[(tid + TH * i) / 8] = z;
         }
         se = wave_sum(se);
-        if (lane == 0) sums.se[w] = se;
+        if (lane == 0 && i0 == 0) sSE[cw] = se;
+        if (c < 4) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int row = 16 * i + 4 * q;
-            const f32x4 start = *reinterpret_cast<const f32x4*>(dec + row), left = *reinterpret_cast<const f32x4*>(dec + 64 + row),
-                        beta = *reinterpret_cast<const f32x4*>(dec + 128 + row);
-            dq[i] += p.scale * start * U[i];
-            dk[i] += left * L[i] - start * beta * B[i];
-            const f32x4 x = qv[i] * U[i], y = kv[i] * B[i], z = kv[i] * L[i];
+            for (int i = 0; i < RT; ++i) {
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const float a = row16_sum(x[r]), b = row16_sum(y[r]), l = row16_sum(z[r]);
-                if (c == 0) {
-                    sums.dot[0][w][row + r] = a;
-                    sums.dot[1][w][row + r] = b;
-                    sums.dot[2][w][row + r] = l;
-                }
+                for (int j = 0; j < 3; ++j) sDot[j][cw][16 * (i0 + i) + 4 * q + c] = dots[j][i];
             }
-        }
-        __syncthreads();
-#pragma unroll
-        for (int k = 0; k < TILES; ++k) {
-            if (w + W * k > 9) continue;
-            const int tb = tb_of(k), jb = jb_of(k), j = 16 * jb + c;
-            const double Gj = sums.G[j];
-            const f32x4 beta = *reinterpret_cast<const f32x4*>(dec + 128 + 16 * tb + 4 * q);
-            float col = 0.0f;
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int i = 16 * tb + 4 * q + r;
-                const float e = j <= i ? exp_diff(sums.G[i], Gj) : 0.0f, ea = j < i ? -(e * dA[k][r]) : 0.0f;
-                const float m = j <= i ? p.scale * (e * dP[k][r]) : 0.0f, n = beta[r] * ea;
-                mp[k][r] += m;
-                ma[k][r] += n;
-                const float b = ea * kk[k][r], pair = m * qk[k][r] + beta[r] * b;
-                col += pair;
-                const float row = row16_sum(pair), bs = row16_sum(b);
-                if (c == 0) {
-                    sums.row[jb][i] = row;
-                    sums.beta[jb][i] = bs;
-                }
-            }
-            col += __shfl_xor(col, 16, 64);
-            col += __shfl_xor(col, 32, 64);
-            if (q == 0) sums.col[tb][j] = col;
         }
         __syncthreads();
         if (w == 0) {
             // Lane = token.
-            float dots[3];
+            const int h = hk * p.share + hs;
+            const long long at = (((long long)seq * p.n_head + h) * p.n_chunk + ch) * DR_C + lane;
+            double own = p.pair_g[at];
+            const float db = p.pair_b[at];
+            float dot[3];
 #pragma unroll
             for (int j = 0; j < 3; ++j) {
-                dots[j] = 0.0f;
+                dot[j] = 0.0f;
 #pragma unroll
-                for (int x = 0; x < W; ++x) dots[j] += sums.dot[j][x][lane];
+                for (int x = 0; x < W; ++x) dot[j] += sDot[j][x][lane];
             }
             float sse = 0.0f;
 #pragma unroll
-            for (int x = 0; x < W; ++x) sse += sums.se[x];
-            const float start = dec[lane], left = dec[64 + lane], beta = dec[128 + lane];
-            const int tile = lane >> 4;
-            double own = 0.0;
-            float db = 0.0f;
-#pragma unroll
-            for (int x = 0; x < 4; ++x) {
-                if (x <= tile) {
-                    own += sums.row[x][lane];
-                    db += sums.beta[x][lane];
-                }
-                if (x >= tile) own -= sums.col[x][lane];
-            }
-            const double tail = (double)left * dots[2];
-            own += (double)(p.scale * start) * dots[0] - (double)(start * beta) * dots[1] - tail;
+            for (int x = 0; x < W; ++x) sse += sSE[x];
+            const float start = sDec[lane], left = sDec[64 + lane], beta = sDec[128 + lane];
+            const double tail = (double)left * dot[2];
+            own += (double)(p.scale * start) * dot[0] - (double)(start * beta) * dot[1] - tail;
             const double tails = __shfl(wave_incl_sum(tail), 63, 64);
-            if (lane == 63) own += tails + (double)dec[63] * sse;
+            if (lane == 63) own += tails + (double)sDec[63] * sse;
             const double incl = wave_incl_sum(own);
             const double dg = __shfl(incl, 63, 64) - incl + own;
             if (lane < len) {
                 const long long to = ((long long)seq * p.n_tok + t0 + lane) * p.n_head + h;
                 p.dg[to] = (float)dg;
-                p.dbeta[to] = sums.zv[lane] - start * dots[1] + db;
+                p.dbeta[to] = db - start * dot[1];
             }
         }
     }
     // The triangles' products, once for all heads.
     __syncthreads();
-    stage_kq();
 #pragma unroll
-    for (int k = 0; k < TILES; ++k) {
-        if (w + W * k > 9) continue;
-        const int tb = tb_of(k), jb = jb_of(k);
-        // Stored by columns: M[j][i].
-        dr_put4<NO, DR_C, DR_C>(sM + 0 * NO * DR_C * DR_C, 16 * jb + c, 16 * tb + 4 * q, mp[k][0], mp[k][1], mp[k][2], mp[k][3]);
-        dr_put4<NO, DR_C, DR_C>(sM + 1 * NO * DR_C * DR_C, 16 * jb + c, 16 * tb + 4 * q, ma[k][0], ma[k][1], ma[k][2], ma[k][3]);
-        if (tb != jb) {   // 0 above the diagonal
-            dr_put4<NO, DR_C, DR_C>(sM + 0 * NO * DR_C * DR_C, 16 * tb + c, 16 * jb + 4 * q, 0.0f, 0.0f, 0.0f, 0.0f);
-            dr_put4<NO, DR_C, DR_C>(sM + 1 * NO * DR_C * DR_C, 16 * tb + c, 16 * jb + 4 * q, 0.0f, 0.0f, 0.0f, 0.0f);
-        }
+    for (int i = 0; i < DR_C * (NK / 8) / TH; ++i) {
+        const int row = (tid + TH * i) / (NK / 8), col = 8 * ((tid + TH * i) % (NK / 8));
+        const Raw8<T> kr = rk.load8(row, col), qr = rq.load8(row, col);
+        bf16x8 k[NPL], qq[NPL];
+        dr_operand<T>(kr, N - col, k);
+        dr_operand<T>(qr, N - col, qq);
+        dr_put8<NPL, NK, DR_C>(sK, row, col, k);
+        dr_put8<NPL, NK, DR_C>(sQ, row, col, qq);
+    }
+    for (int x = w; x < 20; x += 8) {
+        // Stored by columns: M[j][i]; 0 above the diagonal.
+        const int k = x % 10, tb = (k >= 1) + (k >= 3) + (k >= 6), jb = k - tb * (tb + 1) / 2;
+        const f32x4 m = *reinterpret_cast<const f32x4*>(p.tri + (long long)id * (2 * 10 * 256) + 256 * x + 4 * lane);
+        __bf16* to = sM + x / 10 * NO * DR_C * DR_C;
+        dr_put4<NO, DR_C, DR_C>(to, 16 * jb + c, 16 * tb + 4 * q, m[0], m[1], m[2], m[3]);
+        if (tb != jb) dr_put4<NO, DR_C, DR_C>(to, 16 * tb + c, 16 * jb + 4 * q, 0.0f, 0.0f, 0.0f, 0.0f);
     }
     __syncthreads();
 #pragma unroll
@@ -1011,19 +1097,20 @@ __device__ void delta_grad(const HelixDeltaParams& p) {
         dr_get8_t<NPL, NK, DR_C>(sK, 32 * ks + 8 * q, n0, c, bk);
         dr_get8_t<NPL, NK, DR_C>(sQ, 32 * ks + 8 * q, n0, c, bq);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < RT; ++i) {
             bf16x8 a[NO];
+            const int tile = i0 + i;
             // M[i][j] over j: columns of what is stored; M'[j][i] over i: its rows.
-            if (2 * ks <= i) {
-                dr_get8_t<NO, DR_C, DR_C>(sM + 0 * NO * DR_C * DR_C, 32 * ks + 8 * q, 16 * i, c, a);
+            if (2 * ks <= tile) {
+                dr_get8_t<NO, DR_C, DR_C>(sM, 32 * ks + 8 * q, 16 * tile, c, a);
                 dq[i] = dr_mfma<NO, NPL, NO>(a, bk, dq[i]);
-                dr_get8_t<NO, DR_C, DR_C>(sM + 1 * NO * DR_C * DR_C, 32 * ks + 8 * q, 16 * i, c, a);
+                dr_get8_t<NO, DR_C, DR_C>(sM + NO * DR_C * DR_C, 32 * ks + 8 * q, 16 * tile, c, a);
                 dk[i] = dr_mfma<NO, NPL, NO>(a, bk, dk[i]);
             }
-            if (2 * ks + 1 >= i) {
-                dr_get8<NO, DR_C, DR_C>(sM + 0 * NO * DR_C * DR_C, 16 * i + c, 32 * ks + 8 * q, a);
+            if (2 * ks + 1 >= tile) {
+                dr_get8<NO, DR_C, DR_C>(sM, 16 * tile + c, 32 * ks + 8 * q, a);
                 dk[i] = dr_mfma<NO, NPL, NO>(a, bq, dk[i]);
-                dr_get8<NO, DR_C, DR_C>(sM + 1 * NO * DR_C * DR_C, 16 * i + c, 32 * ks + 8 * q, a);
+                dr_get8<NO, DR_C, DR_C>(sM + NO * DR_C * DR_C, 16 * tile + c, 32 * ks + 8 * q, a);
                 dk[i] = dr_mfma<NO, NPL, NO>(a, bk, dk[i]);
             }
         }
@@ -1031,11 +1118,11 @@ __device__ void delta_grad(const HelixDeltaParams& p) {
     const long long to = (((long long)seq * p.n_tok + t0) * p.n_qk + hk) * N;
     const Rows<T> oq(p.dq, to, (long long)p.n_qk * N, len, N), ok(p.dk, to, (long long)p.n_qk * N, len, N);
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < RT; ++i)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-            oq.store(16 * i + 4 * q + r, n0 + c, dq[i][r]);
-            ok.store(16 * i + 4 * q + r, n0 + c, dk[i][r]);
+            oq.store(16 * (i0 + i) + 4 * q + r, n0 + c, dq[i][r]);
+            ok.store(16 * (i0 + i) + 4 * q + r, n0 + c, dk[i][r]);
         }
 }
 
@@ -1050,7 +1137,8 @@ __device__ void delta_grad(const HelixDeltaParams& p) {
     extern "C" __global__ __launch_bounds__(256) void helix_delta_prep_bwd_##TAG##_##NK##SUF(HelixDeltaParams p) { delta_prep<T, NK, ODD, true>(p); } \
     extern "C" __global__ __launch_bounds__(512) void helix_delta_keep_##TAG##_##NK##SUF(HelixDeltaParams p) { delta_walk<T, NK, ODD, true>(p); }     \
     extern "C" __global__ __launch_bounds__(256) void helix_delta_back_##TAG##_##NK##SUF(HelixDeltaParams p) { delta_back<T, NK, ODD>(p); }           \
-    extern "C" __global__ __launch_bounds__(4 * NK) void helix_delta_grad_##TAG##_##NK##SUF(HelixDeltaParams p) { delta_grad<T, NK, ODD>(p); }
+    extern "C" __global__ __launch_bounds__(640) void helix_delta_pairs_##TAG##_##NK##SUF(HelixDeltaParams p) { delta_pairs<T, NK, ODD>(p); }                   \
+    extern "C" __global__ __launch_bounds__(512) void helix_delta_grad_##TAG##_##NK##SUF(HelixDeltaParams p) { delta_grad<T, NK, ODD>(p); }
 DR_STEPS(f32, float, 64)
 DR_KERNELS(f32, float, 64, , false)
 DR_STEPS(f32, float, 128)

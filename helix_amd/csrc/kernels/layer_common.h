@@ -225,4 +225,14 @@ HELIX_DEV float row16_sum(float v) {
     return add_dpp<0x140>(v);
 }
 
+// Of four values, the sums over each sixteen lanes: lane c has that of value c % 4.
+HELIX_DEV float row16_sum4(float a, float b, float c, float d, int lane) {
+    const bool odd = lane & 1, high = lane & 2;
+    const float ab = (odd ? b : a) + as_f32((unsigned)__builtin_amdgcn_update_dpp(0, (int)as_u32(odd ? a : b), 0xb1, 0xf, 0xf, true));
+    const float cd = (odd ? d : c) + as_f32((unsigned)__builtin_amdgcn_update_dpp(0, (int)as_u32(odd ? c : d), 0xb1, 0xf, 0xf, true));
+    float v = (high ? cd : ab) + as_f32((unsigned)__builtin_amdgcn_update_dpp(0, (int)as_u32(high ? ab : cd), 0x4e, 0xf, 0xf, true));
+    v = add_dpp<0x128>(v);   // row_ror:8
+    return add_dpp<0x124>(v);   // row_ror:4
+}
+
 #endif

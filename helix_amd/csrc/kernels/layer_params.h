@@ -190,6 +190,9 @@ typedef struct {
     float*       keep_e;    /* the same of the state's gradient after them     */
     float*       keep_d;    /* [sequence x head][chunk][64][n_val] D           */
     float*       keep_z;    /* and Z                                           */
+    double*      pair_g;    /* [sequence x head][chunk][64] what the triangles bring G */
+    float*       pair_b;    /* and beta, with Z . V                            */
+    float*       tri;       /* [sequence x qk head][chunk][2][10][256] their gradients, by blocks */
 } HelixDeltaParams;
 
 #endif

@@ -839,7 +839,7 @@ extern "C" helix_status helix_gated_scan_backward_encode(helix_ctx* ctx, void* s
 
 namespace {
 
-constexpr int kDeltaThreads = 256;
+constexpr int kDeltaThreads = 256, kDeltaPairThreads = 640;
 
 // Elements of strides that do not overlap: each dimension's stride reaches past what the ones below it span.
 bool disjoint(std::initializer_list<std::pair<long long, long long>> dims) {   // (size, stride)
@@ -1009,7 +1009,7 @@ namespace {
 // The backward pass: what a segment's chunks leave for its kernels, and the states that the segments start from.
 struct DeltaBwdPlan {
     int n_chunk = 0, chunks = 0, n_seg = 0, n_slice = 0;
-    size_t x_at = 0, tt_at = 0, pt_at = 0, decay_at = 0, s_at = 0, e_at = 0, d_at = 0, z_at = 0, start_at = 0, bytes = 0;
+    size_t x_at = 0, tt_at = 0, pt_at = 0, decay_at = 0, s_at = 0, e_at = 0, d_at = 0, z_at = 0, pg_at = 0, pb_at = 0, tri_at = 0, start_at = 0, bytes = 0;
 };
 // Scratch of a segment: up to two gigabytes, and one chunk of every sequence where that is more. More than one segment forms
 // its states twice.
@@ -1021,9 +1021,10 @@ DeltaBwdPlan delta_bwd_plan(const helix_delta_rule_backward_args& a) {
     const size_t sh = (size_t)a.n_seq * a.n_head, x = 6 * 3 * HELIX_DR_FRAG;
     auto up = [](size_t bytes) { return (bytes + 255) & ~(size_t)255; };
     const size_t state = (size_t)a.n_key * a.n_val * 4, rows = (size_t)HELIX_DR_CHUNK * a.n_val * 4;
+    const size_t tri = 2 * 10 * 256 * 4, sk = (size_t)a.n_seq * std::max(1, a.n_qk_head);
     p.n_chunk = (int)ceil_div(a.n_tok, HELIX_DR_CHUNK);
     p.chunks = (int)std::min<size_t>(p.n_chunk,
-                                     std::max<size_t>(1, kDeltaBwdScratch / (sh * (3 * x + HELIX_DR_DECAY + 2 * state + 2 * rows))));
+                                     std::max<size_t>(1, kDeltaBwdScratch / (sh * (3 * x + HELIX_DR_DECAY + 2 * state + 2 * rows + 12 * HELIX_DR_CHUNK) + sk * tri)));
     p.n_seg = (int)ceil_div(p.n_chunk, p.chunks);
     p.n_slice = (int)ceil_div(a.n_val, HELIX_DR_SLICE);
     const size_t each = sh * p.chunks;
@@ -1034,7 +1035,10 @@ DeltaBwdPlan delta_bwd_plan(const helix_delta_rule_backward_args& a) {
     p.e_at = p.s_at + up(each * state);
     p.d_at = p.e_at + up(each * state);
     p.z_at = p.d_at + up(each * rows);
-    p.start_at = p.z_at + up(each * rows);
+    p.pg_at = p.z_at + up(each * rows);
+    p.pb_at = p.pg_at + each * HELIX_DR_CHUNK * 8;
+    p.tri_at = p.pb_at + each * HELIX_DR_CHUNK * 4;
+    p.start_at = p.tri_at + sk * p.chunks * tri;
     p.bytes = p.start_at + (size_t)(p.n_seg - 1) * up(sh * state);
     return p;
 }
@@ -1086,15 +1090,18 @@ extern "C" helix_status helix_delta_rule_backward_encode(helix_ctx* ctx, void* s
         p.keep_e = reinterpret_cast<float*>(sc + plan.e_at);
         p.keep_d = reinterpret_cast<float*>(sc + plan.d_at);
         p.keep_z = reinterpret_cast<float*>(sc + plan.z_at);
+        p.pair_g = reinterpret_cast<double*>(sc + plan.pg_at);
+        p.pair_b = reinterpret_cast<float*>(sc + plan.pb_at);
+        p.tri = reinterpret_cast<float*>(sc + plan.tri_at);
         p.n_slice = (int)ceil_div(a->n_val, HELIX_DR_SLICE);
-        const int keys = delta_keys(a->n_key);
         const std::string form = delta_form(*a);
         const hipFunction_t prep = kernel(ctx, "helix_delta_prep_bwd_" + form), keep = kernel(ctx, "helix_delta_keep_" + form),
-                            back = kernel(ctx, "helix_delta_back_" + form), grad = kernel(ctx, "helix_delta_grad_" + form);
+                            back = kernel(ctx, "helix_delta_back_" + form), pairs = kernel(ctx, "helix_delta_pairs_" + form),
+                            grad = kernel(ctx, "helix_delta_grad_" + form);
         const long long sh = (long long)a->n_seq * a->n_head, sk = (long long)a->n_seq * a->n_qk_head;
         const unsigned gw = grid(sh * p.n_slice, 2 * kDeltaThreads);
         grid(sh * plan.chunks, kDeltaThreads);
-        grid(sk * plan.chunks, 4 * keys);
+        grid(sk * plan.chunks, kDeltaPairThreads);
         const OnDevice on(ctx->device);
         if (!a->n_tok) {
             launch(back, stream, gw, 1, kDeltaThreads, p);
@@ -1118,7 +1125,8 @@ extern "C" helix_status helix_delta_rule_backward_encode(helix_ctx* ctx, void* s
         for (int i = plan.n_seg - 1; i >= 0; --i) {
             states(i);
             launch(back, stream, gw, 1, kDeltaThreads, p);
-            launch(grad, stream, (unsigned)(sk * p.n_chunk), 1, (unsigned)(4 * keys), p);
+            launch(pairs, stream, (unsigned)(sk * p.n_chunk), 1, kDeltaPairThreads, p);
+            launch(grad, stream, (unsigned)(sk * p.n_chunk), 1, 2 * kDeltaThreads, p);
             p.d_s = p.ds0;   // the segment before goes on from here
         }
     });
@@ -1142,7 +1150,7 @@ const std::vector<std::string>& layer_kernel_names() {
         for (const char* tag : kTags)
             for (const char* n : {"_64", "_128"}) {
                 v.push_back(std::string("helix_delta_steps_") + tag + n);
-                for (const char* k : {"prep_", "walk_", "prep_bwd_", "keep_", "back_", "grad_"})
+                for (const char* k : {"prep_", "walk_", "prep_bwd_", "keep_", "back_", "pairs_", "grad_"})
                     for (const char* s : {"", "_s"})
                         if (!*s || tag != kTags[HELIX_F32]) v.push_back(std::string("helix_delta_") + k + tag + n + s);
             }
