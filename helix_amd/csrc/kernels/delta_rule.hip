@@ -567,32 +567,168 @@ __device__ void delta_walk(const HelixDeltaParams& p) {
 // caller's):
 //     dD = P' dO + (e^(G_63 - G) K) E,   Z = T' dD,   dV = beta Z
 //     dS = e^(G_63) E + scale (e^G Q)' dO - (e^G K)' dV
-// from the last chunk to the first: helix_delta_back_*, spread and laid out as the walk, dO
-// and e^G dO in V's place. It leaves E and Z for helix_delta_grad_*.
+// from the last chunk to the first: helix_delta_back_*, spread and laid out as the walk. Its
+// second four waves bring K, Q and dO and form what does not wait for E, P' dO and
+// scale (e^G Q)' dO of the chunk after the one that the first four are at. It leaves E and Z for
+// the kernels below.
 template <typename T, int NK, bool ODD>
 __device__ void delta_back(const HelixDeltaParams& p) {
     constexpr int NPL = dr_planes<T>, NT = NK / 64, KS = NK / 32;
     __shared__ __attribute__((aligned(16))) __bf16 sK[NPL * DR_C * NK], sQ[NPL * DR_C * NK], sE[3 * 16 * NK];
     __shared__ __attribute__((aligned(16))) __bf16 sO[NPL * 16 * DR_C], sW[3 * 16 * DR_C], sR[3 * 16 * DR_C], sU[3 * 16 * DR_C];
-    const int tid = threadIdx.x, lane = lane_id(), w = wave_uniform(), c = lane & 15, q = lane >> 4;
+    __shared__ f32x4 sPO[4][64], sQW[NT][4][64];   // P' dO, where Z then is, and Q' (scale e^G dO), as lanes hold them
+    __shared__ __attribute__((aligned(16))) float sDec[2][HELIX_DR_DECAY / 4];
+    const int tid = threadIdx.x & 255, lane = lane_id(), w = wave_uniform() & 3, c = lane & 15, q = lane >> 4;
     const unsigned id = xcd_logical_id(blockIdx.x, gridDim.x);
     const int slice = (int)(id % (unsigned)p.n_slice);
     const unsigned sh = id / (unsigned)p.n_slice;
     const int seq = (int)(sh / (unsigned)p.n_head), h = (int)(sh % (unsigned)p.n_head), hk = h / p.share;
     const int p0 = 16 * slice, P = p.n_val, N = p.n_key;
     const unsigned state_bytes = (unsigned)N * (unsigned)P * 4u;
-    const int row0 = 16 * w + 4 * q;
+    const int row0 = 16 * w + 4 * q, last = p.n_chunk - 1;
+    const long long base = (long long)sh * p.n_chunk;
+    auto first = [&](int ch) { return (long long)(p.chunk0 + ch) * DR_C; };
+    auto tokens = [&](int ch) { return (int)min((long long)DR_C, p.n_tok - first(ch)); };
+
+    if (wave_uniform() >= 4) {
+        if (last < 0) return;
+        constexpr int PER = DR_C * (NK / 8) / 256;
+        Raw8<T> kr[PER], qr[PER];
+        bf16x8 pf[2][3];
+        unsigned vo[4];
+        f32x4 start, dec;
+        auto load_q = [&](int ch) {   // Q's rows, dO and its decays
+            ch = max(ch, 0);
+            const Rows<T, ODD> rq(p.q, seq * p.seq_q + hk * p.head_q + first(ch) * p.tok_q, p.tok_q, tokens(ch), N);
+            const Rows<T> ro(p.d_o, seq * p.seq_o + h * p.head_o + first(ch) * p.tok_o, p.tok_o, tokens(ch), P);
+#pragma unroll
+            for (int i = 0; i < PER; ++i) qr[i] = rq.load8((tid + 256 * i) / (NK / 8), 8 * ((tid + 256 * i) % (NK / 8)));
+#pragma unroll
+            for (int r = 0; r < 4; ++r) vo[r] = ro.raw(row0 + r, p0 + c);
+            start = *reinterpret_cast<const f32x4*>(p.decay + (base + ch) * (HELIX_DR_DECAY / 4) + row0);
+        };
+        auto load_k = [&](int ch) {   // K's rows, all decays, and the fragments of P'
+            ch = max(ch, 0);
+            const Rows<T, ODD> rk(p.k, seq * p.seq_k + hk * p.head_k + first(ch) * p.tok_k, p.tok_k, tokens(ch), N);
+#pragma unroll
+            for (int i = 0; i < PER; ++i) kr[i] = rk.load8((tid + 256 * i) / (NK / 8), 8 * ((tid + 256 * i) % (NK / 8)));
+            if (tid < HELIX_DR_DECAY / 16) dec = *reinterpret_cast<const f32x4*>(p.decay + (base + ch) * (HELIX_DR_DECAY / 4) + 4 * tid);
+            const char* pt = p.pt + (base + ch) * (6 * 3 * HELIX_DR_FRAG) + 16 * lane;
+#pragma unroll
+            for (int ks = 0; ks < 2; ++ks) {
+                if (ks == 0 && w > 1) continue;
+#pragma unroll
+                for (int k = 0; k < 3; ++k) pf[ks][k] = *reinterpret_cast<const bf16x8*>(pt + (dr_up(w, ks) * 3 + k) * HELIX_DR_FRAG);
+            }
+        };
+        auto put_rows = [&](__bf16* to, const Raw8<T> (&v)[PER]) {
+#pragma unroll
+            for (int i = 0; i < PER; ++i) {
+                const int row = (tid + 256 * i) / (NK / 8), col = 8 * ((tid + 256 * i) % (NK / 8));
+                bf16x8 o[NPL];
+                dr_operand<T>(v[i], N - col, o);
+                dr_put8<NPL, NK, DR_C>(to, row, col, o);
+            }
+        };
+        auto put_q = [&] {
+            put_rows(sQ, qr);
+            float o[4];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) o[r] = raw_f32<T>(vo[r]);
+            dr_put4<NPL, DR_C, 16>(sO, c, row0, o[0], o[1], o[2], o[3]);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) o[r] *= p.scale * start[r];
+            dr_put4<3, DR_C, 16>(sW, c, row0, o[0], o[1], o[2], o[3]);
+        };
+        auto put_k = [&](int ch) {
+            put_rows(sK, kr);
+            if (tid < HELIX_DR_DECAY / 16) *reinterpret_cast<f32x4*>(&sDec[ch & 1][4 * tid]) = dec;
+        };
+        f32x4 po, qw[NT];
+        auto form = [&] {
+            DrAcc a0, a1[NT];
+#pragma unroll
+            for (int ks = 0; ks < 2; ++ks) {
+                bf16x8 b[3];
+                if (ks == 1 || w < 2) {
+                    bf16x8 o[NPL];
+                    dr_get8<NPL, DR_C, 16>(sO, c, 32 * ks + 8 * q, o);
+                    dr_mfma<3, NPL>(pf[ks], o, a0);
+                }
+                dr_get8<3, DR_C, 16>(sW, c, 32 * ks + 8 * q, b);
+#pragma unroll
+                for (int i = 0; i < NT; ++i) {
+                    bf16x8 a[NPL];
+                    dr_get8_t<NPL, NK, DR_C>(sQ, 32 * ks + 8 * q, NT * 16 * w + 16 * i, c, a);
+                    dr_mfma<NPL, 3>(a, b, a1[i]);
+                }
+            }
+            po = a0.sum();
+#pragma unroll
+            for (int i = 0; i < NT; ++i) qw[i] = a1[i].sum();
+        };
+        auto leave = [&] {
+            sPO[w][lane] = po;
+#pragma unroll
+            for (int i = 0; i < NT; ++i) sQW[i][w][lane] = qw[i];
+        };
+        load_q(last);
+        load_k(last);
+        put_q();
+        put_k(last);
+        load_q(last - 1);
+        dr_barrier();
+        form();
+        leave();
+        load_k(last - 1);
+        for (int ch = last; ch >= 0; --ch) {
+            dr_barrier();   // K, E and what does not depend on E are there
+            if (ch) put_q();
+            load_q(ch - 2);
+            dr_barrier();   // dD is there; K has been read
+            if (ch) form();
+            put_k(ch - 1);
+            load_k(ch - 2);
+            dr_barrier();   // dV is there
+            const f32x4 Z = sPO[w][lane], beta = *reinterpret_cast<const f32x4*>(&sDec[ch & 1][128 + row0]);
+            const Rows<float> rz(p.keep_z, (base + ch) * DR_C * P, P, DR_C, P);
+            const Rows<T> rv(p.dv, (((long long)seq * p.n_tok + first(ch)) * p.n_head + h) * P, (long long)p.n_head * P, tokens(ch), P);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                rz.store(row0 + r, p0 + c, Z[r]);
+                rv.store(row0 + r, p0 + c, Z[r] * beta[r]);
+            }
+            if (ch) leave();
+        }
+        return;
+    }
+
     auto state_off = [&](int i, int r) {
         const int n = NT * 16 * w + 16 * i + 4 * q + r;
         return n < N && p0 + c < P ? (n * P + p0 + c) * 4 : (int)0x80000000;
     };
-    auto put_state = [&](const f32x4 (&S)[NT], helix_rsrc r0) {
+    f32x4 E[NT];
+    auto put_state = [&](helix_rsrc r0) {
 #pragma unroll
         for (int i = 0; i < NT; ++i)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) __builtin_amdgcn_raw_buffer_store_b32(as_u32(S[i][r]), r0, state_off(i, r), 0, 0);
+            for (int r = 0; r < 4; ++r) __builtin_amdgcn_raw_buffer_store_b32(as_u32(E[i][r]), r0, state_off(i, r), 0, 0);
     };
-    f32x4 E[NT];
+    auto put_e = [&] {
+#pragma unroll
+        for (int i = 0; i < NT; ++i)
+            dr_put4<3, NK, 16>(sE, c, NT * 16 * w + 16 * i + 4 * q, E[i][0], E[i][1], E[i][2], E[i][3]);
+    };
+    bf16x8 tf[2][3];
+    auto load_t = [&](int ch) {
+        const char* tt = p.tt + (base + max(ch, 0)) * (6 * 3 * HELIX_DR_FRAG) + 16 * lane;
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks) {
+            if (ks == 0 && w > 1) continue;
+#pragma unroll
+            for (int k = 0; k < 3; ++k) tf[ks][k] = *reinterpret_cast<const bf16x8*>(tt + (dr_up(w, ks) * 3 + k) * HELIX_DR_FRAG);
+        }
+    };
     {
         const helix_rsrc r0 = make_rsrc_u(p.d_s + (long long)sh * N * P, p.d_s ? state_bytes : 0u);   // none: reads 0
 #pragma unroll
@@ -600,133 +736,63 @@ __device__ void delta_back(const HelixDeltaParams& p) {
 #pragma unroll
             for (int r = 0; r < 4; ++r) E[i][r] = buf_f32(r0, state_off(i, r), 0);
     }
-    constexpr int PER = DR_C * (NK / 8) / 256;
-    struct Ahead {
-        Raw8<T> k[PER], q[PER];
-        bf16x8 t[2][3], p[2][3];
-        unsigned o[4];
-        f32x4 start, left, beta;
-        float all;
-    } next;
-    auto load = [&](int ch) {
-        const long long t0 = (long long)(p.chunk0 + ch) * DR_C;
-        const int len = (int)min((long long)DR_C, p.n_tok - t0);
-        const Rows<T, ODD> rk(p.k, seq * p.seq_k + hk * p.head_k + t0 * p.tok_k, p.tok_k, len, N);
-        const Rows<T, ODD> rq(p.q, seq * p.seq_q + hk * p.head_q + t0 * p.tok_q, p.tok_q, len, N);
-        const Rows<T> ro(p.d_o, seq * p.seq_o + h * p.head_o + t0 * p.tok_o, p.tok_o, len, P);
-#pragma unroll
-        for (int i = 0; i < PER; ++i) {
-            const int row = (tid + 256 * i) / (NK / 8), col = 8 * ((tid + 256 * i) % (NK / 8));
-            next.k[i] = rk.load8(row, col);
-            next.q[i] = rq.load8(row, col);
-        }
-        const long long at = (long long)sh * p.n_chunk + ch;
-        const char* tt = p.tt + at * (6 * 3 * HELIX_DR_FRAG) + 16 * lane;
-        const char* pt = p.pt + at * (6 * 3 * HELIX_DR_FRAG) + 16 * lane;
-#pragma unroll
-        for (int ks = 0; ks < 2; ++ks) {
-            if (ks == 0 && w > 1) continue;
-#pragma unroll
-            for (int k = 0; k < 3; ++k) {
-                next.t[ks][k] = *reinterpret_cast<const bf16x8*>(tt + (dr_up(w, ks) * 3 + k) * HELIX_DR_FRAG);
-                next.p[ks][k] = *reinterpret_cast<const bf16x8*>(pt + (dr_up(w, ks) * 3 + k) * HELIX_DR_FRAG);
-            }
-        }
-#pragma unroll
-        for (int r = 0; r < 4; ++r) next.o[r] = ro.raw(row0 + r, p0 + c);
-        const float* dec = p.decay + at * (HELIX_DR_DECAY / 4);
-        next.start = *reinterpret_cast<const f32x4*>(dec + row0);
-        next.left = *reinterpret_cast<const f32x4*>(dec + 64 + row0);
-        next.beta = *reinterpret_cast<const f32x4*>(dec + 128 + row0);
-        next.all = dec[63];
-    };
-    if (p.n_chunk) load(p.n_chunk - 1);
-    for (int ch = p.n_chunk - 1; ch >= 0; --ch) {
-        const Ahead now = next;
-#pragma unroll
-        for (int i = 0; i < PER; ++i) {
-            const int row = (tid + 256 * i) / (NK / 8), col = 8 * ((tid + 256 * i) % (NK / 8));
-            bf16x8 k[NPL], qq[NPL];
-            dr_operand<T>(now.k[i], N - col, k);
-            dr_operand<T>(now.q[i], N - col, qq);
-            dr_put8<NPL, NK, DR_C>(sK, row, col, k);
-            dr_put8<NPL, NK, DR_C>(sQ, row, col, qq);
-        }
-        {
-            float o[4];
-#pragma unroll
-            for (int r = 0; r < 4; ++r) o[r] = raw_f32<T>(now.o[r]);
-            dr_put4<NPL, DR_C, 16>(sO, c, row0, o[0], o[1], o[2], o[3]);
-#pragma unroll
-            for (int r = 0; r < 4; ++r) o[r] *= p.scale * now.start[r];
-            dr_put4<3, DR_C, 16>(sW, c, row0, o[0], o[1], o[2], o[3]);
-        }
-#pragma unroll
-        for (int i = 0; i < NT; ++i)
-            dr_put4<3, NK, 16>(sE, c, NT * 16 * w + 16 * i + 4 * q, E[i][0], E[i][1], E[i][2], E[i][3]);
-        if (ch) load(ch - 1);
-        const long long at = (long long)sh * p.n_chunk + ch;
-        const long long t0 = (long long)(p.chunk0 + ch) * DR_C;
-        const int len = (int)min((long long)DR_C, p.n_tok - t0);
-        __syncthreads();
-        put_state(E, make_rsrc_u(p.keep_e + at * N * P, state_bytes));
-        f32x4 ke = zero4();
+    if (last >= 0) {
+        load_t(last);
+        put_e();
+        dr_barrier();
+    }
+    for (int ch = last; ch >= 0; --ch) {
+        dr_barrier();   // K, E and what does not depend on E are there
+        put_state(make_rsrc_u(p.keep_e + (base + ch) * N * P, state_bytes));
+        const float* const dec = sDec[ch & 1];
+        DrAcc ke;
 #pragma unroll
         for (int s = 0; s < KS; ++s) {
             const int col = 32 * s + 8 * q;
             bf16x8 a[NPL], b[3];
             dr_get8<NPL, NK, DR_C>(sK, 16 * w + c, col, a);
             dr_get8<3, NK, 16>(sE, c, col, b);
-            ke = dr_mfma<NPL, 3>(a, b, ke);
+            dr_mfma<NPL, 3>(a, b, ke);
         }
-        f32x4 dd = ke * now.left;
+        bf16x8 kt[2][NT][NPL];
 #pragma unroll
-        for (int ks = 0; ks < 2; ++ks) {
-            if (ks == 0 && w > 1) continue;
-            bf16x8 b[NPL];
-            dr_get8<NPL, DR_C, 16>(sO, c, 32 * ks + 8 * q, b);
-            dd = dr_mfma<3, NPL>(now.p[ks], b, dd);
-        }
+        for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+            for (int i = 0; i < NT; ++i) dr_get8_t<NPL, NK, DR_C>(sK, 32 * ks + 8 * q, NT * 16 * w + 16 * i, c, kt[ks][i]);
+        f32x4 qw[NT];
+#pragma unroll
+        for (int i = 0; i < NT; ++i) qw[i] = sQW[i][w][lane];
+        const f32x4 dd = ke.sum() * *reinterpret_cast<const f32x4*>(dec + 64 + row0) + sPO[w][lane];
         dr_put4<3, DR_C, 16>(sR, c, row0, dd[0], dd[1], dd[2], dd[3]);
-        __syncthreads();
-        f32x4 Z = zero4();
+        dr_barrier();   // dD is there; K has been read
+        DrAcc zs;
 #pragma unroll
         for (int ks = 0; ks < 2; ++ks) {
             if (ks == 0 && w > 1) continue;
             bf16x8 b[3];
             dr_get8<3, DR_C, 16>(sR, c, 32 * ks + 8 * q, b);
-            Z = dr_mfma<3, 3>(now.t[ks], b, Z);
+            dr_mfma<3, 3>(tf[ks], b, zs);
         }
-        const f32x4 dv = Z * now.beta;
-        const f32x4 u = -(dv * now.start);
+        const f32x4 Z = zs.sum();
+        const f32x4 u = -(Z * *reinterpret_cast<const f32x4*>(dec + 128 + row0) * *reinterpret_cast<const f32x4*>(dec + row0));
         dr_put4<3, DR_C, 16>(sU, c, row0, u[0], u[1], u[2], u[3]);
-        const Rows<float> rz(p.keep_z, at * DR_C * P, P, DR_C, P);
-        const Rows<T> rv(p.dv, (((long long)seq * p.n_tok + t0) * p.n_head + h) * P, (long long)p.n_head * P, len, P);
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            rz.store(row0 + r, p0 + c, Z[r]);
-            rv.store(row0 + r, p0 + c, dv[r]);
-        }
-        __syncthreads();
-#pragma unroll
-        for (int i = 0; i < NT; ++i) E[i] *= now.all;
+        sPO[w][lane] = Z;
+        load_t(ch - 1);
+        const float all = dec[63];
+        dr_barrier();   // dV is there
+        DrAcc up[NT];
 #pragma unroll
         for (int ks = 0; ks < 2; ++ks) {
-            bf16x8 bw[3], bu[3];
-            dr_get8<3, DR_C, 16>(sW, c, 32 * ks + 8 * q, bw);
-            dr_get8<3, DR_C, 16>(sU, c, 32 * ks + 8 * q, bu);
+            bf16x8 b[3];
+            dr_get8<3, DR_C, 16>(sU, c, 32 * ks + 8 * q, b);
 #pragma unroll
-            for (int i = 0; i < NT; ++i) {
-                bf16x8 a[NPL];
-                dr_get8_t<NPL, NK, DR_C>(sQ, 32 * ks + 8 * q, NT * 16 * w + 16 * i, c, a);
-                E[i] = dr_mfma<NPL, 3>(a, bw, E[i]);
-                dr_get8_t<NPL, NK, DR_C>(sK, 32 * ks + 8 * q, NT * 16 * w + 16 * i, c, a);
-                E[i] = dr_mfma<NPL, 3>(a, bu, E[i]);
-            }
+            for (int i = 0; i < NT; ++i) dr_mfma<NPL, 3>(kt[ks][i], b, up[i]);
         }
-        __syncthreads();   // K, Q and the operands are written again
+#pragma unroll
+        for (int i = 0; i < NT; ++i) E[i] = all * E[i] + (qw[i] + up[i].sum());
+        put_e();
     }
-    put_state(E, make_rsrc_u(p.ds0 + (long long)sh * N * P, state_bytes));
+    put_state(make_rsrc_u(p.ds0 + (long long)sh * N * P, state_bytes));
 }
 
 // The other gradients, a chunk of a head of queries and keys a workgroup, its value heads one
@@ -1136,7 +1202,7 @@ __device__ void delta_grad(const HelixDeltaParams& p) {
     extern "C" __global__ __launch_bounds__(512) void helix_delta_walk_##TAG##_##NK##SUF(HelixDeltaParams p) { delta_walk<T, NK, ODD, false>(p); }    \
     extern "C" __global__ __launch_bounds__(256) void helix_delta_prep_bwd_##TAG##_##NK##SUF(HelixDeltaParams p) { delta_prep<T, NK, ODD, true>(p); } \
     extern "C" __global__ __launch_bounds__(512) void helix_delta_keep_##TAG##_##NK##SUF(HelixDeltaParams p) { delta_walk<T, NK, ODD, true>(p); }     \
-    extern "C" __global__ __launch_bounds__(256) void helix_delta_back_##TAG##_##NK##SUF(HelixDeltaParams p) { delta_back<T, NK, ODD>(p); }           \
+    extern "C" __global__ __launch_bounds__(512) void helix_delta_back_##TAG##_##NK##SUF(HelixDeltaParams p) { delta_back<T, NK, ODD>(p); }           \
     extern "C" __global__ __launch_bounds__(640) void helix_delta_pairs_##TAG##_##NK##SUF(HelixDeltaParams p) { delta_pairs<T, NK, ODD>(p); }                   \
     extern "C" __global__ __launch_bounds__(512) void helix_delta_grad_##TAG##_##NK##SUF(HelixDeltaParams p) { delta_grad<T, NK, ODD>(p); }
 DR_STEPS(f32, float, 64)

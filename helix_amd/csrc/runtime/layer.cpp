@@ -1104,7 +1104,7 @@ extern "C" helix_status helix_delta_rule_backward_encode(helix_ctx* ctx, void* s
         grid(sk * plan.chunks, kDeltaPairThreads);
         const OnDevice on(ctx->device);
         if (!a->n_tok) {
-            launch(back, stream, gw, 1, kDeltaThreads, p);
+            launch(back, stream, gw, 1, 2 * kDeltaThreads, p);
             return;
         }
         const size_t state = ((size_t)sh * a->n_key * a->n_val * 4 + 255) & ~(size_t)255;
@@ -1124,7 +1124,7 @@ extern "C" helix_status helix_delta_rule_backward_encode(helix_ctx* ctx, void* s
         p.s = nullptr;
         for (int i = plan.n_seg - 1; i >= 0; --i) {
             states(i);
-            launch(back, stream, gw, 1, kDeltaThreads, p);
+            launch(back, stream, gw, 1, 2 * kDeltaThreads, p);
             launch(pairs, stream, (unsigned)(sk * p.n_chunk), 1, kDeltaPairThreads, p);
             launch(grad, stream, (unsigned)(sk * p.n_chunk), 1, 2 * kDeltaThreads, p);
             p.d_s = p.ds0;   // the segment before goes on from here
