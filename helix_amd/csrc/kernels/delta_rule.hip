@@ -363,8 +363,9 @@ __device__ void delta_walk(const HelixDeltaParams& p) {
         constexpr int PER = DR_C * (NK / 8) / 256;
         Raw8<T> kr[PER], vr;
         f32x4 dec;
-        const int vrow = (tid >> 1) & 63, vcol = 8 * (tid & 1);
+        // (The addresses of all this are formed where they are used: kept, they would take a second workgroup's registers.)
         auto load_k = [&](int ch) {
+            const int tid = vgpr_fresh(threadIdx.x) & 255, vrow = (tid >> 1) & 63, vcol = 8 * (tid & 1);
             ch = min(ch, last);
             const Rows<T, ODD> rk(p.k, seq * p.seq_k + hk * p.head_k + first(ch) * p.tok_k, p.tok_k, tokens(ch), N);
             const Rows<T, ODD> rv(p.v, seq * p.seq_v + h * p.head_v + first(ch) * p.tok_v, p.tok_v, tokens(ch), P);
@@ -375,6 +376,7 @@ __device__ void delta_walk(const HelixDeltaParams& p) {
                 dec = *reinterpret_cast<const f32x4*>(p.decay + (base + ch) * (HELIX_DR_DECAY / 4) + 4 * (tid - 128));
         };
         auto put_k = [&](int ch) {
+            const int tid = vgpr_fresh(threadIdx.x) & 255, vrow = (tid >> 1) & 63, vcol = 8 * (tid & 1);
 #pragma unroll
             for (int i = 0; i < PER; ++i) {
                 const int row = (tid + 256 * i) / (NK / 8), col = 8 * ((tid + 256 * i) % (NK / 8));
@@ -387,6 +389,7 @@ __device__ void delta_walk(const HelixDeltaParams& p) {
         };
         // What a chunk left in sOut, by the lanes that have V's places.
         auto store_out = [&](int ch) {
+            const int tid = vgpr_fresh(threadIdx.x) & 255, vrow = (tid >> 1) & 63, vcol = 8 * (tid & 1);
             if (tid >= 128) return;
             const Raw8<Out> v = *reinterpret_cast<const Raw8<Out>*>(&sOut[vrow][vcol]);
             if constexpr (KEEP) {
@@ -399,6 +402,7 @@ __device__ void delta_walk(const HelixDeltaParams& p) {
         Raw8<T> qr[KS];
         bf16x8 pf[2][NO];
         auto load_q = [&](int ch) {
+            const int tid = vgpr_fresh(threadIdx.x) & 255, c = tid & 15, q = (tid & 63) >> 4;
             ch = min(ch, last);
             const Rows<T, ODD> rq(p.q, seq * p.seq_q + hk * p.head_q + first(ch) * p.tok_q, p.tok_q, tokens(ch), N);
 #pragma unroll
@@ -597,7 +601,9 @@ __device__ void delta_back(const HelixDeltaParams& p) {
         bf16x8 pf[2][3];
         unsigned vo[4];
         f32x4 start, dec;
+        // (The addresses of all this are formed where they are used: kept, they would take a second workgroup's registers.)
         auto load_q = [&](int ch) {   // Q's rows, dO and its decays
+            const int tid = vgpr_fresh(threadIdx.x) & 255, c = tid & 15, row0 = tid >> 4 << 2;
             ch = max(ch, 0);
             const Rows<T, ODD> rq(p.q, seq * p.seq_q + hk * p.head_q + first(ch) * p.tok_q, p.tok_q, tokens(ch), N);
             const Rows<T> ro(p.d_o, seq * p.seq_o + h * p.head_o + first(ch) * p.tok_o, p.tok_o, tokens(ch), P);
@@ -608,6 +614,7 @@ __device__ void delta_back(const HelixDeltaParams& p) {
             start = *reinterpret_cast<const f32x4*>(p.decay + (base + ch) * (HELIX_DR_DECAY / 4) + row0);
         };
         auto load_k = [&](int ch) {   // K's rows, all decays, and the fragments of P'
+            const int tid = vgpr_fresh(threadIdx.x) & 255, lane = tid & 63;
             ch = max(ch, 0);
             const Rows<T, ODD> rk(p.k, seq * p.seq_k + hk * p.head_k + first(ch) * p.tok_k, p.tok_k, tokens(ch), N);
 #pragma unroll
@@ -622,6 +629,7 @@ __device__ void delta_back(const HelixDeltaParams& p) {
             }
         };
         auto put_rows = [&](__bf16* to, const Raw8<T> (&v)[PER]) {
+            const int tid = vgpr_fresh(threadIdx.x) & 255;
 #pragma unroll
             for (int i = 0; i < PER; ++i) {
                 const int row = (tid + 256 * i) / (NK / 8), col = 8 * ((tid + 256 * i) % (NK / 8));
@@ -632,6 +640,7 @@ __device__ void delta_back(const HelixDeltaParams& p) {
         };
         auto put_q = [&] {
             put_rows(sQ, qr);
+            const int tid = vgpr_fresh(threadIdx.x) & 255, c = tid & 15, row0 = tid >> 4 << 2;
             float o[4];
 #pragma unroll
             for (int r = 0; r < 4; ++r) o[r] = raw_f32<T>(vo[r]);
@@ -646,26 +655,26 @@ __device__ void delta_back(const HelixDeltaParams& p) {
         };
         f32x4 po, qw[NT];
         auto form = [&] {
-            DrAcc a0, a1[NT];
+            const int fresh = vgpr_fresh(lane), c = fresh & 15, q = fresh >> 4;   // (addresses are formed here)
+            po = zero4();
+#pragma unroll
+            for (int i = 0; i < NT; ++i) qw[i] = zero4();
 #pragma unroll
             for (int ks = 0; ks < 2; ++ks) {
                 bf16x8 b[3];
                 if (ks == 1 || w < 2) {
                     bf16x8 o[NPL];
                     dr_get8<NPL, DR_C, 16>(sO, c, 32 * ks + 8 * q, o);
-                    dr_mfma<3, NPL>(pf[ks], o, a0);
+                    po = dr_mfma<3, NPL>(pf[ks], o, po);
                 }
                 dr_get8<3, DR_C, 16>(sW, c, 32 * ks + 8 * q, b);
 #pragma unroll
                 for (int i = 0; i < NT; ++i) {
                     bf16x8 a[NPL];
                     dr_get8_t<NPL, NK, DR_C>(sQ, 32 * ks + 8 * q, NT * 16 * w + 16 * i, c, a);
-                    dr_mfma<NPL, 3>(a, b, a1[i]);
+                    qw[i] = dr_mfma<NPL, 3>(a, b, qw[i]);
                 }
             }
-            po = a0.sum();
-#pragma unroll
-            for (int i = 0; i < NT; ++i) qw[i] = a1[i].sum();
         };
         auto leave = [&] {
             sPO[w][lane] = po;
@@ -690,6 +699,7 @@ __device__ void delta_back(const HelixDeltaParams& p) {
             put_k(ch - 1);
             load_k(ch - 2);
             dr_barrier();   // dV is there
+            const int tid = vgpr_fresh(threadIdx.x) & 255, lane = tid & 63, c = tid & 15, row0 = tid >> 4 << 2;
             const f32x4 Z = sPO[w][lane], beta = *reinterpret_cast<const f32x4*>(&sDec[ch & 1][128 + row0]);
             const Rows<float> rz(p.keep_z, (base + ch) * DR_C * P, P, DR_C, P);
             const Rows<T> rv(p.dv, (((long long)seq * p.n_tok + first(ch)) * p.n_head + h) * P, (long long)p.n_head * P, tokens(ch), P);
