@@ -335,23 +335,23 @@ __device__ void delta_prep(const HelixDeltaParams& p) {
 // wait for one another.
 // KEEP: no outputs and no waves for them; the states before the chunks and D are stored (fp32)
 // for the backward pass.
-template <typename T, int NK, bool ODD, bool KEEP>
+template <typename T, int NK, bool ODD, bool KEEP, int NC>
 __device__ void delta_walk(const HelixDeltaParams& p) {
     constexpr int NPL = dr_planes<T>, NO = dr_out_planes<T>, NT = NK / 64, KS = NK / 32;
-    constexpr int VP = 16 + 16 / sizeof(T);   // rows of V and of outputs in LDS
+    constexpr int COLS = 16 * NC, VP = COLS + 16 / sizeof(T);   // columns of the workgroup; rows of V and of outputs in LDS
     __shared__ __attribute__((aligned(16))) __bf16 sK[NPL * DR_C * NK];
-    __shared__ __attribute__((aligned(16))) __bf16 sS[3 * 16 * NK];
-    __shared__ __attribute__((aligned(16))) __bf16 sR[3 * 16 * DR_C], sU[3 * 16 * DR_C], sD[KEEP ? 8 : NO * 16 * DR_C];
+    __shared__ __attribute__((aligned(16))) __bf16 sS[3 * COLS * NK];
+    __shared__ __attribute__((aligned(16))) __bf16 sR[3 * COLS * DR_C], sU[3 * COLS * DR_C], sD[KEEP ? 8 : NO * COLS * DR_C];
     __shared__ __attribute__((aligned(16))) T sV[DR_C][VP];
     __shared__ __attribute__((aligned(16))) float sDec[2][HELIX_DR_DECAY / 4];
     typedef typename std::conditional<KEEP, float, T>::type Out;   // D, or o
-    __shared__ __attribute__((aligned(16))) Out sOut[DR_C][16 + 16 / sizeof(Out)];
+    __shared__ __attribute__((aligned(16))) Out sOut[DR_C][COLS + 16 / sizeof(Out)];
     const int tid = threadIdx.x & 255, lane = lane_id(), w = wave_uniform() & 3, c = lane & 15, q = lane >> 4;
     const unsigned id = xcd_logical_id(blockIdx.x, gridDim.x);   // a head's slices share an XCD's cache
     const int slice = (int)(id % (unsigned)p.n_slice);
     const unsigned sh = id / (unsigned)p.n_slice;
     const int seq = (int)(sh / (unsigned)p.n_head), h = (int)(sh % (unsigned)p.n_head), hk = h / p.share;
-    const int p0 = 16 * slice, P = p.n_val, N = p.n_key;
+    const int p0 = COLS * slice, P = p.n_val, N = p.n_key;
     const unsigned state_bytes = (unsigned)N * (unsigned)P * 4u;
     const int row0 = 16 * w + 4 * q, last = p.n_chunk - 1;
     const long long base = (long long)sh * p.n_chunk;
@@ -359,24 +359,24 @@ __device__ void delta_walk(const HelixDeltaParams& p) {
     auto tokens = [&](int ch) { return (int)min((long long)DR_C, p.n_tok - first(ch)); };
 
     if (wave_uniform() >= 4) {
-        // K's rows, 16 columns of V's (two lanes a row) and the decays: loaded, and laid out in LDS.
+        // K's rows, the columns of V's (two or four lanes a row) and the decays: loaded, and laid out in LDS.
         constexpr int PER = DR_C * (NK / 8) / 256;
         Raw8<T> kr[PER], vr;
         f32x4 dec;
         // (The addresses of all this are formed where they are used: kept, they would take a second workgroup's registers.)
         auto load_k = [&](int ch) {
-            const int tid = vgpr_fresh(threadIdx.x) & 255, vrow = (tid >> 1) & 63, vcol = 8 * (tid & 1);
+            const int tid = vgpr_fresh(threadIdx.x) & 255, vrow = tid / (2 * NC) & 63, vcol = 8 * (tid % (2 * NC));
             ch = min(ch, last);
             const Rows<T, ODD> rk(p.k, seq * p.seq_k + hk * p.head_k + first(ch) * p.tok_k, p.tok_k, tokens(ch), N);
             const Rows<T, ODD> rv(p.v, seq * p.seq_v + h * p.head_v + first(ch) * p.tok_v, p.tok_v, tokens(ch), P);
 #pragma unroll
             for (int i = 0; i < PER; ++i) kr[i] = rk.load8((tid + 256 * i) / (NK / 8), 8 * ((tid + 256 * i) % (NK / 8)));
-            if (tid < 128) vr = rv.load8(vrow, p0 + vcol);
-            else if (tid < 128 + HELIX_DR_DECAY / 16)
-                dec = *reinterpret_cast<const f32x4*>(p.decay + (base + ch) * (HELIX_DR_DECAY / 4) + 4 * (tid - 128));
+            if (tid < 128 * NC) vr = rv.load8(vrow, p0 + vcol);
+            if (tid >= 256 - HELIX_DR_DECAY / 16)
+                dec = *reinterpret_cast<const f32x4*>(p.decay + (base + ch) * (HELIX_DR_DECAY / 4) + 4 * (tid - (256 - HELIX_DR_DECAY / 16)));
         };
         auto put_k = [&](int ch) {
-            const int tid = vgpr_fresh(threadIdx.x) & 255, vrow = (tid >> 1) & 63, vcol = 8 * (tid & 1);
+            const int tid = vgpr_fresh(threadIdx.x) & 255, vrow = tid / (2 * NC) & 63, vcol = 8 * (tid % (2 * NC));
 #pragma unroll
             for (int i = 0; i < PER; ++i) {
                 const int row = (tid + 256 * i) / (NK / 8), col = 8 * ((tid + 256 * i) % (NK / 8));
@@ -384,13 +384,13 @@ __device__ void delta_walk(const HelixDeltaParams& p) {
                 dr_operand<T>(kr[i], N - col, o);
                 dr_put8<NPL, NK, DR_C>(sK, row, col, o);
             }
-            if (tid < 128) *reinterpret_cast<Raw8<T>*>(&sV[vrow][vcol]) = vr;
-            else if (tid < 128 + HELIX_DR_DECAY / 16) *reinterpret_cast<f32x4*>(&sDec[ch & 1][4 * (tid - 128)]) = dec;
+            if (tid < 128 * NC) *reinterpret_cast<Raw8<T>*>(&sV[vrow][vcol]) = vr;
+            if (tid >= 256 - HELIX_DR_DECAY / 16) *reinterpret_cast<f32x4*>(&sDec[ch & 1][4 * (tid - (256 - HELIX_DR_DECAY / 16))]) = dec;
         };
         // What a chunk left in sOut, by the lanes that have V's places.
         auto store_out = [&](int ch) {
-            const int tid = vgpr_fresh(threadIdx.x) & 255, vrow = (tid >> 1) & 63, vcol = 8 * (tid & 1);
-            if (tid >= 128) return;
+            const int tid = vgpr_fresh(threadIdx.x) & 255, vrow = tid / (2 * NC) & 63, vcol = 8 * (tid % (2 * NC));
+            if (tid >= 128 * NC) return;
             const Raw8<Out> v = *reinterpret_cast<const Raw8<Out>*>(&sOut[vrow][vcol]);
             if constexpr (KEEP) {
                 store8_at<float>(p.keep_d + ((base + ch) * DR_C + vrow) * P + p0 + vcol, v, P - p0 - vcol);
@@ -426,18 +426,23 @@ __device__ void delta_walk(const HelixDeltaParams& p) {
         load_k(1);
         for (int ch = 0; ch <= last; ++ch) {
             dr_barrier();   // K, V and S are there
-            f32x4 o;
+            f32x4 o[NC];
             if constexpr (!KEEP) {
-                DrAcc qs;
+                DrAcc qs[NC];
 #pragma unroll
                 for (int s = 0; s < KS; ++s) {
                     const int col = 32 * s + 8 * q;
                     bf16x8 a[NPL], b[NO];
                     dr_operand<T>(qr[s], N - col, a);
-                    dr_get8<NO, NK, 16>(sS, c, col, b);
-                    dr_mfma<NPL, NO, NO>(a, b, qs);
+#pragma unroll
+                    for (int n = 0; n < NC; ++n) {
+                        dr_get8<NO, NK, COLS>(sS, 16 * n + c, col, b);
+                        dr_mfma<NPL, NO, NO>(a, b, qs[n]);
+                    }
                 }
-                o = qs.sum() * (p.scale * *reinterpret_cast<const f32x4*>(&sDec[ch & 1][row0]));
+                const f32x4 start = p.scale * *reinterpret_cast<const f32x4*>(&sDec[ch & 1][row0]);
+#pragma unroll
+                for (int n = 0; n < NC; ++n) o[n] = qs[n].sum() * start;
                 load_q(ch + 1);
             }
             if (ch) store_out(ch - 1);
@@ -449,13 +454,18 @@ __device__ void delta_walk(const HelixDeltaParams& p) {
 #pragma unroll
                 for (int ks = 0; ks < 2; ++ks) {
                     if (ks && w < 2) break;
-                    bf16x8 b[NO];
-                    dr_get8<NO, DR_C, 16>(sD, c, 32 * ks + 8 * q, b);
-                    o = dr_mfma<NO, NO, NO>(pf[ks], b, o);
+#pragma unroll
+                    for (int n = 0; n < NC; ++n) {
+                        bf16x8 b[NO];
+                        dr_get8<NO, DR_C, COLS>(sD, 16 * n + c, 32 * ks + 8 * q, b);
+                        o[n] = dr_mfma<NO, NO, NO>(pf[ks], b, o[n]);
+                    }
                 }
                 load_p(ch + 1);
 #pragma unroll
-                for (int r = 0; r < 4; ++r) sOut[row0 + r][c] = (T)o[r];
+                for (int n = 0; n < NC; ++n)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) sOut[row0 + r][16 * n + c] = (T)o[n][r];
             }
         }
         dr_barrier();   // the last outputs are there
@@ -463,13 +473,21 @@ __device__ void delta_walk(const HelixDeltaParams& p) {
         return;
     }
 
-    // Register r of tile i: S[n = NT 16 w + 16 i + 4 q + r][p0 + c].
-    auto state_off = [&](int i, int r) {
-        const int n = NT * 16 * w + 16 * i + 4 * q + r;
-        return n < N && p0 + c < P ? (n * P + p0 + c) * 4 : (int)0x80000000;
+    // Register r of tile i, columns n: S[NT 16 w + 16 i + 4 q + r][p0 + 16 n + c].
+    auto state_off = [&](int i, int n, int r) {
+        const int row = NT * 16 * w + 16 * i + 4 * q + r, col = p0 + 16 * n + c;
+        return row < N && col < P ? (row * P + col) * 4 : (int)0x80000000;
     };
-    f32x4 S[NT];
+    f32x4 S[NT][NC];
     bf16x8 xf[2][3];
+    auto put_state = [&](helix_rsrc to) {
+#pragma unroll
+        for (int i = 0; i < NT; ++i)
+#pragma unroll
+            for (int n = 0; n < NC; ++n)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) __builtin_amdgcn_raw_buffer_store_b32(as_u32(S[i][n][r]), to, state_off(i, n, r), 0, 0);
+    };
     auto load_x = [&](int ch) {
         const char* x = p.x + (base + min(ch, last)) * (6 * 3 * HELIX_DR_FRAG) + 16 * lane;
 #pragma unroll
@@ -482,35 +500,36 @@ __device__ void delta_walk(const HelixDeltaParams& p) {
     auto put_s = [&] {
 #pragma unroll
         for (int i = 0; i < NT; ++i)
-            dr_put4<3, NK, 16>(sS, c, NT * 16 * w + 16 * i + 4 * q, S[i][0], S[i][1], S[i][2], S[i][3]);
+#pragma unroll
+            for (int n = 0; n < NC; ++n)
+                dr_put4<3, NK, COLS>(sS, 16 * n + c, NT * 16 * w + 16 * i + 4 * q, S[i][n][0], S[i][n][1], S[i][n][2], S[i][n][3]);
     };
     {
         const helix_rsrc r0 = make_rsrc_u(p.s0 + (long long)sh * N * P, p.s0 ? state_bytes : 0u);   // none: reads 0
 #pragma unroll
         for (int i = 0; i < NT; ++i)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) S[i][r] = buf_f32(r0, state_off(i, r), 0);
+            for (int n = 0; n < NC; ++n)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) S[i][n][r] = buf_f32(r0, state_off(i, n, r), 0);
     }
     load_x(0);
     put_s();
     for (int ch = 0; ch <= last; ++ch) {
         dr_barrier();   // K, V and S are there
-        if constexpr (KEEP) {
-            const helix_rsrc rs = make_rsrc_u(p.keep_s + (base + ch) * N * P, state_bytes);
-#pragma unroll
-            for (int i = 0; i < NT; ++i)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) __builtin_amdgcn_raw_buffer_store_b32(as_u32(S[i][r]), rs, state_off(i, r), 0, 0);
-        }
+        if constexpr (KEEP) put_state(make_rsrc_u(p.keep_s + (base + ch) * N * P, state_bytes));
         const float* const dec = sDec[ch & 1];
-        DrAcc ks_;
+        DrAcc ks_[NC];
 #pragma unroll
         for (int s = 0; s < KS; ++s) {
             const int col = 32 * s + 8 * q;
             bf16x8 a[NPL], b[3];
             dr_get8<NPL, NK, DR_C>(sK, 16 * w + c, col, a);
-            dr_get8<3, NK, 16>(sS, c, col, b);
-            dr_mfma<NPL, 3>(a, b, ks_);
+#pragma unroll
+            for (int n = 0; n < NC; ++n) {
+                dr_get8<3, NK, COLS>(sS, 16 * n + c, col, b);
+                dr_mfma<NPL, 3>(a, b, ks_[n]);
+            }
         }
         bf16x8 kt[2][NT][NPL];
 #pragma unroll
@@ -518,51 +537,58 @@ __device__ void delta_walk(const HelixDeltaParams& p) {
 #pragma unroll
             for (int i = 0; i < NT; ++i) dr_get8_t<NPL, NK, DR_C>(sK, 32 * ks + 8 * q, NT * 16 * w + 16 * i, c, kt[ks][i]);
         const f32x4 start = *reinterpret_cast<const f32x4*>(dec + row0);
-        f32x4 R = ks_.sum();
 #pragma unroll
-        for (int r = 0; r < 4; ++r) R[r] = (float)sV[row0 + r][c] - start[r] * R[r];
-        dr_put4<3, DR_C, 16>(sR, c, row0, R[0], R[1], R[2], R[3]);
+        for (int n = 0; n < NC; ++n) {
+            f32x4 R = ks_[n].sum();
+#pragma unroll
+            for (int r = 0; r < 4; ++r) R[r] = (float)sV[row0 + r][16 * n + c] - start[r] * R[r];
+            dr_put4<3, DR_C, COLS>(sR, 16 * n + c, row0, R[0], R[1], R[2], R[3]);
+        }
         dr_barrier();   // R is there; K and V have been read
-        DrAcc ds;
+        DrAcc ds[NC];
 #pragma unroll
         for (int ks = 0; ks < 2; ++ks) {
             if (ks && w < 2) break;
-            bf16x8 b[3];
-            dr_get8<3, DR_C, 16>(sR, c, 32 * ks + 8 * q, b);
-            dr_mfma<3, 3>(xf[ks], b, ds);
+#pragma unroll
+            for (int n = 0; n < NC; ++n) {
+                bf16x8 b[3];
+                dr_get8<3, DR_C, COLS>(sR, 16 * n + c, 32 * ks + 8 * q, b);
+                dr_mfma<3, 3>(xf[ks], b, ds[n]);
+            }
         }
         const f32x4 left = *reinterpret_cast<const f32x4*>(dec + 64 + row0);
-        const f32x4 D = ds.sum();
-        dr_put4<3, DR_C, 16>(sU, c, row0, D[0] * left[0], D[1] * left[1], D[2] * left[2], D[3] * left[3]);
-        if constexpr (KEEP) {
 #pragma unroll
-            for (int r = 0; r < 4; ++r) sOut[row0 + r][c] = D[r];
-        } else {
-            dr_put4<NO, DR_C, 16>(sD, c, row0, D[0], D[1], D[2], D[3]);
+        for (int n = 0; n < NC; ++n) {
+            const f32x4 D = ds[n].sum();
+            dr_put4<3, DR_C, COLS>(sU, 16 * n + c, row0, D[0] * left[0], D[1] * left[1], D[2] * left[2], D[3] * left[3]);
+            if constexpr (KEEP) {
+#pragma unroll
+                for (int r = 0; r < 4; ++r) sOut[row0 + r][16 * n + c] = D[r];
+            } else {
+                dr_put4<NO, DR_C, COLS>(sD, 16 * n + c, row0, D[0], D[1], D[2], D[3]);
+            }
         }
         load_x(ch + 1);
         const float all = dec[63];
         dr_barrier();   // D is there
-        DrAcc up[NT];
+        DrAcc up[NT][NC];
 #pragma unroll
-        for (int ks = 0; ks < 2; ++ks) {
-            bf16x8 b[3];
-            dr_get8<3, DR_C, 16>(sU, c, 32 * ks + 8 * q, b);
+        for (int ks = 0; ks < 2; ++ks)
 #pragma unroll
-            for (int i = 0; i < NT; ++i) dr_mfma<NPL, 3>(kt[ks][i], b, up[i]);
-        }
+            for (int n = 0; n < NC; ++n) {
+                bf16x8 b[3];
+                dr_get8<3, DR_C, COLS>(sU, 16 * n + c, 32 * ks + 8 * q, b);
 #pragma unroll
-        for (int i = 0; i < NT; ++i) S[i] = all * S[i] + up[i].sum();
-        put_s();
-    }
-    dr_barrier();
-    if (p.s) {
-        const helix_rsrc r1 = make_rsrc_u(p.s + (long long)sh * N * P, state_bytes);
+                for (int i = 0; i < NT; ++i) dr_mfma<NPL, 3>(kt[ks][i], b, up[i][n]);
+            }
 #pragma unroll
         for (int i = 0; i < NT; ++i)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) __builtin_amdgcn_raw_buffer_store_b32(as_u32(S[i][r]), r1, state_off(i, r), 0, 0);
+            for (int n = 0; n < NC; ++n) S[i][n] = all * S[i][n] + up[i][n].sum();
+        put_s();
     }
+    dr_barrier();
+    if (p.s) put_state(make_rsrc_u(p.s + (long long)sh * N * P, state_bytes));
 }
 
 // ---- backward -----------------------------------------------------------------------------
@@ -575,19 +601,19 @@ __device__ void delta_walk(const HelixDeltaParams& p) {
 // second four waves bring K, Q and dO and form what does not wait for E, P' dO and
 // scale (e^G Q)' dO of the chunk after the one that the first four are at. It leaves E and Z for
 // the kernels below.
-template <typename T, int NK, bool ODD>
+template <typename T, int NK, bool ODD, int NC>
 __device__ void delta_back(const HelixDeltaParams& p) {
-    constexpr int NPL = dr_planes<T>, NT = NK / 64, KS = NK / 32;
-    __shared__ __attribute__((aligned(16))) __bf16 sK[NPL * DR_C * NK], sQ[NPL * DR_C * NK], sE[3 * 16 * NK];
-    __shared__ __attribute__((aligned(16))) __bf16 sO[NPL * 16 * DR_C], sW[3 * 16 * DR_C], sR[3 * 16 * DR_C], sU[3 * 16 * DR_C];
-    __shared__ f32x4 sPO[4][64], sQW[NT][4][64];   // P' dO, where Z then is, and Q' (scale e^G dO), as lanes hold them
+    constexpr int NPL = dr_planes<T>, NT = NK / 64, KS = NK / 32, COLS = 16 * NC;
+    __shared__ __attribute__((aligned(16))) __bf16 sK[NPL * DR_C * NK], sQ[NPL * DR_C * NK], sE[3 * COLS * NK];
+    __shared__ __attribute__((aligned(16))) __bf16 sO[NPL * COLS * DR_C], sW[3 * COLS * DR_C], sR[3 * COLS * DR_C], sU[3 * COLS * DR_C];
+    __shared__ f32x4 sPO[NC][4][64], sQW[NC][NT][4][64];   // P' dO, where Z then is, and Q' (scale e^G dO), as lanes hold them
     __shared__ __attribute__((aligned(16))) float sDec[2][HELIX_DR_DECAY / 4];
     const int tid = threadIdx.x & 255, lane = lane_id(), w = wave_uniform() & 3, c = lane & 15, q = lane >> 4;
     const unsigned id = xcd_logical_id(blockIdx.x, gridDim.x);
     const int slice = (int)(id % (unsigned)p.n_slice);
     const unsigned sh = id / (unsigned)p.n_slice;
     const int seq = (int)(sh / (unsigned)p.n_head), h = (int)(sh % (unsigned)p.n_head), hk = h / p.share;
-    const int p0 = 16 * slice, P = p.n_val, N = p.n_key;
+    const int p0 = COLS * slice, P = p.n_val, N = p.n_key;
     const unsigned state_bytes = (unsigned)N * (unsigned)P * 4u;
     const int row0 = 16 * w + 4 * q, last = p.n_chunk - 1;
     const long long base = (long long)sh * p.n_chunk;
@@ -599,7 +625,7 @@ __device__ void delta_back(const HelixDeltaParams& p) {
         constexpr int PER = DR_C * (NK / 8) / 256;
         Raw8<T> kr[PER], qr[PER];
         bf16x8 pf[2][3];
-        unsigned vo[4];
+        unsigned vo[NC][4];
         f32x4 start, dec;
         // (The addresses of all this are formed where they are used: kept, they would take a second workgroup's registers.)
         auto load_q = [&](int ch) {   // Q's rows, dO and its decays
@@ -610,7 +636,9 @@ __device__ void delta_back(const HelixDeltaParams& p) {
 #pragma unroll
             for (int i = 0; i < PER; ++i) qr[i] = rq.load8((tid + 256 * i) / (NK / 8), 8 * ((tid + 256 * i) % (NK / 8)));
 #pragma unroll
-            for (int r = 0; r < 4; ++r) vo[r] = ro.raw(row0 + r, p0 + c);
+            for (int n = 0; n < NC; ++n)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) vo[n][r] = ro.raw(row0 + r, p0 + 16 * n + c);
             start = *reinterpret_cast<const f32x4*>(p.decay + (base + ch) * (HELIX_DR_DECAY / 4) + row0);
         };
         auto load_k = [&](int ch) {   // K's rows, all decays, and the fragments of P'
@@ -641,45 +669,60 @@ __device__ void delta_back(const HelixDeltaParams& p) {
         auto put_q = [&] {
             put_rows(sQ, qr);
             const int tid = vgpr_fresh(threadIdx.x) & 255, c = tid & 15, row0 = tid >> 4 << 2;
-            float o[4];
 #pragma unroll
-            for (int r = 0; r < 4; ++r) o[r] = raw_f32<T>(vo[r]);
-            dr_put4<NPL, DR_C, 16>(sO, c, row0, o[0], o[1], o[2], o[3]);
+            for (int n = 0; n < NC; ++n) {
+                float o[4];
 #pragma unroll
-            for (int r = 0; r < 4; ++r) o[r] *= p.scale * start[r];
-            dr_put4<3, DR_C, 16>(sW, c, row0, o[0], o[1], o[2], o[3]);
+                for (int r = 0; r < 4; ++r) o[r] = raw_f32<T>(vo[n][r]);
+                dr_put4<NPL, DR_C, COLS>(sO, 16 * n + c, row0, o[0], o[1], o[2], o[3]);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) o[r] *= p.scale * start[r];
+                dr_put4<3, DR_C, COLS>(sW, 16 * n + c, row0, o[0], o[1], o[2], o[3]);
+            }
         };
         auto put_k = [&](int ch) {
             put_rows(sK, kr);
             if (tid < HELIX_DR_DECAY / 16) *reinterpret_cast<f32x4*>(&sDec[ch & 1][4 * tid]) = dec;
         };
-        f32x4 po, qw[NT];
+        f32x4 po[NC], qw[NC][NT];
         auto form = [&] {
-            const int fresh = vgpr_fresh(lane), c = fresh & 15, q = fresh >> 4;   // (addresses are formed here)
-            po = zero4();
+            const int fresh = vgpr_fresh(lane), c = fresh & 15, q = fresh >> 4;
 #pragma unroll
-            for (int i = 0; i < NT; ++i) qw[i] = zero4();
+            for (int n = 0; n < NC; ++n) {
+                po[n] = zero4();
+#pragma unroll
+                for (int i = 0; i < NT; ++i) qw[n][i] = zero4();
+            }
 #pragma unroll
             for (int ks = 0; ks < 2; ++ks) {
-                bf16x8 b[3];
                 if (ks == 1 || w < 2) {
-                    bf16x8 o[NPL];
-                    dr_get8<NPL, DR_C, 16>(sO, c, 32 * ks + 8 * q, o);
-                    po = dr_mfma<3, NPL>(pf[ks], o, po);
+#pragma unroll
+                    for (int n = 0; n < NC; ++n) {
+                        bf16x8 o[NPL];
+                        dr_get8<NPL, DR_C, COLS>(sO, 16 * n + c, 32 * ks + 8 * q, o);
+                        po[n] = dr_mfma<3, NPL>(pf[ks], o, po[n]);
+                    }
                 }
-                dr_get8<3, DR_C, 16>(sW, c, 32 * ks + 8 * q, b);
 #pragma unroll
                 for (int i = 0; i < NT; ++i) {
                     bf16x8 a[NPL];
                     dr_get8_t<NPL, NK, DR_C>(sQ, 32 * ks + 8 * q, NT * 16 * w + 16 * i, c, a);
-                    qw[i] = dr_mfma<NPL, 3>(a, b, qw[i]);
+#pragma unroll
+                    for (int n = 0; n < NC; ++n) {
+                        bf16x8 b[3];
+                        dr_get8<3, DR_C, COLS>(sW, 16 * n + c, 32 * ks + 8 * q, b);
+                        qw[n][i] = dr_mfma<NPL, 3>(a, b, qw[n][i]);
+                    }
                 }
             }
         };
         auto leave = [&] {
-            sPO[w][lane] = po;
 #pragma unroll
-            for (int i = 0; i < NT; ++i) sQW[i][w][lane] = qw[i];
+            for (int n = 0; n < NC; ++n) {
+                sPO[n][w][lane] = po[n];
+#pragma unroll
+                for (int i = 0; i < NT; ++i) sQW[n][i][w][lane] = qw[n][i];
+            }
         };
         load_q(last);
         load_k(last);
@@ -700,34 +743,42 @@ __device__ void delta_back(const HelixDeltaParams& p) {
             load_k(ch - 2);
             dr_barrier();   // dV is there
             const int tid = vgpr_fresh(threadIdx.x) & 255, lane = tid & 63, c = tid & 15, row0 = tid >> 4 << 2;
-            const f32x4 Z = sPO[w][lane], beta = *reinterpret_cast<const f32x4*>(&sDec[ch & 1][128 + row0]);
+            const f32x4 beta = *reinterpret_cast<const f32x4*>(&sDec[ch & 1][128 + row0]);
             const Rows<float> rz(p.keep_z, (base + ch) * DR_C * P, P, DR_C, P);
             const Rows<T> rv(p.dv, (((long long)seq * p.n_tok + first(ch)) * p.n_head + h) * P, (long long)p.n_head * P, tokens(ch), P);
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                rz.store(row0 + r, p0 + c, Z[r]);
-                rv.store(row0 + r, p0 + c, Z[r] * beta[r]);
+            for (int n = 0; n < NC; ++n) {
+                const f32x4 Z = sPO[n][w][lane];
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    rz.store(row0 + r, p0 + 16 * n + c, Z[r]);
+                    rv.store(row0 + r, p0 + 16 * n + c, Z[r] * beta[r]);
+                }
             }
             if (ch) leave();
         }
         return;
     }
 
-    auto state_off = [&](int i, int r) {
-        const int n = NT * 16 * w + 16 * i + 4 * q + r;
-        return n < N && p0 + c < P ? (n * P + p0 + c) * 4 : (int)0x80000000;
+    auto state_off = [&](int i, int n, int r) {
+        const int row = NT * 16 * w + 16 * i + 4 * q + r, col = p0 + 16 * n + c;
+        return row < N && col < P ? (row * P + col) * 4 : (int)0x80000000;
     };
-    f32x4 E[NT];
-    auto put_state = [&](helix_rsrc r0) {
+    f32x4 E[NT][NC];
+    auto put_state = [&](helix_rsrc to) {
 #pragma unroll
         for (int i = 0; i < NT; ++i)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) __builtin_amdgcn_raw_buffer_store_b32(as_u32(E[i][r]), r0, state_off(i, r), 0, 0);
+            for (int n = 0; n < NC; ++n)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) __builtin_amdgcn_raw_buffer_store_b32(as_u32(E[i][n][r]), to, state_off(i, n, r), 0, 0);
     };
     auto put_e = [&] {
 #pragma unroll
         for (int i = 0; i < NT; ++i)
-            dr_put4<3, NK, 16>(sE, c, NT * 16 * w + 16 * i + 4 * q, E[i][0], E[i][1], E[i][2], E[i][3]);
+#pragma unroll
+            for (int n = 0; n < NC; ++n)
+                dr_put4<3, NK, COLS>(sE, 16 * n + c, NT * 16 * w + 16 * i + 4 * q, E[i][n][0], E[i][n][1], E[i][n][2], E[i][n][3]);
     };
     bf16x8 tf[2][3];
     auto load_t = [&](int ch) {
@@ -744,7 +795,9 @@ __device__ void delta_back(const HelixDeltaParams& p) {
 #pragma unroll
         for (int i = 0; i < NT; ++i)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) E[i][r] = buf_f32(r0, state_off(i, r), 0);
+            for (int n = 0; n < NC; ++n)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) E[i][n][r] = buf_f32(r0, state_off(i, n, r), 0);
     }
     if (last >= 0) {
         load_t(last);
@@ -755,51 +808,66 @@ __device__ void delta_back(const HelixDeltaParams& p) {
         dr_barrier();   // K, E and what does not depend on E are there
         put_state(make_rsrc_u(p.keep_e + (base + ch) * N * P, state_bytes));
         const float* const dec = sDec[ch & 1];
-        DrAcc ke;
+        DrAcc ke[NC];
 #pragma unroll
         for (int s = 0; s < KS; ++s) {
             const int col = 32 * s + 8 * q;
             bf16x8 a[NPL], b[3];
             dr_get8<NPL, NK, DR_C>(sK, 16 * w + c, col, a);
-            dr_get8<3, NK, 16>(sE, c, col, b);
-            dr_mfma<NPL, 3>(a, b, ke);
+#pragma unroll
+            for (int n = 0; n < NC; ++n) {
+                dr_get8<3, NK, COLS>(sE, 16 * n + c, col, b);
+                dr_mfma<NPL, 3>(a, b, ke[n]);
+            }
         }
         bf16x8 kt[2][NT][NPL];
 #pragma unroll
         for (int ks = 0; ks < 2; ++ks)
 #pragma unroll
             for (int i = 0; i < NT; ++i) dr_get8_t<NPL, NK, DR_C>(sK, 32 * ks + 8 * q, NT * 16 * w + 16 * i, c, kt[ks][i]);
-        f32x4 qw[NT];
+        const f32x4 left = *reinterpret_cast<const f32x4*>(dec + 64 + row0);
 #pragma unroll
-        for (int i = 0; i < NT; ++i) qw[i] = sQW[i][w][lane];
-        const f32x4 dd = ke.sum() * *reinterpret_cast<const f32x4*>(dec + 64 + row0) + sPO[w][lane];
-        dr_put4<3, DR_C, 16>(sR, c, row0, dd[0], dd[1], dd[2], dd[3]);
+        for (int n = 0; n < NC; ++n) {
+#pragma unroll
+            for (int i = 0; i < NT; ++i) E[i][n] = dec[63] * E[i][n] + sQW[n][i][w][lane];
+            const f32x4 dd = ke[n].sum() * left + sPO[n][w][lane];
+            dr_put4<3, DR_C, COLS>(sR, 16 * n + c, row0, dd[0], dd[1], dd[2], dd[3]);
+        }
         dr_barrier();   // dD is there; K has been read
-        DrAcc zs;
+        DrAcc zs[NC];
 #pragma unroll
         for (int ks = 0; ks < 2; ++ks) {
             if (ks == 0 && w > 1) continue;
-            bf16x8 b[3];
-            dr_get8<3, DR_C, 16>(sR, c, 32 * ks + 8 * q, b);
-            dr_mfma<3, 3>(tf[ks], b, zs);
+#pragma unroll
+            for (int n = 0; n < NC; ++n) {
+                bf16x8 b[3];
+                dr_get8<3, DR_C, COLS>(sR, 16 * n + c, 32 * ks + 8 * q, b);
+                dr_mfma<3, 3>(tf[ks], b, zs[n]);
+            }
         }
-        const f32x4 Z = zs.sum();
-        const f32x4 u = -(Z * *reinterpret_cast<const f32x4*>(dec + 128 + row0) * *reinterpret_cast<const f32x4*>(dec + row0));
-        dr_put4<3, DR_C, 16>(sU, c, row0, u[0], u[1], u[2], u[3]);
-        sPO[w][lane] = Z;
+        const f32x4 factor = -(*reinterpret_cast<const f32x4*>(dec + 128 + row0) * *reinterpret_cast<const f32x4*>(dec + row0));
+#pragma unroll
+        for (int n = 0; n < NC; ++n) {
+            const f32x4 Z = zs[n].sum(), u = Z * factor;
+            dr_put4<3, DR_C, COLS>(sU, 16 * n + c, row0, u[0], u[1], u[2], u[3]);
+            sPO[n][w][lane] = Z;
+        }
         load_t(ch - 1);
-        const float all = dec[63];
         dr_barrier();   // dV is there
-        DrAcc up[NT];
+        DrAcc up[NT][NC];
 #pragma unroll
-        for (int ks = 0; ks < 2; ++ks) {
-            bf16x8 b[3];
-            dr_get8<3, DR_C, 16>(sU, c, 32 * ks + 8 * q, b);
+        for (int ks = 0; ks < 2; ++ks)
 #pragma unroll
-            for (int i = 0; i < NT; ++i) dr_mfma<NPL, 3>(kt[ks][i], b, up[i]);
-        }
+            for (int n = 0; n < NC; ++n) {
+                bf16x8 b[3];
+                dr_get8<3, DR_C, COLS>(sU, 16 * n + c, 32 * ks + 8 * q, b);
 #pragma unroll
-        for (int i = 0; i < NT; ++i) E[i] = all * E[i] + (qw[i] + up[i].sum());
+                for (int i = 0; i < NT; ++i) dr_mfma<NPL, 3>(kt[ks][i], b, up[i][n]);
+            }
+#pragma unroll
+        for (int i = 0; i < NT; ++i)
+#pragma unroll
+            for (int n = 0; n < NC; ++n) E[i][n] += up[i][n].sum();
         put_e();
     }
     put_state(make_rsrc_u(p.ds0 + (long long)sh * N * P, state_bytes));
@@ -1206,28 +1274,42 @@ __device__ void delta_grad(const HelixDeltaParams& p) {
 
 #define DR_STEPS(TAG, T, NK)                                                                                                             \
     extern "C" __global__ __launch_bounds__(256) void helix_delta_steps_##TAG##_##NK(HelixDeltaParams p) { delta_steps<T, NK / 16>(p); }
-// _s: rows of an odd width.
-#define DR_KERNELS(TAG, T, NK, SUF, ODD)                                                                                                              \
-    extern "C" __global__ __launch_bounds__(256) void helix_delta_prep_##TAG##_##NK##SUF(HelixDeltaParams p) { delta_prep<T, NK, ODD, false>(p); }    \
-    extern "C" __global__ __launch_bounds__(512) void helix_delta_walk_##TAG##_##NK##SUF(HelixDeltaParams p) { delta_walk<T, NK, ODD, false>(p); }    \
-    extern "C" __global__ __launch_bounds__(256) void helix_delta_prep_bwd_##TAG##_##NK##SUF(HelixDeltaParams p) { delta_prep<T, NK, ODD, true>(p); } \
-    extern "C" __global__ __launch_bounds__(512) void helix_delta_keep_##TAG##_##NK##SUF(HelixDeltaParams p) { delta_walk<T, NK, ODD, true>(p); }     \
-    extern "C" __global__ __launch_bounds__(512) void helix_delta_back_##TAG##_##NK##SUF(HelixDeltaParams p) { delta_back<T, NK, ODD>(p); }           \
-    extern "C" __global__ __launch_bounds__(640) void helix_delta_pairs_##TAG##_##NK##SUF(HelixDeltaParams p) { delta_pairs<T, NK, ODD>(p); }                   \
-    extern "C" __global__ __launch_bounds__(512) void helix_delta_grad_##TAG##_##NK##SUF(HelixDeltaParams p) { delta_grad<T, NK, ODD>(p); }
+// _s: rows of an odd width. _c16, _c32: columns of a workgroup.
+#define DR_KERNELS(TAG, T, NK, SUF, ODD)                                                                                                                    \
+    extern "C" __global__ __launch_bounds__(256) void helix_delta_prep_##TAG##_##NK##SUF(HelixDeltaParams p) { delta_prep<T, NK, ODD, false>(p); }          \
+    extern "C" __global__ __launch_bounds__(256) void helix_delta_prep_bwd_##TAG##_##NK##SUF(HelixDeltaParams p) { delta_prep<T, NK, ODD, true>(p); }       \
+    extern "C" __global__ __launch_bounds__(640) void helix_delta_pairs_##TAG##_##NK##SUF(HelixDeltaParams p) { delta_pairs<T, NK, ODD>(p); }               \
+    extern "C" __global__ __launch_bounds__(512) void helix_delta_grad_##TAG##_##NK##SUF(HelixDeltaParams p) { delta_grad<T, NK, ODD>(p); }                 \
+    extern "C" __global__ __launch_bounds__(512) void helix_delta_walk_##TAG##_##NK##SUF##_c16(HelixDeltaParams p) { delta_walk<T, NK, ODD, false, 1>(p); } \
+    extern "C" __global__ __launch_bounds__(512) void helix_delta_keep_##TAG##_##NK##SUF##_c16(HelixDeltaParams p) { delta_walk<T, NK, ODD, true, 1>(p); }  \
+    extern "C" __global__ __launch_bounds__(512) void helix_delta_back_##TAG##_##NK##SUF##_c16(HelixDeltaParams p) { delta_back<T, NK, ODD, 1>(p); }        \
+    extern "C" __global__ __launch_bounds__(512) void helix_delta_walk_##TAG##_##NK##SUF##_c32(HelixDeltaParams p) { delta_walk<T, NK, ODD, false, 2>(p); } \
+    extern "C" __global__ __launch_bounds__(512) void helix_delta_keep_##TAG##_##NK##SUF##_c32(HelixDeltaParams p) { delta_walk<T, NK, ODD, true, 2>(p); }
+// (fp32 of 128 keys and 32 columns would not fit in LDS.)
+#define DR_BACK(TAG, T, NK, SUF, ODD)                                                                                                                \
+    extern "C" __global__ __launch_bounds__(512) void helix_delta_back_##TAG##_##NK##SUF##_c32(HelixDeltaParams p) { delta_back<T, NK, ODD, 2>(p); }
 DR_STEPS(f32, float, 64)
 DR_KERNELS(f32, float, 64, , false)
+DR_BACK(f32, float, 64, , false)
 DR_STEPS(f32, float, 128)
 DR_KERNELS(f32, float, 128, , false)
 DR_STEPS(f16, _Float16, 64)
 DR_KERNELS(f16, _Float16, 64, , false)
+DR_BACK(f16, _Float16, 64, , false)
 DR_KERNELS(f16, _Float16, 64, _s, true)
+DR_BACK(f16, _Float16, 64, _s, true)
 DR_STEPS(f16, _Float16, 128)
 DR_KERNELS(f16, _Float16, 128, , false)
+DR_BACK(f16, _Float16, 128, , false)
 DR_KERNELS(f16, _Float16, 128, _s, true)
+DR_BACK(f16, _Float16, 128, _s, true)
 DR_STEPS(bf16, __bf16, 64)
 DR_KERNELS(bf16, __bf16, 64, , false)
+DR_BACK(bf16, __bf16, 64, , false)
 DR_KERNELS(bf16, __bf16, 64, _s, true)
+DR_BACK(bf16, __bf16, 64, _s, true)
 DR_STEPS(bf16, __bf16, 128)
 DR_KERNELS(bf16, __bf16, 128, , false)
+DR_BACK(bf16, __bf16, 128, , false)
 DR_KERNELS(bf16, __bf16, 128, _s, true)
+DR_BACK(bf16, __bf16, 128, _s, true)

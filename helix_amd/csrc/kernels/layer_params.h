@@ -145,10 +145,8 @@ typedef struct {
     HelixGatedScanJoin join;
 } HelixGatedScanBwdParams;
 
-/* Delta rule: tokens of a chunk, columns of the state that a workgroup of the
- * walks owns, and most tokens that go one by one. */
+/* Delta rule: tokens of a chunk, and most tokens that go one by one. */
 #define HELIX_DR_CHUNK 64
-#define HELIX_DR_SLICE 16
 #define HELIX_DR_STEPS 16
 
 /* Bytes, per chunk of a head, of the operands that the first kernel leaves for
@@ -180,7 +178,7 @@ typedef struct {
     int          n_seq, n_tok, n_qk, n_head, share, n_key, n_val;   /* share = n_head / n_qk */
     float        scale;
     /* Chunked: the chunks chunk0 .. chunk0 + n_chunk - 1 of every sequence. */
-    int          chunk0, n_chunk, n_slice;
+    int          chunk0, n_chunk, n_slice;   /* n_slice: workgroups of a walk for each head */
     char*        x;         /* [sequence x head][chunk] fragments of X         */
     char*        p;         /* of scale P                                      */
     char*        tt;        /* of T^T and scale P^T (backward)                 */

@@ -891,9 +891,12 @@ std::string delta_form(const A& a, bool steps = false) {
     return std::string(kTags[a.io_dtype]) + "_" + std::to_string(delta_keys(a.n_key)) + (odd ? "_s" : "");
 }
 
+// Columns of the state that a workgroup of the walks has: 32 where that still gives every CU a workgroup.
+int delta_columns(long long heads, int n_val) { return n_val > 16 && heads * ceil_div(n_val, 32) >= 256 ? 32 : 16; }
+
 // How the rule is cut: segments of `chunks` chunks of every sequence, whose operands scratch holds at a time.
 struct DeltaPlan {
-    int n_chunk = 0, chunks = 0, n_slice = 0;
+    int n_chunk = 0, chunks = 0, columns = 0;
     size_t x_at = 0, p_at = 0, decay_at = 0, bytes = 0;
 };
 // Scratch of a segment: up to a gigabyte, and one chunk of every sequence where that is more.
@@ -906,7 +909,7 @@ DeltaPlan delta_plan(const helix_delta_rule_args& a) {
     const size_t x = 6 * 3 * HELIX_DR_FRAG, pp = 6 * out * HELIX_DR_FRAG, each = sh * (x + pp + HELIX_DR_DECAY);
     p.n_chunk = (int)ceil_div(a.n_tok, HELIX_DR_CHUNK);
     p.chunks = (int)std::min<size_t>(p.n_chunk, std::max<size_t>(1, kDeltaScratch / each));
-    p.n_slice = (int)ceil_div(a.n_val, HELIX_DR_SLICE);
+    p.columns = delta_columns((long long)sh, a.n_val);
     p.p_at = p.x_at + sh * p.chunks * x;
     p.decay_at = p.p_at + sh * p.chunks * pp;
     p.bytes = p.decay_at + sh * p.chunks * HELIX_DR_DECAY;
@@ -987,13 +990,14 @@ extern "C" helix_status helix_delta_rule_encode(helix_ctx* ctx, void* stream, co
             launch(f, stream, gx, 1, kDeltaThreads, p);
             return;
         }
-        const hipFunction_t prep = kernel(ctx, "helix_delta_prep_" + form), walk = kernel(ctx, "helix_delta_walk_" + form);
-        const unsigned gp = grid(sh * plan.chunks, kDeltaThreads), gw = grid(sh * plan.n_slice, 2 * kDeltaThreads);
+        const hipFunction_t prep = kernel(ctx, "helix_delta_prep_" + form),
+                            walk = kernel(ctx, "helix_delta_walk_" + form + "_c" + std::to_string(plan.columns));
+        p.n_slice = (int)ceil_div(a->n_val, plan.columns);
+        const unsigned gp = grid(sh * plan.chunks, kDeltaThreads), gw = grid(sh * p.n_slice, 2 * kDeltaThreads);
         char* sc = static_cast<char*>(a->scratch);
         p.x = sc + plan.x_at;
         p.p = sc + plan.p_at;
         p.decay = reinterpret_cast<float*>(sc + plan.decay_at);
-        p.n_slice = plan.n_slice;
         const OnDevice on(ctx->device);
         for (p.chunk0 = 0; p.chunk0 < plan.n_chunk; p.chunk0 += plan.chunks) {
             p.n_chunk = std::min(plan.chunks, plan.n_chunk - p.chunk0);
@@ -1008,7 +1012,7 @@ namespace {
 
 // The backward pass: what a segment's chunks leave for its kernels, and the states that the segments start from.
 struct DeltaBwdPlan {
-    int n_chunk = 0, chunks = 0, n_seg = 0, n_slice = 0;
+    int n_chunk = 0, chunks = 0, n_seg = 0;
     size_t x_at = 0, tt_at = 0, pt_at = 0, decay_at = 0, s_at = 0, e_at = 0, d_at = 0, z_at = 0, pg_at = 0, pb_at = 0, tri_at = 0, start_at = 0, bytes = 0;
 };
 // Scratch of a segment: up to two gigabytes, and one chunk of every sequence where that is more. More than one segment forms
@@ -1026,7 +1030,6 @@ DeltaBwdPlan delta_bwd_plan(const helix_delta_rule_backward_args& a) {
     p.chunks = (int)std::min<size_t>(p.n_chunk,
                                      std::max<size_t>(1, kDeltaBwdScratch / (sh * (3 * x + HELIX_DR_DECAY + 2 * state + 2 * rows + 12 * HELIX_DR_CHUNK) + sk * tri)));
     p.n_seg = (int)ceil_div(p.n_chunk, p.chunks);
-    p.n_slice = (int)ceil_div(a.n_val, HELIX_DR_SLICE);
     const size_t each = sh * p.chunks;
     p.tt_at = p.x_at + each * x;
     p.pt_at = p.tt_at + each * x;
@@ -1093,10 +1096,12 @@ extern "C" helix_status helix_delta_rule_backward_encode(helix_ctx* ctx, void* s
         p.pair_g = reinterpret_cast<double*>(sc + plan.pg_at);
         p.pair_b = reinterpret_cast<float*>(sc + plan.pb_at);
         p.tri = reinterpret_cast<float*>(sc + plan.tri_at);
-        p.n_slice = (int)ceil_div(a->n_val, HELIX_DR_SLICE);
-        const std::string form = delta_form(*a);
-        const hipFunction_t prep = kernel(ctx, "helix_delta_prep_bwd_" + form), keep = kernel(ctx, "helix_delta_keep_" + form),
-                            back = kernel(ctx, "helix_delta_back_" + form), pairs = kernel(ctx, "helix_delta_pairs_" + form),
+        // (fp32 of 128 keys and 32 columns would not fit in LDS.)
+        const int columns = a->io_dtype == HELIX_F32 && a->n_key > 64 ? 16 : delta_columns((long long)a->n_seq * a->n_head, a->n_val);
+        p.n_slice = (int)ceil_div(a->n_val, columns);
+        const std::string form = delta_form(*a), wide = form + "_c" + std::to_string(columns);
+        const hipFunction_t prep = kernel(ctx, "helix_delta_prep_bwd_" + form), keep = kernel(ctx, "helix_delta_keep_" + wide),
+                            back = kernel(ctx, "helix_delta_back_" + wide), pairs = kernel(ctx, "helix_delta_pairs_" + form),
                             grad = kernel(ctx, "helix_delta_grad_" + form);
         const long long sh = (long long)a->n_seq * a->n_head, sk = (long long)a->n_seq * a->n_qk_head;
         const unsigned gw = grid(sh * p.n_slice, 2 * kDeltaThreads);
@@ -1150,9 +1155,13 @@ const std::vector<std::string>& layer_kernel_names() {
         for (const char* tag : kTags)
             for (const char* n : {"_64", "_128"}) {
                 v.push_back(std::string("helix_delta_steps_") + tag + n);
-                for (const char* k : {"prep_", "walk_", "prep_bwd_", "keep_", "back_", "pairs_", "grad_"})
-                    for (const char* s : {"", "_s"})
-                        if (!*s || tag != kTags[HELIX_F32]) v.push_back(std::string("helix_delta_") + k + tag + n + s);
+                for (const char* s : {"", "_s"}) {
+                    if (*s && tag == kTags[HELIX_F32]) continue;
+                    for (const char* k : {"prep_", "prep_bwd_", "pairs_", "grad_"}) v.push_back(std::string("helix_delta_") + k + tag + n + s);
+                    for (const char* k : {"walk_", "keep_", "back_"})
+                        for (const char* c : {"_c16", "_c32"})
+                            if (std::string(k) + tag + n + c != "back_f32_128_c32") v.push_back(std::string("helix_delta_") + k + tag + n + s + c);
+                }
             }
         v.push_back("helix_group_norm_dw");
         for (const char* tag : kTags) {
