@@ -46,6 +46,19 @@ struct DrAcc {
     __device__ __forceinline__ DrAcc() { s[0] = s[1] = s[2] = f32x4{0.0f, 0.0f, 0.0f, 0.0f}; }
     __device__ __forceinline__ f32x4 sum() const { return (s[2] + s[1]) + s[0]; }
 };
+// Sums of a wave that has NC blocks of columns: with two, their chains are enough side by side, and one sum for each spares
+// registers.
+struct DrAcc1 {
+    f32x4 s;
+    __device__ __forceinline__ DrAcc1() { s = f32x4{0.0f, 0.0f, 0.0f, 0.0f}; }
+    __device__ __forceinline__ f32x4 sum() const { return s; }
+};
+template <int NC> struct DrAccOf { typedef DrAcc type; };
+template <> struct DrAccOf<2> { typedef DrAcc1 type; };
+template <int NA, int NB, int MAX = 3>
+HELIX_DEV void dr_mfma(const bf16x8 (&a)[NA], const bf16x8 (&b)[NB], DrAcc1& acc) {
+    acc.s = dr_mfma<NA, NB, MAX>(a, b, acc.s);
+}
 // Of products with NPL parts on both sides; one part's have one sum.
 template <int NPL>
 HELIX_DEV f32x4 dr_sum(const DrAcc& a) { return NPL == 1 ? a.s[0] : a.sum(); }

@@ -428,7 +428,7 @@ __device__ void delta_walk(const HelixDeltaParams& p) {
             dr_barrier();   // K, V and S are there
             f32x4 o[NC];
             if constexpr (!KEEP) {
-                DrAcc qs[NC];
+                typename DrAccOf<NC>::type qs[NC];
 #pragma unroll
                 for (int s = 0; s < KS; ++s) {
                     const int col = 32 * s + 8 * q;
@@ -519,7 +519,7 @@ __device__ void delta_walk(const HelixDeltaParams& p) {
         dr_barrier();   // K, V and S are there
         if constexpr (KEEP) put_state(make_rsrc_u(p.keep_s + (base + ch) * N * P, state_bytes));
         const float* const dec = sDec[ch & 1];
-        DrAcc ks_[NC];
+        typename DrAccOf<NC>::type ks_[NC];
 #pragma unroll
         for (int s = 0; s < KS; ++s) {
             const int col = 32 * s + 8 * q;
@@ -545,7 +545,7 @@ __device__ void delta_walk(const HelixDeltaParams& p) {
             dr_put4<3, DR_C, COLS>(sR, 16 * n + c, row0, R[0], R[1], R[2], R[3]);
         }
         dr_barrier();   // R is there; K and V have been read
-        DrAcc ds[NC];
+        typename DrAccOf<NC>::type ds[NC];
 #pragma unroll
         for (int ks = 0; ks < 2; ++ks) {
             if (ks && w < 2) break;
@@ -571,7 +571,7 @@ __device__ void delta_walk(const HelixDeltaParams& p) {
         load_x(ch + 1);
         const float all = dec[63];
         dr_barrier();   // D is there
-        DrAcc up[NT][NC];
+        typename DrAccOf<NC>::type up[NT][NC];
 #pragma unroll
         for (int ks = 0; ks < 2; ++ks)
 #pragma unroll
@@ -808,7 +808,7 @@ __device__ void delta_back(const HelixDeltaParams& p) {
         dr_barrier();   // K, E and what does not depend on E are there
         put_state(make_rsrc_u(p.keep_e + (base + ch) * N * P, state_bytes));
         const float* const dec = sDec[ch & 1];
-        DrAcc ke[NC];
+        typename DrAccOf<NC>::type ke[NC];
 #pragma unroll
         for (int s = 0; s < KS; ++s) {
             const int col = 32 * s + 8 * q;
@@ -834,7 +834,7 @@ __device__ void delta_back(const HelixDeltaParams& p) {
             dr_put4<3, DR_C, COLS>(sR, 16 * n + c, row0, dd[0], dd[1], dd[2], dd[3]);
         }
         dr_barrier();   // dD is there; K has been read
-        DrAcc zs[NC];
+        typename DrAccOf<NC>::type zs[NC];
 #pragma unroll
         for (int ks = 0; ks < 2; ++ks) {
             if (ks == 0 && w > 1) continue;
@@ -854,7 +854,7 @@ __device__ void delta_back(const HelixDeltaParams& p) {
         }
         load_t(ch - 1);
         dr_barrier();   // dV is there
-        DrAcc up[NT][NC];
+        typename DrAccOf<NC>::type up[NT][NC];
 #pragma unroll
         for (int ks = 0; ks < 2; ++ks)
 #pragma unroll
@@ -892,6 +892,7 @@ __device__ void delta_pairs(const HelixDeltaParams& p) {
     constexpr int kKQ = 2 * NPL * DR_C * NK, kOZD = (NPL + 6) * DR_C * DR_C;
     __shared__ __attribute__((aligned(16))) __bf16 sBig[kKQ > kOZD ? kKQ : kOZD];
     __shared__ double sG[DR_C];
+    __shared__ __attribute__((aligned(16))) float sB[DR_C];
     __shared__ float sRow[4][DR_C], sCol[4][DR_C], sBeta[4][DR_C], sZV[DR_C];
     __bf16* const sK = sBig;
     __bf16* const sQ = sBig + NPL * DR_C * NK;
@@ -919,12 +920,12 @@ __device__ void delta_pairs(const HelixDeltaParams& p) {
         }
     }
     // A pass over 64 columns of a head's values, loaded while the one before is at work: a row's eight by the first 512 threads.
-    const int srow = tid / 8, scol = 8 * (tid % 8);
     Raw8<T> no, nv;
     Raw8<float> nz, nd;
-    float ng;
+    float ng, nb;
     auto load = [&](int hs, int pb) {
         if (hs >= p.share) return;
+        const int tid = vgpr_fresh(threadIdx.x), srow = tid / 8, scol = 8 * (tid % 8), lane = tid & 63;
         const int h = hk * p.share + hs;
         const long long at = ((long long)seq * p.n_head + h) * p.n_chunk + ch;
         const Rows<T, ODD> ro(p.d_o, seq * p.seq_o + h * p.head_o + t0 * p.tok_o, p.tok_o, len, P);
@@ -936,6 +937,7 @@ __device__ void delta_pairs(const HelixDeltaParams& p) {
             nd = rd.load8(srow, pb + scol);
             nv = rv.load8(srow, pb + scol);
         }
+        nb = p.decay[at * (HELIX_DR_DECAY / 4) + 128 + lane];
         ng = lane < len ? p.g[seq * p.seq_g + (t0 + lane) * p.tok_g + h] : 0.0f;
     };
     load(0, 0);
@@ -958,11 +960,13 @@ __device__ void delta_pairs(const HelixDeltaParams& p) {
     }
     for (int hs = 0; hs < p.share; ++hs) {
         const long long at = ((long long)seq * p.n_head + hk * p.share + hs) * p.n_chunk + ch;
-        const float* dec = p.decay + at * (HELIX_DR_DECAY / 4);
         const double G = dr_log_decay(ng) * 1.4426950408889634074;
-        DrAcc dP, dA;
+        const float bl = nb;
+        f32x4 dP = zero4(), dA = zero4();
         float zv = 0.0f;
         for (int pb = 0; pb < P; pb += 64) {
+            // (Addresses formed from these are formed here, not kept over the loop.)
+            const int tid = vgpr_fresh(threadIdx.x), srow = tid / 8, scol = 8 * (tid % 8), c = tid & 15, q = (tid & 63) >> 4;
             __syncthreads();   // what these overwrite has been read
             if (tid < 512) {
                 const int n = P - pb - scol;
@@ -984,31 +988,34 @@ __device__ void delta_pairs(const HelixDeltaParams& p) {
                 bf16x8 ao[NPL], az[3], bd[3];
                 dr_get8<3, DR_C, DR_C>(sD, 16 * jb + c, col, bd);
                 dr_get8<NPL, DR_C, DR_C>(sO, 16 * tb + c, col, ao);
-                dr_mfma<NPL, 3>(ao, bd, dP);
+                dP = dr_mfma<NPL, 3>(ao, bd, dP);
                 dr_get8<3, DR_C, DR_C>(sZ, 16 * tb + c, col, az);
-                dr_mfma<3, 3>(az, bd, dA);
+                dA = dr_mfma<3, 3>(az, bd, dA);
             }
         }
-        if (w == 0) sG[lane] = G;
+        const int tid = vgpr_fresh(threadIdx.x), lane = tid & 63, c = tid & 15, q = lane >> 4;
+        if (w == 0) {
+            sG[lane] = G;
+            sB[lane] = bl;
+        }
         if (tid < 512) {
             zv = add_dpp<0xb1>(zv);   // eight lanes a row
             zv = add_dpp<0x4e>(zv);
             zv = add_dpp<0x141>(zv);
-            if ((tid & 7) == 0) sZV[srow] = zv;
+            if ((tid & 7) == 0) sZV[tid / 8] = zv;
         }
         __syncthreads();
         {
-            const f32x4 x = dP.sum(), y = dA.sum();
-            const int j = 16 * jb + c;
+                        const int j = 16 * jb + c;
             const double Gj = sG[j];
-            const f32x4 beta = *reinterpret_cast<const f32x4*>(dec + 128 + 16 * tb + 4 * q);
+            const f32x4 beta = *reinterpret_cast<const f32x4*>(&sB[16 * tb + 4 * q]);
             float pair[4], bs[4];
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 const int i = 16 * tb + 4 * q + r;
                 const float e = __builtin_amdgcn_exp2f((float)(sG[i] - Gj));
                 const bool in = tb > jb || j <= i, below = tb > jb || j < i;
-                const float m = in ? p.scale * (e * x[r]) : 0.0f, a = below ? -(e * y[r]) : 0.0f;
+                const float m = in ? p.scale * (e * dP[r]) : 0.0f, a = below ? -(e * dA[r]) : 0.0f;
                 mp[r] += m;
                 ma[r] += beta[r] * a;
                 bs[r] = below ? a * kk[r] : 0.0f;
@@ -1115,6 +1122,13 @@ __device__ void delta_grad(const HelixDeltaParams& p) {
     };
     load(0, 0);
     for (int hs = 0; hs < p.share; ++hs) {
+        const long long at = (((long long)seq * p.n_head + hk * p.share + hs) * p.n_chunk + ch) * DR_C + lane;
+        double own = 0.0;
+        float db = 0.0f;
+        if (w == 0) {
+            own = p.pair_g[at];
+            db = p.pair_b[at];
+        }
         float se = 0.0f, dots[3][RT];   // (of row 16 (i0 + i) + 4 q + c % 4)
 #pragma unroll
         for (int i = 0; i < RT; ++i) dots[0][i] = dots[1][i] = dots[2][i] = 0.0f;
@@ -1187,9 +1201,6 @@ __device__ void delta_grad(const HelixDeltaParams& p) {
         if (w == 0) {
             // Lane = token.
             const int h = hk * p.share + hs;
-            const long long at = (((long long)seq * p.n_head + h) * p.n_chunk + ch) * DR_C + lane;
-            double own = p.pair_g[at];
-            const float db = p.pair_b[at];
             float dot[3];
 #pragma unroll
             for (int j = 0; j < 3; ++j) {
@@ -1278,13 +1289,13 @@ __device__ void delta_grad(const HelixDeltaParams& p) {
 #define DR_KERNELS(TAG, T, NK, SUF, ODD)                                                                                                                    \
     extern "C" __global__ __launch_bounds__(256) void helix_delta_prep_##TAG##_##NK##SUF(HelixDeltaParams p) { delta_prep<T, NK, ODD, false>(p); }          \
     extern "C" __global__ __launch_bounds__(256) void helix_delta_prep_bwd_##TAG##_##NK##SUF(HelixDeltaParams p) { delta_prep<T, NK, ODD, true>(p); }       \
-    extern "C" __global__ __launch_bounds__(640) void helix_delta_pairs_##TAG##_##NK##SUF(HelixDeltaParams p) { delta_pairs<T, NK, ODD>(p); }               \
+    extern "C" __global__ __launch_bounds__(640, 5) void helix_delta_pairs_##TAG##_##NK##SUF(HelixDeltaParams p) { delta_pairs<T, NK, ODD>(p); }               \
     extern "C" __global__ __launch_bounds__(512) void helix_delta_grad_##TAG##_##NK##SUF(HelixDeltaParams p) { delta_grad<T, NK, ODD>(p); }                 \
     extern "C" __global__ __launch_bounds__(512) void helix_delta_walk_##TAG##_##NK##SUF##_c16(HelixDeltaParams p) { delta_walk<T, NK, ODD, false, 1>(p); } \
     extern "C" __global__ __launch_bounds__(512) void helix_delta_keep_##TAG##_##NK##SUF##_c16(HelixDeltaParams p) { delta_walk<T, NK, ODD, true, 1>(p); }  \
     extern "C" __global__ __launch_bounds__(512) void helix_delta_back_##TAG##_##NK##SUF##_c16(HelixDeltaParams p) { delta_back<T, NK, ODD, 1>(p); }        \
     extern "C" __global__ __launch_bounds__(512) void helix_delta_walk_##TAG##_##NK##SUF##_c32(HelixDeltaParams p) { delta_walk<T, NK, ODD, false, 2>(p); } \
-    extern "C" __global__ __launch_bounds__(512) void helix_delta_keep_##TAG##_##NK##SUF##_c32(HelixDeltaParams p) { delta_walk<T, NK, ODD, true, 2>(p); }
+    extern "C" __global__ __launch_bounds__(512, 4) void helix_delta_keep_##TAG##_##NK##SUF##_c32(HelixDeltaParams p) { delta_walk<T, NK, ODD, true, 2>(p); }
 // (fp32 of 128 keys and 32 columns would not fit in LDS.)
 #define DR_BACK(TAG, T, NK, SUF, ODD)                                                                                                                \
     extern "C" __global__ __launch_bounds__(512) void helix_delta_back_##TAG##_##NK##SUF##_c32(HelixDeltaParams p) { delta_back<T, NK, ODD, 2>(p); }

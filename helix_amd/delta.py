@@ -13,28 +13,27 @@ from . import abi
 from .layer import device_index, expect, io_code, packed, ptr, run, run_with_scratch, scratch, stream_handle, under
 
 
-def _strides(name: str, t: torch.Tensor) -> tuple[int, int, int]:
-    if t.stride(3) != 1 and t.shape[3] > 1:
-        raise ValueError(f"{name}: the channels must be contiguous")
-    return t.stride(0), t.stride(1), t.stride(2)
-
-
-def _gate_strides(name: str, t: torch.Tensor) -> tuple[int, int]:
-    if t.stride(2) != 1 and t.shape[2] > 1:
-        raise ValueError(f"{name}: the heads must be contiguous")
-    return t.stride(0), t.stride(1)
+def _tensor(name: str, t: torch.Tensor, dtype: torch.dtype, shape, like: torch.Tensor, inner: str) -> tuple[int, ...]:
+    """Checks t, and returns its strides but the last dimension's, whose elements have to be neighbours."""
+    if t.dtype != dtype or t.shape != shape or t.get_device() != like.get_device():
+        expect(name, t, dtype, shape, like)
+    strides = t.stride()
+    if strides[-1] != 1 and shape[-1] > 1:
+        raise ValueError(f"{name}: the {inner} must be contiguous")
+    return strides[:-1]
 
 
 def _state(name: str, t: torch.Tensor | None, like: torch.Tensor, shape) -> None:
     if t is None:
         return
-    expect(name, t, torch.float32, shape, like)
+    if t.dtype != torch.float32 or t.shape != shape or t.get_device() != like.get_device():
+        expect(name, t, torch.float32, shape, like)
     if not t.is_contiguous():
         raise ValueError(f"{name} must be contiguous")
 
 
 def _inputs(op, q, k, v, g, beta, s0, scale):
-    """Checks: (device, io, the sizes' fields of the arguments, the inputs' strides)."""
+    """Checks: (device, the sizes' fields of the arguments, the inputs' strides)."""
     index = device_index(op, q)
     io = io_code("q", q)
     if q.dim() != 4 or v.dim() != 4:
@@ -43,16 +42,14 @@ def _inputs(op, q, k, v, g, beta, s0, scale):
     H, P = v.shape[2:]
     if N < 1 or P < 1:
         raise ValueError("heads must have at least one key and one value channel")
-    if (Hk and H % Hk) or (H and not Hk):
+    if H % Hk if Hk else H:
         raise ValueError(f"the {Hk} heads of q and k must divide the {H} heads of v")
-    expect("k", k, q.dtype, q.shape, q)
-    expect("v", v, q.dtype, (S, L, H, P), q)
-    expect("g", g, torch.float32, (S, L, H), q)
-    expect("beta", beta, torch.float32, (S, L, H), q)
+    dtype, gates = q.dtype, (S, L, H)
+    strides = (*_tensor("q", q, dtype, q.shape, q, "channels"), *_tensor("k", k, dtype, q.shape, q, "channels"),
+               *_tensor("v", v, dtype, (S, L, H, P), q, "channels"), *_tensor("g", g, torch.float32, gates, q, "heads"),
+               *_tensor("beta", beta, torch.float32, gates, q, "heads"))
     _state("s0", s0, q, (S, H, N, P))
-    sizes = (S, L, Hk, H, N, P, io, N ** -0.5 if scale is None else scale)
-    strides = (*_strides("q", q), *_strides("k", k), *_strides("v", v), *_gate_strides("g", g), *_gate_strides("beta", beta))
-    return index, sizes, strides
+    return index, (S, L, Hk, H, N, P, io, N ** -0.5 if scale is None else scale), strides
 
 
 def delta_rule(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Tensor, beta: torch.Tensor,
@@ -87,7 +84,7 @@ def delta_rule_backward(do: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: t
     are formed again. dq and dk of a head that several heads of v share are the sums over them."""
     index, sizes, strides = _inputs("delta_rule_backward", q, k, v, g, beta, s0, scale)
     S, L, Hk, H, N, P = sizes[:6]
-    expect("do", do, q.dtype, (S, L, H, P), q)
+    strides = (*_tensor("do", do, q.dtype, (S, L, H, P), q, "channels"), *strides)
     _state("ds", ds, q, (S, H, N, P))
     with under(index, stream):
         dq, dk = (torch.empty(S, L, Hk, N, dtype=q.dtype, device=q.device) for _ in range(2))
@@ -95,7 +92,6 @@ def delta_rule_backward(do: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: t
         dg, dbeta = (torch.empty(S, L, H, dtype=torch.float32, device=q.device) for _ in range(2))
         ds0 = torch.empty(S, H, N, P, dtype=torch.float32, device=q.device)
     st = stream_handle(index, stream)
-    strides = (*_strides("do", do), *strides)
 
     def pack(buf, nbytes):
         return abi.DELTA_RULE_BACKWARD_STRUCT.pack(*sizes, do.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(),
