@@ -311,7 +311,7 @@ struct GroupBwdPlan {
     long long gx = 0, parts = 0;   // workgroups along the groups and along the rows
 };
 // A workgroup has as many groups side by side as there are, up to its room, and rows in what is left of it. Along the
-// rows four workgroups a CU in all, of four rows a slot at least.
+// rows four workgroups a CU in all, of two rows a slot at least.
 GroupBwdPlan group_bwd_plan(long long rows, int dim, int groups) {
     GroupBwdPlan p;
     p.form = group_form(dim / groups);
@@ -319,7 +319,7 @@ GroupBwdPlan group_bwd_plan(long long rows, int dim, int groups) {
     while (p.group_slots < room && p.group_slots < groups) p.group_slots *= 2;
     p.row_slots = room / p.group_slots;
     p.gx = ceil_div(groups, p.group_slots);
-    p.parts = std::max(1LL, std::min(ceil_div(4 * 256, p.gx), rows / (4 * p.row_slots)));
+    p.parts = std::max(1LL, std::min(ceil_div(4 * 256, p.gx), rows / (2 * p.row_slots)));
     return p;
 }
 
