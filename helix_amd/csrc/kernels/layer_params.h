@@ -145,7 +145,8 @@ typedef struct {
     HelixGatedScanJoin join;
 } HelixGatedScanBwdParams;
 
-/* Delta rule: tokens of a chunk, and most tokens that go one by one. */
+/* Delta rule: tokens of a chunk, and those of a call that goes token by token
+ * whose keys and queries are in LDS at a time. */
 #define HELIX_DR_CHUNK 64
 #define HELIX_DR_STEPS 16
 

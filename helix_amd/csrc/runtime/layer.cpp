@@ -894,6 +894,16 @@ std::string delta_form(const A& a, bool steps = false) {
 // Columns of the state that a workgroup of the walks has: 32 where that still gives every CU a workgroup.
 int delta_columns(long long heads, int n_val) { return n_val > 16 && heads * ceil_div(n_val, 32) >= 256 ? 32 : 16; }
 
+// The most tokens that go one by one, by the workgroups that their kernel has. One by one a token costs 1.1 to 1.4 us where
+// all of them run at once; a chunk costs about the same for 1 token as for 64, and more in fp32. Measured, us one by one | as a
+// chunk, 128 keys: 16 bits, 64 workgroups, 4 tokens 9 | 13, 8 tokens 14 | 13; 256, 8 tokens 15 | 21, 12 tokens 21 | 21; 384,
+// 16 tokens 28 | 29; 4096, 16 tokens 168 | 210, 24 tokens 246 | 215. fp32, 64 workgroups, 12 tokens 17 | 18, 16 tokens
+// 21 | 18; 384, 32 tokens 45 | 42; 1024, 32 tokens 71 | 86, 64 tokens 130 | 96.
+int delta_steps(long long heads, int n_val, int io) {
+    const long long groups = heads * ceil_div(n_val, 64);
+    return (io == HELIX_F32 ? 2 : 1) * (groups < 256 ? 6 : groups < 384 ? 10 : 16);
+}
+
 // How the rule is cut: segments of `chunks` chunks of every sequence, whose operands scratch holds at a time.
 struct DeltaPlan {
     int n_chunk = 0, chunks = 0, columns = 0;
@@ -904,7 +914,8 @@ constexpr size_t kDeltaScratch = (size_t)1 << 30;
 
 DeltaPlan delta_plan(const helix_delta_rule_args& a) {
     DeltaPlan p;
-    if (a.n_seq <= 0 || a.n_head <= 0 || a.n_tok <= HELIX_DR_STEPS || a.n_key <= 0 || a.n_val <= 0) return p;
+    if (a.n_seq <= 0 || a.n_head <= 0 || a.n_key <= 0 || a.n_val <= 0) return p;
+    if (a.n_tok <= delta_steps((long long)a.n_seq * a.n_head, a.n_val, a.io_dtype)) return p;
     const size_t sh = (size_t)a.n_seq * a.n_head, out = a.io_dtype == HELIX_F32 ? 3 : 2;
     const size_t x = 6 * 3 * HELIX_DR_FRAG, pp = 6 * out * HELIX_DR_FRAG, each = sh * (x + pp + HELIX_DR_DECAY);
     p.n_chunk = (int)ceil_div(a.n_tok, HELIX_DR_CHUNK);

@@ -69,7 +69,7 @@ BOTH = [
     (dict(o=0), HELIX_ERR_INVALID_ARG), (dict(s=0), HELIX_ERR_INVALID_ARG), (dict(s=P + 2), HELIX_ERR_INVALID_ARG),
     (dict(tok_o=127), HELIX_ERR_INVALID_ARG), (dict(seq_o=12799), HELIX_ERR_INVALID_ARG), (dict(head_o=31), HELIX_ERR_INVALID_ARG),
     (dict(head_o=3200, tok_o=32), HELIX_ERR_NO_DEVICE),   # heads outside tokens
-    (dict(L=1, scratch=0, nbytes=0), HELIX_ERR_NO_DEVICE), (dict(L=16, scratch=0, nbytes=0), HELIX_ERR_NO_DEVICE),
+    (dict(L=1, scratch=0, nbytes=0), HELIX_ERR_NO_DEVICE), (dict(L=6, scratch=0, nbytes=0), HELIX_ERR_NO_DEVICE),
     (dict(L=0, q=0, k=0, v=0, g=0, beta=0, o=0, scratch=0, nbytes=0), HELIX_ERR_NO_DEVICE),
 ])
 def test_checks(host, change, status):

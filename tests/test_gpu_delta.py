@@ -63,7 +63,7 @@ def check_backward(q, k, v, g, beta, s0, ds=True, scale=None, seed=90, amp=None)
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("L", [1, 2, 15, 16, 17, 31, 63, 64, 65, 127, 128, 129, 200, 333])
+@pytest.mark.parametrize("L", [1, 2, 3, 6, 7, 12, 13, 15, 16, 17, 31, 63, 64, 65, 127, 128, 129, 200, 333])
 def test_lengths(gpu, L, dtype):
     p = problem(2, L, 1, 2, 64, 32, dtype, seed=L, packed_rows=L % 2 == 1, carry=L % 3 != 0)
     check(*p)
@@ -73,7 +73,7 @@ def test_lengths(gpu, L, dtype):
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("N,P", [(1, 1), (2, 3), (5, 7), (8, 64), (31, 17), (40, 72), (63, 15), (64, 128), (65, 16), (66, 33),
                                  (100, 130), (127, 65), (128, 192), (128, 1)])
-@pytest.mark.parametrize("L", [9, 100])
+@pytest.mark.parametrize("L", [5, 9, 100])
 def test_widths(gpu, L, N, P, dtype):
     p = problem(1, L, 2, 2, N, P, dtype, seed=N + P, packed_rows=(N + P) % 2 == 0)
     check(*p)
@@ -97,6 +97,14 @@ def test_long_and_many(gpu, S, L, Hk, H, N, P, dtype):
     check_backward(*p)
 
 
+# Where many heads share the machine, more tokens go one by one: up to 32 in fp32, more than LDS has the keys of at a time.
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("S,L,Hk,H,N,P", [(4, 10, 4, 64, 32, 16), (4, 11, 4, 64, 32, 16), (4, 20, 4, 64, 32, 16), (4, 21, 4, 64, 32, 16),
+                                          (6, 16, 8, 64, 24, 20), (6, 17, 8, 64, 24, 20), (3, 32, 8, 64, 40, 72), (6, 33, 8, 64, 24, 20)])
+def test_some_tokens_of_many_heads(gpu, S, L, Hk, H, N, P, dtype):
+    check(*problem(S, L, Hk, H, N, P, dtype, seed=L, packed_rows=L % 2 == 0))
+
+
 def test_scale(gpu):
     p = problem(1, 80, 1, 2, 32, 16, torch.float32, seed=3)
     for scale in (1.0, -0.7, 0.0):
@@ -104,7 +112,7 @@ def test_scale(gpu):
         check_backward(*p, scale=scale)
 
 
-@pytest.mark.parametrize("L", [10, 150])
+@pytest.mark.parametrize("L", [5, 10, 150])
 def test_long_memory(gpu, L):
     # No decay at all, and a state that is large against what the tokens bring.
     q, k, v, g, beta, s0 = problem(1, L, 2, 2, 64, 32, torch.bfloat16, seed=8)
