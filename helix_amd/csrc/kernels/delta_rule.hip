@@ -144,18 +144,23 @@ constexpr int DR_LD = DR_C + 4;   // fp32 rows of a chunk's square matrices in L
 // on fp32 matrix instructions, T_jw staying in the registers it was formed in. (Products of powers of A would be fewer steps,
 // but keys that repeat make the powers large, and they cancel.) BWD: T' and P' with X, without P.
 // Four workgroups a CU hide one another's chains: P takes the place of K's parts in LDS, T that of A.
+template <typename T, int NK>
+struct PrepLds {
+    union {
+        __bf16 k[dr_planes<T> * DR_C * NK];
+        float p[DR_C][DR_LD];
+    };
+    float a[DR_C][DR_LD], d[4][16][20], b[DR_C];
+    double g[DR_C];
+};
 template <typename T, int NK, bool ODD, bool BWD>
-__device__ void delta_prep(const HelixDeltaParams& p) {
+__device__ void delta_prep(const HelixDeltaParams& p, unsigned id, PrepLds<T, NK>& lds) {
     constexpr int NPL = dr_planes<T>, NO = dr_out_planes<T>;
-    constexpr int kK = NPL * DR_C * NK * 2, kP = DR_C * DR_LD * 4;
-    __shared__ __attribute__((aligned(16))) char sKP[kK > kP ? kK : kP];
-    __shared__ __attribute__((aligned(16))) float sA[DR_C][DR_LD];
-    __shared__ __attribute__((aligned(16))) float sD[4][16][20];
-    __shared__ double sG[DR_C];
-    __shared__ __attribute__((aligned(16))) float sB[DR_C];
-    __bf16* const sK = reinterpret_cast<__bf16*>(sKP);
-    float (*const sP)[DR_LD] = reinterpret_cast<float (*)[DR_LD]>(sKP);
-    const unsigned id = blockIdx.x;
+    __bf16* const sK = lds.k;
+    auto &sP = lds.p, &sA = lds.a;
+    auto& sD = lds.d;
+    auto& sG = lds.g;
+    auto& sB = lds.b;
     // (Wave w has w + 1 blocks of the products: turned from workgroup to workgroup, every SIMD gets each.)
     const int tid = threadIdx.x, lane = lane_id(), w = (wave_uniform() + (int)id) & 3, c = lane & 15, q = lane >> 4;
     const int ch = (int)(id % (unsigned)p.n_chunk);
@@ -335,19 +340,27 @@ __device__ void delta_prep(const HelixDeltaParams& p) {
 // wait for one another.
 // KEEP: no outputs and no waves for them; the states before the chunks and D are stored (fp32)
 // for the backward pass.
-template <typename T, int NK, bool ODD, bool KEEP, int NC>
-__device__ void delta_walk(const HelixDeltaParams& p) {
-    constexpr int NPL = dr_planes<T>, NO = dr_out_planes<T>, NT = NK / 64, KS = NK / 32;
-    constexpr int COLS = 16 * NC, VP = COLS + 16 / sizeof(T);   // columns of the workgroup; rows of V and of outputs in LDS
-    __shared__ __attribute__((aligned(16))) __bf16 sK[NPL * DR_C * NK];
-    __shared__ __attribute__((aligned(16))) __bf16 sS[3 * COLS * NK];
-    __shared__ __attribute__((aligned(16))) __bf16 sR[3 * COLS * DR_C], sU[3 * COLS * DR_C], sD[KEEP ? 8 : NO * COLS * DR_C];
-    __shared__ __attribute__((aligned(16))) T sV[DR_C][VP];
-    __shared__ __attribute__((aligned(16))) float sDec[2][HELIX_DR_DECAY / 4];
+template <typename T, int NK, bool KEEP, int NC>
+struct WalkLds {
+    static constexpr int COLS = 16 * NC;   // columns of the workgroup
     typedef typename std::conditional<KEEP, float, T>::type Out;   // D, or o
-    __shared__ __attribute__((aligned(16))) Out sOut[DR_C][COLS + 16 / sizeof(Out)];
+    __bf16 k[dr_planes<T> * DR_C * NK], s[3 * COLS * NK], r[3 * COLS * DR_C], u[3 * COLS * DR_C];
+    __bf16 d[KEEP ? 8 : dr_out_planes<T> * COLS * DR_C];
+    T v[DR_C][COLS + 16 / sizeof(T)];
+    float dec[2][HELIX_DR_DECAY / 4];
+    Out out[DR_C][COLS + 16 / sizeof(Out)];
+};
+template <typename T, int NK, bool ODD, bool KEEP, int NC>
+__device__ void delta_walk(const HelixDeltaParams& p, WalkLds<T, NK, KEEP, NC>& lds) {
+    constexpr int NPL = dr_planes<T>, NO = dr_out_planes<T>, NT = NK / 64, KS = NK / 32;
+    constexpr int COLS = 16 * NC;
+    typedef typename WalkLds<T, NK, KEEP, NC>::Out Out;
+    __bf16 *const sK = lds.k, *const sS = lds.s, *const sR = lds.r, *const sU = lds.u, *const sD = lds.d;
+    auto& sV = lds.v;
+    auto& sDec = lds.dec;
+    auto& sOut = lds.out;
     const int tid = threadIdx.x & 255, lane = lane_id(), w = wave_uniform() & 3, c = lane & 15, q = lane >> 4;
-    const unsigned id = xcd_logical_id(blockIdx.x, gridDim.x);   // a head's slices share an XCD's cache
+    const unsigned id = xcd_logical_id(blockIdx.x, p.n_walk);   // a head's slices share an XCD's cache
     const int slice = (int)(id % (unsigned)p.n_slice);
     const unsigned sh = id / (unsigned)p.n_slice;
     const int seq = (int)(sh / (unsigned)p.n_head), h = (int)(sh % (unsigned)p.n_head), hk = h / p.share;
@@ -589,6 +602,36 @@ __device__ void delta_walk(const HelixDeltaParams& p) {
     }
     dr_barrier();
     if (p.s) put_state(make_rsrc_u(p.s + (long long)sh * N * P, state_bytes));
+}
+
+template <typename T, int NK, bool ODD, bool BWD>
+__device__ void prep_kernel(const HelixDeltaParams& p) {
+    __shared__ __attribute__((aligned(16))) PrepLds<T, NK> lds;
+    delta_prep<T, NK, ODD, BWD>(p, blockIdx.x, lds);
+}
+template <typename T, int NK, bool ODD, bool KEEP, int NC>
+__device__ void walk_kernel(const HelixDeltaParams& p) {
+    __shared__ __attribute__((aligned(16))) WalkLds<T, NK, KEEP, NC> lds;
+    delta_walk<T, NK, ODD, KEEP, NC>(p, lds);
+}
+
+// A walk whose workgroups leave room on every CU, and behind it the operands of the chunks that the next walk takes.
+template <typename T, int NK, bool ODD>
+__device__ void delta_walk_ahead(const HelixDeltaParams& p) {
+    if constexpr (sizeof(T) == 4) return walk_kernel<T, NK, ODD, false, 1>(p);   // (fp32's take a CU's LDS and registers)
+    __shared__ __attribute__((aligned(16))) union {
+        WalkLds<T, NK, false, 1> walk;
+        PrepLds<T, NK> prep;
+    } lds;
+    if (blockIdx.x < p.n_walk) return delta_walk<T, NK, ODD, false, 1>(p, lds.walk);
+    if (threadIdx.x >= 256) return;   // (barriers wait for the waves that are left)
+    HelixDeltaParams n = p;
+    n.chunk0 += n.n_chunk;
+    n.n_chunk = n.n_next;
+    n.x = n.next_x;
+    n.p = n.next_p;
+    n.decay = n.next_decay;
+    delta_prep<T, NK, ODD, false>(n, blockIdx.x - p.n_walk, lds.prep);
 }
 
 // ---- backward -----------------------------------------------------------------------------
@@ -1287,15 +1330,15 @@ __device__ void delta_grad(const HelixDeltaParams& p) {
     extern "C" __global__ __launch_bounds__(256) void helix_delta_steps_##TAG##_##NK(HelixDeltaParams p) { delta_steps<T, NK / 16>(p); }
 // _s: rows of an odd width. _c16, _c32: columns of a workgroup.
 #define DR_KERNELS(TAG, T, NK, SUF, ODD)                                                                                                                    \
-    extern "C" __global__ __launch_bounds__(256) void helix_delta_prep_##TAG##_##NK##SUF(HelixDeltaParams p) { delta_prep<T, NK, ODD, false>(p); }          \
-    extern "C" __global__ __launch_bounds__(256) void helix_delta_prep_bwd_##TAG##_##NK##SUF(HelixDeltaParams p) { delta_prep<T, NK, ODD, true>(p); }       \
+    extern "C" __global__ __launch_bounds__(256) void helix_delta_prep_##TAG##_##NK##SUF(HelixDeltaParams p) { prep_kernel<T, NK, ODD, false>(p); }          \
+    extern "C" __global__ __launch_bounds__(256) void helix_delta_prep_bwd_##TAG##_##NK##SUF(HelixDeltaParams p) { prep_kernel<T, NK, ODD, true>(p); }       \
     extern "C" __global__ __launch_bounds__(640, 5) void helix_delta_pairs_##TAG##_##NK##SUF(HelixDeltaParams p) { delta_pairs<T, NK, ODD>(p); }               \
     extern "C" __global__ __launch_bounds__(512) void helix_delta_grad_##TAG##_##NK##SUF(HelixDeltaParams p) { delta_grad<T, NK, ODD>(p); }                 \
-    extern "C" __global__ __launch_bounds__(512) void helix_delta_walk_##TAG##_##NK##SUF##_c16(HelixDeltaParams p) { delta_walk<T, NK, ODD, false, 1>(p); } \
-    extern "C" __global__ __launch_bounds__(512) void helix_delta_keep_##TAG##_##NK##SUF##_c16(HelixDeltaParams p) { delta_walk<T, NK, ODD, true, 1>(p); }  \
+    extern "C" __global__ __launch_bounds__(512, sizeof(T) == 4 ? 2 : 4) void helix_delta_walk_##TAG##_##NK##SUF##_c16(HelixDeltaParams p) { delta_walk_ahead<T, NK, ODD>(p); } \
+    extern "C" __global__ __launch_bounds__(512) void helix_delta_keep_##TAG##_##NK##SUF##_c16(HelixDeltaParams p) { walk_kernel<T, NK, ODD, true, 1>(p); }  \
     extern "C" __global__ __launch_bounds__(512) void helix_delta_back_##TAG##_##NK##SUF##_c16(HelixDeltaParams p) { delta_back<T, NK, ODD, 1>(p); }        \
-    extern "C" __global__ __launch_bounds__(512) void helix_delta_walk_##TAG##_##NK##SUF##_c32(HelixDeltaParams p) { delta_walk<T, NK, ODD, false, 2>(p); } \
-    extern "C" __global__ __launch_bounds__(512, 4) void helix_delta_keep_##TAG##_##NK##SUF##_c32(HelixDeltaParams p) { delta_walk<T, NK, ODD, true, 2>(p); }
+    extern "C" __global__ __launch_bounds__(512) void helix_delta_walk_##TAG##_##NK##SUF##_c32(HelixDeltaParams p) { walk_kernel<T, NK, ODD, false, 2>(p); } \
+    extern "C" __global__ __launch_bounds__(512, 4) void helix_delta_keep_##TAG##_##NK##SUF##_c32(HelixDeltaParams p) { walk_kernel<T, NK, ODD, true, 2>(p); }
 // (fp32 of 128 keys and 32 columns would not fit in LDS.)
 #define DR_BACK(TAG, T, NK, SUF, ODD)                                                                                                                \
     extern "C" __global__ __launch_bounds__(512) void helix_delta_back_##TAG##_##NK##SUF##_c32(HelixDeltaParams p) { delta_back<T, NK, ODD, 2>(p); }

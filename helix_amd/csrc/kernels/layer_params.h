@@ -192,6 +192,12 @@ typedef struct {
     double*      pair_g;    /* [sequence x head][chunk][64] what the triangles bring G */
     float*       pair_b;    /* and beta, with Z . V                            */
     float*       tri;       /* [sequence x qk head][chunk][2][10][256] their gradients, by blocks */
+    /* Of a walk: its workgroups. The launch's others form the operands of the n_next chunks that follow, here. */
+    unsigned     n_walk;
+    int          n_next;
+    char*        next_x;
+    char*        next_p;
+    float*       next_decay;
 } HelixDeltaParams;
 
 #endif

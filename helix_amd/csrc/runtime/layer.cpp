@@ -892,6 +892,8 @@ std::string delta_form(const A& a, bool steps = false) {
 }
 
 // Columns of the state that a workgroup of the walks has: 32 where that still gives every CU a workgroup.
+// (2048 tokens, bf16, 128 keys x 64, us with 16 | 32, forward and backward: 64 heads 95 | 101, 297 | 329; 128 heads
+// 130 | 116, 556 | 503; 256 heads 293 | 252, 1103 | 953. fp32, 64 keys x 128: 64 heads 133 | 115, 509 | 428.)
 int delta_columns(long long heads, int n_val) { return n_val > 16 && heads * ceil_div(n_val, 32) >= 256 ? 32 : 16; }
 
 // The most tokens that go one by one, by the workgroups that their kernel has. One by one a token costs 1.1 to 1.4 us where
@@ -904,10 +906,20 @@ int delta_steps(long long heads, int n_val, int io) {
     return (io == HELIX_F32 ? 2 : 1) * (groups < 256 ? 6 : groups < 384 ? 10 : 16);
 }
 
+// Whether a long call goes in segments, and the walk of each takes along the kernel that forms the next one's operands: where
+// walks leave CUs room for it (16 bits, at most three workgroups of 16 columns for two CUs) and there is less to form than to
+// walk. Segments of 2048 chunks of heads at least, whose operands take as long as some launches. Measured, us in one piece |
+// in segments, bf16: 8192 tokens of 64 heads of 128 x 64 330 | 300; of 96 heads 509 | 430; 32768 tokens of 32 heads of
+// 128 x 128 1072 | 943; with 8 heads and 64 chunks a segment 225 | 228. f16: 477 | 458, 670 | 655, 1618 | 1401. Past the
+// bounds, f16: 127 heads of 128 x 64 836 | 907, 128 of 128 x 32 630 | 704, 256 of 128 x 16 877 | 1047.
+bool delta_ahead(long long heads, int columns, const helix_delta_rule_args& a) {
+    return columns == 16 && a.io_dtype != HELIX_F32 && heads <= 96 && heads * ceil_div(a.n_val, 16) <= 384;
+}
+
 // How the rule is cut: segments of `chunks` chunks of every sequence, whose operands scratch holds at a time.
 struct DeltaPlan {
-    int n_chunk = 0, chunks = 0, columns = 0;
-    size_t x_at = 0, p_at = 0, decay_at = 0, bytes = 0;
+    int n_chunk = 0, chunks = 0, columns = 0, sets = 1;   // sets: of a segment's operands
+    size_t x_at = 0, p_at = 0, decay_at = 0, set = 0, bytes = 0;
 };
 // Scratch of a segment: up to a gigabyte, and one chunk of every sequence where that is more.
 constexpr size_t kDeltaScratch = (size_t)1 << 30;
@@ -921,9 +933,17 @@ DeltaPlan delta_plan(const helix_delta_rule_args& a) {
     p.n_chunk = (int)ceil_div(a.n_tok, HELIX_DR_CHUNK);
     p.chunks = (int)std::min<size_t>(p.n_chunk, std::max<size_t>(1, kDeltaScratch / each));
     p.columns = delta_columns((long long)sh, a.n_val);
+    if (delta_ahead((long long)sh, p.columns, a)) {
+        const int least = (int)std::max<size_t>(32, 2048 / sh), n = std::max<int>(p.n_chunk / least, (int)ceil_div(2 * p.n_chunk, p.chunks));
+        if (n > 2) {
+            p.chunks = (int)ceil_div(p.n_chunk, n);
+            p.sets = 2;
+        }
+    }
     p.p_at = p.x_at + sh * p.chunks * x;
     p.decay_at = p.p_at + sh * p.chunks * pp;
-    p.bytes = p.decay_at + sh * p.chunks * HELIX_DR_DECAY;
+    p.set = p.decay_at + sh * p.chunks * HELIX_DR_DECAY;
+    p.bytes = p.sets * p.set;
     return p;
 }
 
@@ -1004,16 +1024,25 @@ extern "C" helix_status helix_delta_rule_encode(helix_ctx* ctx, void* stream, co
         const hipFunction_t prep = kernel(ctx, "helix_delta_prep_" + form),
                             walk = kernel(ctx, "helix_delta_walk_" + form + "_c" + std::to_string(plan.columns));
         p.n_slice = (int)ceil_div(a->n_val, plan.columns);
-        const unsigned gp = grid(sh * plan.chunks, kDeltaThreads), gw = grid(sh * p.n_slice, 2 * kDeltaThreads);
+        const unsigned gw = grid(sh * p.n_slice, 2 * kDeltaThreads);
+        grid(gw + sh * plan.chunks, 2 * kDeltaThreads);
         char* sc = static_cast<char*>(a->scratch);
-        p.x = sc + plan.x_at;
-        p.p = sc + plan.p_at;
-        p.decay = reinterpret_cast<float*>(sc + plan.decay_at);
         const OnDevice on(ctx->device);
-        for (p.chunk0 = 0; p.chunk0 < plan.n_chunk; p.chunk0 += plan.chunks) {
-            p.n_chunk = std::min(plan.chunks, plan.n_chunk - p.chunk0);
-            launch(prep, stream, p.n_chunk == plan.chunks ? gp : (unsigned)(sh * p.n_chunk), 1, kDeltaThreads, p);
-            launch(walk, stream, gw, 1, 2 * kDeltaThreads, p);
+        p.n_walk = gw;
+        for (int first = 0, set = 0; first < plan.n_chunk; first += plan.chunks, set ^= plan.sets - 1) {
+            auto at = [&](int i, size_t off) { return sc + i * plan.set + off; };
+            const int other = set ^ (plan.sets - 1), next = first + plan.chunks;
+            p.x = at(set, plan.x_at);
+            p.p = at(set, plan.p_at);
+            p.decay = reinterpret_cast<float*>(at(set, plan.decay_at));
+            p.chunk0 = first;
+            p.n_chunk = std::min(plan.chunks, plan.n_chunk - first);
+            if (!first || plan.sets == 1) launch(prep, stream, (unsigned)(sh * p.n_chunk), 1, kDeltaThreads, p);
+            p.n_next = plan.sets == 2 ? std::max(0, std::min(plan.chunks, plan.n_chunk - next)) : 0;
+            p.next_x = at(other, plan.x_at);
+            p.next_p = at(other, plan.p_at);
+            p.next_decay = reinterpret_cast<float*>(at(other, plan.decay_at));
+            launch(walk, stream, gw + (unsigned)(sh * p.n_next), 1, 2 * kDeltaThreads, p);
             p.s0 = p.s;   // the next segment starts where this one ends
         }
     });
@@ -1116,6 +1145,7 @@ extern "C" helix_status helix_delta_rule_backward_encode(helix_ctx* ctx, void* s
                             grad = kernel(ctx, "helix_delta_grad_" + form);
         const long long sh = (long long)a->n_seq * a->n_head, sk = (long long)a->n_seq * a->n_qk_head;
         const unsigned gw = grid(sh * p.n_slice, 2 * kDeltaThreads);
+        p.n_walk = gw;
         grid(sh * plan.chunks, kDeltaThreads);
         grid(sk * plan.chunks, kDeltaPairThreads);
         const OnDevice on(ctx->device);

@@ -97,6 +97,13 @@ def test_long_and_many(gpu, S, L, Hk, H, N, P, dtype):
     check_backward(*p)
 
 
+# Long calls of some heads go in segments whose operands are formed while the one before is walked.
+@pytest.mark.parametrize("S,L,Hk,H,N,P,dtype", [(1, 6200, 2, 64, 8, 8, torch.bfloat16), (1, 6145, 64, 64, 66, 17, torch.float16),
+                                                (2, 6300, 3, 48, 16, 24, torch.bfloat16), (1, 12800, 16, 32, 65, 4, torch.bfloat16)])
+def test_segments_ahead(gpu, S, L, Hk, H, N, P, dtype):
+    check(*problem(S, L, Hk, H, N, P, dtype, seed=L, packed_rows=S == 1))
+
+
 # Where many heads share the machine, more tokens go one by one: up to 32 in fp32, more than LDS has the keys of at a time.
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("S,L,Hk,H,N,P", [(4, 10, 4, 64, 32, 16), (4, 11, 4, 64, 32, 16), (4, 20, 4, 64, 32, 16), (4, 21, 4, 64, 32, 16),
