@@ -7,8 +7,11 @@
 // below the diagonal and X = (1 + A)^-1 diag(beta),
 //     D = X (V - e^G K S),   O = scale (e^G Q S + (E . Q K') D),   S' = e^(G_63) S + (e^(G_63 - G) K)' D
 // X and P = scale E . Q K' need no state: helix_delta_prep_* forms them for all chunks at once.
-// helix_delta_walk_* then goes through the chunks of a sequence, a workgroup for 16 columns of
-// a head's state, whose columns do not meet.
+// helix_delta_walk_* then goes through the chunks of a sequence, a workgroup for 16 or 32 columns
+// of a head's state, whose columns do not meet.
+//
+// 8192 tokens of 64 heads of 128 x 64 in bf16: 300 us, where memory's part is 34 (174 MB). 28 us
+// form the first segment's operands, the rest are 128 steps of the walk (below).
 #include "delta_common.h"
 
 namespace {
@@ -18,7 +21,9 @@ namespace {
 // A workgroup has 64 columns of a state in registers: lane 16 kg + cl of wave w columns
 // 4 cl .. + 3 of the rows 16 i + 4 w + kg. k'S and q'S are summed over a token's old state
 // together (q'S' = e^g q'S + (q . k) d), so that a token meets one barrier. Memory binds a
-// batch of single tokens (the state is read and written once), latency few sequences.
+// batch of single tokens (the state is read and written once: 64 of 64 heads of 128 x 64, 270 MB,
+// 47 us, 5.7 TB/s with the cache's part), latency few sequences (one token of one 5.2 us, 1.1 to
+// 1.4 for each that follows: the loads of its row, nine sums over lanes and a meeting in LDS).
 template <typename T, int NR>
 __device__ void delta_steps(const HelixDeltaParams& p) {
     __shared__ float kq[2][HELIX_DR_STEPS][16 * NR];
@@ -143,7 +148,8 @@ constexpr int DR_LD = DR_C + 4;   // fp32 rows of a chunk's square matrices in L
 //     T_iw = -T_ii (sum over j of A_ij T_jw),  w <= j < i
 // on fp32 matrix instructions, T_jw staying in the registers it was formed in. (Products of powers of A would be fewer steps,
 // but keys that repeat make the powers large, and they cancel.) BWD: T' and P' with X, without P.
-// Four workgroups a CU hide one another's chains: P takes the place of K's parts in LDS, T that of A.
+// Four workgroups a CU hide one another's chains: P takes the place of K's parts in LDS, T that of A (8192 tokens of 64 heads,
+// bf16, 128 keys: two workgroups a CU 169 us, four 87, of which 50 are the writing of 30 KB a chunk).
 template <typename T, int NK>
 struct PrepLds {
     union {
@@ -336,8 +342,15 @@ __device__ void delta_prep(const HelixDeltaParams& p, unsigned id, PrepLds<T, NK
 // a row. A chunk is three barriers; what does not depend on the state is loaded as soon as the
 // chunk before has used its registers. K is read in the first phase alone (K' as operands of
 // the third is kept in registers), so that its next rows can take its place.
-// What bounds it is the chain of a chunk, with the latencies of LDS and of three products that
-// wait for one another.
+// What bounds it is the chain of a chunk: three products that wait for one another, each with its
+// way through LDS, beside 64 KB of loads into the CU. 8192 tokens of 64 heads of 128 x 64, bf16,
+// 128 chunks: 2 us a chunk; without the loads 1.4, the state's waves alone 1.2. The two kinds
+// of waves took a prompt from 555 us to 424; LDS rows turned by their number (dr_at), V and outputs
+// through LDS and prep's workgroups to 348. No gain: loads two
+// chunks ahead, LDS reads moved before the barriers, priorities of the waves. Slower: Q S in the
+// second phase (353 us for 275 of the walk), K's operands straight from memory (370).
+// With 32 columns a product's operands are loaded and split once for two blocks of columns
+// (128 chunks of 256 heads, KEEP: 240 us with 16 columns, 167 with 32 and two workgroups a CU).
 // KEEP: no outputs and no waves for them; the states before the chunks and D are stored (fp32)
 // for the backward pass.
 template <typename T, int NK, bool KEEP, int NC>
@@ -615,7 +628,8 @@ __device__ void walk_kernel(const HelixDeltaParams& p) {
     delta_walk<T, NK, ODD, KEEP, NC>(p, lds);
 }
 
-// A walk whose workgroups leave room on every CU, and behind it the operands of the chunks that the next walk takes.
+// A walk whose workgroups leave room on every CU, and behind it the operands of the chunks that the next walk takes: 32 chunks
+// of 64 heads take 63 us by themselves, and 79 with the next 32 chunks' operands, which are 28 in a launch of their own.
 template <typename T, int NK, bool ODD>
 __device__ void delta_walk_ahead(const HelixDeltaParams& p) {
     if constexpr (sizeof(T) == 4) return walk_kernel<T, NK, ODD, false, 1>(p);   // (fp32's take a CU's LDS and registers)
@@ -643,7 +657,8 @@ __device__ void delta_walk_ahead(const HelixDeltaParams& p) {
 // from the last chunk to the first: helix_delta_back_*, spread and laid out as the walk. Its
 // second four waves bring K, Q and dO and form what does not wait for E, P' dO and
 // scale (e^G Q)' dO of the chunk after the one that the first four are at. It leaves E and Z for
-// the kernels below.
+// the kernels below. Bound as the walk is: 32 chunks of 256 heads of 128 x 64, bf16, 333 us with 16
+// columns a workgroup, 256 with 32.
 template <typename T, int NK, bool ODD, int NC>
 __device__ void delta_back(const HelixDeltaParams& p) {
     constexpr int NPL = dr_planes<T>, NT = NK / 64, KS = NK / 32, COLS = 16 * NC;
@@ -928,7 +943,9 @@ __device__ void delta_back(const HelixDeltaParams& p) {
 // sum of e^(G_63 - G) (K . L) and e^(G_63) (S . E); in fp64, as neighbours nearly cancel.
 // Two kernels, as the registers do not hold both: the triangles first (helix_delta_pairs_*, a
 // wave a block of 16 x 16), which read dO, Z, D and V, then the products with the states
-// (helix_delta_grad_*), which read dO, Z and D again, S and E.
+// (helix_delta_grad_*), which read dO, Z and D again, S and E. Memory binds both, behind the LDS
+// that dO, Z and D pass: 8192 chunks of heads of 128 x 64, bf16, 440 MB in 130 us and 970 MB
+// in 300, 3.3 TB/s.
 template <typename T, int NK, bool ODD>
 __device__ void delta_pairs(const HelixDeltaParams& p) {
     constexpr int NPL = dr_planes<T>, TH = 640;

@@ -8,6 +8,12 @@
 // lanes and by shuffles above; the variance is the mean square of x - mean, not a
 // difference of sums. A last vector that the group's end cuts is read whole where the
 // row goes on behind it, and is written in pieces of four, two and one.
+//
+// Measured: 8192 rows of 64 groups of 64 with a gate, bf16 into 8 bits, 168 MB in 40 us
+// (4.2 TB/s, as a large copy of that share of writes); 2871 rows of 27 groups of 192 in
+// fp32, 120 MB in 24 us; backward, 32768 rows of 80 groups of 64 with a gate, bf16,
+// 1.7 GB in 370 us (4.6 TB/s). Kept from it, as slower: the next row's loads before this
+// one's sums, tails read by element in the same instructions as whole vectors (492 us).
 #include "layer_common.h"
 
 namespace {

@@ -282,7 +282,9 @@ extern "C" helix_status helix_norm_backward_encode(helix_ctx* ctx, void* stream,
 
 namespace {
 
-// Lanes and vectors of eight of a group of `width` channels (kernels/group_norm.hip).
+// Lanes and vectors of eight of a group of `width` channels (kernels/group_norm.hip): the least that hold it. 8192 rows of 4096
+// channels with a gate in bf16, us with these | the next ones, forward and backward: groups of 64 39 | 71, 78 | 105; of 1024
+// (two vectors a lane, or a workgroup) 35 | 64, 93 | 103; of 2048 (a workgroup) 38 | 59, 77 | 131.
 struct GroupForm {
     int lanes = 256, vectors = 4;
     std::string name() const { return "_l" + std::to_string(lanes) + "_" + std::to_string(vectors); }
@@ -311,7 +313,8 @@ struct GroupBwdPlan {
     long long gx = 0, parts = 0;   // workgroups along the groups and along the rows
 };
 // A workgroup has as many groups side by side as there are, up to its room, and rows in what is left of it. Along the
-// rows four workgroups a CU in all, of two rows a slot at least.
+// rows four workgroups a CU in all (32768 rows of 80 groups of 64, with a gate, bf16: two 448 us, four 370, eight 372), of two
+// rows a slot at least (256 rows of 64 groups of 64: of one 12.4 us, of two 11.2, of four 13.0).
 GroupBwdPlan group_bwd_plan(long long rows, int dim, int groups) {
     GroupBwdPlan p;
     p.form = group_form(dim / groups);
