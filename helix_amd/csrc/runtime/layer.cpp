@@ -882,8 +882,16 @@ bool delta_shape(const A& a) {
     need(dtype_ok(a.io_dtype), "io_dtype is none of HELIX_F32, HELIX_F16 and HELIX_BF16");
     need(std::isfinite(a.scale), "scale is not finite");
     if (!a.n_seq || !a.n_head) return false;
+    need((long long)a.n_seq * a.n_head < 1LL << 31, "n_seq * n_head out of range", HELIX_ERR_UNSUPPORTED_SHAPE);
     need(a.n_qk_head >= 1 && a.n_head % a.n_qk_head == 0, "n_qk_head does not divide n_head", HELIX_ERR_UNSUPPORTED_SHAPE);
     return true;
+}
+
+// Whether sizes are such as a call takes and needs scratch for (those that it refuses may be any here).
+template <typename A>
+bool delta_sizes(const A& a) {
+    return a.n_seq > 0 && a.n_head > 0 && a.n_tok > 0 && a.n_key > 0 && a.n_key <= HELIX_DELTA_MAX_KEY && a.n_val > 0 &&
+           a.n_val <= HELIX_DELTA_MAX_VAL && (long long)a.n_seq * a.n_head < 1LL << 31;
 }
 
 int delta_keys(int n_key) { return n_key <= 64 ? 64 : 128; }   // of the kernels
@@ -929,8 +937,7 @@ constexpr size_t kDeltaScratch = (size_t)1 << 30;
 
 DeltaPlan delta_plan(const helix_delta_rule_args& a) {
     DeltaPlan p;
-    if (a.n_seq <= 0 || a.n_head <= 0 || a.n_key <= 0 || a.n_val <= 0) return p;
-    if (a.n_tok <= delta_steps((long long)a.n_seq * a.n_head, a.n_val, a.io_dtype)) return p;
+    if (!delta_sizes(a) || a.n_tok <= delta_steps((long long)a.n_seq * a.n_head, a.n_val, a.io_dtype)) return p;
     const size_t sh = (size_t)a.n_seq * a.n_head, out = a.io_dtype == HELIX_F32 ? 3 : 2;
     const size_t x = 6 * 3 * HELIX_DR_FRAG, pp = 6 * out * HELIX_DR_FRAG, each = sh * (x + pp + HELIX_DR_DECAY);
     p.n_chunk = (int)ceil_div(a.n_tok, HELIX_DR_CHUNK);
@@ -1064,7 +1071,7 @@ constexpr size_t kDeltaBwdScratch = (size_t)2 << 30;
 
 DeltaBwdPlan delta_bwd_plan(const helix_delta_rule_backward_args& a) {
     DeltaBwdPlan p;
-    if (a.n_seq <= 0 || a.n_head <= 0 || a.n_tok <= 0 || a.n_key <= 0 || a.n_val <= 0) return p;
+    if (!delta_sizes(a)) return p;
     const size_t sh = (size_t)a.n_seq * a.n_head, x = 6 * 3 * HELIX_DR_FRAG;
     auto up = [](size_t bytes) { return (bytes + 255) & ~(size_t)255; };
     const size_t state = (size_t)a.n_key * a.n_val * 4, rows = (size_t)HELIX_DR_CHUNK * a.n_val * 4;

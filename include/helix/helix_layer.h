@@ -312,7 +312,8 @@ helix_status helix_gated_scan_backward_encode(helix_ctx* ctx, void* stream,
  * (n_seq, n_head, n_key, n_val). */
 typedef struct {
     int32_t      n_seq, n_tok;       /* n_seq or n_head 0: nothing is done;
-                                        n_tok 0: s = s0                       */
+                                        n_tok 0: s = s0; n_seq * n_head is
+                                        below 2^31                            */
     int32_t      n_qk_head, n_head;  /* the first divides the second          */
     int32_t      n_key, n_val;
     int32_t      io_dtype;           /* of q, k, v and o                      */

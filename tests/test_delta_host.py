@@ -61,6 +61,7 @@ BOTH = [
     (dict(s0=P + 2), HELIX_ERR_INVALID_ARG), (dict(tok=-1), HELIX_ERR_INVALID_ARG), (dict(seq=-1), HELIX_ERR_INVALID_ARG),
     (dict(tok=1 << 24), HELIX_ERR_UNSUPPORTED_SHAPE), (dict(scratch=0), HELIX_ERR_SCRATCH_TOO_SMALL),
     (dict(nbytes=16), HELIX_ERR_SCRATCH_TOO_SMALL), (dict(scratch=P + 4), HELIX_ERR_INVALID_ARG),
+    (dict(S=1 << 28, Hk=1 << 28, H=1 << 28), HELIX_ERR_UNSUPPORTED_SHAPE), (dict(S=1 << 16, H=1 << 15, Hk=1), HELIX_ERR_UNSUPPORTED_SHAPE),
     (dict(tok=0, seq=0), HELIX_ERR_NO_DEVICE),   # inputs may be one row, read for every token
 ]
 
@@ -96,6 +97,14 @@ def test_scratch_stays_bounded():
         assert size(make(S=1, L=65, Hk=1, H=1)) > small
         assert size(make(S=4, L=1 << 18, Hk=8, H=64, N=128, V=64)) <= most
         assert size(make(S=4, L=1 << 18, Hk=8, H=64, N=128, V=64)) > most // 3
+
+
+@pytest.mark.parametrize("sizes", [dict(S=1 << 28, Hk=1 << 28, H=1 << 28), dict(S=1 << 16, H=1 << 15), dict(N=1 << 30, V=1 << 30),
+                                   dict(N=129), dict(V=-1), dict(S=-1, H=-1), dict(L=-(1 << 31)), dict(Hk=-1, H=0)])
+def test_scratch_of_sizes_that_are_refused(sizes):
+    # A size for every argument; what a call then refuses needs none.
+    L = abi.lib()
+    assert L.helix_delta_rule_scratch_size(args(**sizes)) == 0 and L.helix_delta_rule_backward_scratch_size(bwd(**sizes)) == 0
 
 
 def test_oracle_gradients_by_differentiation():
