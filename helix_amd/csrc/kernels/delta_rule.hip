@@ -1345,17 +1345,17 @@ __device__ void delta_grad(const HelixDeltaParams& p) {
 
 #define DR_STEPS(TAG, T, NK)                                                                                                             \
     extern "C" __global__ __launch_bounds__(256) void helix_delta_steps_##TAG##_##NK(HelixDeltaParams p) { delta_steps<T, NK / 16>(p); }
-// _s: rows of an odd width. _c16, _c32: columns of a workgroup.
+// _s: rows of an odd width. _c16, _c32: columns of a workgroup. Waves a SIMD where LDS has room for two workgroups a CU.
 #define DR_KERNELS(TAG, T, NK, SUF, ODD)                                                                                                                    \
     extern "C" __global__ __launch_bounds__(256) void helix_delta_prep_##TAG##_##NK##SUF(HelixDeltaParams p) { prep_kernel<T, NK, ODD, false>(p); }          \
     extern "C" __global__ __launch_bounds__(256) void helix_delta_prep_bwd_##TAG##_##NK##SUF(HelixDeltaParams p) { prep_kernel<T, NK, ODD, true>(p); }       \
-    extern "C" __global__ __launch_bounds__(640, 5) void helix_delta_pairs_##TAG##_##NK##SUF(HelixDeltaParams p) { delta_pairs<T, NK, ODD>(p); }               \
+    extern "C" __global__ __launch_bounds__(640, sizeof(T) == 4 && NK == 128 ? 3 : 5) void helix_delta_pairs_##TAG##_##NK##SUF(HelixDeltaParams p) { delta_pairs<T, NK, ODD>(p); }               \
     extern "C" __global__ __launch_bounds__(512) void helix_delta_grad_##TAG##_##NK##SUF(HelixDeltaParams p) { delta_grad<T, NK, ODD>(p); }                 \
     extern "C" __global__ __launch_bounds__(512, sizeof(T) == 4 ? 2 : 4) void helix_delta_walk_##TAG##_##NK##SUF##_c16(HelixDeltaParams p) { delta_walk_ahead<T, NK, ODD>(p); } \
     extern "C" __global__ __launch_bounds__(512) void helix_delta_keep_##TAG##_##NK##SUF##_c16(HelixDeltaParams p) { walk_kernel<T, NK, ODD, true, 1>(p); }  \
     extern "C" __global__ __launch_bounds__(512) void helix_delta_back_##TAG##_##NK##SUF##_c16(HelixDeltaParams p) { delta_back<T, NK, ODD, 1>(p); }        \
     extern "C" __global__ __launch_bounds__(512) void helix_delta_walk_##TAG##_##NK##SUF##_c32(HelixDeltaParams p) { walk_kernel<T, NK, ODD, false, 2>(p); } \
-    extern "C" __global__ __launch_bounds__(512, 4) void helix_delta_keep_##TAG##_##NK##SUF##_c32(HelixDeltaParams p) { walk_kernel<T, NK, ODD, true, 2>(p); }
+    extern "C" __global__ __launch_bounds__(512, sizeof(WalkLds<T, NK, true, 2>) <= 81920 ? 4 : 2) void helix_delta_keep_##TAG##_##NK##SUF##_c32(HelixDeltaParams p) { walk_kernel<T, NK, ODD, true, 2>(p); }
 // (fp32 of 128 keys and 32 columns would not fit in LDS.)
 #define DR_BACK(TAG, T, NK, SUF, ODD)                                                                                                                \
     extern "C" __global__ __launch_bounds__(512) void helix_delta_back_##TAG##_##NK##SUF##_c32(HelixDeltaParams p) { delta_back<T, NK, ODD, 2>(p); }
