@@ -72,6 +72,11 @@ def backward(do, q, k, v, g, beta, s0, ds, scale):
     size["ds0"] = top
     share = H // Hk
     dq, dk = dq.unflatten(2, (Hk, share)).sum(3), dk.unflatten(2, (Hk, share)).sum(3)
+    # The heads that share are added one after another in fp32. With terms of norm s each, size = s sqrt(share), the sum of
+    # the first h has s sqrt(h), and its rounding E of that: together E s sqrt(1 + 2 + .. + share) = E size sqrt(share / 2),
+    # beside the 32 E of the size that the terms are off by.
+    for n in ("dq", "dk"):
+        size[n] *= (1 + (share / 2) ** 0.5 / 32) ** 2   # (sizes are squares here)
     return (dq, dk, dv, dg, db, dS), {n: float(x) ** 0.5 for n, x in size.items()}
 
 

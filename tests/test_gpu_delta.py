@@ -90,7 +90,9 @@ def test_heads(gpu, S, Hk, H, L, dtype):
 
 
 @pytest.mark.parametrize("S,L,Hk,H,N,P,dtype", [(1, 1500, 2, 4, 128, 64, torch.bfloat16), (3, 1003, 2, 2, 64, 48, torch.float32),
-                                                (1, 2050, 1, 1, 96, 20, torch.float16), (64, 1, 2, 8, 128, 64, torch.bfloat16)])
+                                                (1, 2050, 1, 1, 96, 20, torch.float16), (64, 1, 2, 8, 128, 64, torch.bfloat16),
+                                                (1, 70, 1, 1, 128, 65536, torch.bfloat16), (1, 2, 1, 2, 128, 65535, torch.float16),
+                                                (1, 66, 1, 8192, 1, 1, torch.float32), (70000, 7, 1, 1, 2, 2, torch.bfloat16)])
 def test_long_and_many(gpu, S, L, Hk, H, N, P, dtype):
     p = problem(S, L, Hk, H, N, P, dtype, seed=7)
     check(*p)
@@ -102,6 +104,52 @@ def test_long_and_many(gpu, S, L, Hk, H, N, P, dtype):
                                                 (2, 6300, 3, 48, 16, 24, torch.bfloat16), (1, 12800, 16, 32, 65, 4, torch.bfloat16)])
 def test_segments_ahead(gpu, S, L, Hk, H, N, P, dtype):
     check(*problem(S, L, Hk, H, N, P, dtype, seed=L, packed_rows=S == 1))
+
+
+def test_segments_ahead_in_place_and_captured(gpu):
+    # The state goes from segment to segment through s, which may be s0; a graph's segments follow each other on every replay.
+    q, k, v, g, beta, s0 = problem(1, 6211, 2, 64, 24, 16, torch.bfloat16, seed=80)
+    o, s = delta_rule(q, k, v, g, beta, s0)
+    state, out = s0.clone(), torch.empty_like(o)
+    encode(q, k, v, g, beta, state, out, state)
+    assert torch.equal(out, o) and torch.equal(state, s)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = delta_rule(q, k, v, g, beta, s0)
+    for i in range(3):
+        v.copy_(normal(*v.shape, seed=81 + i, dtype=v.dtype))
+        eager = [t.clone() for t in delta_rule(q, k, v, g, beta, s0)]
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, eager))
+
+
+@pytest.mark.parametrize("L,tok,seq", [(300, (1 << 23) + 24, 64), (3, 200, (1 << 31) + 72), (70, 200, (1 << 31) + 72)])
+def test_offsets_past_32_bits(gpu, L, tok, seq):
+    # Tokens, or sequences, that lie gigabytes apart in one buffer; only what belongs to them is written.
+    S, Hk, H, N, P = 2, 1, 2, 24, 32
+    p = problem(S, L, Hk, H, N, P, torch.bfloat16, seed=95)
+    d = normal(S, L, H, P, seed=96, dtype=torch.bfloat16)
+    want, grads = delta_rule(*p), delta_rule_backward(d, *p)
+    q, k, v, g, beta, s0 = p
+    if seq < tok:
+        seq *= 3   # (the sequences' rows side by side)
+    buf = torch.empty((S - 1) * seq + L * tok, dtype=torch.bfloat16, device="cuda")
+
+    def place(t, at):
+        heads, width = t.shape[2:]
+        view = buf.as_strided((S, L, heads, width), (seq, tok, width, 1), at)
+        view.copy_(t)
+        return view
+
+    far = [place(t, at) for t, at in ((q, 0), (k, N), (v, 2 * N))]
+    got = delta_rule(*far, g, beta, s0)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    assert all(torch.equal(a, b) for a, b in zip(delta_rule_backward(d, *far, g, beta, s0), grads))
+    out = buf.as_strided((S, L, H, P), (seq, tok, P, 1), 2 * N)   # (over v's place, which another copy of it then is read from)
+    state = torch.empty_like(want[1])
+    encode(far[0], far[1], v, g, beta, s0, out, state)
+    assert torch.equal(out, want[0]) and torch.equal(state, want[1]) and torch.equal(far[0], q) and torch.equal(far[1], k)
 
 
 # Where many heads share the machine, more tokens go one by one: up to 32 in fp32, more than LDS has the keys of at a time.
