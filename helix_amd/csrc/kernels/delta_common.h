@@ -6,7 +6,8 @@
 //
 // An fp32 value is three bf16 parts, and a product of two the six products of parts i, j
 // with i + j <= 2: fp32's own accuracy (helix_common.h). A bf16 element is one part, an f16
-// one two, exactly.
+// one two, exactly. Operands that only a 16-bit output takes are in three parts too: an output
+// may be a small difference of large sums, which two parts (2^-18 of each) would be seen in.
 #ifndef HELIX_DELTA_COMMON_H
 #define HELIX_DELTA_COMMON_H
 
@@ -26,14 +27,12 @@ HELIX_DEV int dr_at(int row, int chunk) {
 }
 
 template <typename T> constexpr int dr_planes = __is_same(T, float) ? 3 : __is_same(T, _Float16) ? 2 : 1;
-// Parts of operands that meet outputs of the storage type alone: two (2^-18) where that has 16 bits.
-template <typename T> constexpr int dr_out_planes = __is_same(T, float) ? 3 : 2;
 
-// Products of the parts i, j with i + j < MAX, smallest first.
-template <int NA, int NB, int MAX = 3>
+// Products of the parts i, j with i + j < 3, smallest first.
+template <int NA, int NB>
 HELIX_DEV f32x4 dr_mfma(const bf16x8 (&a)[NA], const bf16x8 (&b)[NB], f32x4 acc) {
 #pragma unroll
-    for (int sum = MAX - 1; sum >= 0; --sum)
+    for (int sum = 2; sum >= 0; --sum)
 #pragma unroll
         for (int i = sum; i >= 0; --i)
             if (i < NA && sum - i < NB) acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[i], b[sum - i], acc, 0, 0, 0);
@@ -55,19 +54,19 @@ struct DrAcc1 {
 };
 template <int NC> struct DrAccOf { typedef DrAcc type; };
 template <> struct DrAccOf<2> { typedef DrAcc1 type; };
-template <int NA, int NB, int MAX = 3>
+template <int NA, int NB>
 HELIX_DEV void dr_mfma(const bf16x8 (&a)[NA], const bf16x8 (&b)[NB], DrAcc1& acc) {
-    acc.s = dr_mfma<NA, NB, MAX>(a, b, acc.s);
+    acc.s = dr_mfma<NA, NB>(a, b, acc.s);
 }
 // Of products with NPL parts on both sides; one part's have one sum.
 template <int NPL>
 HELIX_DEV f32x4 dr_sum(const DrAcc& a) { return NPL == 1 ? a.s[0] : a.sum(); }
-template <int NA, int NB, int MAX = 3>
+template <int NA, int NB>
 HELIX_DEV void dr_mfma(const bf16x8 (&a)[NA], const bf16x8 (&b)[NB], DrAcc& acc) {
 #pragma unroll
     for (int i = 0; i < NA; ++i)
 #pragma unroll
-        for (int sum = MAX - 1; sum >= 0; --sum)
+        for (int sum = 2; sum >= 0; --sum)
             if (sum - i >= 0 && sum - i < NB)
                 acc.s[sum] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[i], b[sum - i], acc.s[sum], 0, 0, 0);
 }

@@ -161,7 +161,7 @@ struct PrepLds {
 };
 template <typename T, int NK, bool ODD, bool BWD>
 __device__ void delta_prep(const HelixDeltaParams& p, unsigned id, PrepLds<T, NK>& lds) {
-    constexpr int NPL = dr_planes<T>, NO = dr_out_planes<T>;
+    constexpr int NPL = dr_planes<T>;
     __bf16* const sK = lds.k;
     auto &sP = lds.p, &sA = lds.a;
     auto& sD = lds.d;
@@ -297,13 +297,12 @@ __device__ void delta_prep(const HelixDeltaParams& p, unsigned id, PrepLds<T, NK
         }
     __syncthreads();
     // Fragments: row 16 w + c, columns 32 ks + 8 q ..
-    auto emit = [&](char* to, int frag, const float (&v)[8], auto parts) {
-        constexpr int M = decltype(parts)::value;
-        bf16x8 o[M];
-        dr_split8<M>(v, o);
+    auto emit = [&](char* to, int frag, const float (&v)[8]) {
+        bf16x8 o[3];
+        dr_split8<3>(v, o);
 #pragma unroll
-        for (int k = 0; k < M; ++k)
-            *reinterpret_cast<bf16x8*>(to + ((long long)id * 6 * M + frag * M + k) * HELIX_DR_FRAG + 16 * lane) = o[k];
+        for (int k = 0; k < 3; ++k)
+            *reinterpret_cast<bf16x8*>(to + ((long long)id * 18 + frag * 3 + k) * HELIX_DR_FRAG + 16 * lane) = o[k];
     };
 #pragma unroll
     for (int ks = 0; ks < 2; ++ks) {
@@ -312,21 +311,21 @@ __device__ void delta_prep(const HelixDeltaParams& p, unsigned id, PrepLds<T, NK
         if (ks == 0 || w > 1) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) v[e] = sA[row][col + e] * sB[col + e];
-            emit(p.x, dr_low(w, ks), v, std::integral_constant<int, 3>{});
+            emit(p.x, dr_low(w, ks), v);
             if constexpr (!BWD) {
 #pragma unroll
                 for (int e = 0; e < 8; ++e) v[e] = sP[row][col + e];
-                emit(p.p, dr_low(w, ks), v, std::integral_constant<int, NO>{});
+                emit(p.p, dr_low(w, ks), v);
             }
         }
         if constexpr (BWD) {
             if (ks == 1 || w < 2) {
 #pragma unroll
                 for (int e = 0; e < 8; ++e) v[e] = sA[col + e][row];
-                emit(p.tt, dr_up(w, ks), v, std::integral_constant<int, 3>{});
+                emit(p.tt, dr_up(w, ks), v);
 #pragma unroll
                 for (int e = 0; e < 8; ++e) v[e] = sP[col + e][row];
-                emit(p.pt, dr_up(w, ks), v, std::integral_constant<int, 3>{});
+                emit(p.pt, dr_up(w, ks), v);
             }
         }
     }
@@ -358,14 +357,14 @@ struct WalkLds {
     static constexpr int COLS = 16 * NC;   // columns of the workgroup
     typedef typename std::conditional<KEEP, float, T>::type Out;   // D, or o
     __bf16 k[dr_planes<T> * DR_C * NK], s[3 * COLS * NK], r[3 * COLS * DR_C], u[3 * COLS * DR_C];
-    __bf16 d[KEEP ? 8 : dr_out_planes<T> * COLS * DR_C];
+    __bf16 d[KEEP ? 8 : 3 * COLS * DR_C];
     T v[DR_C][COLS + 16 / sizeof(T)];
     float dec[2][HELIX_DR_DECAY / 4];
     Out out[DR_C][COLS + 16 / sizeof(Out)];
 };
 template <typename T, int NK, bool ODD, bool KEEP, int NC>
 __device__ void delta_walk(const HelixDeltaParams& p, WalkLds<T, NK, KEEP, NC>& lds) {
-    constexpr int NPL = dr_planes<T>, NO = dr_out_planes<T>, NT = NK / 64, KS = NK / 32;
+    constexpr int NPL = dr_planes<T>, NT = NK / 64, KS = NK / 32;
     constexpr int COLS = 16 * NC;
     typedef typename WalkLds<T, NK, KEEP, NC>::Out Out;
     __bf16 *const sK = lds.k, *const sS = lds.s, *const sR = lds.r, *const sU = lds.u, *const sD = lds.d;
@@ -426,7 +425,7 @@ __device__ void delta_walk(const HelixDeltaParams& p, WalkLds<T, NK, KEEP, NC>& 
             }
         };
         Raw8<T> qr[KS];
-        bf16x8 pf[2][NO];
+        bf16x8 pf[2][3];
         auto load_q = [&](int ch) {
             const int tid = vgpr_fresh(threadIdx.x) & 255, c = tid & 15, q = (tid & 63) >> 4;
             ch = min(ch, last);
@@ -435,12 +434,12 @@ __device__ void delta_walk(const HelixDeltaParams& p, WalkLds<T, NK, KEEP, NC>& 
             for (int s = 0; s < KS; ++s) qr[s] = rq.load8(16 * w + c, 32 * s + 8 * q);
         };
         auto load_p = [&](int ch) {
-            const char* pp = p.p + (base + min(ch, last)) * (6 * NO * HELIX_DR_FRAG) + 16 * lane;
+            const char* pp = p.p + (base + min(ch, last)) * (6 * 3 * HELIX_DR_FRAG) + 16 * lane;
 #pragma unroll
             for (int ks = 0; ks < 2; ++ks) {
                 if (ks && w < 2) break;
 #pragma unroll
-                for (int k = 0; k < NO; ++k) pf[ks][k] = *reinterpret_cast<const bf16x8*>(pp + (dr_low(w, ks) * NO + k) * HELIX_DR_FRAG);
+                for (int k = 0; k < 3; ++k) pf[ks][k] = *reinterpret_cast<const bf16x8*>(pp + (dr_low(w, ks) * 3 + k) * HELIX_DR_FRAG);
             }
         };
         load_k(0);
@@ -458,12 +457,12 @@ __device__ void delta_walk(const HelixDeltaParams& p, WalkLds<T, NK, KEEP, NC>& 
 #pragma unroll
                 for (int s = 0; s < KS; ++s) {
                     const int col = 32 * s + 8 * q;
-                    bf16x8 a[NPL], b[NO];
+                    bf16x8 a[NPL], b[3];
                     dr_operand<T>(qr[s], N - col, a);
 #pragma unroll
                     for (int n = 0; n < NC; ++n) {
-                        dr_get8<NO, NK, COLS>(sS, 16 * n + c, col, b);
-                        dr_mfma<NPL, NO, NO>(a, b, qs[n]);
+                        dr_get8<3, NK, COLS>(sS, 16 * n + c, col, b);
+                        dr_mfma<NPL, 3>(a, b, qs[n]);
                     }
                 }
                 const f32x4 start = p.scale * *reinterpret_cast<const f32x4*>(&sDec[ch & 1][row0]);
@@ -482,9 +481,9 @@ __device__ void delta_walk(const HelixDeltaParams& p, WalkLds<T, NK, KEEP, NC>& 
                     if (ks && w < 2) break;
 #pragma unroll
                     for (int n = 0; n < NC; ++n) {
-                        bf16x8 b[NO];
-                        dr_get8<NO, DR_C, COLS>(sD, 16 * n + c, 32 * ks + 8 * q, b);
-                        o[n] = dr_mfma<NO, NO, NO>(pf[ks], b, o[n]);
+                        bf16x8 b[3];
+                        dr_get8<3, DR_C, COLS>(sD, 16 * n + c, 32 * ks + 8 * q, b);
+                        o[n] = dr_mfma<3, 3>(pf[ks], b, o[n]);
                     }
                 }
                 load_p(ch + 1);
@@ -591,7 +590,7 @@ __device__ void delta_walk(const HelixDeltaParams& p, WalkLds<T, NK, KEEP, NC>& 
 #pragma unroll
                 for (int r = 0; r < 4; ++r) sOut[row0 + r][16 * n + c] = D[r];
             } else {
-                dr_put4<NO, DR_C, COLS>(sD, 16 * n + c, row0, D[0], D[1], D[2], D[3]);
+                dr_put4<3, DR_C, COLS>(sD, 16 * n + c, row0, D[0], D[1], D[2], D[3]);
             }
         }
         load_x(ch + 1);
@@ -1119,9 +1118,9 @@ __device__ void delta_pairs(const HelixDeltaParams& p) {
 // 64 columns at a time; K, Q and the triangles at the end.
 template <typename T, int NK, bool ODD>
 __device__ void delta_grad(const HelixDeltaParams& p) {
-    constexpr int NPL = dr_planes<T>, NO = dr_out_planes<T>, W = NK / 16, TH = 512;
+    constexpr int NPL = dr_planes<T>, W = NK / 16, TH = 512;
     constexpr int RG = 8 / W, RT = 4 / RG;   // groups of waves along the tokens, and row tiles of a wave
-    constexpr int kKQ = 2 * NPL * DR_C * NK, kM = 2 * NO * DR_C * DR_C, kOZD = (NPL + 6) * DR_C * DR_C;
+    constexpr int kKQ = 2 * NPL * DR_C * NK, kM = 3 * DR_C * DR_C, kOZD = (NPL + 6) * DR_C * DR_C;
     __shared__ __attribute__((aligned(16))) __bf16 sBig[kKQ + kM > kOZD ? kKQ + kM : kOZD];
     __shared__ __attribute__((aligned(16))) float sDec[HELIX_DR_DECAY / 4];
     __shared__ float sDot[3][W][DR_C], sSE[W];
@@ -1297,36 +1296,37 @@ __device__ void delta_grad(const HelixDeltaParams& p) {
         dr_put8<NPL, NK, DR_C>(sK, row, col, k);
         dr_put8<NPL, NK, DR_C>(sQ, row, col, qq);
     }
-    for (int x = w; x < 20; x += 8) {
-        // Stored by columns: M[j][i]; 0 above the diagonal.
-        const int k = x % 10, tb = (k >= 1) + (k >= 3) + (k >= 6), jb = k - tb * (tb + 1) / 2;
-        const f32x4 m = *reinterpret_cast<const f32x4*>(p.tri + (long long)id * (2 * 10 * 256) + 256 * x + 4 * lane);
-        __bf16* to = sM + x / 10 * NO * DR_C * DR_C;
-        dr_put4<NO, DR_C, DR_C>(to, 16 * jb + c, 16 * tb + 4 * q, m[0], m[1], m[2], m[3]);
-        if (tb != jb) dr_put4<NO, DR_C, DR_C>(to, 16 * tb + c, 16 * jb + 4 * q, 0.0f, 0.0f, 0.0f, 0.0f);
-    }
-    __syncthreads();
 #pragma unroll
-    for (int ks = 0; ks < 2; ++ks) {
-        bf16x8 bk[NPL], bq[NPL];
-        dr_get8_t<NPL, NK, DR_C>(sK, 32 * ks + 8 * q, n0, c, bk);
-        dr_get8_t<NPL, NK, DR_C>(sQ, 32 * ks + 8 * q, n0, c, bq);
+    for (int m = 0; m < 2; ++m) {   // M_P, then M_A
+        if (m) __syncthreads();   // M_P has been read
+        for (int x = w; x < 10; x += 8) {
+            // Stored by columns: M[j][i]; 0 above the diagonal.
+            const int tb = (x >= 1) + (x >= 3) + (x >= 6), jb = x - tb * (tb + 1) / 2;
+            const f32x4 v = *reinterpret_cast<const f32x4*>(p.tri + (long long)id * (2 * 10 * 256) + 256 * (10 * m + x) + 4 * lane);
+            dr_put4<3, DR_C, DR_C>(sM, 16 * jb + c, 16 * tb + 4 * q, v[0], v[1], v[2], v[3]);
+            if (tb != jb) dr_put4<3, DR_C, DR_C>(sM, 16 * tb + c, 16 * jb + 4 * q, 0.0f, 0.0f, 0.0f, 0.0f);
+        }
+        __syncthreads();
 #pragma unroll
-        for (int i = 0; i < RT; ++i) {
-            bf16x8 a[NO];
-            const int tile = i0 + i;
-            // M[i][j] over j: columns of what is stored; M'[j][i] over i: its rows.
-            if (2 * ks <= tile) {
-                dr_get8_t<NO, DR_C, DR_C>(sM, 32 * ks + 8 * q, 16 * tile, c, a);
-                dq[i] = dr_mfma<NO, NPL, NO>(a, bk, dq[i]);
-                dr_get8_t<NO, DR_C, DR_C>(sM + NO * DR_C * DR_C, 32 * ks + 8 * q, 16 * tile, c, a);
-                dk[i] = dr_mfma<NO, NPL, NO>(a, bk, dk[i]);
-            }
-            if (2 * ks + 1 >= tile) {
-                dr_get8<NO, DR_C, DR_C>(sM, 16 * tile + c, 32 * ks + 8 * q, a);
-                dk[i] = dr_mfma<NO, NPL, NO>(a, bq, dk[i]);
-                dr_get8<NO, DR_C, DR_C>(sM + NO * DR_C * DR_C, 16 * tile + c, 32 * ks + 8 * q, a);
-                dk[i] = dr_mfma<NO, NPL, NO>(a, bk, dk[i]);
+        for (int ks = 0; ks < 2; ++ks) {
+            bf16x8 bk[NPL], bq[NPL];
+            dr_get8_t<NPL, NK, DR_C>(sK, 32 * ks + 8 * q, n0, c, bk);
+            if (m == 0) dr_get8_t<NPL, NK, DR_C>(sQ, 32 * ks + 8 * q, n0, c, bq);
+#pragma unroll
+            for (int i = 0; i < RT; ++i) {
+                bf16x8 a[3];
+                const int tile = i0 + i;
+                // M[i][j] over j: columns of what is stored; M'[j][i] over i: its rows.
+                if (2 * ks <= tile) {
+                    dr_get8_t<3, DR_C, DR_C>(sM, 32 * ks + 8 * q, 16 * tile, c, a);
+                    if (m == 0) dq[i] = dr_mfma<3, NPL>(a, bk, dq[i]);
+                    else dk[i] = dr_mfma<3, NPL>(a, bk, dk[i]);
+                }
+                if (2 * ks + 1 >= tile) {
+                    dr_get8<3, DR_C, DR_C>(sM, 16 * tile + c, 32 * ks + 8 * q, a);
+                    if (m == 0) dk[i] = dr_mfma<3, NPL>(a, bq, dk[i]);
+                    else dk[i] = dr_mfma<3, NPL>(a, bk, dk[i]);
+                }
             }
         }
     }

@@ -938,8 +938,7 @@ constexpr size_t kDeltaScratch = (size_t)1 << 30;
 DeltaPlan delta_plan(const helix_delta_rule_args& a) {
     DeltaPlan p;
     if (!delta_sizes(a) || a.n_tok <= delta_steps((long long)a.n_seq * a.n_head, a.n_val, a.io_dtype)) return p;
-    const size_t sh = (size_t)a.n_seq * a.n_head, out = a.io_dtype == HELIX_F32 ? 3 : 2;
-    const size_t x = 6 * 3 * HELIX_DR_FRAG, pp = 6 * out * HELIX_DR_FRAG, each = sh * (x + pp + HELIX_DR_DECAY);
+    const size_t sh = (size_t)a.n_seq * a.n_head, x = 6 * 3 * HELIX_DR_FRAG, each = sh * (2 * x + HELIX_DR_DECAY);
     p.n_chunk = (int)ceil_div(a.n_tok, HELIX_DR_CHUNK);
     p.chunks = (int)std::min<size_t>(p.n_chunk, std::max<size_t>(1, kDeltaScratch / each));
     p.columns = delta_columns((long long)sh, a.n_val);
@@ -951,7 +950,7 @@ DeltaPlan delta_plan(const helix_delta_rule_args& a) {
         }
     }
     p.p_at = p.x_at + sh * p.chunks * x;
-    p.decay_at = p.p_at + sh * p.chunks * pp;
+    p.decay_at = p.p_at + sh * p.chunks * x;
     p.set = p.decay_at + sh * p.chunks * HELIX_DR_DECAY;
     p.bytes = p.sets * p.set;
     return p;
