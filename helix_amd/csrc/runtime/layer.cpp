@@ -891,7 +891,8 @@ bool delta_shape(const A& a) {
 template <typename A>
 bool delta_sizes(const A& a) {
     return a.n_seq > 0 && a.n_head > 0 && a.n_tok > 0 && a.n_key > 0 && a.n_key <= HELIX_DELTA_MAX_KEY && a.n_val > 0 &&
-           a.n_val <= HELIX_DELTA_MAX_VAL && (long long)a.n_seq * a.n_head < 1LL << 31;
+           a.n_val <= HELIX_DELTA_MAX_VAL && (long long)a.n_seq * a.n_head < 1LL << 31 && a.n_qk_head > 0 &&
+           a.n_head % a.n_qk_head == 0;
 }
 
 int delta_keys(int n_key) { return n_key <= 64 ? 64 : 128; }   // of the kernels
@@ -1074,7 +1075,7 @@ DeltaBwdPlan delta_bwd_plan(const helix_delta_rule_backward_args& a) {
     const size_t sh = (size_t)a.n_seq * a.n_head, x = 6 * 3 * HELIX_DR_FRAG;
     auto up = [](size_t bytes) { return (bytes + 255) & ~(size_t)255; };
     const size_t state = (size_t)a.n_key * a.n_val * 4, rows = (size_t)HELIX_DR_CHUNK * a.n_val * 4;
-    const size_t tri = 2 * 10 * 256 * 4, sk = (size_t)a.n_seq * std::max(1, a.n_qk_head);
+    const size_t tri = 2 * 10 * 256 * 4, sk = (size_t)a.n_seq * a.n_qk_head;
     p.n_chunk = (int)ceil_div(a.n_tok, HELIX_DR_CHUNK);
     p.chunks = (int)std::min<size_t>(p.n_chunk,
                                      std::max<size_t>(1, kDeltaBwdScratch / (sh * (3 * x + HELIX_DR_DECAY + 2 * state + 2 * rows + 12 * HELIX_DR_CHUNK) + sk * tri)));
