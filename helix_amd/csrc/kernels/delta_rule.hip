@@ -802,7 +802,7 @@ __device__ void delta_back(const HelixDeltaParams& p) {
             const int tid = vgpr_fresh(threadIdx.x) & 255, lane = tid & 63, c = tid & 15, row0 = tid >> 4 << 2;
             const f32x4 beta = *reinterpret_cast<const f32x4*>(&sDec[ch & 1][128 + row0]);
             const Rows<float> rz(p.keep_z, (base + ch) * DR_C * P, P, DR_C, P);
-            const Rows<T> rv(p.dv, (((long long)seq * p.n_tok + first(ch)) * p.n_head + h) * P, (long long)p.n_head * P, tokens(ch), P);
+            const Rows<T> rv(p.dv, (((long long)seq * p.n_tok + first(ch)) * p.row_head + h) * P, (long long)p.row_head * P, tokens(ch), P);
 #pragma unroll
             for (int n = 0; n < NC; ++n) {
                 const f32x4 Z = sPO[n][w][lane];
@@ -1278,7 +1278,7 @@ __device__ void delta_grad(const HelixDeltaParams& p) {
             const double incl = wave_incl_sum(own);
             const double dg = __shfl(incl, 63, 64) - incl + own;
             if (lane < len) {
-                const long long to = ((long long)seq * p.n_tok + t0 + lane) * p.n_head + h;
+                const long long to = ((long long)seq * p.n_tok + t0 + lane) * p.row_head + h;
                 p.dg[to] = (float)dg;
                 p.dbeta[to] = db - start * dot[1];
             }
@@ -1330,8 +1330,8 @@ __device__ void delta_grad(const HelixDeltaParams& p) {
             }
         }
     }
-    const long long to = (((long long)seq * p.n_tok + t0) * p.n_qk + hk) * N;
-    const Rows<T> oq(p.dq, to, (long long)p.n_qk * N, len, N), ok(p.dk, to, (long long)p.n_qk * N, len, N);
+    const long long to = (((long long)seq * p.n_tok + t0) * p.row_qk + hk) * N;
+    const Rows<T> oq(p.dq, to, (long long)p.row_qk * N, len, N), ok(p.dk, to, (long long)p.row_qk * N, len, N);
 #pragma unroll
     for (int i = 0; i < RT; ++i)
 #pragma unroll

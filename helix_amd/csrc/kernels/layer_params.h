@@ -178,6 +178,7 @@ typedef struct {
     long long    seq_g, tok_g, seq_b, tok_b, seq_o, tok_o, head_o;   /* (o, or its gradient) */
     int          n_seq, n_tok, n_qk, n_head, share, n_key, n_val;   /* share = n_head / n_qk */
     float        scale;
+    int          row_qk, row_head;   /* heads of a row of dq and dk, and of dv, dg and dbeta (a launch may have a part of them) */
     /* Chunked: the chunks chunk0 .. chunk0 + n_chunk - 1 of every sequence. */
     int          chunk0, n_chunk, n_slice;   /* n_slice: workgroups of a walk for each head */
     char*        x;         /* [sequence x head][chunk] fragments of X         */

@@ -985,6 +985,8 @@ HelixDeltaParams delta_params(const A& a) {
     p.n_qk = a.n_qk_head;
     p.n_head = a.n_head;
     p.share = a.n_head / a.n_qk_head;
+    p.row_qk = a.n_qk_head;
+    p.row_head = a.n_head;
     p.n_key = a.n_key;
     p.n_val = a.n_val;
     p.scale = a.scale;
@@ -1060,39 +1062,93 @@ extern "C" helix_status helix_delta_rule_encode(helix_ctx* ctx, void* stream, co
 
 namespace {
 
-// The backward pass: what a segment's chunks leave for its kernels, and the states that the segments start from.
-struct DeltaBwdPlan {
-    int n_chunk = 0, chunks = 0, n_seg = 0;
-    size_t x_at = 0, tt_at = 0, pt_at = 0, decay_at = 0, s_at = 0, e_at = 0, d_at = 0, z_at = 0, pg_at = 0, pb_at = 0, tri_at = 0, start_at = 0, bytes = 0;
+// Heads of a call that go together, part after part through the same scratch: those of `seqs` sequences or, where `heads` are
+// fewer than there are, so many of one sequence's. A part's heads do not meet another's.
+struct DeltaParts {
+    int seqs = 0, heads = 0;
+    long long all() const { return (long long)seqs * heads; }
 };
-// Scratch of a segment: up to two gigabytes, and one chunk of every sequence where that is more. More than one segment forms
-// its states twice.
-constexpr size_t kDeltaBwdScratch = (size_t)2 << 30;
+// Parts of at most `most` heads, as alike as may be; the heads that share one of the queries' stay together.
+DeltaParts delta_parts(long long n_seq, long long n_qk, long long share, long long most) {
+    const long long n_head = n_qk * share;
+    DeltaParts p{1, (int)n_head};
+    if (most >= n_head) p.seqs = (int)ceil_div(n_seq, ceil_div(n_seq, most / n_head));
+    else p.heads = (int)(share * ceil_div(n_qk, ceil_div(n_qk, std::max(1LL, most / share))));
+    return p;
+}
+
+// What is the whole call's in p, for the part that begins at a sequence and a head (a call's last parts may be smaller).
+HelixDeltaParams delta_part(HelixDeltaParams p, const DeltaParts& part, long long seq, long long head, size_t es) {
+    const long long qk = head / p.share, state = (seq * p.n_head + head) * p.n_key * p.n_val;
+    advance(p.q, seq * p.seq_q + qk * p.head_q, es);
+    advance(p.k, seq * p.seq_k + qk * p.head_k, es);
+    advance(p.v, seq * p.seq_v + head * p.head_v, es);
+    advance(p.g, seq * p.seq_g + head, 4);
+    advance(p.beta, seq * p.seq_b + head, 4);
+    advance(p.d_o, seq * p.seq_o + head * p.head_o, es);
+    for (const float** s : {&p.s0, &p.d_s}) advance(*s, state, 4);
+    advance(p.ds0, state, 4);
+    const long long row = seq * p.n_tok;   // dense ones
+    advance(p.dq, (row * p.n_qk + qk) * p.n_key, es);
+    advance(p.dk, (row * p.n_qk + qk) * p.n_key, es);
+    advance(p.dv, (row * p.n_head + head) * p.n_val, es);
+    advance(p.dg, row * p.n_head + head, 4);
+    advance(p.dbeta, row * p.n_head + head, 4);
+    p.n_seq = (int)std::min<long long>(part.seqs, p.n_seq - seq);
+    p.n_head = (int)std::min<long long>(part.heads, p.n_head - head);
+    p.n_qk = p.n_head / p.share;
+    return p;
+}
+
+// The backward pass: its parts, what a segment's chunks leave for its kernels, and the states that the segments start from.
+struct DeltaBwdPlan {
+    DeltaParts part;
+    int n_chunk = 0, chunks = 0, n_seg = 0, columns = 0;
+    size_t x_at = 0, tt_at = 0, pt_at = 0, decay_at = 0, s_at = 0, e_at = 0, d_at = 0, z_at = 0, pg_at = 0, pb_at = 0, tri_at = 0, start_at = 0, state = 0, bytes = 0;
+};
+// Scratch of a segment: up to two gigabytes, and up to one for the states that a part's segments start from. Where a call wants
+// more it goes in parts: heads with all their tokens, if those that fit give every CU a workgroup of 32 columns, else as many as
+// do that, in segments, whose states are formed twice. bf16, heads of 128 x 64, ms with parts of whole tokens | with all heads
+// in segments: 32 x 4096 tokens of 64 heads 16.4 | 19.9, 1000 x 256 of 16 heads 6.4 | 9.4. Segments, with workgroups for half
+// the CUs | for each | two for each: 2 x 65536 tokens of 64 heads 23.8 | 20.8 | 20.8, 4 x 32768 23.9 | 20.2 | 19.7. (The heads
+// of one query head may take more than two gigabytes for a chunk, or than one for the states.)
+constexpr size_t kDeltaBwdScratch = (size_t)2 << 30, kDeltaBwdStates = (size_t)1 << 30;
 
 DeltaBwdPlan delta_bwd_plan(const helix_delta_rule_backward_args& a) {
     DeltaBwdPlan p;
     if (!delta_sizes(a)) return p;
-    const size_t sh = (size_t)a.n_seq * a.n_head, x = 6 * 3 * HELIX_DR_FRAG;
+    const size_t x = 6 * 3 * HELIX_DR_FRAG, tri = 2 * 10 * 256 * 4, share = a.n_head / a.n_qk_head, sh = (size_t)a.n_seq * a.n_head;
     auto up = [](size_t bytes) { return (bytes + 255) & ~(size_t)255; };
     const size_t state = (size_t)a.n_key * a.n_val * 4, rows = (size_t)HELIX_DR_CHUNK * a.n_val * 4;
-    const size_t tri = 2 * 10 * 256 * 4, sk = (size_t)a.n_seq * a.n_qk_head;
+    const size_t each = 3 * x + HELIX_DR_DECAY + 2 * state + 2 * rows + 12 * HELIX_DR_CHUNK + tri / share + 1;   // of a chunk of a head
     p.n_chunk = (int)ceil_div(a.n_tok, HELIX_DR_CHUNK);
-    p.chunks = (int)std::min<size_t>(p.n_chunk,
-                                     std::max<size_t>(1, kDeltaBwdScratch / (sh * (3 * x + HELIX_DR_DECAY + 2 * state + 2 * rows + 12 * HELIX_DR_CHUNK) + sk * tri)));
+    auto chunks = [&](size_t heads) { return (int)std::min<size_t>(p.n_chunk, std::max<size_t>(1, kDeltaBwdScratch / (heads * each))); };
+    size_t most = sh;
+    if (chunks(sh) < p.n_chunk || sh * each > kDeltaBwdScratch) {
+        most = std::max<size_t>(kDeltaBwdScratch / (p.n_chunk * each), ceil_div(256, ceil_div(a.n_val, 32)));
+        while (most > share && (most * each > kDeltaBwdScratch || (ceil_div(p.n_chunk, chunks(most)) - 1) * most * state > kDeltaBwdStates)) most /= 2;
+    }
+    most = std::min<size_t>(most, most_groups(2 * kDeltaThreads) / ceil_div(a.n_val, 16));
+    p.part = delta_parts(a.n_seq, a.n_qk_head, share, (long long)most);
+    const size_t heads = p.part.all(), qk = heads / share;
+    p.chunks = chunks(heads);
     p.n_seg = (int)ceil_div(p.n_chunk, p.chunks);
-    const size_t each = sh * p.chunks;
-    p.tt_at = p.x_at + each * x;
-    p.pt_at = p.tt_at + each * x;
-    p.decay_at = p.pt_at + each * x;
-    p.s_at = p.decay_at + up(each * HELIX_DR_DECAY);
-    p.e_at = p.s_at + up(each * state);
-    p.d_at = p.e_at + up(each * state);
-    p.z_at = p.d_at + up(each * rows);
-    p.pg_at = p.z_at + up(each * rows);
-    p.pb_at = p.pg_at + each * HELIX_DR_CHUNK * 8;
-    p.tri_at = p.pb_at + each * HELIX_DR_CHUNK * 4;
-    p.start_at = p.tri_at + sk * p.chunks * tri;
-    p.bytes = p.start_at + (size_t)(p.n_seg - 1) * up(sh * state);
+    // (fp32 of 128 keys and 32 columns would not fit in LDS.)
+    p.columns = a.io_dtype == HELIX_F32 && a.n_key > 64 ? 16 : delta_columns((long long)heads, a.n_val);
+    const size_t of = heads * p.chunks;
+    p.tt_at = p.x_at + of * x;
+    p.pt_at = p.tt_at + of * x;
+    p.decay_at = p.pt_at + of * x;
+    p.s_at = p.decay_at + up(of * HELIX_DR_DECAY);
+    p.e_at = p.s_at + up(of * state);
+    p.d_at = p.e_at + up(of * state);
+    p.z_at = p.d_at + up(of * rows);
+    p.pg_at = p.z_at + up(of * rows);
+    p.pb_at = p.pg_at + of * HELIX_DR_CHUNK * 8;
+    p.tri_at = p.pb_at + of * HELIX_DR_CHUNK * 4;
+    p.start_at = p.tri_at + qk * p.chunks * tri;
+    p.state = up(heads * state);
+    p.bytes = p.start_at + (size_t)(p.n_seg - 1) * p.state;
     return p;
 }
 
@@ -1118,73 +1174,76 @@ extern "C" helix_status helix_delta_rule_backward_encode(helix_ctx* ctx, void* s
              "ds0 is NULL, or it or d_s not aligned to its elements");
         need((long long)a->n_head * a->n_val < (1LL << 31) / 64 / (long long)es && (long long)a->n_qk_head * a->n_key < (1LL << 31) / 64 / (long long)es,
              "64 tokens of dq, dk or dv span 2^31 bytes or more", HELIX_ERR_UNSUPPORTED_SHAPE);
-        const DeltaBwdPlan plan = delta_bwd_plan(*a);
+        DeltaBwdPlan plan = delta_bwd_plan(*a);
+        if (!a->n_tok) {
+            plan.columns = 16;
+            plan.part = delta_parts(a->n_seq, a->n_qk_head, a->n_head / a->n_qk_head, most_groups(2 * kDeltaThreads) / ceil_div(a->n_val, 16));
+        }
         need(plan.bytes == 0 || (a->scratch && a->scratch_bytes >= plan.bytes),
              "scratch smaller than helix_delta_rule_backward_scratch_size()", HELIX_ERR_SCRATCH_TOO_SMALL);
         need(aligned(a->scratch, 16), "scratch is not 16-byte aligned");
-        HelixDeltaParams p = delta_params(*a);
-        p.d_o = a->d_o;
-        p.d_s = a->d_s;
-        p.seq_o = a->seq_do;
-        p.tok_o = a->tok_do;
-        p.head_o = a->head_do;
-        p.dq = a->dq;
-        p.dk = a->dk;
-        p.dv = a->dv;
-        p.dg = a->dg;
-        p.dbeta = a->dbeta;
-        p.ds0 = a->ds0;
+        HelixDeltaParams call = delta_params(*a);
+        call.d_o = a->d_o;
+        call.d_s = a->d_s;
+        call.seq_o = a->seq_do;
+        call.tok_o = a->tok_do;
+        call.head_o = a->head_do;
+        call.dq = a->dq;
+        call.dk = a->dk;
+        call.dv = a->dv;
+        call.dg = a->dg;
+        call.dbeta = a->dbeta;
+        call.ds0 = a->ds0;
         char* sc = static_cast<char*>(a->scratch);
-        p.x = sc + plan.x_at;
-        p.tt = sc + plan.tt_at;
-        p.pt = sc + plan.pt_at;
-        p.decay = reinterpret_cast<float*>(sc + plan.decay_at);
-        p.keep_s = reinterpret_cast<float*>(sc + plan.s_at);
-        p.keep_e = reinterpret_cast<float*>(sc + plan.e_at);
-        p.keep_d = reinterpret_cast<float*>(sc + plan.d_at);
-        p.keep_z = reinterpret_cast<float*>(sc + plan.z_at);
-        p.pair_g = reinterpret_cast<double*>(sc + plan.pg_at);
-        p.pair_b = reinterpret_cast<float*>(sc + plan.pb_at);
-        p.tri = reinterpret_cast<float*>(sc + plan.tri_at);
-        // (fp32 of 128 keys and 32 columns would not fit in LDS.)
-        const int columns = a->io_dtype == HELIX_F32 && a->n_key > 64 ? 16 : delta_columns((long long)a->n_seq * a->n_head, a->n_val);
-        p.n_slice = (int)ceil_div(a->n_val, columns);
-        const std::string form = delta_form(*a), wide = form + "_c" + std::to_string(columns);
+        call.x = sc + plan.x_at;
+        call.tt = sc + plan.tt_at;
+        call.pt = sc + plan.pt_at;
+        call.decay = reinterpret_cast<float*>(sc + plan.decay_at);
+        call.keep_s = reinterpret_cast<float*>(sc + plan.s_at);
+        call.keep_e = reinterpret_cast<float*>(sc + plan.e_at);
+        call.keep_d = reinterpret_cast<float*>(sc + plan.d_at);
+        call.keep_z = reinterpret_cast<float*>(sc + plan.z_at);
+        call.pair_g = reinterpret_cast<double*>(sc + plan.pg_at);
+        call.pair_b = reinterpret_cast<float*>(sc + plan.pb_at);
+        call.tri = reinterpret_cast<float*>(sc + plan.tri_at);
+        call.n_slice = (int)ceil_div(a->n_val, plan.columns);
+        const std::string form = delta_form(*a), wide = form + "_c" + std::to_string(plan.columns);
         const hipFunction_t prep = kernel(ctx, "helix_delta_prep_bwd_" + form), keep = kernel(ctx, "helix_delta_keep_" + wide),
                             back = kernel(ctx, "helix_delta_back_" + wide), pairs = kernel(ctx, "helix_delta_pairs_" + form),
                             grad = kernel(ctx, "helix_delta_grad_" + form);
-        const long long sh = (long long)a->n_seq * a->n_head, sk = (long long)a->n_seq * a->n_qk_head;
-        const unsigned gw = grid(sh * p.n_slice, 2 * kDeltaThreads);
-        p.n_walk = gw;
-        grid(sh * plan.chunks, kDeltaThreads);
-        grid(sk * plan.chunks, kDeltaPairThreads);
+        grid(plan.part.all() * call.n_slice, 2 * kDeltaThreads);
+        grid(plan.part.all() * std::max(1, plan.chunks), kDeltaPairThreads);
         const OnDevice on(ctx->device);
-        if (!a->n_tok) {
-            launch(back, stream, gw, 1, 2 * kDeltaThreads, p);
-            return;
-        }
-        const size_t state = ((size_t)sh * a->n_key * a->n_val * 4 + 255) & ~(size_t)255;
-        // The state before segment i (i > 0).
-        auto start = [&](int i) { return reinterpret_cast<float*>(sc + plan.start_at + (size_t)(i - 1) * state); };
-        auto states = [&](int i) {
-            p.chunk0 = i * plan.chunks;
-            p.n_chunk = std::min(plan.chunks, plan.n_chunk - p.chunk0);
-            p.s0 = i ? start(i) : a->s0;
-            launch(prep, stream, (unsigned)(sh * p.n_chunk), 1, kDeltaThreads, p);
-            launch(keep, stream, gw, 1, 2 * kDeltaThreads, p);
+        // A part: the states that its segments start from (that of segment i > 0 at i - 1), then its segments from the last on.
+        auto run = [&](HelixDeltaParams p) {
+            const long long sh = (long long)p.n_seq * p.n_head, sk = (long long)p.n_seq * p.n_qk;
+            const unsigned gw = (unsigned)(sh * p.n_slice);
+            p.n_walk = gw;
+            const float* const s0 = p.s0;
+            auto start = [&](int i) { return reinterpret_cast<float*>(sc + plan.start_at + (size_t)(i - 1) * plan.state); };
+            auto states = [&](int i) {
+                p.chunk0 = i * plan.chunks;
+                p.n_chunk = std::min(plan.chunks, plan.n_chunk - p.chunk0);
+                p.s0 = i ? start(i) : s0;
+                launch(prep, stream, (unsigned)(sh * p.n_chunk), 1, kDeltaThreads, p);
+                launch(keep, stream, gw, 1, 2 * kDeltaThreads, p);
+            };
+            for (int i = 0; i + 1 < plan.n_seg; ++i) {
+                p.s = start(i + 1);
+                states(i);
+            }
+            p.s = nullptr;
+            for (int i = plan.n_seg - 1; i >= 0; --i) {
+                states(i);
+                launch(back, stream, gw, 1, 2 * kDeltaThreads, p);
+                launch(pairs, stream, (unsigned)(sk * p.n_chunk), 1, kDeltaPairThreads, p);
+                launch(grad, stream, (unsigned)(sk * p.n_chunk), 1, 2 * kDeltaThreads, p);
+                p.d_s = p.ds0;   // the segment before goes on from here
+            }
+            if (!plan.n_seg) launch(back, stream, gw, 1, 2 * kDeltaThreads, p);   // no tokens: ds0 = d_s
         };
-        for (int i = 0; i + 1 < plan.n_seg; ++i) {
-            p.s = start(i + 1);
-            states(i);
-        }
-        p.s = nullptr;
-        for (int i = plan.n_seg - 1; i >= 0; --i) {
-            states(i);
-            launch(back, stream, gw, 1, 2 * kDeltaThreads, p);
-            launch(pairs, stream, (unsigned)(sk * p.n_chunk), 1, kDeltaPairThreads, p);
-            launch(grad, stream, (unsigned)(sk * p.n_chunk), 1, 2 * kDeltaThreads, p);
-            p.d_s = p.ds0;   // the segment before goes on from here
-        }
+        for (long long seq = 0; seq < a->n_seq; seq += plan.part.seqs)
+            for (long long head = 0; head < a->n_head; head += plan.part.heads) run(delta_part(call, plan.part, seq, head, es));
     });
 }
 

@@ -33,3 +33,16 @@ def test_every_size_has_an_answer():
     for S, L, Hk, H in itertools.product(edge, repeat=4):
         for N, P in ((1, 1), (128, 3), (128, 1 << 16), (129, 1), (I32, I32), (0, 0)):
             sizes(S, L, Hk, H, N, P)
+
+
+GIB = 1 << 30
+
+
+# Many sequences, heads and tokens at once, each and together.
+@pytest.mark.parametrize("io", [0, 2])
+@pytest.mark.parametrize("a", [(64, 4096, 8, 64, 128, 64), (64, 8192, 4, 32, 128, 128), (256, 4096, 4, 32, 128, 128), (64, 8192, 8, 64, 128, 64),
+                               (64, 2048, 8, 64, 128, 64), (32, 4096, 8, 64, 128, 128), (256, 2048, 8, 64, 128, 128), (8, 1 << 17, 16, 64, 128, 64),
+                               (1, 1 << 20, 128, 128, 128, 128), (1, 1 << 21, 8, 64, 128, 64), (2, 1 << 22, 4, 4, 128, 256), (1, 4096, 2, 2, 128, 1 << 14),
+                               (100000, 100, 1, 2, 16, 16), (2, 200, 1000, 8000, 40, 24), (1 << 20, 65, 1, 1, 128, 64), (3, 16000, 100, 300, 16, 16)])
+def test_backward_scratch_stays_bounded(a, io):
+    assert 0 < sizes(*a, io)[1] <= 3 * GIB
