@@ -889,8 +889,8 @@ bool delta_shape(const A& a) {
 
 // Whether sizes are such as a call takes and needs scratch for (those that it refuses may be any here).
 template <typename A>
-bool delta_sizes(const A& a) {
-    return a.n_seq > 0 && a.n_head > 0 && a.n_tok > 0 && a.n_key > 0 && a.n_key <= HELIX_DELTA_MAX_KEY && a.n_val > 0 &&
+bool delta_heads(const A& a) {
+    return a.n_seq > 0 && a.n_head > 0 && a.n_tok >= 0 && a.n_key > 0 && a.n_key <= HELIX_DELTA_MAX_KEY && a.n_val > 0 &&
            a.n_val <= HELIX_DELTA_MAX_VAL && (long long)a.n_seq * a.n_head < 1LL << 31 && a.n_qk_head > 0 &&
            a.n_head % a.n_qk_head == 0;
 }
@@ -928,20 +928,80 @@ bool delta_ahead(long long heads, int columns, const helix_delta_rule_args& a) {
     return columns == 16 && a.io_dtype != HELIX_F32 && heads <= 96 && heads * ceil_div(a.n_val, 16) <= 384;
 }
 
-// How the rule is cut: segments of `chunks` chunks of every sequence, whose operands scratch holds at a time.
+// Heads of a call that go together, part after part through the same scratch: those of `seqs` sequences or, where `heads` are
+// fewer than there are, so many of one sequence's. A part's heads do not meet another's.
+struct DeltaParts {
+    int seqs = 0, heads = 0;
+    long long all() const { return (long long)seqs * heads; }
+};
+// Parts of at most `most` heads, as alike as may be. Heads that share one of the queries' stay together unless `split`.
+DeltaParts delta_parts(long long n_seq, long long n_qk, long long share, long long most, bool split = false) {
+    const long long n_head = n_qk * share;
+    DeltaParts p{1, (int)n_head};
+    if (most >= n_head) p.seqs = (int)ceil_div(n_seq, ceil_div(n_seq, most / n_head));
+    else if (split && most < share) p.heads = (int)ceil_div(share, ceil_div(share, most));
+    else p.heads = (int)(share * ceil_div(n_qk, ceil_div(n_qk, std::max(1LL, most / share))));
+    return p;
+}
+
+// What is the whole call's in p, for the part that begins at a sequence and a head (a call's last parts may be smaller).
+HelixDeltaParams delta_part(HelixDeltaParams p, const DeltaParts& part, long long seq, long long head, size_t es) {
+    const long long qk = head / p.share, state = (seq * p.n_head + head) * p.n_key * p.n_val;
+    advance(p.q, seq * p.seq_q + qk * p.head_q, es);
+    advance(p.k, seq * p.seq_k + qk * p.head_k, es);
+    advance(p.v, seq * p.seq_v + head * p.head_v, es);
+    advance(p.g, seq * p.seq_g + head, 4);
+    advance(p.beta, seq * p.seq_b + head, 4);
+    advance(p.o, seq * p.seq_o + head * p.head_o, es);
+    advance(p.d_o, seq * p.seq_o + head * p.head_o, es);
+    for (const float** s : {&p.s0, &p.d_s}) advance(*s, state, 4);
+    for (float** s : {&p.s, &p.ds0}) advance(*s, state, 4);
+    const long long row = seq * p.n_tok;   // dense ones
+    advance(p.dq, (row * p.n_qk + qk) * p.n_key, es);
+    advance(p.dk, (row * p.n_qk + qk) * p.n_key, es);
+    advance(p.dv, (row * p.n_head + head) * p.n_val, es);
+    advance(p.dg, row * p.n_head + head, 4);
+    advance(p.dbeta, row * p.n_head + head, 4);
+    p.n_seq = (int)std::min<long long>(part.seqs, p.n_seq - seq);
+    p.n_head = (int)std::min<long long>(part.heads, p.n_head - head);
+    if (part.heads < p.share) p.n_head = (int)std::min<long long>(p.n_head, p.share - head % p.share);
+    p.share = std::min(p.share, p.n_head);
+    p.n_qk = p.n_head / p.share;
+    return p;
+}
+// f(parameters) for every part of a call.
+template <typename F>
+void each_part(const HelixDeltaParams& call, const DeltaParts& part, size_t es, F&& f) {
+    for (long long seq = 0; seq < call.n_seq; seq += part.seqs)
+        for (long long head = 0; head < call.n_head;) {
+            const HelixDeltaParams p = delta_part(call, part, seq, head, es);
+            head += p.n_head;
+            f(p);
+        }
+}
+
+// How the rule is cut: parts, and segments of `chunks` chunks of them, whose operands scratch holds at a time.
 struct DeltaPlan {
+    DeltaParts part;
     int n_chunk = 0, chunks = 0, columns = 0, sets = 1;   // sets: of a segment's operands
     size_t x_at = 0, p_at = 0, decay_at = 0, set = 0, bytes = 0;
 };
-// Scratch of a segment: up to a gigabyte, and one chunk of every sequence where that is more.
+// Scratch: up to a gigabyte.
 constexpr size_t kDeltaScratch = (size_t)1 << 30;
 
 DeltaPlan delta_plan(const helix_delta_rule_args& a) {
     DeltaPlan p;
-    if (!delta_sizes(a) || a.n_tok <= delta_steps((long long)a.n_seq * a.n_head, a.n_val, a.io_dtype)) return p;
-    const size_t sh = (size_t)a.n_seq * a.n_head, x = 6 * 3 * HELIX_DR_FRAG, each = sh * (2 * x + HELIX_DR_DECAY);
+    if (!delta_heads(a)) return p;
+    const long long all = (long long)a.n_seq * a.n_head, share = a.n_head / a.n_qk_head;
+    if (a.n_tok <= delta_steps(all, a.n_val, a.io_dtype)) {
+        p.part = delta_parts(a.n_seq, a.n_qk_head, share, most_groups(kDeltaThreads) / ceil_div(a.n_val, 64), true);
+        return p;
+    }
+    const size_t x = 6 * 3 * HELIX_DR_FRAG, each = 2 * x + HELIX_DR_DECAY;   // of a chunk of a head
+    p.part = delta_parts(a.n_seq, a.n_qk_head, share, std::min<long long>(kDeltaScratch / each, most_groups(2 * kDeltaThreads) / ceil_div(a.n_val, 16)), true);
+    const size_t sh = p.part.all();
     p.n_chunk = (int)ceil_div(a.n_tok, HELIX_DR_CHUNK);
-    p.chunks = (int)std::min<size_t>(p.n_chunk, std::max<size_t>(1, kDeltaScratch / each));
+    p.chunks = (int)std::min<size_t>(p.n_chunk, kDeltaScratch / (sh * each));
     p.columns = delta_columns((long long)sh, a.n_val);
     if (delta_ahead((long long)sh, p.columns, a)) {
         const int least = (int)std::max<size_t>(32, 2048 / sh), n = std::max<int>(p.n_chunk / least, (int)ceil_div(2 * p.n_chunk, p.chunks));
@@ -1018,87 +1078,51 @@ extern "C" helix_status helix_delta_rule_encode(helix_ctx* ctx, void* stream, co
         need(plan.bytes == 0 || (a->scratch && a->scratch_bytes >= plan.bytes),
              "scratch smaller than helix_delta_rule_scratch_size()", HELIX_ERR_SCRATCH_TOO_SMALL);
         need(aligned(a->scratch, 16), "scratch is not 16-byte aligned");
-        HelixDeltaParams p = delta_params(*a);
-        p.o = a->o;
-        p.s = a->s;
-        p.seq_o = a->seq_o;
-        p.tok_o = a->tok_o;
-        p.head_o = a->head_o;
+        HelixDeltaParams call = delta_params(*a);
+        call.o = a->o;
+        call.s = a->s;
+        call.seq_o = a->seq_o;
+        call.tok_o = a->tok_o;
+        call.head_o = a->head_o;
         const std::string form = delta_form(*a, !plan.bytes);
-        const long long sh = (long long)a->n_seq * a->n_head;
         if (!plan.bytes) {
             const hipFunction_t f = kernel(ctx, "helix_delta_steps_" + form);
-            const unsigned gx = grid(sh * ceil_div(a->n_val, 64), kDeltaThreads);
+            const long long slices = ceil_div(a->n_val, 64);
             const OnDevice on(ctx->device);
-            launch(f, stream, gx, 1, kDeltaThreads, p);
+            each_part(call, plan.part, es, [&](HelixDeltaParams p) {
+                launch(f, stream, (unsigned)((long long)p.n_seq * p.n_head * slices), 1, kDeltaThreads, p);
+            });
             return;
         }
         const hipFunction_t prep = kernel(ctx, "helix_delta_prep_" + form),
                             walk = kernel(ctx, "helix_delta_walk_" + form + "_c" + std::to_string(plan.columns));
-        p.n_slice = (int)ceil_div(a->n_val, plan.columns);
-        const unsigned gw = grid(sh * p.n_slice, 2 * kDeltaThreads);
-        grid(gw + sh * plan.chunks, 2 * kDeltaThreads);
+        call.n_slice = (int)ceil_div(a->n_val, plan.columns);
         char* sc = static_cast<char*>(a->scratch);
         const OnDevice on(ctx->device);
-        p.n_walk = gw;
-        for (int first = 0, set = 0; first < plan.n_chunk; first += plan.chunks, set ^= plan.sets - 1) {
-            auto at = [&](int i, size_t off) { return sc + i * plan.set + off; };
-            const int other = set ^ (plan.sets - 1), next = first + plan.chunks;
-            p.x = at(set, plan.x_at);
-            p.p = at(set, plan.p_at);
-            p.decay = reinterpret_cast<float*>(at(set, plan.decay_at));
-            p.chunk0 = first;
-            p.n_chunk = std::min(plan.chunks, plan.n_chunk - first);
-            if (!first || plan.sets == 1) launch(prep, stream, (unsigned)(sh * p.n_chunk), 1, kDeltaThreads, p);
-            p.n_next = plan.sets == 2 ? std::max(0, std::min(plan.chunks, plan.n_chunk - next)) : 0;
-            p.next_x = at(other, plan.x_at);
-            p.next_p = at(other, plan.p_at);
-            p.next_decay = reinterpret_cast<float*>(at(other, plan.decay_at));
-            launch(walk, stream, gw + (unsigned)(sh * p.n_next), 1, 2 * kDeltaThreads, p);
-            p.s0 = p.s;   // the next segment starts where this one ends
-        }
+        each_part(call, plan.part, es, [&](HelixDeltaParams p) {
+            const long long sh = (long long)p.n_seq * p.n_head;
+            p.n_walk = (unsigned)(sh * p.n_slice);
+            for (int first = 0, set = 0; first < plan.n_chunk; first += plan.chunks, set ^= plan.sets - 1) {
+                auto at = [&](int i, size_t off) { return sc + i * plan.set + off; };
+                const int other = set ^ (plan.sets - 1), next = first + plan.chunks;
+                p.x = at(set, plan.x_at);
+                p.p = at(set, plan.p_at);
+                p.decay = reinterpret_cast<float*>(at(set, plan.decay_at));
+                p.chunk0 = first;
+                p.n_chunk = std::min(plan.chunks, plan.n_chunk - first);
+                if (!first || plan.sets == 1) launch(prep, stream, (unsigned)(sh * p.n_chunk), 1, kDeltaThreads, p);
+                p.n_next = plan.sets == 2 ? std::max(0, std::min(plan.chunks, plan.n_chunk - next)) : 0;
+                p.next_x = at(other, plan.x_at);
+                p.next_p = at(other, plan.p_at);
+                p.next_decay = reinterpret_cast<float*>(at(other, plan.decay_at));
+                launch(walk, stream, p.n_walk + (unsigned)(sh * p.n_next), 1, 2 * kDeltaThreads, p);
+                p.s0 = p.s;   // the next segment starts where this one ends
+            }
+        });
     });
 }
 
 namespace {
-
-// Heads of a call that go together, part after part through the same scratch: those of `seqs` sequences or, where `heads` are
-// fewer than there are, so many of one sequence's. A part's heads do not meet another's.
-struct DeltaParts {
-    int seqs = 0, heads = 0;
-    long long all() const { return (long long)seqs * heads; }
-};
-// Parts of at most `most` heads, as alike as may be; the heads that share one of the queries' stay together.
-DeltaParts delta_parts(long long n_seq, long long n_qk, long long share, long long most) {
-    const long long n_head = n_qk * share;
-    DeltaParts p{1, (int)n_head};
-    if (most >= n_head) p.seqs = (int)ceil_div(n_seq, ceil_div(n_seq, most / n_head));
-    else p.heads = (int)(share * ceil_div(n_qk, ceil_div(n_qk, std::max(1LL, most / share))));
-    return p;
-}
-
-// What is the whole call's in p, for the part that begins at a sequence and a head (a call's last parts may be smaller).
-HelixDeltaParams delta_part(HelixDeltaParams p, const DeltaParts& part, long long seq, long long head, size_t es) {
-    const long long qk = head / p.share, state = (seq * p.n_head + head) * p.n_key * p.n_val;
-    advance(p.q, seq * p.seq_q + qk * p.head_q, es);
-    advance(p.k, seq * p.seq_k + qk * p.head_k, es);
-    advance(p.v, seq * p.seq_v + head * p.head_v, es);
-    advance(p.g, seq * p.seq_g + head, 4);
-    advance(p.beta, seq * p.seq_b + head, 4);
-    advance(p.d_o, seq * p.seq_o + head * p.head_o, es);
-    for (const float** s : {&p.s0, &p.d_s}) advance(*s, state, 4);
-    advance(p.ds0, state, 4);
-    const long long row = seq * p.n_tok;   // dense ones
-    advance(p.dq, (row * p.n_qk + qk) * p.n_key, es);
-    advance(p.dk, (row * p.n_qk + qk) * p.n_key, es);
-    advance(p.dv, (row * p.n_head + head) * p.n_val, es);
-    advance(p.dg, row * p.n_head + head, 4);
-    advance(p.dbeta, row * p.n_head + head, 4);
-    p.n_seq = (int)std::min<long long>(part.seqs, p.n_seq - seq);
-    p.n_head = (int)std::min<long long>(part.heads, p.n_head - head);
-    p.n_qk = p.n_head / p.share;
-    return p;
-}
 
 // The backward pass: its parts, what a segment's chunks leave for its kernels, and the states that the segments start from.
 struct DeltaBwdPlan {
@@ -1116,7 +1140,13 @@ constexpr size_t kDeltaBwdScratch = (size_t)2 << 30, kDeltaBwdStates = (size_t)1
 
 DeltaBwdPlan delta_bwd_plan(const helix_delta_rule_backward_args& a) {
     DeltaBwdPlan p;
-    if (!delta_sizes(a)) return p;
+    if (!delta_heads(a)) return p;
+    const long long launch_heads = most_groups(kDeltaPairThreads) / ceil_div(a.n_val, 16);
+    if (!a.n_tok) {   // ds0 = d_s
+        p.part = delta_parts(a.n_seq, a.n_qk_head, a.n_head / a.n_qk_head, launch_heads);
+        p.columns = 16;
+        return p;
+    }
     const size_t x = 6 * 3 * HELIX_DR_FRAG, tri = 2 * 10 * 256 * 4, share = a.n_head / a.n_qk_head, sh = (size_t)a.n_seq * a.n_head;
     auto up = [](size_t bytes) { return (bytes + 255) & ~(size_t)255; };
     const size_t state = (size_t)a.n_key * a.n_val * 4, rows = (size_t)HELIX_DR_CHUNK * a.n_val * 4;
@@ -1128,8 +1158,7 @@ DeltaBwdPlan delta_bwd_plan(const helix_delta_rule_backward_args& a) {
         most = std::max<size_t>(kDeltaBwdScratch / (p.n_chunk * each), ceil_div(256, ceil_div(a.n_val, 32)));
         while (most > share && (most * each > kDeltaBwdScratch || (ceil_div(p.n_chunk, chunks(most)) - 1) * most * state > kDeltaBwdStates)) most /= 2;
     }
-    most = std::min<size_t>(most, most_groups(2 * kDeltaThreads) / ceil_div(a.n_val, 16));
-    p.part = delta_parts(a.n_seq, a.n_qk_head, share, (long long)most);
+    p.part = delta_parts(a.n_seq, a.n_qk_head, share, std::min((long long)most, launch_heads));
     const size_t heads = p.part.all(), qk = heads / share;
     p.chunks = chunks(heads);
     p.n_seg = (int)ceil_div(p.n_chunk, p.chunks);
@@ -1174,11 +1203,9 @@ extern "C" helix_status helix_delta_rule_backward_encode(helix_ctx* ctx, void* s
              "ds0 is NULL, or it or d_s not aligned to its elements");
         need((long long)a->n_head * a->n_val < (1LL << 31) / 64 / (long long)es && (long long)a->n_qk_head * a->n_key < (1LL << 31) / 64 / (long long)es,
              "64 tokens of dq, dk or dv span 2^31 bytes or more", HELIX_ERR_UNSUPPORTED_SHAPE);
-        DeltaBwdPlan plan = delta_bwd_plan(*a);
-        if (!a->n_tok) {
-            plan.columns = 16;
-            plan.part = delta_parts(a->n_seq, a->n_qk_head, a->n_head / a->n_qk_head, most_groups(2 * kDeltaThreads) / ceil_div(a->n_val, 16));
-        }
+        const DeltaBwdPlan plan = delta_bwd_plan(*a);
+        need(plan.part.all() * std::max<long long>(plan.chunks, ceil_div(a->n_val, plan.columns)) <= most_groups(kDeltaPairThreads),
+             "the heads that share a query head exceed a launch", HELIX_ERR_UNSUPPORTED_SHAPE);
         need(plan.bytes == 0 || (a->scratch && a->scratch_bytes >= plan.bytes),
              "scratch smaller than helix_delta_rule_backward_scratch_size()", HELIX_ERR_SCRATCH_TOO_SMALL);
         need(aligned(a->scratch, 16), "scratch is not 16-byte aligned");
@@ -1211,8 +1238,6 @@ extern "C" helix_status helix_delta_rule_backward_encode(helix_ctx* ctx, void* s
         const hipFunction_t prep = kernel(ctx, "helix_delta_prep_bwd_" + form), keep = kernel(ctx, "helix_delta_keep_" + wide),
                             back = kernel(ctx, "helix_delta_back_" + wide), pairs = kernel(ctx, "helix_delta_pairs_" + form),
                             grad = kernel(ctx, "helix_delta_grad_" + form);
-        grid(plan.part.all() * call.n_slice, 2 * kDeltaThreads);
-        grid(plan.part.all() * std::max(1, plan.chunks), kDeltaPairThreads);
         const OnDevice on(ctx->device);
         // A part: the states that its segments start from (that of segment i > 0 at i - 1), then its segments from the last on.
         auto run = [&](HelixDeltaParams p) {
@@ -1242,8 +1267,7 @@ extern "C" helix_status helix_delta_rule_backward_encode(helix_ctx* ctx, void* s
             }
             if (!plan.n_seg) launch(back, stream, gw, 1, 2 * kDeltaThreads, p);   // no tokens: ds0 = d_s
         };
-        for (long long seq = 0; seq < a->n_seq; seq += plan.part.seqs)
-            for (long long head = 0; head < a->n_head; head += plan.part.heads) run(delta_part(call, plan.part, seq, head, es));
+        each_part(call, plan.part, es, run);
     });
 }
 

@@ -339,7 +339,8 @@ helix_status helix_delta_rule_encode(helix_ctx* ctx, void* stream, const helix_d
 
 /* Gradients, from d_o (of every o) and d_s (of s). The states are formed again.
  * dq and dk of a head that value heads share are the sums over them, in fp32 and in
- * the heads' order. Of a non-finite input the gradients of its heads (of its column,
+ * the heads' order; the heads that share one have n_head / n_qk_head * ceil(n_val /
+ * 16) below 2^32 / 640. Of a non-finite input the gradients of its heads (of its column,
  * for v and d_o: also dq, dk, dg and dbeta of the head) are not finite either. */
 typedef struct {
     int32_t      n_seq, n_tok;       /* n_seq or n_head 0: nothing is done;

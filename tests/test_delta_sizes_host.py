@@ -4,6 +4,7 @@ import itertools
 import pytest
 
 from helix_amd import abi
+from helix_amd.desc import HELIX_ERR_NO_DEVICE, HELIX_ERR_UNSUPPORTED_SHAPE
 
 I32 = 2 ** 31 - 1
 
@@ -46,3 +47,32 @@ GIB = 1 << 30
                                (100000, 100, 1, 2, 16, 16), (2, 200, 1000, 8000, 40, 24), (1 << 20, 65, 1, 1, 128, 64), (3, 16000, 100, 300, 16, 16)])
 def test_backward_scratch_stays_bounded(a, io):
     assert 0 < sizes(*a, io)[1] <= 3 * GIB
+
+
+@pytest.mark.parametrize("io", [0, 2])
+@pytest.mark.parametrize("a", [(3000, 200, 1, 16, 16, 16), (100000, 100, 1, 2, 16, 16), (1, 70, 1, 40000, 128, 64), (1, 1 << 20, 40000, 40000, 16, 16),
+                               (1 << 20, 65, 64, 64, 128, 64), (1, 1 << 21, 8, 64, 128, 64), ((1 << 31) - 1, 100, 1, 1, 1, 1)])
+def test_forward_scratch_stays_bounded(a, io):
+    assert 0 < sizes(*a, io)[0] <= GIB
+
+
+# A launch holds 2^32 threads; calls of more heads than that go in parts. Only heads that share one of the queries' stay
+# together, backward.
+@pytest.mark.parametrize("a,status", [((1 << 25, 3, 1, 1, 8, 8), (HELIX_ERR_NO_DEVICE,) * 2), ((1 << 25, 70, 1, 1, 8, 8), (HELIX_ERR_NO_DEVICE,) * 2),
+                                      ((1, 1, 1 << 25, 1 << 25, 8, 8), (HELIX_ERR_NO_DEVICE, HELIX_ERR_UNSUPPORTED_SHAPE)),   # (dv's rows: 2^31 bytes)
+                                      ((1, 1, 1, (1 << 23) - 1, 8, 1), (HELIX_ERR_NO_DEVICE, HELIX_ERR_UNSUPPORTED_SHAPE)),
+                                      ((1, 1, 1, 6710886, 8, 1), (HELIX_ERR_NO_DEVICE,) * 2), ((1, 0, 1, 6710886, 8, 1), (HELIX_ERR_NO_DEVICE,) * 2),
+                                      ((1, 0, 1, 6710887, 8, 1), (HELIX_ERR_NO_DEVICE, HELIX_ERR_UNSUPPORTED_SHAPE)),
+                                      ((1, 1, 1, 6710887, 8, 1), (HELIX_ERR_NO_DEVICE, HELIX_ERR_UNSUPPORTED_SHAPE)),
+                                      ((300, 70, 16, 64, 128, 1 << 16), (HELIX_ERR_NO_DEVICE,) * 2)])
+def test_heads_of_more_than_one_launch(a, status):
+    S, L, Hk, H, N, P = a
+    host, lib = abi.Context(host_only=True), abi.lib()
+    at = 1 << 12   # an address that nothing reads
+    qk, v, g = (L * Hk * N, Hk * N, N), (L * H * P, H * P, P), (L * H, H)
+    strides = (*qk, *qk, *v, *g, *g)
+    fwd = abi.DELTA_RULE_STRUCT.pack(*a, 2, 1.0, *[at] * 5, 0, *[at] * 3, 1 << 50, *strides, *v)
+    bwd = abi.DELTA_RULE_BACKWARD_STRUCT.pack(*a, 2, 1.0, *[at] * 15, 1 << 50, *v, *strides)
+    got = tuple(int(f(host.handle, None, x)) for f, x in ((lib.helix_delta_rule_encode, fwd), (lib.helix_delta_rule_backward_encode, bwd)))
+    host.close()
+    assert got == status

@@ -4,7 +4,7 @@ import pytest
 import torch
 
 from helix_amd import abi
-from helix_amd.delta import delta_rule_backward
+from helix_amd.delta import delta_rule, delta_rule_backward
 
 pytestmark = pytest.mark.gpu
 
@@ -59,3 +59,35 @@ def test_backward_in_parts(gpu, S, L, Hk, H, N, P, dtype, some):
         for n, x, y in zip(NAMES, one, grads):
             y = y[a:b, c:e] if n == "ds0" else y[a:b, :, c // share:e // share] if n in ("dq", "dk") else y[a:b, :, c:e]
             assert torch.equal(x, y), (n, seqs, heads)
+
+
+@pytest.mark.parametrize("S,L,Hk,H,N,P,dtype,some", [
+    (40000, 70, 1, 1, 16, 8, torch.bfloat16, [((0, 3), (0, 1)), ((19999, 20002), (0, 1)), ((39997, 40000), (0, 1))]),   # sequences
+    (2, 200, 20000, 40000, 8, 12, torch.float16, [((0, 1), (0, 4)), ((1, 2), (19996, 20004)), ((1, 2), (39998, 40000))]),   # heads
+    (1, 70, 1, 40000, 40, 8, torch.float32, [((0, 1), (0, 5)), ((0, 1), (19996, 20004)), ((0, 1), (39999, 40000))]),   # of one query head
+    (2, 130, 3, 90000, 16, 4, torch.bfloat16, [((0, 1), (14997, 15003)), ((1, 2), (29997, 30000)), ((1, 2), (44998, 45006)), ((1, 2), (89993, 90000))]),
+])
+def test_forward_in_parts(gpu, S, L, Hk, H, N, P, dtype, some):
+    p = problem(S, L, Hk, H, N, P, dtype, seed=20)
+    o, s = delta_rule(*p)
+    for seqs, heads in some:
+        (a, b), (c, d) = seqs, heads
+        o1, s1 = delta_rule(*of(p, seqs, heads, H // Hk))
+        assert torch.equal(o1, o[a:b, :, c:d]) and torch.equal(s1, s[a:b, c:d])
+
+
+# Token by token: 2^24 - 1 workgroups a launch.
+@pytest.mark.parametrize("S,L,Hk,H,P", [((1 << 24) + 5, 3, 1, 1, 2), (1, 1, (1 << 24) + 6, (1 << 24) + 6, 1), (1, 1, 1, (1 << 24) + 6, 1),
+                                        (1 << 17, 2, 1, 1, (1 << 13) + 1)])
+def test_steps_of_more_than_one_launch(gpu, S, L, Hk, H, P):
+    torch.cuda.empty_cache()
+    if torch.cuda.mem_get_info()[0] < 60 << 30:
+        pytest.skip("needs 60 GB of GPU memory")
+    p = problem(S, L, Hk, H, 1, P, torch.bfloat16, seed=30)
+    o, s = delta_rule(*p)
+    seqs, heads = (S, H // 2) if S == 1 else (S // 2, H)
+    for first in (True, False):
+        at = ((0, seqs) if first else (S - seqs, S)) if S > 1 else (0, 1), ((0, heads) if first else (H - heads, H)) if S == 1 else (0, H)
+        (a, b), (c, d) = at
+        o1, s1 = delta_rule(*of(p, *at, H // Hk))
+        assert torch.equal(o1, o[a:b, :, c:d]) and torch.equal(s1, s[a:b, c:d])
