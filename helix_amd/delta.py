@@ -87,7 +87,7 @@ def delta_rule_backward(do: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: t
     strides = (*_tensor("do", do, q.dtype, (S, L, H, P), q, "channels"), *strides)
     _state("ds", ds, q, (S, H, N, P))
     with under(index, stream):
-        dq, dk = (torch.empty(S, L, Hk, N, dtype=q.dtype, device=q.device) for _ in range(2))
+        dq, dk = ((torch.empty if H else torch.zeros)(S, L, Hk, N, dtype=q.dtype, device=q.device) for _ in range(2))
         dv = torch.empty(S, L, H, P, dtype=q.dtype, device=q.device)
         dg, dbeta = (torch.empty(S, L, H, dtype=torch.float32, device=q.device) for _ in range(2))
         ds0 = torch.empty(S, H, N, P, dtype=torch.float32, device=q.device)
