@@ -71,19 +71,25 @@ HELIX_DEV void dr_mfma(const bf16x8 (&a)[NA], const bf16x8 (&b)[NB], DrAcc& acc)
                 acc.s[sum] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[i], b[sum - i], acc.s[sum], 0, 0, 0);
 }
 
-template <int NPL>
+// END: of values that may reach the end of fp32, which lies past bf16's: the first part stays a number, the others have the rest.
+// (What is not finite stays so: the rest of an infinity is one.)
+template <int NPL, bool END = false>
 HELIX_DEV void dr_split2(float a, float b, unsigned (&w)[NPL]) {
-    if constexpr (NPL == 3) split3_pair(a, b, w[0], w[1], w[2]);
+    if constexpr (NPL == 3 && END) {
+        constexpr float kTop = 0x1.fep127f;   // bf16's largest
+        w[0] = pk_bf16(__builtin_amdgcn_fmed3f(a, -kTop, kTop), __builtin_amdgcn_fmed3f(b, -kTop, kTop));
+        split2_pair(sub_lo(a, w[0]), sub_hi(b, w[0]), w[1], w[2]);
+    } else if constexpr (NPL == 3) split3_pair(a, b, w[0], w[1], w[2]);
     else if constexpr (NPL == 2) split2_pair(a, b, w[0], w[1]);
     else w[0] = pk_bf16(a, b);
 }
-template <int NPL>
+template <int NPL, bool END = false>
 HELIX_DEV void dr_split8(const float (&v)[8], bf16x8 (&o)[NPL]) {
     u32x4 q[NPL];
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
         unsigned w[NPL];
-        dr_split2<NPL>(v[2 * e], v[2 * e + 1], w);
+        dr_split2<NPL, END>(v[2 * e], v[2 * e + 1], w);
 #pragma unroll
         for (int k = 0; k < NPL; ++k) q[k][e] = w[k];
     }
@@ -91,8 +97,8 @@ HELIX_DEV void dr_split8(const float (&v)[8], bf16x8 (&o)[NPL]) {
     for (int k = 0; k < NPL; ++k) o[k] = __builtin_bit_cast(bf16x8, q[k]);
 }
 
-// Eight stored elements as an operand's parts, those from n on cleared.
-template <typename T>
+// Eight stored elements as an operand's parts, those from n on cleared. OWN: of what the kernels stored, not the caller.
+template <typename T, bool OWN = false>
 HELIX_DEV void dr_operand(const Raw8<T>& v, int n, bf16x8 (&o)[dr_planes<T>]) {
     if constexpr (__is_same(T, __bf16)) {
         u32x4 w = v.w[0];
@@ -105,7 +111,7 @@ HELIX_DEV void dr_operand(const Raw8<T>& v, int n, bf16x8 (&o)[dr_planes<T>]) {
         float f[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) f[e] = e < n ? at8(v, e) : 0.0f;
-        dr_split8<dr_planes<T>>(f, o);
+        dr_split8<dr_planes<T>, !OWN>(f, o);
     }
 }
 
@@ -152,11 +158,11 @@ HELIX_DEV float raw_f32(unsigned w) {
 
 // Four values of a result's registers (rows i .. i + 3, i a multiple of 4, of a column) as parts, side by side in row `row`
 // of planes of ROWS rows of W.
-template <int NPL, int W, int ROWS>
+template <int NPL, int W, int ROWS, bool END = false>
 HELIX_DEV void dr_put4(__bf16* planes, int row, int i, float a, float b, float c, float d) {
     unsigned lo[NPL], hi[NPL];
-    dr_split2<NPL>(a, b, lo);
-    dr_split2<NPL>(c, d, hi);
+    dr_split2<NPL, END>(a, b, lo);
+    dr_split2<NPL, END>(c, d, hi);
     __bf16* to = planes + dr_at<W>(row, i >> 3) + (i & 4);
 #pragma unroll
     for (int k = 0; k < NPL; ++k) *reinterpret_cast<u32x2*>(to + k * ROWS * W) = u32x2{lo[k], hi[k]};

@@ -567,7 +567,7 @@ __device__ void delta_walk(const HelixDeltaParams& p, WalkLds<T, NK, KEEP, NC>& 
             f32x4 R = ks_[n].sum();
 #pragma unroll
             for (int r = 0; r < 4; ++r) R[r] = (float)sV[row0 + r][16 * n + c] - start[r] * R[r];
-            dr_put4<3, DR_C, COLS>(sR, 16 * n + c, row0, R[0], R[1], R[2], R[3]);
+            dr_put4<3, DR_C, COLS, sizeof(T) == 4>(sR, 16 * n + c, row0, R[0], R[1], R[2], R[3]);   // (V at the end of fp32)
         }
         dr_barrier();   // R is there; K and V have been read
         typename DrAccOf<NC>::type ds[NC];
@@ -731,7 +731,7 @@ __device__ void delta_back(const HelixDeltaParams& p) {
                 float o[4];
 #pragma unroll
                 for (int r = 0; r < 4; ++r) o[r] = raw_f32<T>(vo[n][r]);
-                dr_put4<NPL, DR_C, COLS>(sO, 16 * n + c, row0, o[0], o[1], o[2], o[3]);
+                dr_put4<NPL, DR_C, COLS, sizeof(T) == 4>(sO, 16 * n + c, row0, o[0], o[1], o[2], o[3]);
 #pragma unroll
                 for (int r = 0; r < 4; ++r) o[r] *= p.scale * start[r];
                 dr_put4<3, DR_C, COLS>(sW, 16 * n + c, row0, o[0], o[1], o[2], o[3]);
@@ -1031,8 +1031,8 @@ __device__ void delta_pairs(const HelixDeltaParams& p) {
                 const int n = P - pb - scol;
                 bf16x8 o[NPL], z[3], d[3];
                 dr_operand<T>(no, n, o);
-                dr_operand<float>(nz, n, z);
-                dr_operand<float>(nd, n, d);
+                dr_operand<float, true>(nz, n, z);
+                dr_operand<float, true>(nd, n, d);
 #pragma unroll
                 for (int e = 0; e < 8; ++e) zv += e < n ? at8(nz, e) * at8(nv, e) : 0.0f;
                 dr_put8<NPL, DR_C, DR_C>(sO, srow, scol, o);
@@ -1199,8 +1199,8 @@ __device__ void delta_grad(const HelixDeltaParams& p) {
                 const int row = fresh / 8, col = 8 * (fresh % 8), n = P - pb - col;
                 bf16x8 o[NPL], z[3], d[3];
                 dr_operand<T>(next.o, n, o);
-                dr_operand<float>(next.z, n, z);
-                dr_operand<float>(next.d, n, d);
+                dr_operand<float, true>(next.z, n, z);
+                dr_operand<float, true>(next.d, n, d);
                 dr_put8<NPL, DR_C, DR_C>(sO, row, col, o);
                 dr_put8<3, DR_C, DR_C>(sZ, row, col, z);
                 dr_put8<3, DR_C, DR_C>(sD, row, col, d);
@@ -1210,8 +1210,8 @@ __device__ void delta_grad(const HelixDeltaParams& p) {
 #pragma unroll
             for (int ks = 0; ks < 2; ++ks) {
                 const int n = P - pb - 32 * ks - 8 * q;
-                dr_operand<float>(next.s[ks], n, bs[ks]);
-                dr_operand<float>(next.e[ks], n, be[ks]);
+                dr_operand<float, true>(next.s[ks], n, bs[ks]);
+                dr_operand<float, true>(next.e[ks], n, be[ks]);
 #pragma unroll
                 for (int e = 0; e < 8; ++e) se += e < n ? at8(next.s[ks], e) * at8(next.e[ks], e) : 0.0f;
             }

@@ -300,8 +300,9 @@ helix_status helix_gated_scan_backward_encode(helix_ctx* ctx, void* stream,
  * and beta = 0 leaves the state as it is. Keys are taken as they are: of length
  * one at most, with beta up to 2, they keep the state bounded.
  *
- * Products keep fp32 accuracy (operands in three bf16 parts, fp32 sums), whatever
- * the storage type; o is rounded to it once.
+ * Products keep fp32 accuracy (operands in three bf16 parts, fp32 sums; of a
+ * chunk's operands below 2^-110, 2^-134), whatever the storage type; o is rounded
+ * to it once. Inputs may be any finite numbers, the type's largest too.
  * Where an element of v is infinite or NaN, its column of the state and of o is
  * from the chunk of 64 tokens on that it lies in; where one of q, k, g or beta
  * is, its heads are. Other heads and sequences are not touched.
