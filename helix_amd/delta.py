@@ -3,7 +3,8 @@
     S_t = e^(g_t) S_(t-1) + beta_t k_t (v_t - e^(g_t) S_(t-1)' k_t)',  o_t = scale S_t' q_t,  S_(-1) = s0
 
 The state, keys x values, is float32 throughout. Keys are taken as they are: a layer norms them (and the queries) to
-length one, rms_norm with a weight of keys ** -0.5, say. A token that is to leave the state as it is has g = 0 and beta = 0.
+length one, rms_norm with a weight of keys ** -0.5, say. A token that is to leave the state as it is has g = 0, beta = 0 and
+any finite q, k and v (0 times a NaN is a NaN: memory that nothing has written is no padding). g = -inf forgets all before.
 """
 from __future__ import annotations
 

@@ -303,9 +303,11 @@ helix_status helix_gated_scan_backward_encode(helix_ctx* ctx, void* stream,
  * Products keep fp32 accuracy (operands in three bf16 parts, fp32 sums; of a
  * chunk's operands below 2^-110, 2^-134), whatever the storage type; o is rounded
  * to it once. Inputs may be any finite numbers, the type's largest too.
- * Where an element of v is infinite or NaN, its column of the state and of o is
- * from the chunk of 64 tokens on that it lies in; where one of q, k, g or beta
- * is, its heads are. Other heads and sequences are not touched.
+ * What is not finite (g = -inf apart) stays where the formulas take it: an element
+ * of v or s0 in its column of o and s, one of q in its token's o, one of k, g or
+ * beta in its heads' o and s; but in a call of chunks the o of tokens before it in
+ * its chunk of 64 may be NaN too. Other heads and sequences are not touched. A
+ * masked token's q, k and v have to be finite, as 0 times a NaN is one.
  *
  * n_tok = 1 is the step of a single token; s may be s0. Strides are any that are
  * not negative (o's elements do not overlap); 64 tokens of q, k, v or o span
@@ -341,8 +343,10 @@ helix_status helix_delta_rule_encode(helix_ctx* ctx, void* stream, const helix_d
 /* Gradients, from d_o (of every o) and d_s (of s). The states are formed again.
  * dq and dk of a head that value heads share are the sums over them, in fp32 and in
  * the heads' order; the heads that share one have n_head / n_qk_head * ceil(n_val /
- * 16) below 2^32 / 640. Of a non-finite input the gradients of its heads (of its column,
- * for v and d_o: also dq, dk, dg and dbeta of the head) are not finite either. */
+ * 16) below 2^32 / 640. What is not finite (g = -inf apart) may reach every gradient
+ * of its sequence's heads that the formulas give it a part in, at tokens before and
+ * after it; one of v and s0 has none in dv and ds0, one of d_o and d_s only its
+ * column of them. Other heads and sequences are not touched. */
 typedef struct {
     int32_t      n_seq, n_tok;       /* n_seq or n_head 0: nothing is done;
                                         n_tok 0: ds0 = d_s                    */
