@@ -858,6 +858,15 @@ bool disjoint(std::initializer_list<std::pair<long long, long long>> dims) {   /
     return true;
 }
 
+// Gates (n_seq, n_tok, heads), fp32 with dense heads, at any distance of their tokens: the kernels' offsets in them are 64 bits.
+void gates(const char* name, const float* p, long long n_tok, long long seq, long long tok) {
+    if (!n_tok) return;
+    const std::string n = name;
+    if (!p) throw Bad{HELIX_ERR_INVALID_ARG, n + " is NULL"};
+    if (!aligned(p, 4)) throw Bad{HELIX_ERR_INVALID_ARG, n + " is not aligned to its elements"};
+    if (seq < 0 || tok < 0) throw Bad{HELIX_ERR_INVALID_ARG, n + ": negative stride"};
+}
+
 // A tensor (n_seq, n_tok, heads, width) with contiguous last dimension: present, aligned, and within the kernels' reach.
 void heads(const char* name, const void* p, long long n_seq, long long n_tok, long long n_head, long long width, long long seq,
            long long tok, long long head, size_t es, bool written) {
@@ -904,15 +913,16 @@ std::string delta_form(const A& a, bool steps = false) {
 }
 
 // Columns of the state that a workgroup of the walks has: 32 where that still gives every CU a workgroup.
-// (2048 tokens, bf16, 128 keys x 64, us with 16 | 32, forward and backward: 64 heads 95 | 101, 297 | 329; 128 heads
-// 130 | 116, 556 | 503; 256 heads 293 | 252, 1103 | 953. fp32, 64 keys x 128: 64 heads 133 | 115, 509 | 428.)
+// (2048 tokens, bf16, 128 keys x 64, us with 16 | 32, forward and backward: 64 heads 96 | 108, 306 | 344; 128 heads
+// 134 | 125, 550 | 498; 256 heads 322 | 259, 1070 | 923. fp32, 64 keys x 128: 32 heads 92 | 106, 279 | 311; 64 heads
+// 140 | 123, 539 | 447.)
 int delta_columns(long long heads, int n_val) { return n_val > 16 && heads * ceil_div(n_val, 32) >= 256 ? 32 : 16; }
 
 // The most tokens that go one by one, by the workgroups that their kernel has. One by one a token costs 1.1 to 1.4 us where
 // all of them run at once; a chunk costs about the same for 1 token as for 64, and more in fp32. Measured, us one by one | as a
-// chunk, 128 keys: 16 bits, 64 workgroups, 4 tokens 9 | 13, 8 tokens 14 | 13; 256, 8 tokens 15 | 21, 12 tokens 21 | 21; 384,
-// 16 tokens 28 | 29; 4096, 16 tokens 168 | 210, 24 tokens 246 | 215. fp32, 64 workgroups, 12 tokens 17 | 18, 16 tokens
-// 21 | 18; 384, 32 tokens 45 | 42; 1024, 32 tokens 71 | 86, 64 tokens 130 | 96.
+// chunk, 128 keys: bf16, 64 workgroups, 4 tokens 9 | 14, 8 tokens 15 | 14; 256, 8 tokens 16 | 23, 12 tokens 22 | 23; 384,
+// 16 tokens 29 | 31; 4096, 16 tokens 173 | 223, 24 tokens 247 | 226. fp32, 64 workgroups, 12 tokens 17 | 19, 16 tokens
+// 22 | 19; 384, 32 tokens 46 | 43; 1024, 32 tokens 73 | 87, 64 tokens 132 | 98.
 int delta_steps(long long heads, int n_val, int io) {
     const long long groups = heads * ceil_div(n_val, 64);
     return (io == HELIX_F32 ? 2 : 1) * (groups < 256 ? 6 : groups < 384 ? 10 : 16);
@@ -921,9 +931,10 @@ int delta_steps(long long heads, int n_val, int io) {
 // Whether a long call goes in segments, and the walk of each takes along the kernel that forms the next one's operands: where
 // walks leave CUs room for it (16 bits, at most three workgroups of 16 columns for two CUs) and there is less to form than to
 // walk. Segments of 2048 chunks of heads at least, whose operands take as long as some launches. Measured, us in one piece |
-// in segments, bf16: 8192 tokens of 64 heads of 128 x 64 330 | 300; of 96 heads 509 | 430; 32768 tokens of 32 heads of
-// 128 x 128 1072 | 943; with 8 heads and 64 chunks a segment 225 | 228. f16: 477 | 458, 670 | 655, 1618 | 1401. Past the
-// bounds, f16: 127 heads of 128 x 64 836 | 907, 128 of 128 x 32 630 | 704, 256 of 128 x 16 877 | 1047.
+// in segments, bf16: 8192 tokens of 64 heads of 128 x 64 349 | 317; of 96 heads 546 | 490; 32768 tokens of 32 heads of
+// 128 x 128 1181 | 1045. f16: 486 | 476, 699 | 684, 1646 | 1470. Past the bounds: 104 heads of 128 x 64 bf16 572 | 536, f16
+// 721 | 729; 112 heads 595 | 587, 747 | 773; 120 heads 616 | 620, 770 | 816; 128 heads of 128 x 32 547 | 530, 659 | 731; 192 of
+// them 704 | 745, 919 | 983; 256 of 128 x 16 748 | 754, 930 | 1085: one bound for both types.
 bool delta_ahead(long long heads, int columns, const helix_delta_rule_args& a) {
     return columns == 16 && a.io_dtype != HELIX_F32 && heads <= 96 && heads * ceil_div(a.n_val, 16) <= 384;
 }
@@ -1057,8 +1068,8 @@ void delta_inputs(const A& a, size_t es) {
     heads("q", a.q, a.n_seq, a.n_tok, a.n_qk_head, a.n_key, a.seq_q, a.tok_q, a.head_q, es, false);
     heads("k", a.k, a.n_seq, a.n_tok, a.n_qk_head, a.n_key, a.seq_k, a.tok_k, a.head_k, es, false);
     heads("v", a.v, a.n_seq, a.n_tok, a.n_head, a.n_val, a.seq_v, a.tok_v, a.head_v, es, false);
-    heads("g", a.g, a.n_seq, a.n_tok, 1, a.n_head, a.seq_g, a.tok_g, 0, 4, false);
-    heads("beta", a.beta, a.n_seq, a.n_tok, 1, a.n_head, a.seq_beta, a.tok_beta, 0, 4, false);
+    gates("g", a.g, a.n_tok, a.seq_g, a.tok_g);
+    gates("beta", a.beta, a.n_tok, a.seq_beta, a.tok_beta);
     need(aligned(a.s0, 4), "s0 is not aligned to its elements");
 }
 

@@ -76,3 +76,20 @@ def test_heads_of_more_than_one_launch(a, status):
     got = tuple(int(f(host.handle, None, x)) for f, x in ((lib.helix_delta_rule_encode, fwd), (lib.helix_delta_rule_backward_encode, bwd)))
     host.close()
     assert got == status
+
+
+def test_gates_at_any_distance():
+    # What 64 tokens of q, k, v and o span is bounded, of g and beta it is not: 2^23 heads and more of two tokens are taken.
+    host, lib = abi.Context(host_only=True), abi.lib()
+    at, H = 1 << 12, 1 << 23
+    far = 1 << 40
+    for a, gate in (((1, 2, 1, H, 8, 1), (2 * H, H)), ((2, 100, 2, 4, 16, 8), (far, far // 200)), ((2, 5, 2, 4, 16, 8), (4, far))):
+        S, L, Hk, H_, N, P = a
+        qk, v = (L * Hk * N, Hk * N, N), (L * H_ * P, H_ * P, P)
+        strides = (*qk, *qk, *v, *gate, *gate)
+        fwd = abi.DELTA_RULE_STRUCT.pack(*a, 2, 1.0, *[at] * 5, 0, *[at] * 3, 1 << 50, *strides, *v)
+        assert int(lib.helix_delta_rule_encode(host.handle, None, fwd)) == HELIX_ERR_NO_DEVICE
+        if P > 1:
+            bwd = abi.DELTA_RULE_BACKWARD_STRUCT.pack(*a, 2, 1.0, *[at] * 15, 1 << 50, *v, *strides)
+            assert int(lib.helix_delta_rule_backward_encode(host.handle, None, bwd)) == HELIX_ERR_NO_DEVICE
+    host.close()

@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from helix_amd.delta import delta_rule_backward
+from helix_amd.delta import delta_rule, delta_rule_backward
 
 pytestmark = pytest.mark.gpu
 
@@ -45,3 +45,19 @@ def test_gradients_of_outputs_past_32_bits(gpu, L, tok, seq):
     do.copy_(normal(S, L, H, P, seed=4, dtype=torch.bfloat16))
     want = delta_rule_backward(do.contiguous(), q, k, v, g, beta)
     assert all(torch.equal(a, b) for a, b in zip(delta_rule_backward(do, q, k, v, g, beta), want))
+
+
+@pytest.mark.parametrize("L,tok", [(5, (1 << 31) + 8), (300, (1 << 23) + 8)])
+def test_gates_past_32_bits(gpu, L, tok):
+    # Gates whose tokens lie gigabytes apart.
+    S, H, N, P = 2, 3, 24, 32
+    q, k = (normal(S, L, 1, N, seed=i, dtype=torch.bfloat16) / 5 for i in (1, 2))
+    v, do = (normal(S, L, H, P, seed=i, dtype=torch.bfloat16) for i in (3, 4))
+    g, beta = -torch.rand(S, L, H, device="cuda"), torch.rand(S, L, H, device="cuda")
+    want = (*delta_rule(q, k, v, g, beta), *delta_rule_backward(do, q, k, v, g, beta))
+    buf = torch.empty((L - 1) * tok + 64, device="cuda")
+    far = [buf.as_strided((S, L, H), (8, tok, 1), at) for at in (0, 32)]
+    for x, y in zip(far, (g, beta)):
+        x.copy_(y)
+    got = (*delta_rule(q, k, v, *far), *delta_rule_backward(do, q, k, v, *far))
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
