@@ -10,7 +10,7 @@
 // helix_delta_walk_* then goes through the chunks of a sequence, a workgroup for 16 or 32 columns
 // of a head's state, whose columns do not meet.
 //
-// 8192 tokens of 64 heads of 128 x 64 in bf16: 300 us, where memory's part is 34 (174 MB). 28 us
+// 8192 tokens of 64 heads of 128 x 64 in bf16: 318 us, where memory's part is 34 (174 MB). 28 us
 // form the first segment's operands, the rest are 128 steps of the walk (below).
 #include "delta_common.h"
 
@@ -148,8 +148,8 @@ constexpr int DR_LD = DR_C + 4;   // fp32 rows of a chunk's square matrices in L
 //     T_iw = -T_ii (sum over j of A_ij T_jw),  w <= j < i
 // on fp32 matrix instructions, T_jw staying in the registers it was formed in. (Products of powers of A would be fewer steps,
 // but keys that repeat make the powers large, and they cancel.) BWD: T' and P' with X, without P.
-// Four workgroups a CU hide one another's chains: P takes the place of K's parts in LDS, T that of A (8192 tokens of 64 heads,
-// bf16, 128 keys: two workgroups a CU 169 us, four 87, of which 50 are the writing of 30 KB a chunk).
+// Four workgroups a CU hide one another's chains: P takes the place of K's parts in LDS, T that of A (twice as fast as two a
+// CU). 2048 tokens of 64 heads, bf16, 128 keys: 27 us, the writing of 37 KB a chunk at 2.8 TB/s.
 template <typename T, int NK>
 struct PrepLds {
     union {
@@ -342,14 +342,14 @@ __device__ void delta_prep(const HelixDeltaParams& p, unsigned id, PrepLds<T, NK
 // chunk before has used its registers. K is read in the first phase alone (K' as operands of
 // the third is kept in registers), so that its next rows can take its place.
 // What bounds it is the chain of a chunk: three products that wait for one another, each with its
-// way through LDS, beside 64 KB of loads into the CU. 8192 tokens of 64 heads of 128 x 64, bf16,
-// 128 chunks: 2 us a chunk; without the loads 1.4, the state's waves alone 1.2. The two kinds
-// of waves took a prompt from 555 us to 424; LDS rows turned by their number (dr_at), V and outputs
-// through LDS and prep's workgroups to 348. No gain: loads two
-// chunks ahead, LDS reads moved before the barriers, priorities of the waves. Slower: Q S in the
-// second phase (353 us for 275 of the walk), K's operands straight from memory (370).
+// way through LDS, beside 70 KB of loads into the CU. 2048 tokens of 64 heads of 128 x 64, bf16,
+// 32 chunks: 70 us, 2.2 a chunk; without the loads 1.7, without the outputs 1.6, the state's waves
+// alone 1.4. Tried on earlier forms, of the time of a whole prompt of 8192 tokens: the two kinds
+// of waves 0.76, rows in LDS turned by their number (dr_at) with V and outputs through LDS 0.82. No
+// gain: loads two chunks ahead, LDS reads moved before the barriers, priorities of the waves. Slower:
+// Q S in the second phase (1.28 of the walk's time), K's operands straight from memory (1.35).
 // With 32 columns a product's operands are loaded and split once for two blocks of columns
-// (128 chunks of 256 heads, KEEP: 240 us with 16 columns, 167 with 32 and two workgroups a CU).
+// (32 chunks of 256 heads, KEEP: 240 us with 16 columns, 167 with 32 and two workgroups a CU).
 // KEEP: no outputs and no waves for them; the states before the chunks and D are stored (fp32)
 // for the backward pass.
 template <typename T, int NK, bool KEEP, int NC>
@@ -628,7 +628,7 @@ __device__ void walk_kernel(const HelixDeltaParams& p) {
 }
 
 // A walk whose workgroups leave room on every CU, and behind it the operands of the chunks that the next walk takes: 32 chunks
-// of 64 heads take 63 us by themselves, and 79 with the next 32 chunks' operands, which are 28 in a launch of their own.
+// of 64 heads take 70 us by themselves, and 94 with the next 32 chunks' operands, which are 28 in a launch of their own.
 template <typename T, int NK, bool ODD>
 __device__ void delta_walk_ahead(const HelixDeltaParams& p) {
     if constexpr (sizeof(T) == 4) return walk_kernel<T, NK, ODD, false, 1>(p);   // (fp32's take a CU's LDS and registers)
@@ -657,7 +657,7 @@ __device__ void delta_walk_ahead(const HelixDeltaParams& p) {
 // second four waves bring K, Q and dO and form what does not wait for E, P' dO and
 // scale (e^G Q)' dO of the chunk after the one that the first four are at. It leaves E and Z for
 // the kernels below. Bound as the walk is: 32 chunks of 256 heads of 128 x 64, bf16, 333 us with 16
-// columns a workgroup, 256 with 32.
+// columns a workgroup, 257 with 32.
 template <typename T, int NK, bool ODD, int NC>
 __device__ void delta_back(const HelixDeltaParams& p) {
     constexpr int NPL = dr_planes<T>, NT = NK / 64, KS = NK / 32, COLS = 16 * NC;
@@ -1065,7 +1065,7 @@ __device__ void delta_pairs(const HelixDeltaParams& p) {
         }
         __syncthreads();
         {
-                        const int j = 16 * jb + c;
+            const int j = 16 * jb + c;
             const double Gj = sG[j];
             const f32x4 beta = *reinterpret_cast<const f32x4*>(&sB[16 * tb + 4 * q]);
             float pair[4], bs[4];
