@@ -734,7 +734,7 @@ __device__ void delta_back(const HelixDeltaParams& p) {
                 dr_put4<NPL, DR_C, COLS, sizeof(T) == 4>(sO, 16 * n + c, row0, o[0], o[1], o[2], o[3]);
 #pragma unroll
                 for (int r = 0; r < 4; ++r) o[r] *= p.scale * start[r];
-                dr_put4<3, DR_C, COLS>(sW, 16 * n + c, row0, o[0], o[1], o[2], o[3]);
+                dr_put4<3, DR_C, COLS, sizeof(T) == 4>(sW, 16 * n + c, row0, o[0], o[1], o[2], o[3]);   // (dO at the end of fp32)
             }
         };
         auto put_k = [&](int ch) {

@@ -896,7 +896,7 @@ bool delta_shape(const A& a) {
     return true;
 }
 
-// Whether sizes are such as a call takes and needs scratch for (those that it refuses may be any here).
+// Whether sizes are such as a call takes, of some heads (those that it refuses may be any here).
 template <typename A>
 bool delta_heads(const A& a) {
     return a.n_seq > 0 && a.n_head > 0 && a.n_tok >= 0 && a.n_key > 0 && a.n_key <= HELIX_DELTA_MAX_KEY && a.n_val > 0 &&

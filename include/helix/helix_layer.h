@@ -302,8 +302,9 @@ helix_status helix_gated_scan_backward_encode(helix_ctx* ctx, void* stream,
  *
  * Products keep fp32 accuracy (operands in three bf16 parts, fp32 sums; of a
  * chunk's operands below 2^-110, 2^-134), whatever the storage type; o is rounded
- * to it once. Inputs may be any finite numbers, the type's largest too, whose sums
- * (S' k, S' q and the products of a chunk's keys and queries) stay finite in fp32.
+ * to it once. Inputs may be any finite numbers, the type's largest too; what is
+ * formed of them (S, S' k, S' q, what a token brings, the products of a chunk's keys
+ * and queries) has to stay below bf16's largest, 3.3895e38.
  * What is not finite (g = -inf apart) stays where the formulas take it: an element
  * of v or s0 in its column of o and s, one of q in its token's o, one of k, g or
  * beta in its heads' o and s; but in a call of chunks the o of tokens before it in

@@ -80,3 +80,19 @@ def test_values_at_the_end_of_fp32(gpu, L):
     least = float((sc * lo.f64(big)[0, :, 0].norm(dim=-1) * 8 ** 0.5 * 2.0 ** -134 * d).norm())
     off = float((lo.f64(o) - want).norm())
     assert off <= do_.FP32 * so + least, (off, do_.FP32 * so, least)
+
+
+@pytest.mark.parametrize("N", [8, 72])
+@pytest.mark.parametrize("L", [5, 70])
+def test_gradients_of_outputs_at_the_end_of_fp32(gpu, L, N):
+    # With scale 1 and no decay, what multiplies the queries is at the end too. (Small q and v: all that follows stays finite.)
+    q, k, v, g, beta, _ = problem(1, L, 1, 1, N, 16, torch.float32, 5)
+    q, v, g = 1e-3 * q, 1e-2 * v, torch.zeros_like(g)
+    do = torch.zeros_like(v)
+    do[:, 2, :, :8] = torch.finfo(torch.float32).max * (1 - torch.arange(8, device="cuda") * 2.0 ** -12)
+    want, size = do_.backward(do, q, k, v, g, beta, None, None, 1.0)
+    got = delta_rule_backward(do, q, k, v, g, beta, scale=1.0)
+    for n, a, b in zip(("dq", "dk", "dv", "dg", "dbeta", "ds0"), got, want):
+        assert a.isfinite().all(), n
+        # (In units of 2^100, whose squares a norm can add.)
+        do_.close(a.double() * 2.0 ** -100, b * 2.0 ** -100, size[n] * 2.0 ** -100, torch.float32, n)
